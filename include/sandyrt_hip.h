@@ -57,7 +57,9 @@ enum SandyDeviceError {
     SANDY_DEVERR_GATHER_ID = 1u << 3,   /* embedding id out of range */
     SANDY_DEVERR_OFFSETS = 1u << 4,     /* moe_matmul invalid expert offsets */
     SANDY_DEVERR_BLOCK = 1u << 5,       /* paged block id outside the pool */
-    SANDY_DEVERR_ATTN_POS = 1u << 6     /* attention position_offsets must be non-negative */
+    SANDY_DEVERR_ATTN_POS = 1u << 6,    /* attention position_offsets must be non-negative */
+    SANDY_DEVERR_QUANT_ROWS = 1u << 7,  /* quant_paged rows before 0 or past the block table */
+    SANDY_DEVERR_QUANT_COUNT = 1u << 8  /* quant_paged count below 0 or above the row count */
 };
 
 /* A strided view of device memory (TensorViewDesc, src/device/DeviceTypes.h:25-29). */
@@ -136,6 +138,32 @@ typedef struct SandyPagedTensor {
 } SandyPagedTensor;
 
 #define SANDY_HIP_PAGED_STAGE_SLOTS 8
+
+/* Payload types of a quantised paged cache. */
+enum SandyQuantFormat {
+    SANDY_QUANT_INT8 = 0, /* two's complement, -127..127 */
+    SANDY_QUANT_E4M3 = 1  /* OCP float8 e4m3 (no infinities), magnitudes up to 448 */
+};
+
+/*
+ * A paged K or V cache held in 8 bits.  pool [num_pages, prefix, page_size,
+ * inner] bytes, scales [num_pages, prefix] bytes, both contiguous.  A block is
+ * one page of one head: its values are payload * 2^(c - 127) with c the
+ * block's scale byte; c = 255 stands for NaN and makes every value of the
+ * block NaN.  Powers of two keep every value exact in bf16, and a block whose
+ * scale grows while it fills loses nothing but the bits that the larger scale
+ * cannot hold.
+ */
+typedef struct SandyQuantCache {
+    void* pool;
+    void* scales;
+    int32_t format;           /* enum SandyQuantFormat */
+    int32_t reserved;
+    int64_t page_size;        /* rows of a page (power of two) */
+    int64_t prefix;           /* kv heads */
+    int64_t inner;            /* head dim */
+    int64_t num_pages;
+} SandyQuantCache;
 
 /* One node of a fused element-wise scalar DAG (ScalarNode, src/ir/KernelIR.h:346-355). */
 typedef struct SandyScalarNode {
@@ -341,6 +369,76 @@ int sandy_hip_paged_attention_noalloc(const SandyTensor* q, const SandyPagedCach
                                       const SandyPagedCache* v_cache, const SandyTensor* block_table,
                                       const SandyTensor* position_offsets, int64_t window, double scale,
                                       const SandyTensor* out, void* stream, char* err, size_t err_cap);
+
+/* ---------------------------------------------------------------- quantised paged K/V cache */
+
+/*
+ * No counterpart in the reference, whose paged tensors keep the model's type.
+ * K and V caches share format and geometry; block_table [B, max_blocks] int32
+ * lists each sequence's pages in order (max_blocks * page_size <= 2^30);
+ * position_offsets [B] (i32/i64) is each sequence's first row or query of the
+ * call; counts (NULL or [B], i32/i64) how many of the T rows or queries it has,
+ * the rest being padding of a ragged batch.  A count outside 0..T is recorded
+ * (SANDY_DEVERR_QUANT_COUNT) and clamped.  A block id outside the pool is
+ * recorded (SANDY_DEVERR_BLOCK): its rows are not written, read as zero, and
+ * contribute no keys.  Table entries past a sequence's rows are not read.
+ */
+
+/*
+ * Quantise rows as they are written: k and v [B, prefix, T, inner] (F32 or
+ * BF16, any strides) into rows position .. position + count - 1 of each
+ * sequence.  v and v_cache may both be NULL.  The scale of a block is the
+ * smallest power of two (2^-126 at the least) that holds the largest magnitude
+ * written to it since its first row: a block that already has rows keeps the
+ * larger of its scale and the new rows' one, and its rows are rounded again
+ * when the scale grows (nearest even, as every value is; whatever the number of
+ * times, an int8 value ends within one final step).  A write at a page's first row
+ * starts its block anew.  New values that are not finite (or above 127 * 2^121 for
+ * int8, 448 * 2^119 for e4m3, next to 2^128) make the block's scale NaN (c =
+ * 255, until it starts anew) with payload 0.  Rows of a page
+ * past the last one written are left as they were.  Sequences that write to
+ * the same page in one call race on it.  Rows outside the block table are
+ * recorded (SANDY_DEVERR_QUANT_ROWS) and that sequence writes nothing.
+ */
+int sandy_hip_quant_paged_append(const SandyTensor* k, const SandyTensor* v, const SandyQuantCache* k_cache,
+                                 const SandyQuantCache* v_cache, const SandyTensor* block_table,
+                                 const SandyTensor* position_offsets, const SandyTensor* counts, void* stream,
+                                 char* err, size_t err_cap);
+
+/*
+ * Rows position .. position + count - 1 of each sequence back: k_out and v_out
+ * [B, prefix, T, inner] contiguous, F32 or BF16 (every value exact in either,
+ * but for bf16 below 2^-126).  v_out and v_cache may both be NULL.  Rows from
+ * count on and rows outside the block table (SANDY_DEVERR_QUANT_ROWS) are zero.
+ */
+int sandy_hip_quant_paged_read(const SandyQuantCache* k_cache, const SandyQuantCache* v_cache,
+                               const SandyTensor* block_table, const SandyTensor* position_offsets,
+                               const SandyTensor* counts, const SandyTensor* k_out, const SandyTensor* v_out,
+                               void* stream, char* err, size_t err_cap);
+
+/*
+ * Causal attention over the cache: q [B, Hq, T, inner] (F32 or BF16, any
+ * strides; Hq a multiple of prefix), query t of a sequence at position
+ * position + t sees keys 0 .. position + t (and >= position + t + 1 - window
+ * when window > 0) that the block table covers.  scale <= 0 means
+ * 1/sqrt(inner); inner <= 512.  Queries from count on, and queries that see no
+ * key, give zero; a negative position is recorded (SANDY_DEVERR_ATTN_POS) and
+ * its sequence gives zero.  Scores, softmax and sums are fp32 or wider, for
+ * values the cache holds exactly.  out has q's shape and type and may be q
+ * itself.  `workspace` holds sandy_hip_quant_paged_attention_workspace() bytes
+ * (16-byte aligned; NULL where that is 0): the call's alone while it runs, its
+ * contents need not be kept or cleared.
+ */
+int sandy_hip_quant_paged_attention(const SandyTensor* q, const SandyQuantCache* k_cache,
+                                    const SandyQuantCache* v_cache, const SandyTensor* block_table,
+                                    const SandyTensor* position_offsets, const SandyTensor* counts, int64_t window,
+                                    double scale, const SandyTensor* out, void* workspace, size_t workspace_bytes,
+                                    void* stream, char* err, size_t err_cap);
+
+/* Workspace bytes of an attention call with this q, cache and block table. */
+int sandy_hip_quant_paged_attention_workspace(const SandyTensor* q, const SandyQuantCache* k_cache,
+                                              const SandyTensor* block_table, size_t* bytes, char* err,
+                                              size_t err_cap);
 
 /* ---------------------------------------------------------------- layout */
 

@@ -88,6 +88,19 @@ class SandyPagedView(C.Structure):
     ]
 
 
+class SandyQuantCache(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p),
+        ("scales", C.c_void_p),
+        ("format", C.c_int32),
+        ("reserved", C.c_int32),
+        ("page_size", C.c_int64),
+        ("prefix", C.c_int64),
+        ("inner", C.c_int64),
+        ("num_pages", C.c_int64),
+    ]
+
+
 class SandyRowStats(C.Structure):
     _fields_ = [
         ("sumsq", C.c_void_p),
@@ -153,6 +166,7 @@ T = C.POINTER(SandyTensor)
 P = C.POINTER(SandyPagedCache)
 PV = C.POINTER(SandyPagedView)
 RS = C.POINTER(SandyRowStats)
+Q8 = C.POINTER(SandyQuantCache)
 ERR = C.c_char_p
 
 # name -> argtypes (every function returns int; the last three args are
@@ -179,6 +193,10 @@ SIGNATURES = {
     "sandy_hip_layout_transform": [T, T, C.c_int32, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_attention_paged_view": [T, PV, PV, T, C.c_int64, C.c_double, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_paged_attention_noalloc": [T, P, P, T, T, C.c_int64, C.c_double, T, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_paged_append": [T, T, Q8, Q8, T, T, T, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_paged_read": [Q8, Q8, T, T, T, T, T, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_paged_attention": [T, Q8, Q8, T, T, T, C.c_int64, C.c_double, T, C.c_void_p, C.c_size_t,
+                                        C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_topk": [T, C.c_int64, C.c_int64, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_gather": [T, T, T, C.c_int64, C.c_int64, T, T, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_matmul": [T, T, T, C.c_int32, T, C.c_void_p, ERR, C.c_size_t],
@@ -225,6 +243,7 @@ DEVICE_SIGNATURES = {
     "sandy_hip_device_graph_end": ([DEV, U32P], C.c_int),
     "sandy_hip_device_graph_launch": ([DEV, C.c_uint32], C.c_int),
     "sandy_hip_device_graph_destroy": ([DEV, C.c_uint32], C.c_int),
+    "sandy_hip_quant_paged_attention_workspace": ([T, Q8, T, C.POINTER(C.c_size_t)], C.c_int),
 }
 ST = C.c_void_p
 DEVICE_SIGNATURES.update({

@@ -1,0 +1,33 @@
+// quant_attention.h -- attention over the 8-bit paged K/V cache: the arguments
+// its kernels share.
+#pragma once
+#include "quant_cache.h"
+
+namespace sandy_hip {
+
+struct QuantAttnArgs {
+    QuantPages p;  // tokens = queries a sequence
+    const void* q;
+    void* out;
+    int64_t qs[4], os[4];  // element strides over (b, h, t, d)
+    int64_t window;
+    float scale_log2;      // scale * log2(e)
+    int32_t hq, group;     // q heads, of one kv head
+    int32_t f32;           // q and out are f32, else bf16
+};
+
+// Keys [first, last] that query t of a sequence at `pos` sees (none: last < first).
+struct KeyRange {
+    int first, last;
+};
+
+__device__ __forceinline__ KeyRange quant_keys(const QuantAttnArgs& a, int64_t pos, int t) {
+    const int64_t at = pos + t;
+    const int64_t cap = static_cast<int64_t>(a.p.max_blocks) << a.p.log2_page;
+    KeyRange r;
+    r.last = static_cast<int>(min<int64_t>(at, cap - 1));
+    r.first = a.window > 0 ? static_cast<int>(min<int64_t>(max<int64_t>(at - a.window + 1, 0), cap)) : 0;
+    return r;
+}
+
+} // namespace sandy_hip

@@ -1,0 +1,166 @@
+// quant_attention.hip -- causal attention over the 8-bit paged K/V cache.
+//
+// o = sum_k p_k v_k / sum_k p_k, p_k = 2^(s_k - m), s_k = scale log2(e) q . k_k,
+// one pass over the keys with the running maximum m and sum.  A block's scale
+// never touches its payload: K's multiplies the score, V's the weight p.
+#include "quant_attention.h"
+
+#include <algorithm>
+
+namespace sandy_hip {
+namespace {
+
+constexpr int kMaxDim = 512;
+
+// Any head dim and page size: a workgroup per (sequence, q head, query), 256
+// keys at a time -- a thread scores one key, then owns dims tid and tid + 256.
+template <typename T, int FORMAT>
+__global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnArgs a) {
+    constexpr int kDims = kMaxDim / 256;
+    __shared__ float qf[kMaxDim];
+    __shared__ float weight[256];
+    __shared__ const uint8_t* row[256];
+    __shared__ float part[4];
+    __shared__ double sums[4];
+    const QuantPages& p = a.p;
+    const int tid = threadIdx.x;
+    uint32_t at = blockIdx.x;
+    const int t = at % p.tokens;
+    at /= p.tokens;
+    const int h = at % a.hq;
+    const int b = at / a.hq;
+    const int kh = h / a.group;
+    const int D = p.dim;
+    const int64_t pos = load_index(p.pos, p.pos_dt, b);
+    if (pos < 0 && tid == 0) atomicOr(p.errw, static_cast<uint32_t>(SANDY_DEVERR_ATTN_POS));
+    KeyRange keys = quant_keys(a, pos, t);
+    if (pos < 0 || t >= quant_count(p, b)) keys = KeyRange{0, -1};
+    const int64_t q0 = b * a.qs[0] + h * a.qs[1] + t * a.qs[2];
+    for (int d = tid; d < D; d += 256) qf[d] = Vec8<T>::load1(a.q, q0 + d * a.qs[3]);
+    __syncthreads();
+    float m = -INFINITY, acc[kDims];
+    double l = 0.0;
+#pragma unroll
+    for (int i = 0; i < kDims; i++) acc[i] = 0.0f;
+    for (int k0 = keys.first; k0 <= keys.last; k0 += 256) {
+        const int key = k0 + tid;
+        float s = -INFINITY, vs = 0.0f;
+        const uint8_t* vrow = nullptr;
+        if (key <= keys.last) {
+            const int id = quant_block(p, b, key >> p.log2_page);
+            if (id >= 0) {
+                const int64_t block = static_cast<int64_t>(id) * p.heads + kh;
+                const int64_t from = ((block << p.log2_page) + (key & ((1 << p.log2_page) - 1))) * D;
+                const uint8_t* krow = p.pool[0] + from;
+                float dot = 0.0f;
+                for (int d = 0; d < D; d++) dot = fmaf(qf[d], Quant<FORMAT>::template value<0>(krow[d]), dot);
+                s = dot * quant_scale(p.scales[0][block]) * a.scale_log2;
+                vs = quant_scale(p.scales[1][block]);
+                vrow = p.pool[1] + from;
+            }
+        }
+        float mx = wave_max(s);
+        __syncthreads();  // the sums over the chunk before have been read
+        if ((tid & 63) == 0) part[tid >> 6] = mx;
+        __syncthreads();
+        mx = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), m);
+        const float shift = mx == -INFINITY ? 0.0f : mx;
+        const float alpha = __builtin_amdgcn_exp2f(m - shift);
+        const float w = vrow ? __builtin_amdgcn_exp2f(s - shift) : 0.0f;
+        l = l * static_cast<double>(alpha) + static_cast<double>(w);
+        m = mx;
+        weight[tid] = vrow ? w * vs : 0.0f;
+        row[tid] = vrow;
+        __syncthreads();
+        const int n = min(256, keys.last - k0 + 1);
+#pragma unroll
+        for (int i = 0; i < kDims; i++) {
+            const int d = tid + 256 * i;
+            if (d >= D) continue;
+            acc[i] *= alpha;
+            for (int j = 0; j < n; j++)
+                if (row[j]) acc[i] = fmaf(weight[j], Quant<FORMAT>::template value<0>(row[j][d]), acc[i]);
+        }
+    }
+    l = wave_sum(l);
+    if ((tid & 63) == 0) sums[tid >> 6] = l;
+    __syncthreads();
+    const double total = sums[0] + sums[1] + sums[2] + sums[3];
+    const float inv = total == 0.0 ? 0.0f : 1.0f / static_cast<float>(total);
+    const int64_t o0 = b * a.os[0] + h * a.os[1] + t * a.os[2];
+#pragma unroll
+    for (int i = 0; i < kDims; i++) {
+        const int d = tid + 256 * i;
+        if (d < D) Vec8<T>::store1(a.out, o0 + d * a.os[3], acc[i] * inv);
+    }
+}
+
+int check_quant_attention(const SandyTensor* q, const SandyQuantCache* kc, Err e) {
+    if (!valid_rank(q) || !kc) return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires q and caches");
+    if (!is_float(q->dtype)) return fail(e, SANDY_ERR_INVALID, "attention q unsupported dtype");
+    if (q->rank != 4) return fail(e, SANDY_ERR_INVALID, "quant_paged attention expects q [B, Hq, T, D]");
+    if (kc->inner != q->dims[3]) return fail(e, SANDY_ERR_INVALID, "attention head dimension mismatch");
+    if (kc->inner > kMaxDim) return fail(e, SANDY_ERR_UNSUPPORTED, "attention head dimension above 512");
+    if (kc->prefix <= 0 || q->dims[1] <= 0 || q->dims[1] % kc->prefix != 0)
+        return fail(e, SANDY_ERR_INVALID, "attention heads must be divisible by kv_heads");
+    return SANDY_OK;
+}
+
+} // namespace
+} // namespace sandy_hip
+
+using namespace sandy_hip;
+
+extern "C" int sandy_hip_quant_paged_attention_workspace(const SandyTensor* q, const SandyQuantCache* kc,
+                                                         const SandyTensor* table, size_t* bytes, char* err,
+                                                         size_t err_cap) {
+    Err e{err, err_cap};
+    int status = check_quant_attention(q, kc, e);
+    if (status) return status;
+    if (!valid_rank(table) || !bytes) return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires a block table");
+    *bytes = 0;
+    return ok(e);
+}
+
+extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const SandyQuantCache* kc,
+                                               const SandyQuantCache* vc, const SandyTensor* table,
+                                               const SandyTensor* position_offsets, const SandyTensor* counts,
+                                               int64_t window, double scale, const SandyTensor* out, void* workspace,
+                                               size_t workspace_bytes, void* stream, char* err, size_t err_cap) {
+    Err e{err, err_cap};
+    int status = check_quant_attention(q, kc, e);
+    if (status) return status;
+    if (!vc || !valid_rank(out)) return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires q and caches");
+    if (!same_shape(*q, *out) || out->dtype != q->dtype) return fail(e, SANDY_ERR_INVALID, "attention output shape mismatch");
+    if (window < 0) return fail(e, SANDY_ERR_INVALID, "attention window must be >= 0");
+    QuantAttnArgs a{};
+    status = check_quant_pages(kc, vc, table, position_offsets, counts, q->dims[0], q->dims[2], e, &a.p);
+    if (status) return status;
+    if (numel(*q) == 0) return ok(e);
+    a.p.errw = device_error_word(e, &status);
+    if (status) return status;
+    a.q = base_ptr(*q);
+    a.out = base_ptr(*out);
+    for (int i = 0; i < 4; i++) {
+        a.qs[i] = q->strides[i];
+        a.os[i] = out->strides[i];
+    }
+    a.window = window;
+    a.scale_log2 = (scale <= 0.0 ? 1.0f / sqrtf(static_cast<float>(a.p.dim)) : static_cast<float>(scale)) * 1.44269504088896341f;
+    a.hq = static_cast<int32_t>(q->dims[1]);
+    a.group = a.hq / a.p.heads;
+    a.f32 = q->dtype == SANDY_F32;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int64_t wgs = q->dims[0] * q->dims[1] * q->dims[2];
+    if (wgs > UINT32_MAX / 256) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged attention of too many queries");
+    const dim3 grid(static_cast<unsigned>(wgs));
+    if (kc->format == SANDY_QUANT_INT8) {
+        if (a.f32) hipLaunchKernelGGL((quant_attention_general_kernel<F32, SANDY_QUANT_INT8>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((quant_attention_general_kernel<BF16, SANDY_QUANT_INT8>), grid, dim3(256), 0, s, a);
+    } else {
+        if (a.f32) hipLaunchKernelGGL((quant_attention_general_kernel<F32, SANDY_QUANT_E4M3>), grid, dim3(256), 0, s, a);
+        else hipLaunchKernelGGL((quant_attention_general_kernel<BF16, SANDY_QUANT_E4M3>), grid, dim3(256), 0, s, a);
+    }
+    SANDY_HIP_TRY(hipGetLastError(), e, "quant_paged attention launch");
+    return ok(e);
+}

@@ -150,5 +150,7 @@ extern "C" int sandy_hip_take_device_errors(void* stream, uint32_t* flags, char*
     if (host & SANDY_DEVERR_OFFSETS) return fail(e, SANDY_ERR_INVALID, "moe_matmul invalid expert offsets");
     if (host & SANDY_DEVERR_BLOCK) return fail(e, SANDY_ERR_INVALID, "paged attention block id outside the pool");
     if (host & SANDY_DEVERR_ATTN_POS) return fail(e, SANDY_ERR_INVALID, "attention position_offsets must be non-negative");
+    if (host & SANDY_DEVERR_QUANT_ROWS) return fail(e, SANDY_ERR_INVALID, "quant_paged rows outside the block table");
+    if (host & SANDY_DEVERR_QUANT_COUNT) return fail(e, SANDY_ERR_INVALID, "quant_paged counts out of range");
     return ok(e);
 }

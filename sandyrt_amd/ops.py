@@ -417,6 +417,106 @@ def paged_attention_noalloc(q, k_cache: PagedCache, v_cache: PagedCache, block_t
     return out
 
 
+# ------------------------------------------------------------------ quantised paged K/V cache
+_QUANT_FORMATS = {"int8": (torch.int8, 0), "e4m3": (torch.float8_e4m3fn, 1)}
+_QUANT_CODES = dict(_QUANT_FORMATS.values())
+
+
+@dataclass
+class QuantPagedCache:
+    """A paged K or V cache held in 8 bits: pool [num_pages, heads, page_size,
+    dim] of int8 or float8_e4m3fn payloads and scales [num_pages, heads] uint8,
+    both contiguous.  The values of a page's head are payload * 2^(c - 127)
+    with c its scale byte; 255 stands for NaN."""
+
+    pool: torch.Tensor
+    scales: torch.Tensor
+
+    @staticmethod
+    def empty(num_pages: int, heads: int, page_size: int, dim: int, format: str = "int8", device="cuda"):
+        """A cache without rows (every value 0)."""
+        if format not in _QUANT_FORMATS:
+            raise SandyError(1, "quant_paged cache format must be int8 or e4m3")
+        shape = (num_pages, heads, page_size, dim)
+        return QuantPagedCache(torch.zeros(shape, dtype=torch.uint8, device=device).view(_QUANT_FORMATS[format][0]),
+                               torch.zeros(num_pages, heads, dtype=torch.uint8, device=device))
+
+    def struct(self):
+        pool, scales = self.pool, self.scales
+        if pool.dtype not in _QUANT_CODES:
+            raise SandyError(1, "quant_paged cache format must be int8 or e4m3")
+        if pool.dim() != 4 or not pool.is_contiguous():
+            raise SandyError(1, "quant_paged pool must be a contiguous [pages, heads, page_size, dim] tensor")
+        if scales.dtype != torch.uint8 or scales.shape != pool.shape[:2] or not scales.is_contiguous():
+            raise SandyError(1, "quant_paged scales must be a contiguous [pages, heads] uint8 tensor")
+        pages, heads, rows, dim = pool.shape
+        return _lib.SandyQuantCache(pool.data_ptr(), scales.data_ptr(), _QUANT_CODES[pool.dtype], 0, rows, heads, dim,
+                                    pages)
+
+
+def _quant_call(name, tensors, caches, *args):
+    """An entry point of the quantised cache, on its tensors' own device."""
+    tensors = [t for t in tensors if t is not None] + [t for c in caches if c is not None for t in (c.pool, c.scales)]
+    _require_gpu(*tensors)
+    device = tensors[0].device
+    if any(t.device != device for t in tensors):
+        raise SandyError(1, "quant_paged tensors must live on one GPU")
+    if device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
+
+
+def quant_paged_append(k, v, k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_table, position_offsets,
+                       counts=None) -> None:
+    """Quantise k and v [B, heads, T, dim] into rows position_offsets[b] .. of
+    each sequence's pages, one launch for both (v and v_cache None: k alone).
+
+    A block (page and head) takes the smallest power-of-two scale that holds
+    its largest magnitude; rows it already has are rounded again when the scale
+    grows.  A write at a page's first row starts its block anew.  `counts` [B]:
+    the rows each sequence has of the T, the others are padding.  Sequences of
+    one call must not write to the same page."""
+    _quant_call("sandy_hip_quant_paged_append", (k, v, block_table, position_offsets, counts), (k_cache, v_cache),
+                arg(k), arg(v), k_cache.struct(), None if v_cache is None else v_cache.struct(), arg(block_table),
+                arg(position_offsets), arg(counts))
+
+
+def quant_paged_read(k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_table, position_offsets, tokens: int,
+                     counts=None, dtype=torch.bfloat16, k_out=None, v_out=None):
+    """Rows position_offsets[b] .. + tokens of each sequence back, as (k, v)
+    [B, heads, tokens, dim]; zero from counts[b] on.  v_cache None: v is None."""
+    def output(cache, out):
+        if cache is None or out is not None:
+            return out
+        return torch.empty(block_table.shape[0], cache.pool.shape[1], tokens, cache.pool.shape[3], dtype=dtype,
+                           device=cache.pool.device)
+
+    k_out, v_out = output(k_cache, k_out), output(v_cache, v_out)
+    _quant_call("sandy_hip_quant_paged_read", (k_out, v_out, block_table, position_offsets, counts),
+                (k_cache, v_cache), k_cache.struct(), None if v_cache is None else v_cache.struct(), arg(block_table),
+                arg(position_offsets), arg(counts), arg(k_out), arg(v_out))
+    return k_out, v_out
+
+
+def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_table, position_offsets,
+                          counts=None, window: int = 0, scale: float = -1.0, out=None):
+    """Causal attention of q [B, Hq, T, dim] over a quantised cache: query t of
+    a sequence sees keys up to position_offsets[b] + t (its own, which must have
+    been appended).  Queries from counts[b] on give zero."""
+    out = torch.empty_like(q) if out is None else out
+    kc, vc, qa, ta = k_cache.struct(), v_cache.struct(), arg(q), arg(block_table)
+    need = C.c_size_t(0)
+    _lib.dcall("sandy_hip_quant_paged_attention_workspace", qa, kc, ta, C.byref(need))
+    # the call's own: calls on other streams and captured graphs share nothing with it
+    work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    _quant_call("sandy_hip_quant_paged_attention", (q, out, block_table, position_offsets, counts),
+                (k_cache, v_cache), qa, kc, vc, ta, arg(position_offsets), arg(counts), int(window), float(scale),
+                arg(out), work.data_ptr() if work is not None else None, need.value)
+    return out
+
+
 # ------------------------------------------------------------------ MoE
 def topk(x, k: int, axis: int = -1, index_dtype=torch.int64, values=None, indices=None):
     """TopKKernelOp: value descending, index ascending on ties (TensorCalc.cpp:1447-1518)."""
