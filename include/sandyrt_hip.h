@@ -435,9 +435,9 @@ int sandy_hip_quant_paged_attention(const SandyTensor* q, const SandyQuantCache*
                                     double scale, const SandyTensor* out, void* workspace, size_t workspace_bytes,
                                     void* stream, char* err, size_t err_cap);
 
-/* Workspace bytes of an attention call with this q, cache and block table. */
+/* Workspace bytes of an attention call with this q, cache, block table and window. */
 int sandy_hip_quant_paged_attention_workspace(const SandyTensor* q, const SandyQuantCache* k_cache,
-                                              const SandyTensor* block_table, size_t* bytes, char* err,
+                                              const SandyTensor* block_table, int64_t window, size_t* bytes, char* err,
                                               size_t err_cap);
 
 /* ---------------------------------------------------------------- layout */

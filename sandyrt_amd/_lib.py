@@ -243,7 +243,7 @@ DEVICE_SIGNATURES = {
     "sandy_hip_device_graph_end": ([DEV, U32P], C.c_int),
     "sandy_hip_device_graph_launch": ([DEV, C.c_uint32], C.c_int),
     "sandy_hip_device_graph_destroy": ([DEV, C.c_uint32], C.c_int),
-    "sandy_hip_quant_paged_attention_workspace": ([T, Q8, T, C.POINTER(C.c_size_t)], C.c_int),
+    "sandy_hip_quant_paged_attention_workspace": ([T, Q8, T, C.c_int64, C.POINTER(C.c_size_t)], C.c_int),
 }
 ST = C.c_void_p
 DEVICE_SIGNATURES.update({

@@ -22,12 +22,19 @@ struct KeyRange {
 };
 
 __device__ __forceinline__ KeyRange quant_keys(const QuantAttnArgs& a, int64_t pos, int t) {
-    const int64_t at = pos + t;
+    const int64_t at = min<int64_t>(pos, INT64_MAX - INT32_MAX) + t;
     const int64_t cap = static_cast<int64_t>(a.p.max_blocks) << a.p.log2_page;
     KeyRange r;
     r.last = static_cast<int>(min<int64_t>(at, cap - 1));
     r.first = a.window > 0 ? static_cast<int>(min<int64_t>(max<int64_t>(at - a.window + 1, 0), cap)) : 0;
     return r;
 }
+
+// Few queries a sequence (quant_decode.hip): whether the kernel takes the call,
+// its workspace (whatever the call's strides), its launch.
+bool quant_decode_takes(const QuantAttnArgs& a);
+size_t quant_decode_workspace(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t page,
+                              int64_t max_blocks, int64_t window);
+int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace, hipStream_t stream, Err e);
 
 } // namespace sandy_hip

@@ -112,13 +112,15 @@ int check_quant_attention(const SandyTensor* q, const SandyQuantCache* kc, Err e
 using namespace sandy_hip;
 
 extern "C" int sandy_hip_quant_paged_attention_workspace(const SandyTensor* q, const SandyQuantCache* kc,
-                                                         const SandyTensor* table, size_t* bytes, char* err,
-                                                         size_t err_cap) {
+                                                         const SandyTensor* table, int64_t window, size_t* bytes,
+                                                         char* err, size_t err_cap) {
     Err e{err, err_cap};
     int status = check_quant_attention(q, kc, e);
     if (status) return status;
-    if (!valid_rank(table) || !bytes) return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires a block table");
-    *bytes = 0;
+    if (!valid_rank(table) || table->rank != 2 || !bytes)
+        return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires a block table");
+    *bytes = quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner, kc->page_size,
+                                    table->dims[1], window);
     return ok(e);
 }
 
@@ -151,6 +153,13 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     a.group = a.hq / a.p.heads;
     a.f32 = q->dtype == SANDY_F32;
     hipStream_t s = static_cast<hipStream_t>(stream);
+    if (quant_decode_takes(a)) {
+        const size_t need = quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner,
+                                                   kc->page_size, table->dims[1], window);
+        if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
+            return fail(e, SANDY_ERR_INVALID, "quant_paged attention needs a 16-byte aligned workspace of %zu bytes", need);
+        return launch_quant_decode(a, kc->format, workspace, s, e);
+    }
     const int64_t wgs = q->dims[0] * q->dims[1] * q->dims[2];
     if (wgs > UINT32_MAX / 256) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged attention of too many queries");
     const dim3 grid(static_cast<unsigned>(wgs));

@@ -1,0 +1,498 @@
+// quant_decode.hip -- attention of few queries a sequence over the 8-bit paged
+// cache on bf16 MFMA, the keys split over workgroups.
+//
+// Both payload types are exact in bf16, so a payload goes to the matrix unit as
+// it is: S^T = K Q^T with K's scale applied to the scores, O^T += V^T P^T with
+// V's applied to the weights (int8) or in the conversion itself (e4m3: exact,
+// the scale is a power of two).  f32 queries enter as three bf16 operands that
+// hold them exactly, and so do their weights; bf16 queries' weights enter as
+// two (2^-15 of each, against the output's 2^-8).  Tiles are 16 keys; a wave takes two at a time:
+//   - K straight into the A operand: a lane holds 16 consecutive dims of its key,
+//     the first 8 for one MFMA step and the others for the next (the order of the
+//     contraction is free as long as Q has the same);
+//   - V through the wave's own LDS rows, back by ds_read_b64_tr_b8, which gives a
+//     lane one dim of 8 keys -- the A operand of O^T in the order that P leaves S^T.
+#include "quant_attention.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace sandy_hip {
+namespace {
+
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+
+constexpr int kRsrcWord3 = 0x00020000;  // gfx9 buffer resource word 3: raw dword access
+constexpr int kMinPairs = 4;            // pairs of tiles a split has at least: one a wave
+
+// Four payloads as four bf16, times `scale` (e4m3 only; a power of two).
+template <int FORMAT>
+__device__ __forceinline__ void payload_bf16(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
+    if constexpr (FORMAT == SANDY_QUANT_E4M3) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, true));
+    } else {  // at most 8 bits: the upper halves of the floats
+        float v[4];
+        quant_values<FORMAT>(w, v);
+        lo = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
+        hi = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u);
+    }
+}
+
+template <int FORMAT>
+__device__ __forceinline__ bf16x8_t payload_operand(uint32_t w0, uint32_t w1, float s0, float s1) {
+    u32x4_t r;
+    uint32_t a, b;
+    payload_bf16<FORMAT>(w0, s0, a, b);
+    r[0] = a, r[1] = b;
+    payload_bf16<FORMAT>(w1, s1, a, b);
+    r[2] = a, r[3] = b;
+    return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// x and y as NS bf16 parts each, packed in pairs: the first ones cut, the last
+// rounded (three hold a finite float exactly, two to 2^-15)
+template <int NS>
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[NS]) {
+#pragma unroll
+    for (int n = 0; n < NS - 1; n++) {
+        const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
+        part[n] = __builtin_amdgcn_perm(yb, xb, 0x07060302u);  // the upper halves
+        x -= __uint_as_float(xb & 0xffff0000u);
+        y -= __uint_as_float(yb & 0xffff0000u);
+    }
+    part[NS - 1] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+}
+
+struct DecodeArgs {
+    QuantAttnArgs a;
+    int32_t col_tiles;  // 16-column tiles of the (query, head) rows of a kv head
+    int32_t splits;     // workgroups a column tile's keys may be split over
+    float* part_o;      // [unit, split][16][D] sums relative to the maximum
+    float* part_ml;     // [unit, split][16][2] maximum and sum of weights
+};
+
+// The keys of one column tile: pairs of 16-key tiles from `begin`, `per` of them a split.
+struct TileKeys {
+    int begin, last, pairs, per, active;
+};
+
+__device__ __forceinline__ TileKeys tile_keys(const DecodeArgs& d, int64_t pos, int count, int t_lo, int t_hi) {
+    TileKeys k{0, -1, 0, kMinPairs, 1};
+    t_hi = min(t_hi, count - 1);
+    if (pos >= 0 && t_lo <= t_hi) {
+        k.begin = quant_keys(d.a, pos, t_lo).first & ~15;
+        k.last = quant_keys(d.a, pos, t_hi).last;
+        if (k.last >= k.begin) k.pairs = (k.last - k.begin + 32) >> 5;
+        k.per = max((k.pairs + d.splits - 1) / d.splits, kMinPairs);
+        k.active = max((k.pairs + k.per - 1) / k.per, 1);
+    }
+    return k;
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(void* p, int64_t at, f32x4_t v) {
+    if constexpr (std::is_same_v<T, F32>) *reinterpret_cast<f32x4_t*>(static_cast<float*>(p) + at) = v;
+    else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+}
+
+template <typename T, int FORMAT, int DP>
+struct DecodeGeo {
+    static constexpr int kChunks = DP / 64;  // 16-byte pieces a lane holds of a K (V) tile
+    static constexpr int kRing = DP == 256 ? 1 : 2;  // pairs in flight
+    static constexpr int kWaves = DP == 64 ? 3 : DP == 256 && std::is_same_v<T, F32> ? 1 : 2;  // a SIMD
+    static constexpr int VP = DP + 16;       // bytes of a V row in LDS: column reads spread over the banks
+    static constexpr int kV = 32 * VP;       // a wave's V rows
+    static constexpr int kMerge = 4 * (DP / 16) * 64 * 16;  // every wave's accumulators
+    static constexpr int kBytes = std::max(4 * kV, kMerge) + 4 * 16 * 2 * 4;
+};
+
+template <typename T, int FORMAT, int DP>
+__global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant_decode_kernel(DecodeArgs da) {
+    using G = DecodeGeo<T, FORMAT, DP>;
+    constexpr bool kF32 = std::is_same_v<T, F32>;
+    constexpr int NQ = kF32 ? 3 : 1, NP = kF32 ? 3 : 2, NCH = G::kChunks, NT = DP / 16, RING = G::kRing;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+    const QuantAttnArgs& a = da.a;
+    const QuantPages& p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int D = p.dim;
+    // heads vary fastest, then sequences, splits, column tiles
+    uint32_t at = blockIdx.x;
+    const int kh = at % p.heads;
+    at /= p.heads;
+    const int b = at % p.batch;
+    at /= p.batch;
+    const int split = at % da.splits;
+    const int ct = at / da.splits;
+    const int rows = a.group * p.tokens;
+    const int64_t pos = load_index(p.pos, p.pos_dt, b);
+    const int count = quant_count(p, b);
+    const int t_lo = 16 * ct / a.group, t_hi = min(rows - 1, 16 * ct + 15) / a.group;
+    const TileKeys tk = tile_keys(da, pos, count, t_lo, t_hi);
+    if (split >= tk.active) return;
+    if (pos < 0 && tid == 0) atomicOr(p.errw, static_cast<uint32_t>(SANDY_DEVERR_ATTN_POS));
+
+    // this lane's column: query qt, head qg of the group (past the rows: the last one, not stored)
+    const int row = min(16 * ct + col, rows - 1);
+    const int qt = row / a.group, qg = row - qt * a.group;
+    KeyRange mine = quant_keys(a, pos, qt);
+    if (qt >= count) mine.last = -1;
+    // keys that every column sees
+    const int all_first = quant_keys(a, pos, t_hi).first;
+    const int all_last = t_hi < count ? quant_keys(a, pos, t_lo).last : -1;
+
+    // B operands of Q^T: column, dims 64 j + 16 g + 8 s .. + 7 in step 2 j + s
+    u32x4_t qv[NQ][2 * NCH];
+    {
+        const int64_t q0 = b * a.qs[0] + (kh * a.group + qg) * a.qs[1] + qt * a.qs[2];
+#pragma unroll
+        for (int s = 0; s < 2 * NCH; s++) {
+            const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
+            const int64_t from = q0 + (d < D ? d : 0);
+            if constexpr (kF32) {
+                float x[8];
+                Vec8<F32>::load(a.q, from, x);
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    // an infinity leaves inf - inf for its later parts: NaN scores, as an
+                    // infinite score's weight has
+                    uint32_t part[3];
+                    split_pair<3>(d < D ? x[i] : 0.0f, d < D ? x[i + 1] : 0.0f, part);
+#pragma unroll
+                    for (int n = 0; n < 3; n++) qv[n][s][i / 2] = part[n];
+                }
+            } else {
+                const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + from);
+                qv[0][s] = d < D ? raw : u32x4_t{0, 0, 0, 0};
+            }
+        }
+    }
+
+    f32x4_t acc[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+
+    unsigned char* vrows = lds + wave * G::kV;
+    int k_off[NCH], v_to[NCH];  // this lane's bytes of a tile; its V pieces' places in LDS
+#pragma unroll
+    for (int j = 0; j < NCH; j++) {
+        const int d = 64 * j + 16 * g;
+        k_off[j] = d < D ? col * D + d : 0x7ffffff0;  // past every tile: zeros
+        const int piece = lane + 64 * j, per_row = D / 16;
+        const int r = piece / per_row;
+        v_to[j] = r < 16 ? r * G::VP + 16 * (piece - r * per_row) : -1;
+    }
+    // ds_read_b64_tr_b8: lanes 2 n and 2 n + 1 of 16 address row n's 16 bytes, lane i
+    // gets byte i of the 8 rows: keys 4 g + n of the first tile, then of the second
+    const int trow = (lane & 15) >> 1;
+    const unsigned char* v_from = vrows + (trow < 4 ? 4 * g + trow : 16 + 4 * g + trow - 4) * G::VP + 8 * (lane & 1);
+
+    const int last_pair = min((split + 1) * tk.per, tk.pairs);
+    // a wave takes every fourth pair; 32 of them (64 tiles) a round
+    for (int round0 = split * tk.per + wave; round0 < last_pair; round0 += 4 * 32) {
+        const int n_pairs = min(32, (last_pair - round0 + 3) / 4);
+        // lane i looks up tile i & 1 of the round's pair i / 2
+        int id = -1, rows_in = 0;
+        float kf = 0.0f, vf = 1.0f;
+        {
+            const int pair = round0 + 4 * (lane >> 1);
+            const int key0 = tk.begin + 32 * pair + 16 * (lane & 1);
+            if (pair < last_pair && key0 <= tk.last) {
+                id = quant_block(p, b, key0 >> p.log2_page);
+                rows_in = min(16, tk.last - key0 + 1);
+                if (id >= 0) {
+                    const int64_t block = static_cast<int64_t>(id) * p.heads + kh;
+                    const int kc = p.scales[0][block], vc = p.scales[1][block];
+                    // a NaN block: NaN scores for whoever sees it, V's own factor aside
+                    kf = quant_scale(vc == 255 ? 255 : kc) * a.scale_log2;
+                    vf = quant_scale(vc == 255 ? 127 : vc);
+                }
+            }
+        }
+        u32x4_t kr[RING][2][NCH], vr[RING][2][NCH];
+        auto load = [&](int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int tile = min(2 * n + h, 63);
+                const int blk = __builtin_amdgcn_readlane(id, tile);
+                // rows past the last key and tiles without a page: an empty range reads zeros
+                const int bytes = n < n_pairs && blk >= 0 ? __builtin_amdgcn_readlane(rows_in, tile) * D : 0;
+                const int key0 = tk.begin + 32 * (round0 + 4 * n) + 16 * h;
+                const int64_t off = (((static_cast<int64_t>(max(blk, 0)) * p.heads + kh) << p.log2_page) +
+                                     (key0 & ((1 << p.log2_page) - 1))) * D;
+                const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(p.pool[0] + off, 0, bytes, kRsrcWord3);
+                const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(p.pool[1] + off, 0, bytes, kRsrcWord3);
+#pragma unroll
+                for (int j = 0; j < NCH; j++) k[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off[j], 0, 0));
+#pragma unroll
+                for (int j = 0; j < NCH; j++) v[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * (lane + 64 * j), 0, 0));
+            }
+        };
+        auto attend = [&](int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
+            f32x4_t sc[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                sc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < NCH; j++)
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const bf16x8_t ka = payload_operand<FORMAT>(k[h][j][2 * s], k[h][j][2 * s + 1], 1.0f, 1.0f);
+#pragma unroll
+                        for (int c = NQ - 1; c >= 0; c--)
+                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][2 * j + s]), sc[h], 0, 0, 0);
+                    }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < NCH; j++)
+                    if (v_to[j] >= 0) *reinterpret_cast<u32x4_t*>(vrows + 16 * h * G::VP + v_to[j]) = v[h][j];
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            load(n + RING, k, v);
+            const float kf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n));
+            const float kf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n + 1));
+            const float vf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n));
+            const float vf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + 1));
+            const int id0 = __builtin_amdgcn_readlane(id, 2 * n), id1 = __builtin_amdgcn_readlane(id, 2 * n + 1);
+            const int k0 = tk.begin + 32 * (round0 + 4 * n);
+            sc[0] *= kf0;
+            sc[1] *= kf1;
+            if (k0 < all_first || k0 + 31 > all_last || (id0 | id1) < 0) {
+                // element i of tile h: key k0 + 16 h + 4 g + i
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int key = k0 + 4 * g + i;
+                    if (id0 < 0 || key < mine.first || key > mine.last) sc[0][i] = -INFINITY;
+                    if (id1 < 0 || key + 16 < mine.first || key + 16 > mine.last) sc[1][i] = -INFINITY;
+                }
+            }
+            float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+            // a column's reference m moves only once its maximum has grown by 2^8:
+            // weights stay below that, at the same relative precision
+            if (__any(mx > m + 8.0f)) {
+                mx = max_xor32(max_xor16(mx));
+                const float m_new = fmaxf(m, mx);
+                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+                l *= alpha;
+#pragma unroll
+                for (int t = 0; t < NT; t++) acc[t] *= alpha;
+                m = m_new;
+            }
+            const float shift = m == -INFINITY ? 0.0f : m;
+            float w[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(sc[i >> 2][i & 3] - shift);
+            l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            if constexpr (FORMAT == SANDY_QUANT_INT8)
+#pragma unroll
+                for (int i = 0; i < 8; i++) w[i] *= i < 4 ? vf0 : vf1;
+            bf16x8_t pw[NP];
+            {
+                u32x4_t parts[NP];
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    uint32_t part[NP];
+                    split_pair<NP>(w[i], w[i + 1], part);
+#pragma unroll
+                    for (int c = 0; c < NP; c++) parts[c][i / 2] = part[c];
+                }
+#pragma unroll
+                for (int c = 0; c < NP; c++) pw[c] = __builtin_bit_cast(bf16x8_t, parts[c]);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                if (16 * t >= D) continue;
+                const i32x2_t raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * t)));
+                const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(raw[0]), static_cast<uint32_t>(raw[1]), vf0, vf1);
+#pragma unroll
+                for (int c = NP - 1; c >= 0; c--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw[c], acc[t], 0, 0, 0);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        };
+#pragma unroll
+        for (int i = 0; i < RING; i++) load(i, kr[i], vr[i]);
+        for (int n = 0; n < n_pairs; n += RING) {
+#pragma unroll
+            for (int i = 0; i < RING; i++)
+                if (n + i < n_pairs) attend(n + i, kr[i], vr[i]);
+        }
+    }
+
+    // the four waves' maxima and sums, then their accumulators
+    l = sum_xor32(sum_xor16(l));
+    float* ml = reinterpret_cast<float*>(lds + std::max(4 * G::kV, G::kMerge));
+    if (g == 0) {
+        ml[(wave * 16 + col) * 2] = m;
+        ml[(wave * 16 + col) * 2 + 1] = l;
+    }
+    __syncthreads();
+    float mm = -INFINITY, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) mm = fmaxf(mm, ml[(w * 16 + col) * 2]);
+    const float shift = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+    for (int w = 0; w < 4; w++) total += ml[(w * 16 + col) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 16 + col) * 2] - shift);
+    const float f = __builtin_amdgcn_exp2f(m - shift);
+    f32x4_t* red = reinterpret_cast<f32x4_t*>(lds);
+#pragma unroll
+    for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t] * f;
+    __syncthreads();
+    const bool final_out = tk.active == 1;
+    const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
+    const int64_t slot = unit * da.splits + split;
+    const bool stored = 16 * ct + col < rows;
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+    const int64_t o0 = b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2];
+#pragma unroll
+    for (int t4 = 0; t4 < NT; t4 += 4) {
+        const int t = t4 + wave;
+        if (16 * t >= D) continue;
+        const f32x4_t o = (red[t * 64 + lane] + red[(NT + t) * 64 + lane]) + (red[(2 * NT + t) * 64 + lane] + red[(3 * NT + t) * 64 + lane]);
+        const int d = 16 * t + 4 * g;
+        if (!stored) continue;
+        if (final_out) store4<T>(a.out, o0 + d, o * inv);
+        else *reinterpret_cast<f32x4_t*>(da.part_o + (slot * 16 + col) * D + d) = o;
+    }
+    if (!final_out && tid < 16 && stored) {
+        da.part_ml[(slot * 16 + col) * 2] = mm;
+        da.part_ml[(slot * 16 + col) * 2 + 1] = total;
+    }
+}
+
+// Joins the splits of one output row: a workgroup per row, every thread 4 dims
+// of every (256 / (D / 4))-th split.
+template <typename T>
+__global__ __launch_bounds__(256) void quant_decode_merge_kernel(DecodeArgs da) {
+    __shared__ f32x4_t sums[256];
+    const QuantAttnArgs& a = da.a;
+    const QuantPages& p = a.p;
+    const int tid = threadIdx.x, D = p.dim;
+    uint32_t at = blockIdx.x;
+    const int rows = a.group * p.tokens;
+    const int row = at % rows;
+    at /= rows;
+    const int kh = at % p.heads;
+    const int b = at / p.heads;
+    const int ct = row >> 4, col = row & 15;
+    const int t_lo = 16 * ct / a.group, t_hi = min(rows - 1, 16 * ct + 15) / a.group;
+    const int qt = row / a.group, qg = row - qt * a.group;
+    const TileKeys tk = tile_keys(da, load_index(p.pos, p.pos_dt, b), quant_count(p, b), t_lo, t_hi);
+    if (tk.active == 1) return;
+    const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
+    const float* ml = da.part_ml + (unit * da.splits * 16 + col) * 2;
+    const float* po = da.part_o + (unit * da.splits * 16 + col) * D;
+    float m = -INFINITY;
+    for (int s = tid & 63; s < tk.active; s += 64) m = fmaxf(m, ml[s * 32]);
+    m = wave_max(m);
+    const float shift = m == -INFINITY ? 0.0f : m;
+    float total = 0.0f;
+    for (int s = tid & 63; s < tk.active; s += 64) total += ml[s * 32 + 1] * __builtin_amdgcn_exp2f(ml[s * 32] - shift);
+    total = wave_sum(total);
+    const int pieces = D / 4, groups = 256 / pieces;
+    const int piece = tid % pieces, grp = tid / pieces;
+    f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
+    if (grp < groups)
+#pragma unroll 4
+        for (int s = grp; s < tk.active; s += groups)
+            o += *reinterpret_cast<const f32x4_t*>(po + static_cast<int64_t>(s) * 16 * D + 4 * piece) * __builtin_amdgcn_exp2f(ml[s * 32] - shift);
+    sums[tid] = o;
+    __syncthreads();
+    if (tid < pieces) {
+        for (int i = 1; i < groups; i++) o += sums[tid + i * pieces];
+        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+        store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * tid, o * inv);
+    }
+}
+
+template <typename T, int FORMAT, int DP>
+int launch_dim(const DecodeArgs& d, hipStream_t stream, Err e) {
+    using G = DecodeGeo<T, FORMAT, DP>;
+    const void* fn = reinterpret_cast<const void*>(&quant_decode_kernel<T, FORMAT, DP>);
+    if (G::kBytes > 64 * 1024)
+        SANDY_HIP_TRY(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::kBytes), e, "quant_paged attention launch");
+    const QuantPages& p = d.a.p;
+    const int64_t wgs = static_cast<int64_t>(p.batch) * p.heads * d.col_tiles * d.splits;
+    DecodeArgs args = d;
+    void* params[] = {&args};
+    SANDY_HIP_TRY(hipLaunchKernel(fn, dim3(static_cast<unsigned>(wgs)), dim3(256), params, G::kBytes, stream), e,
+                  "quant_paged attention launch");
+    if (d.splits > 1) {
+        const int64_t rows = static_cast<int64_t>(p.batch) * d.a.hq * p.tokens;
+        hipLaunchKernelGGL((quant_decode_merge_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, d);
+        SANDY_HIP_TRY(hipGetLastError(), e, "quant_paged attention launch");
+    }
+    return ok(e);
+}
+
+template <typename T, int FORMAT>
+int launch_format(const DecodeArgs& d, hipStream_t stream, Err e) {
+    if (d.a.p.dim <= 64) return launch_dim<T, FORMAT, 64>(d, stream, e);
+    if (d.a.p.dim <= 128) return launch_dim<T, FORMAT, 128>(d, stream, e);
+    return launch_dim<T, FORMAT, 256>(d, stream, e);
+}
+
+// Splits of a column tile's keys: enough workgroups for the chip, none of less
+// than kMinPairs pairs at the longest context the call can have.
+int decode_splits(int64_t batch, int64_t heads, int64_t col_tiles, int64_t cap, int64_t window, int64_t tokens, int64_t dim) {
+    const int64_t units = batch * heads * col_tiles;
+    const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tokens + 16) : cap;
+    const int64_t most = std::max<int64_t>((keys + 31) / 32 / kMinPairs, 1);
+    const int64_t target = dim > 128 ? 512 : 1024;
+    return static_cast<int>(std::clamp<int64_t>(env_int("SANDY_QUANT_SPLITS", static_cast<int>(std::min<int64_t>((target + units - 1) / units, 256))), 1, std::min<int64_t>(most, 256)));
+}
+
+} // namespace
+
+bool quant_decode_takes(const QuantAttnArgs& a) {
+    const QuantPages& p = a.p;
+    const int64_t es = a.f32 ? 4 : 2;
+    if (p.dim % 16 != 0 || p.dim > 256 || p.log2_page < 4) return false;
+    auto aligned = [](const void* ptr, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(ptr) & (bytes - 1)) == 0; };
+    if (!aligned(p.pool[0], 16) || !aligned(p.pool[1], 16)) return false;
+    // q read and out written in pieces of 16 bytes (out bf16: 8)
+    const int64_t in[3] = {p.batch > 1 ? a.qs[0] : 0, a.hq > 1 ? a.qs[1] : 0, p.tokens > 1 ? a.qs[2] : 0};
+    const int64_t to[3] = {p.batch > 1 ? a.os[0] : 0, a.hq > 1 ? a.os[1] : 0, p.tokens > 1 ? a.os[2] : 0};
+    if (!aligned(a.q, 16) || ((in[0] | in[1] | in[2]) & (16 / es - 1)) || a.qs[3] != 1) return false;
+    if (!aligned(a.out, 4 * es) || ((to[0] | to[1] | to[2]) & 3) || a.os[3] != 1) return false;
+    const int64_t rows = static_cast<int64_t>(a.group) * p.tokens;
+    const int64_t col_tiles = (rows + 15) / 16;
+    const int64_t wgs = col_tiles * p.batch * p.heads *
+                        decode_splits(p.batch, p.heads, col_tiles, static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens, p.dim);
+    return rows < (1 << 30) && wgs <= UINT32_MAX / 256 && static_cast<int64_t>(p.batch) * a.hq * p.tokens <= UINT32_MAX / 256;
+}
+
+size_t quant_decode_workspace(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t page,
+                              int64_t max_blocks, int64_t window) {
+    if (dim % 16 != 0 || dim > 256 || page < 16 || batch == 0 || tokens == 0) return 0;
+    const int64_t cap = max_blocks * page;
+    const int64_t col_tiles = (hq / heads * tokens + 15) / 16;
+    const int64_t splits = decode_splits(batch, heads, col_tiles, cap, window, tokens, dim);
+    return splits == 1 ? 0 : static_cast<size_t>(batch * heads * col_tiles * splits * 16 * (dim + 2)) * sizeof(float);
+}
+
+int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace, hipStream_t stream, Err e) {
+    const QuantPages& p = a.p;
+    DecodeArgs d{};
+    d.a = a;
+    d.col_tiles = (a.group * p.tokens + 15) / 16;
+    d.splits = decode_splits(p.batch, p.heads, d.col_tiles, static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens, p.dim);
+    const int64_t slots = static_cast<int64_t>(p.batch) * p.heads * d.col_tiles * d.splits;
+    d.part_o = static_cast<float*>(workspace);
+    d.part_ml = d.part_o + slots * 16 * p.dim;
+    if (format == SANDY_QUANT_INT8)
+        return a.f32 ? launch_format<F32, SANDY_QUANT_INT8>(d, stream, e) : launch_format<BF16, SANDY_QUANT_INT8>(d, stream, e);
+    return a.f32 ? launch_format<F32, SANDY_QUANT_E4M3>(d, stream, e) : launch_format<BF16, SANDY_QUANT_E4M3>(d, stream, e);
+}
+
+} // namespace sandy_hip

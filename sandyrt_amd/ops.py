@@ -508,7 +508,7 @@ def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
     out = torch.empty_like(q) if out is None else out
     kc, vc, qa, ta = k_cache.struct(), v_cache.struct(), arg(q), arg(block_table)
     need = C.c_size_t(0)
-    _lib.dcall("sandy_hip_quant_paged_attention_workspace", qa, kc, ta, C.byref(need))
+    _lib.dcall("sandy_hip_quant_paged_attention_workspace", qa, kc, ta, int(window), C.byref(need))
     # the call's own: calls on other streams and captured graphs share nothing with it
     work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
     _quant_call("sandy_hip_quant_paged_attention", (q, out, block_table, position_offsets, counts),

@@ -11,6 +11,7 @@ from tests.helpers import from_f32, rng
 pytestmark = pytest.mark.gpu
 
 BF16, F32 = torch.bfloat16, torch.float32
+WEIGHT = 2.0 ** -15
 
 
 @pytest.fixture(scope="module")
@@ -234,9 +235,10 @@ def check(ops, q, kc, vc, table, pos, counts=None, window=0, scale=-1.0, what=""
     ops.check_device_errors()
     assert got is out
     cnt = counts if counts is not None else [q.shape[2]] * q.shape[0]
-    # bf16: weights as two bf16 numbers, 2^-9 of 2^-9 and the cut of the first
+    # bf16: weights may be two bf16 numbers, the first cut (what is left is below
+    # 2^-7 of the weight), the second rounded (2^-8 of that)
     want, slack = R.attention(f64(q), R.Cache.of(kc), R.Cache.of(vc), table, pos, cnt, window, scale,
-                              2.0 ** -17 if q.dtype == BF16 else 0.0)
+                              WEIGHT if q.dtype == BF16 else 0.0)
     R.assert_attention(got, want, slack, what)
     return got
 
@@ -420,7 +422,7 @@ def test_prompt_then_steps_in_a_graph(ops, fmt, dtype):
     out = ops.quant_paged_attention(q, kc, vc, gt, pos, counts=cnt)
     kr.append(f64(k), table, [0] * B, counts)
     vr.append(f64(v), table, [0] * B, counts)
-    weight = 2.0 ** -17 if dtype == BF16 else 0.0
+    weight = WEIGHT if dtype == BF16 else 0.0
     R.assert_attention(out, *R.attention(f64(q), kr, vr, table, [0] * B, counts, 0, -1.0, weight), "prompt")
     pos.copy_(cnt)
 
@@ -505,5 +507,5 @@ def test_offsets_past_32_bits(ops):
     for T in (1, 24):
         q = from_f32(r.standard_normal((1, 16, T, dim)).astype(np.float32), BF16)
         got = ops.quant_paged_attention(q, *c, cuda(table), cuda(np.array([n - T])))
-        R.assert_attention(got, *R.attention(f64(q), *refs, [[0, 1, 2, 3]], [n - T], [T], 0, -1.0, 2.0 ** -17))
+        R.assert_attention(got, *R.attention(f64(q), *refs, [[0, 1, 2, 3]], [n - T], [T], 0, -1.0, WEIGHT))
     ops.check_device_errors()
