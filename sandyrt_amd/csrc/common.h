@@ -119,6 +119,11 @@ void* device_workspace(int slot, size_t bytes, hipStream_t stream, Err e, int* s
 // afterwards by the kernels that use them.
 void* device_counters(int slot, size_t bytes, hipStream_t stream, Err e, int* status);
 
+// Zeroed arrival counters that no other work in flight uses, or null where there
+// are none left (the caller then takes a form that needs none): a region for each
+// stream, whose calls follow one another, and for a call under capture words of
+// its graph's own.  The kernels leave them zero.
+uint32_t* arrival_counters(size_t words, hipStream_t stream, Err e, int* status);
 
 // ---------------------------------------------------------------- device helpers
 __device__ __forceinline__ float bf16_to_f32(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }

@@ -74,7 +74,13 @@ struct DecodeArgs {
     int32_t splits;     // workgroups a column tile's keys may be split over
     float* part_o;      // [unit, split][16][D] sums relative to the maximum
     float* part_ml;     // [unit, split][16][2] maximum and sum of weights
+    uint32_t* arrived;  // [unit][counters_of(splits)] zero between calls, or null: the merge kernel joins the splits
 };
+
+// Splits are joined by the last workgroup to arrive, in groups of 16 and then
+// the groups: a unit's counters are one for the groups (or the only group) and,
+// where there are several, one for each.
+__host__ __device__ constexpr int counters_of(int splits) { return splits <= 16 ? 1 : 1 + (splits + 15) / 16; }
 
 // The keys of one column tile: pairs of 16-key tiles from `begin`, `per` of them a split.
 struct TileKeys {
@@ -100,6 +106,88 @@ __device__ __forceinline__ void store4(void* p, int64_t at, f32x4_t v) {
     else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
 }
 
+// Stores and loads that go through to memory: other XCDs' L2s see them once the
+// storing thread has waited for them.
+__device__ __forceinline__ void put_through(float* to, float x, float y) {
+    const uint64_t v = static_cast<uint64_t>(__float_as_uint(x)) | static_cast<uint64_t>(__float_as_uint(y)) << 32;
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void put_through(float* to, f32x4_t v) {
+    put_through(to, v[0], v[1]);
+    put_through(to + 2, v[2], v[3]);
+}
+__device__ __forceinline__ uint64_t get_through(const float* from) {
+    return __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
+__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
+
+// Counts this workgroup in once its stores are there; true for the last of n,
+// which leaves the counter zero.
+__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, int n) {
+    __shared__ bool last;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(n - 1);
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    return last;
+}
+
+// Slots first, first + stride, .. (n <= 16) of a column tile joined, in slot
+// order: into the output, or into slot `first`.  A thread per column and 4 dims.
+template <typename T>
+__device__ __forceinline__ void join_splits(const DecodeArgs& da, int64_t first, int stride, int n, int ct, int kh, int b, bool final_out) {
+    __shared__ float2 joined[16];
+    const QuantAttnArgs& a = da.a;
+    const int D = a.p.dim, rows = a.group * a.p.tokens;
+    const int per_col = D / 4;
+    const int cols = min(16, rows - 16 * ct);
+    for (int i = threadIdx.x; i < cols * per_col; i += 256) {
+        const int c = i / per_col, d = 4 * (i - c * per_col);
+        float m = -INFINITY, total = 0.0f;
+        f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s0 = 0; s0 < n; s0 += 8) {
+            uint64_t ml[8], x[8], y[8];
+#pragma unroll
+            for (int s = 0; s < 8; s++) {  // past the last: the last again, unused
+                const int64_t slot = first + static_cast<int64_t>(min(s0 + s, n - 1)) * stride;
+                ml[s] = get_through(da.part_ml + (slot * 16 + c) * 2);
+                x[s] = get_through(da.part_o + (slot * 16 + c) * D + d);
+                y[s] = get_through(da.part_o + (slot * 16 + c) * D + d + 2);
+            }
+            float top = m;
+#pragma unroll
+            for (int s = 0; s < 8; s++) top = fmaxf(top, low(ml[s]));
+            const float shift = top == -INFINITY ? 0.0f : top;
+            const float f = __builtin_amdgcn_exp2f(m - shift);
+            total *= f;
+            o *= f;
+            m = top;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                if (s0 + s >= n) continue;
+                const float w = __builtin_amdgcn_exp2f(low(ml[s]) - shift);
+                total += high(ml[s]) * w;
+                o += f32x4_t{low(x[s]), high(x[s]), low(y[s]), high(y[s])} * w;
+            }
+        }
+        const int row = 16 * ct + c, qt = row / a.group, qg = row - qt * a.group;
+        if (final_out) {
+            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+            store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, o * inv);
+        } else {
+            put_through(da.part_o + (first * 16 + c) * D + d, o);
+            if (d == 0) joined[c] = make_float2(m, total);
+        }
+    }
+    if (final_out) return;
+    __syncthreads();  // every thread has read the slot's own maximum and sum
+    if (threadIdx.x < cols) put_through(da.part_ml + (first * 16 + threadIdx.x) * 2, joined[threadIdx.x].x, joined[threadIdx.x].y);
+}
+
 template <typename T, int FORMAT, int DP>
 struct DecodeGeo {
     static constexpr int kChunks = DP / 64;  // 16-byte pieces a lane holds of a K (V) tile
@@ -107,7 +195,8 @@ struct DecodeGeo {
     static constexpr int kWaves = DP == 64 ? 3 : DP == 256 && std::is_same_v<T, F32> ? 1 : 2;  // a SIMD
     static constexpr int VP = DP + 16;       // bytes of a V row in LDS: column reads spread over the banks
     static constexpr int kV = 32 * VP;       // a wave's V rows
-    static constexpr int kMerge = 4 * (DP / 16) * 64 * 16;  // every wave's accumulators
+    static constexpr int kSet = DP == 256 ? 8 : DP / 16;  // accumulator tiles the waves exchange at a time
+    static constexpr int kMerge = 4 * kSet * 64 * 16;
     static constexpr int kBytes = std::max(4 * kV, kMerge) + 4 * 16 * 2 * 4;
 };
 
@@ -149,29 +238,16 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     const int all_last = t_hi < count ? quant_keys(a, pos, t_lo).last : -1;
 
     // B operands of Q^T: column, dims 64 j + 16 g + 8 s .. + 7 in step 2 j + s
-    u32x4_t qv[NQ][2 * NCH];
+    // (past D any of the row's: K is zero there)
+    u32x4_t raw[kF32 ? 2 : 1][2 * NCH], qv[NQ][2 * NCH];
     {
         const int64_t q0 = b * a.qs[0] + (kh * a.group + qg) * a.qs[1] + qt * a.qs[2];
 #pragma unroll
         for (int s = 0; s < 2 * NCH; s++) {
             const int d = 64 * (s >> 1) + 16 * g + 8 * (s & 1);
-            const int64_t from = q0 + (d < D ? d : 0);
-            if constexpr (kF32) {
-                float x[8];
-                Vec8<F32>::load(a.q, from, x);
+            const char* from = static_cast<const char*>(a.q) + (q0 + (d < D ? d : 0)) * (kF32 ? 4 : 2);
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    // an infinity leaves inf - inf for its later parts: NaN scores, as an
-                    // infinite score's weight has
-                    uint32_t part[3];
-                    split_pair<3>(d < D ? x[i] : 0.0f, d < D ? x[i + 1] : 0.0f, part);
-#pragma unroll
-                    for (int n = 0; n < 3; n++) qv[n][s][i / 2] = part[n];
-                }
-            } else {
-                const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + from);
-                qv[0][s] = d < D ? raw : u32x4_t{0, 0, 0, 0};
-            }
+            for (int i = 0; i < (kF32 ? 2 : 1); i++) raw[i][s] = *reinterpret_cast<const u32x4_t*>(from + 16 * i);
         }
     }
 
@@ -188,7 +264,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
         k_off[j] = d < D ? col * D + d : 0x7ffffff0;  // past every tile: zeros
         const int piece = lane + 64 * j, per_row = D / 16;
         const int r = piece / per_row;
-        v_to[j] = r < 16 ? r * G::VP + 16 * (piece - r * per_row) : -1;
+        v_to[j] = r < 16 ? r * G::VP + 16 * (piece - r * per_row) : DP;  // none: the padding of the first row
     }
     // ds_read_b64_tr_b8: lanes 2 n and 2 n + 1 of 16 address row n's 16 bytes, lane i
     // gets byte i of the 8 rows: keys 4 g + n of the first tile, then of the second
@@ -196,136 +272,158 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     const unsigned char* v_from = vrows + (trow < 4 ? 4 * g + trow : 16 + 4 * g + trow - 4) * G::VP + 8 * (lane & 1);
 
     const int last_pair = min((split + 1) * tk.per, tk.pairs);
-    // a wave takes every fourth pair; 32 of them (64 tiles) a round
-    for (int round0 = split * tk.per + wave; round0 < last_pair; round0 += 4 * 32) {
-        const int n_pairs = min(32, (last_pair - round0 + 3) / 4);
-        // lane i looks up tile i & 1 of the round's pair i / 2
-        int id = -1, rows_in = 0;
-        float kf = 0.0f, vf = 1.0f;
-        {
-            const int pair = round0 + 4 * (lane >> 1);
-            const int key0 = tk.begin + 32 * pair + 16 * (lane & 1);
-            if (pair < last_pair && key0 <= tk.last) {
-                id = quant_block(p, b, key0 >> p.log2_page);
-                rows_in = min(16, tk.last - key0 + 1);
-                if (id >= 0) {
-                    const int64_t block = static_cast<int64_t>(id) * p.heads + kh;
-                    const int kc = p.scales[0][block], vc = p.scales[1][block];
-                    // a NaN block: NaN scores for whoever sees it, V's own factor aside
-                    kf = quant_scale(vc == 255 ? 255 : kc) * a.scale_log2;
-                    vf = quant_scale(vc == 255 ? 127 : vc);
-                }
-            }
+    // a wave takes every fourth pair, 32 of them (64 tiles) a round: lane i holds
+    // tile i & 1 of pair i / 2, its bytes' offset, its rows (none: 0) and factors
+    int bytes_in = 0;
+    uint64_t offset = 0;
+    float kf = 0.0f, vf = 1.0f;
+    u32x4_t kr[RING][2][NCH], vr[RING][2][NCH];
+    auto load = [&](int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int tile = (2 * n + h) & 63;
+            // rows past the last key and tiles without a page: an empty range reads zeros
+            const int bytes = n < 32 ? __builtin_amdgcn_readlane(bytes_in, tile) : 0;
+            const uint64_t off = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(offset >> 32), tile)) << 32 |
+                                 static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(offset), tile));
+            const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(p.pool[0] + off, 0, bytes, kRsrcWord3);
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(p.pool[1] + off, 0, bytes, kRsrcWord3);
+#pragma unroll
+            for (int j = 0; j < NCH; j++) k[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off[j], 0, 0));
+#pragma unroll
+            for (int j = 0; j < NCH; j++) v[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * (lane + 64 * j), 0, 0));
         }
-        u32x4_t kr[RING][2][NCH], vr[RING][2][NCH];
-        auto load = [&](int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int tile = min(2 * n + h, 63);
-                const int blk = __builtin_amdgcn_readlane(id, tile);
-                // rows past the last key and tiles without a page: an empty range reads zeros
-                const int bytes = n < n_pairs && blk >= 0 ? __builtin_amdgcn_readlane(rows_in, tile) * D : 0;
-                const int key0 = tk.begin + 32 * (round0 + 4 * n) + 16 * h;
-                const int64_t off = (((static_cast<int64_t>(max(blk, 0)) * p.heads + kh) << p.log2_page) +
-                                     (key0 & ((1 << p.log2_page) - 1))) * D;
-                const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(p.pool[0] + off, 0, bytes, kRsrcWord3);
-                const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(p.pool[1] + off, 0, bytes, kRsrcWord3);
-#pragma unroll
-                for (int j = 0; j < NCH; j++) k[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rk, k_off[j], 0, 0));
-#pragma unroll
-                for (int j = 0; j < NCH; j++) v[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * (lane + 64 * j), 0, 0));
-            }
-        };
-        auto attend = [&](int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
-            f32x4_t sc[2];
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                sc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < NCH; j++)
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const bf16x8_t ka = payload_operand<FORMAT>(k[h][j][2 * s], k[h][j][2 * s + 1], 1.0f, 1.0f);
-#pragma unroll
-                        for (int c = NQ - 1; c >= 0; c--)
-                            sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][2 * j + s]), sc[h], 0, 0, 0);
-                    }
-            }
-#pragma unroll
-            for (int h = 0; h < 2; h++)
-#pragma unroll
-                for (int j = 0; j < NCH; j++)
-                    if (v_to[j] >= 0) *reinterpret_cast<u32x4_t*>(vrows + 16 * h * G::VP + v_to[j]) = v[h][j];
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            load(n + RING, k, v);
-            const float kf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n));
-            const float kf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n + 1));
-            const float vf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n));
-            const float vf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + 1));
-            const int id0 = __builtin_amdgcn_readlane(id, 2 * n), id1 = __builtin_amdgcn_readlane(id, 2 * n + 1);
-            const int k0 = tk.begin + 32 * (round0 + 4 * n);
-            sc[0] *= kf0;
-            sc[1] *= kf1;
-            if (k0 < all_first || k0 + 31 > all_last || (id0 | id1) < 0) {
-                // element i of tile h: key k0 + 16 h + 4 g + i
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int key = k0 + 4 * g + i;
-                    if (id0 < 0 || key < mine.first || key > mine.last) sc[0][i] = -INFINITY;
-                    if (id1 < 0 || key + 16 < mine.first || key + 16 > mine.last) sc[1][i] = -INFINITY;
-                }
-            }
-            float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
-                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
-            // a column's reference m moves only once its maximum has grown by 2^8:
-            // weights stay below that, at the same relative precision
-            if (__any(mx > m + 8.0f)) {
-                mx = max_xor32(max_xor16(mx));
-                const float m_new = fmaxf(m, mx);
-                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-                l *= alpha;
-#pragma unroll
-                for (int t = 0; t < NT; t++) acc[t] *= alpha;
-                m = m_new;
-            }
-            const float shift = m == -INFINITY ? 0.0f : m;
-            float w[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(sc[i >> 2][i & 3] - shift);
-            l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            if constexpr (FORMAT == SANDY_QUANT_INT8)
-#pragma unroll
-                for (int i = 0; i < 8; i++) w[i] *= i < 4 ? vf0 : vf1;
-            bf16x8_t pw[NP];
-            {
-                u32x4_t parts[NP];
-#pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    uint32_t part[NP];
-                    split_pair<NP>(w[i], w[i + 1], part);
-#pragma unroll
-                    for (int c = 0; c < NP; c++) parts[c][i / 2] = part[c];
-                }
-#pragma unroll
-                for (int c = 0; c < NP; c++) pw[c] = __builtin_bit_cast(bf16x8_t, parts[c]);
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                if (16 * t >= D) continue;
-                const i32x2_t raw = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * t)));
-                const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(raw[0]), static_cast<uint32_t>(raw[1]), vf0, vf1);
-#pragma unroll
-                for (int c = NP - 1; c >= 0; c--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw[c], acc[t], 0, 0, 0);
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        };
+    };
+    auto begin_round = [&](int round0) {
+        const int pair = round0 + 4 * (lane >> 1);
+        const int key0 = tk.begin + 32 * pair + 16 * (lane & 1);
+        const bool mine_in = pair < last_pair && key0 <= tk.last;
+        const int id = mine_in ? quant_block(p, b, key0 >> p.log2_page) : -1;
+        bytes_in = id < 0 ? 0 : min(16, tk.last - key0 + 1) * D;
+        const int64_t block = static_cast<int64_t>(max(id, 0)) * p.heads + kh;
+        offset = id < 0 ? 0 : static_cast<uint64_t>((block << p.log2_page) + (key0 & ((1 << p.log2_page) - 1))) * D;
+        const int kc = p.scales[0][block], vc = p.scales[1][block];
 #pragma unroll
         for (int i = 0; i < RING; i++) load(i, kr[i], vr[i]);
-        for (int n = 0; n < n_pairs; n += RING) {
+        // a NaN block: NaN scores for whoever sees it, V's own factor aside
+        kf = quant_scale(vc == 255 ? 255 : kc) * a.scale_log2;
+        vf = quant_scale(vc == 255 ? 127 : vc);
+    };
+    auto attend = [&](int round0, int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
+        f32x4_t sc[2];
 #pragma unroll
-            for (int i = 0; i < RING; i++)
-                if (n + i < n_pairs) attend(n + i, kr[i], vr[i]);
+        for (int h = 0; h < 2; h++) {
+            sc[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < NCH; j++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    const bf16x8_t ka = payload_operand<FORMAT>(k[h][j][2 * s], k[h][j][2 * s + 1], 1.0f, 1.0f);
+#pragma unroll
+                    for (int c = NQ - 1; c >= 0; c--)
+                        sc[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][2 * j + s]), sc[h], 0, 0, 0);
+                }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < NCH; j++) *reinterpret_cast<u32x4_t*>(vrows + 16 * h * G::VP + v_to[j]) = v[h][j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        load(n + RING, k, v);
+        const float kf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n));
+        const float kf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n + 1));
+        const float vf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n));
+        const float vf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + 1));
+        const bool none0 = __builtin_amdgcn_readlane(bytes_in, 2 * n) == 0;
+        const bool none1 = __builtin_amdgcn_readlane(bytes_in, 2 * n + 1) == 0;
+        const int k0 = tk.begin + 32 * (round0 + 4 * n);
+        sc[0] *= kf0;
+        sc[1] *= kf1;
+        if ((k0 < all_first) | (k0 + 31 > all_last) | none0 | none1) {
+            // element i of tile h: key k0 + 16 h + 4 g + i
+            const int end0 = none0 ? -1 : mine.last, end1 = none1 ? -1 : mine.last;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int key = k0 + 4 * g + i;
+                sc[0][i] = (key < mine.first) | (key > end0) ? -INFINITY : sc[0][i];
+                sc[1][i] = (key + 16 < mine.first) | (key + 16 > end1) ? -INFINITY : sc[1][i];
+            }
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        // a column's reference m moves only once its maximum has grown by 2^8:
+        // weights stay below that, at the same relative precision
+        if (__any(mx > m + 8.0f)) {
+            mx = max_xor32(max_xor16(mx));
+            const float m_new = fmaxf(m, mx);
+            const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int t = 0; t < NT; t++) acc[t] *= alpha;
+            m = m_new;
+        }
+        const float shift = m == -INFINITY ? 0.0f : m;
+        float w[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = __builtin_amdgcn_exp2f(sc[i >> 2][i & 3] - shift);
+        l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        if constexpr (FORMAT == SANDY_QUANT_INT8)
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] *= i < 4 ? vf0 : vf1;
+        bf16x8_t pw[NP];
+        {
+            u32x4_t parts[NP];
+#pragma unroll
+            for (int i = 0; i < 8; i += 2) {
+                uint32_t part[NP];
+                split_pair<NP>(w[i], w[i + 1], part);
+#pragma unroll
+                for (int c = 0; c < NP; c++) parts[c][i / 2] = part[c];
+            }
+#pragma unroll
+            for (int c = 0; c < NP; c++) pw[c] = __builtin_bit_cast(bf16x8_t, parts[c]);
+        }
+        // (dims past D: bytes of earlier tiles, in accumulators that nothing stores)
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const i32x2_t eight = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * t)));
+            const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), vf0, vf1);
+#pragma unroll
+            for (int c = NP - 1; c >= 0; c--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw[c], acc[t], 0, 0, 0);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    };
+    int round0 = split * tk.per + wave;
+    if (round0 < last_pair) {
+        begin_round(round0);
+#pragma unroll
+        for (int s = 0; s < 2 * NCH; s++) {
+            if constexpr (kF32) {
+                // an infinity leaves inf - inf for its later parts: NaN scores, as an
+                // infinite score's weight has
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    uint32_t part[3];
+                    split_pair<3>(__uint_as_float(raw[i >> 1][s][2 * (i & 1)]), __uint_as_float(raw[i >> 1][s][2 * (i & 1) + 1]), part);
+#pragma unroll
+                    for (int c = 0; c < 3; c++) qv[c][s][i] = part[c];
+                }
+            } else {
+                qv[0][s] = raw[0][s];
+            }
+        }
+        for (;;) {
+            // no branch around a load: the waits stay exact and later loads in flight
+            const int n_pairs = min(32, (last_pair - round0 + 3) / 4);
+            int n = 0;
+            for (; n + RING <= n_pairs; n += RING)
+#pragma unroll
+                for (int i = 0; i < RING; i++) attend(round0, n + i, kr[i], vr[i]);
+            if (n < n_pairs) attend(round0, n, kr[0], vr[0]);
+            round0 += 4 * 32;
+            if (round0 >= last_pair) break;
+            begin_round(round0);
         }
     }
 
@@ -345,29 +443,40 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     for (int w = 0; w < 4; w++) total += ml[(w * 16 + col) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 16 + col) * 2] - shift);
     const float f = __builtin_amdgcn_exp2f(m - shift);
     f32x4_t* red = reinterpret_cast<f32x4_t*>(lds);
-#pragma unroll
-    for (int t = 0; t < NT; t++) red[(wave * NT + t) * 64 + lane] = acc[t] * f;
-    __syncthreads();
     const bool final_out = tk.active == 1;
     const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
     const int64_t slot = unit * da.splits + split;
     const bool stored = 16 * ct + col < rows;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const int64_t o0 = b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2];
+    constexpr int SET = G::kSet;
 #pragma unroll
-    for (int t4 = 0; t4 < NT; t4 += 4) {
-        const int t = t4 + wave;
-        if (16 * t >= D) continue;
-        const f32x4_t o = (red[t * 64 + lane] + red[(NT + t) * 64 + lane]) + (red[(2 * NT + t) * 64 + lane] + red[(3 * NT + t) * 64 + lane]);
-        const int d = 16 * t + 4 * g;
-        if (!stored) continue;
-        if (final_out) store4<T>(a.out, o0 + d, o * inv);
-        else *reinterpret_cast<f32x4_t*>(da.part_o + (slot * 16 + col) * D + d) = o;
+    for (int s0 = 0; s0 < NT; s0 += SET) {
+        if (s0 > 0) __syncthreads();
+#pragma unroll
+        for (int t = 0; t < SET; t++) red[(wave * SET + t) * 64 + lane] = acc[s0 + t] * f;
+        __syncthreads();
+#pragma unroll
+        for (int t4 = 0; t4 < SET; t4 += 4) {
+            const int t = t4 + wave;
+            const int d = 16 * (s0 + t) + 4 * g;
+            if (d >= D || !stored) continue;
+            const f32x4_t o = (red[t * 64 + lane] + red[(SET + t) * 64 + lane]) +
+                              (red[(2 * SET + t) * 64 + lane] + red[(3 * SET + t) * 64 + lane]);
+            if (final_out) store4<T>(a.out, o0 + d, o * inv);
+            else put_through(da.part_o + (slot * 16 + col) * D + d, o);
+        }
     }
-    if (!final_out && tid < 16 && stored) {
-        da.part_ml[(slot * 16 + col) * 2] = mm;
-        da.part_ml[(slot * 16 + col) * 2 + 1] = total;
-    }
+    if (final_out) return;
+    if (tid < 16 && stored) put_through(da.part_ml + (slot * 16 + col) * 2, mm, total);
+    if (!da.arrived) return;
+    uint32_t* arrived = da.arrived + unit * counters_of(da.splits);
+    const int groups = (tk.active + 15) / 16, grp = split / 16;
+    const int in_group = min(16, tk.active - 16 * grp);
+    if (!last_to_arrive(arrived + (groups > 1 ? 1 + grp : 0), in_group)) return;
+    join_splits<T>(da, unit * da.splits + 16 * grp, 1, in_group, ct, kh, b, groups == 1);
+    if (groups == 1 || !last_to_arrive(arrived, groups)) return;
+    join_splits<T>(da, unit * da.splits, 16, groups, ct, kh, b, true);
 }
 
 // Joins the splits of one output row: a workgroup per row, every thread 4 dims
@@ -427,7 +536,7 @@ int launch_dim(const DecodeArgs& d, hipStream_t stream, Err e) {
     void* params[] = {&args};
     SANDY_HIP_TRY(hipLaunchKernel(fn, dim3(static_cast<unsigned>(wgs)), dim3(256), params, G::kBytes, stream), e,
                   "quant_paged attention launch");
-    if (d.splits > 1) {
+    if (d.splits > 1 && !d.arrived) {
         const int64_t rows = static_cast<int64_t>(p.batch) * d.a.hq * p.tokens;
         hipLaunchKernelGGL((quant_decode_merge_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, d);
         SANDY_HIP_TRY(hipGetLastError(), e, "quant_paged attention launch");
@@ -490,6 +599,12 @@ int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace,
     const int64_t slots = static_cast<int64_t>(p.batch) * p.heads * d.col_tiles * d.splits;
     d.part_o = static_cast<float*>(workspace);
     d.part_ml = d.part_o + slots * 16 * p.dim;
+    if (d.splits > 1 && env_int("SANDY_QUANT_MERGE_KERNEL", 0) == 0) {
+        const size_t words = static_cast<size_t>(slots / d.splits) * counters_of(d.splits);
+        int status = 0;
+        d.arrived = arrival_counters(words, stream, e, &status);
+        if (status) return status;
+    }
     if (format == SANDY_QUANT_INT8)
         return a.f32 ? launch_format<F32, SANDY_QUANT_INT8>(d, stream, e) : launch_format<BF16, SANDY_QUANT_INT8>(d, stream, e);
     return a.f32 ? launch_format<F32, SANDY_QUANT_E4M3>(d, stream, e) : launch_format<BF16, SANDY_QUANT_E4M3>(d, stream, e);

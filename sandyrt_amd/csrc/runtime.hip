@@ -22,9 +22,17 @@ struct Buffer {
     bool in_graph = false;  // its address was given to work under capture
 };
 
+constexpr int kStreamRegions = 64;           // streams with arrival counters of their own
+constexpr size_t kRegionWords = 4096;        // of each
+constexpr size_t kCaptureWords = 1u << 20;   // for calls under capture, never given twice
+
 struct DeviceState {
     uint32_t* error_word = nullptr;
     Buffer ws[kSlots], ctr[kSlots];
+    uint32_t* arrivals = nullptr;
+    hipStream_t streams[kStreamRegions];
+    int stream_count = 0;
+    size_t captured_words = 0;
 };
 
 std::mutex g_mu;
@@ -35,6 +43,9 @@ DeviceState g_dev[kMaxDevices];
 // allocate for it.  Each GPU holds its own copy; host code uses the address
 // hipGetSymbolAddress returns for the current device, never the name.
 static __device__ __align__(256) uint32_t error_words[64];
+
+// Arrival counters: zero when the module loads, like the error words.
+static __device__ __align__(256) uint32_t arrival_words[kStreamRegions * kRegionWords + kCaptureWords];
 
 int current_device(Err e, int* dev) {
     hipError_t st = hipGetDevice(dev);
@@ -124,6 +135,37 @@ void* device_counters(int slot, size_t bytes, hipStream_t stream, Err e, int* st
     }
     c.in_graph = c.in_graph || capturing(stream);
     return c.p;
+}
+
+uint32_t* arrival_counters(size_t words, hipStream_t stream, Err e, int* status) {
+    int dev = 0;
+    *status = current_device(e, &dev);
+    if (*status) return nullptr;
+    if (stream == hipStreamPerThread) return nullptr;  // one handle, a stream for each thread
+    const bool captured = capturing(stream);
+    std::lock_guard<std::mutex> lock(g_mu);
+    DeviceState& s = g_dev[dev];
+    if (!s.arrivals) {
+        void* p = nullptr;
+        hipError_t st = hipGetSymbolAddress(&p, HIP_SYMBOL(arrival_words));
+        if (st != hipSuccess) {
+            *status = fail(e, SANDY_ERR_HIP, "arrival counters: %s", hipGetErrorString(st));
+            return nullptr;
+        }
+        s.arrivals = static_cast<uint32_t*>(p);
+    }
+    if (captured) {
+        if (words > kCaptureWords - s.captured_words) return nullptr;
+        uint32_t* p = s.arrivals + kStreamRegions * kRegionWords + s.captured_words;
+        s.captured_words += words;
+        return p;
+    }
+    if (words > kRegionWords) return nullptr;
+    int i = 0;
+    while (i < s.stream_count && s.streams[i] != stream) i++;
+    if (i == kStreamRegions) return nullptr;
+    if (i == s.stream_count) s.streams[s.stream_count++] = stream;
+    return s.arrivals + i * kRegionWords;
 }
 
 } // namespace sandy_hip

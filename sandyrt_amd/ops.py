@@ -456,16 +456,31 @@ class QuantPagedCache:
 
 def _quant_call(name, tensors, caches, *args):
     """An entry point of the quantised cache, on its tensors' own device."""
-    tensors = [t for t in tensors if t is not None] + [t for c in caches if c is not None for t in (c.pool, c.scales)]
-    _require_gpu(*tensors)
-    device = tensors[0].device
-    if any(t.device != device for t in tensors):
-        raise SandyError(1, "quant_paged tensors must live on one GPU")
-    if device.index == torch.cuda.current_device():
-        call(name, *args)
+    at = caches[0].pool.get_device()
+    for c in caches:
+        if c is not None and (c.pool.get_device() != at or c.scales.get_device() != at):
+            raise SandyError(1, "quant_paged tensors must live on one device")
+    for t in tensors:
+        if t is not None and t.get_device() != at:
+            raise SandyError(1, "quant_paged tensors must live on one device")
+    if at < 0:
+        raise SandyError(1, "sandyrt_amd tensors must live on the GPU")
+    if at == torch.cuda.current_device():
+        call(name, *args, stream=torch._C._cuda_getCurrentRawStream(at))
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(at):
             call(name, *args)
+
+
+@functools.lru_cache(maxsize=1024)
+def _quant_workspace(batch, q_heads, tokens, dim, heads, rows, blocks, window):
+    """Workspace bytes of an attention call of these sizes."""
+    q, table = _lib.SandyTensor(rank=4), _lib.SandyTensor(rank=2)
+    q.dims[:4], table.dims[:2] = (batch, q_heads, tokens, dim), (batch, blocks)
+    need = C.c_size_t(0)
+    _lib.dcall("sandy_hip_quant_paged_attention_workspace", q,
+               _lib.SandyQuantCache(page_size=rows, prefix=heads, inner=dim), table, window, C.byref(need))
+    return need.value
 
 
 def quant_paged_append(k, v, k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_table, position_offsets,
@@ -506,14 +521,15 @@ def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
     a sequence sees keys up to position_offsets[b] + t (its own, which must have
     been appended).  Queries from counts[b] on give zero."""
     out = torch.empty_like(q) if out is None else out
-    kc, vc, qa, ta = k_cache.struct(), v_cache.struct(), arg(q), arg(block_table)
-    need = C.c_size_t(0)
-    _lib.dcall("sandy_hip_quant_paged_attention_workspace", qa, kc, ta, int(window), C.byref(need))
-    # the call's own: calls on other streams and captured graphs share nothing with it
-    work = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+    kc, vc, window = k_cache.struct(), v_cache.struct(), int(window)
+    need, work = 0, None
+    if q.dim() == 4 and block_table.dim() == 2:  # else the call says what is wrong
+        need = _quant_workspace(*q.shape, kc.prefix, kc.page_size, block_table.shape[1], window)
+    if need:  # the call's own: calls on other streams and captured graphs share nothing with it
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
     _quant_call("sandy_hip_quant_paged_attention", (q, out, block_table, position_offsets, counts),
-                (k_cache, v_cache), qa, kc, vc, ta, arg(position_offsets), arg(counts), int(window), float(scale),
-                arg(out), work.data_ptr() if work is not None else None, need.value)
+                (k_cache, v_cache), arg(q), kc, vc, arg(block_table), arg(position_offsets), arg(counts), window,
+                float(scale), arg(out), None if work is None else work.data_ptr(), need)
     return out
 
 

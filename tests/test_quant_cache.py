@@ -141,6 +141,9 @@ def test_python_refusals():
         ops.quant_paged_read(c, None, table, pos, 3)
     with pytest.raises(_lib.SandyError, match="must live on the GPU"):
         ops.quant_paged_attention(x, c, c, table, pos)
+    far = ops.QuantPagedCache(pool.to("meta"), scales.to("meta"))
+    with pytest.raises(_lib.SandyError, match="must live on"):
+        ops.quant_paged_read(far, None, table, pos, 3)
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
