@@ -37,4 +37,9 @@ size_t quant_decode_workspace(int64_t batch, int64_t hq, int64_t heads, int64_t 
                               int64_t max_blocks, int64_t window);
 int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace, hipStream_t stream, Err e);
 
+// Many queries a sequence (quant_prefill.hip), of the calls that quant_decode_takes; no workspace.
+bool quant_prefill_takes(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t max_blocks,
+                         bool f32);
+int launch_quant_prefill(const QuantAttnArgs& a, int32_t format, hipStream_t stream, Err e);
+
 } // namespace sandy_hip

@@ -95,6 +95,16 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
     }
 }
 
+// Whether a call of these sizes has rows enough for the prompt kernel.
+bool is_prompt(const SandyTensor* q, const SandyQuantCache* kc, const SandyTensor* table) {
+    return quant_prefill_takes(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner, table->dims[1], q->dtype == SANDY_F32);
+}
+
+size_t workspace_of(const SandyTensor* q, const SandyQuantCache* kc, const SandyTensor* table, int64_t window) {
+    if (is_prompt(q, kc, table)) return 0;
+    return quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner, kc->page_size, table->dims[1], window);
+}
+
 int check_quant_attention(const SandyTensor* q, const SandyQuantCache* kc, Err e) {
     if (!valid_rank(q) || !kc) return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires q and caches");
     if (!is_float(q->dtype)) return fail(e, SANDY_ERR_INVALID, "attention q unsupported dtype");
@@ -119,8 +129,7 @@ extern "C" int sandy_hip_quant_paged_attention_workspace(const SandyTensor* q, c
     if (status) return status;
     if (!valid_rank(table) || table->rank != 2 || !bytes)
         return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires a block table");
-    *bytes = quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner, kc->page_size,
-                                    table->dims[1], window);
+    *bytes = workspace_of(q, kc, table, window);
     return ok(e);
 }
 
@@ -154,8 +163,8 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     a.f32 = q->dtype == SANDY_F32;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (quant_decode_takes(a)) {
-        const size_t need = quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner,
-                                                   kc->page_size, table->dims[1], window);
+        if (is_prompt(q, kc, table)) return launch_quant_prefill(a, kc->format, s, e);
+        const size_t need = workspace_of(q, kc, table, window);
         if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
             return fail(e, SANDY_ERR_INVALID, "quant_paged attention needs a 16-byte aligned workspace of %zu bytes", need);
         return launch_quant_decode(a, kc->format, workspace, s, e);

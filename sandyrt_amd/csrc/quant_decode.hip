@@ -557,7 +557,7 @@ int decode_splits(int64_t batch, int64_t heads, int64_t col_tiles, int64_t cap, 
     const int64_t units = batch * heads * col_tiles;
     const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tokens + 16) : cap;
     const int64_t most = std::max<int64_t>((keys + 31) / 32 / kMinPairs, 1);
-    const int64_t target = dim > 128 ? 512 : 1024;
+    const int64_t target = dim > 128 ? 256 : 512;
     return static_cast<int>(std::clamp<int64_t>(env_int("SANDY_QUANT_SPLITS", static_cast<int>(std::min<int64_t>((target + units - 1) / units, 256))), 1, std::min<int64_t>(most, 256)));
 }
 

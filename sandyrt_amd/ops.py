@@ -473,9 +473,9 @@ def _quant_call(name, tensors, caches, *args):
 
 
 @functools.lru_cache(maxsize=1024)
-def _quant_workspace(batch, q_heads, tokens, dim, heads, rows, blocks, window):
+def _quant_workspace(batch, q_heads, tokens, dim, dtype, heads, rows, blocks, window):
     """Workspace bytes of an attention call of these sizes."""
-    q, table = _lib.SandyTensor(rank=4), _lib.SandyTensor(rank=2)
+    q, table = _lib.SandyTensor(rank=4, dtype=_lib._TORCH_TO_CODE[dtype]), _lib.SandyTensor(rank=2)
     q.dims[:4], table.dims[:2] = (batch, q_heads, tokens, dim), (batch, blocks)
     need = C.c_size_t(0)
     _lib.dcall("sandy_hip_quant_paged_attention_workspace", q,
@@ -524,7 +524,7 @@ def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
     kc, vc, window = k_cache.struct(), v_cache.struct(), int(window)
     need, work = 0, None
     if q.dim() == 4 and block_table.dim() == 2:  # else the call says what is wrong
-        need = _quant_workspace(*q.shape, kc.prefix, kc.page_size, block_table.shape[1], window)
+        need = _quant_workspace(*q.shape, q.dtype, kc.prefix, kc.page_size, block_table.shape[1], window)
     if need:  # the call's own: calls on other streams and captured graphs share nothing with it
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
     _quant_call("sandy_hip_quant_paged_attention", (q, out, block_table, position_offsets, counts),
