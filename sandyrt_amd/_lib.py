@@ -193,9 +193,10 @@ SIGNATURES = {
     "sandy_hip_layout_transform": [T, T, C.c_int32, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_attention_paged_view": [T, PV, PV, T, C.c_int64, C.c_double, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_paged_attention_noalloc": [T, P, P, T, T, C.c_int64, C.c_double, T, C.c_void_p, ERR, C.c_size_t],
-    "sandy_hip_quant_paged_append": [T, T, Q8, Q8, T, T, T, C.c_void_p, ERR, C.c_size_t],
-    "sandy_hip_quant_paged_read": [Q8, Q8, T, T, T, T, T, C.c_void_p, ERR, C.c_size_t],
-    "sandy_hip_quant_paged_attention": [T, Q8, Q8, T, T, T, C.c_int64, C.c_double, T, C.c_void_p, C.c_size_t,
+    # their structs go as packed bytes (pack, pack_quant), which a typed pointer does not take
+    "sandy_hip_quant_paged_append": [*[C.c_void_p] * 7, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_paged_read": [*[C.c_void_p] * 7, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_paged_attention": [*[C.c_void_p] * 6, C.c_int64, C.c_double, C.c_void_p, C.c_void_p, C.c_size_t,
                                         C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_topk": [T, C.c_int64, C.c_int64, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_gather": [T, T, T, C.c_int64, C.c_int64, T, T, T, T, C.c_void_p, ERR, C.c_size_t],
@@ -307,6 +308,10 @@ def pack(t: torch.Tensor) -> bytes:
     if rank > MAX_RANK:
         raise SandyError(1, f"tensor rank {rank} exceeds {MAX_RANK}")
     return _TENSOR_LAYOUT[rank].pack(t.data_ptr(), _TORCH_TO_CODE[t.dtype], rank, *t.shape, *t.stride(), 0)
+
+
+# SandyQuantCache: pool, scales, format, reserved, page_size, prefix, inner, num_pages
+pack_quant = struct.Struct("=QQiiqqqq").pack
 
 
 def arg(t: torch.Tensor | None):

@@ -47,24 +47,29 @@ struct QGeo {
     static constexpr int THREADS = 256 * DS;
     static constexpr int DT = DP / 32 / DS;  // 32-dim tiles of O^T a wave owns
     static constexpr int KW = 4 / RW;
-    static constexpr int CK = 32 * KW;       // keys of a chunk, 32 a wave
+    static constexpr int SUB = RW == 4 ? 2 : 1;  // 32-key blocks of a chunk a wave takes
+    static constexpr int CK = 32 * SUB * KW;     // keys of a chunk
     static constexpr int KP = 2 * DP + 16;   // bytes of a K row in LDS: reads down a column touch every bank once
     static constexpr int VP = 2 * DP + 64;   // of a V row: 4 rows x 64 bytes a transposing read
     static constexpr int kBuf = CK * (KP + VP);
     static constexpr int NB = 2 * kBuf <= 144 * 1024 ? 2 : 1;
     static constexpr int NPC = CK * DP / 16 / THREADS;  // 16-byte pieces of K (of V) a thread stages
-    static constexpr int kMerge = (KW - 1) * RW * DP * 32 * 4 + 4 * 32 * 8;
+    static constexpr int kMerge = KW == 1 ? 0 : (KW - 1) * RW * DP * 32 * 4 + 4 * 32 * 8;
     static constexpr int kBytes = std::max(NB * kBuf, kMerge);
 };
 
-template <int FORMAT>
-__device__ __forceinline__ void to_bf16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+// Four payloads times `scale`, a power of two, as bf16 (exact).
+template <int FORMAT, bool SCALED>
+__device__ __forceinline__ void to_bf16(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
     if constexpr (FORMAT == SANDY_QUANT_E4M3) {
-        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true));
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, SCALED ? scale : 1.0f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, SCALED ? scale : 1.0f, true));
     } else {
         float v[4];
         quant_values<FORMAT>(w, v);
+        if constexpr (SCALED)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[i] *= scale;
         lo = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
         hi = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u);
     }
@@ -83,6 +88,13 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[NS
     part[NS - 1] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
 }
 
+// Workgroup i's place in the list by falling length: every second round of the
+// 256 CUs backwards, so that the workgroups a CU gets add up to about the same.
+__device__ __forceinline__ int snake(int i, int n) {
+    const int round = i & ~255;
+    return (i & 256) ? round + min(256, n - round) - 1 - (i - round) : i;
+}
+
 template <typename T, int FORMAT, int DP, int RW>
 __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_prefill_kernel(PrefillQArgs pa) {
     using G = QGeo<T, FORMAT, DP, RW>;
@@ -97,10 +109,11 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
     const int rw = wave % RW, kw = (wave & 3) / RW, ds = wave >> 2;
     const int col = lane & 31, half = lane >> 5;
     const int D = p.dim;
-    // heads vary fastest (an XCD serves few), the longest row blocks start first
+    // heads vary fastest (an XCD serves few), the longest row blocks first
     const int heads = p.batch * p.heads;
-    const int bh = static_cast<int>(blockIdx.x) % heads;
-    const int rb = pa.row_blocks - 1 - static_cast<int>(blockIdx.x) / heads;
+    const int at = snake(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    const int bh = at % heads;
+    const int rb = pa.row_blocks - 1 - at / heads;
     const int b = bh / p.heads, kh = bh % p.heads;
     const int rows = a.group * p.tokens;
     const int64_t pos = load_index(p.pos, p.pos_dt, b);
@@ -160,12 +173,14 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
     const int page_mask = (1 << p.log2_page) - 1;
     u32x4_t kr[NPC], vr[NPC];
     bool there[NPC];
+    float vs[NPC];
     auto load = [&](int c0, int page0) {
 #pragma unroll
         for (int i = 0; i < NPC; i++) {
             const int key = min(c0 + prow + i * kRowStep, k_end - 1);
             const u32x4_t e = table[(key >> p.log2_page) - page0];
             const bool page = e[1] != kNoPage && in_dim;
+            vs[i] = __uint_as_float(e[3]);
             there[i] = page && c0 + prow + i * kRowStep < k_end;
             const uint64_t off = page ? (static_cast<uint64_t>(e[1]) << 32 | e[0]) + static_cast<uint32_t>(key & page_mask) * static_cast<uint32_t>(D) + 16 * ppc : 0;
             kr[i] = *reinterpret_cast<const u32x4_t*>(p.pool[0] + off);
@@ -185,7 +200,7 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 uint32_t lo, hi;
-                to_bf16<FORMAT>(k[w], lo, hi);
+                to_bf16<FORMAT, false>(k[w], 1.0f, lo, hi);
                 o[w >> 1][2 * (w & 1)] = lo, o[w >> 1][2 * (w & 1) + 1] = hi;
             }
             *reinterpret_cast<u32x4_t*>(kt + r * KP + 32 * ppc) = o[0];
@@ -193,7 +208,7 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
 #pragma unroll
             for (int w = 0; w < 4; w++) {
                 uint32_t lo, hi;
-                to_bf16<FORMAT>(v[w], lo, hi);
+                to_bf16<FORMAT, true>(v[w], vs[i], lo, hi);
                 o[w >> 1][2 * (w & 1)] = lo, o[w >> 1][2 * (w & 1) + 1] = hi;
             }
             *reinterpret_cast<u32x4_t*>(vt + r * VP + 32 * ppc) = o[0];
@@ -226,7 +241,7 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
                 // a NaN block: NaN scores for the rows that see it, V's own factor aside
                 const float f = kc == 255 || vc == 255 ? quant_scale(255) : fmaxf(quant_scale(kc) * a.scale_log2, 0x1p-126f);
                 e = u32x4_t{static_cast<uint32_t>(off), static_cast<uint32_t>(off >> 32), __float_as_uint(f),
-                            static_cast<uint32_t>(vc == 255 ? 0 : vc - 127)};
+                            __float_as_uint(quant_scale(vc == 255 ? 127 : vc))};
             }
             table[i] = e;
         }
@@ -237,48 +252,57 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
             store(buf);
             __syncthreads();
             if (c0 + CK < seg_end) load(c0 + CK, page0);
-            const int k0 = c0 + 32 * kw;
-            if (k0 > any_last || k0 + 31 < any_first) continue;  // wave-uniform
-            const unsigned char* kt = lds + buf * G::kBuf + (32 * kw + col) * KP + 16 * half;
-            const unsigned char* vt = lds + buf * G::kBuf + CK * KP + 32 * kw * VP;
-            // the two 16-key tiles' factors (the second may lie past the last key)
-            const u32x4_t e0 = table[(k0 >> p.log2_page) - page0];
-            const u32x4_t e1 = table[(min(k0 + 16, k_end - 1) >> p.log2_page) - page0];
-            f32x16_t sc;
+            const int k0 = c0 + 32 * G::SUB * kw;
+            if (k0 > any_last || k0 + 32 * G::SUB - 1 < any_first) continue;  // wave-uniform
+            const unsigned char* kt = lds + buf * G::kBuf + (32 * G::SUB * kw + col) * KP + 16 * half;
+            const unsigned char* vt = lds + buf * G::kBuf + CK * KP + 32 * G::SUB * kw * VP;
+            f32x16_t sc[G::SUB];
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i] = 0.0f;
+            for (int u = 0; u < G::SUB; u++) {
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const bf16x8_t ka = *reinterpret_cast<const bf16x8_t*>(kt + 32 * s);
+                for (int i = 0; i < 16; i++) sc[u][i] = 0.0f;
 #pragma unroll
-                for (int c = NQ - 1; c >= 0; c--)
-                    sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][s]), sc, 0, 0, 0);
+                for (int s = 0; s < KS; s++) {
+                    const bf16x8_t ka = *reinterpret_cast<const bf16x8_t*>(kt + 32 * u * KP + 32 * s);
+#pragma unroll
+                    for (int c = NQ - 1; c >= 0; c--)
+                        sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][s]), sc[u], 0, 0, 0);
+                }
             }
-            const bool none0 = __builtin_amdgcn_readfirstlane(e0[1]) == kNoPage;
-            const bool none1 = __builtin_amdgcn_readfirstlane(e1[1]) == kNoPage;
-            float f0 = __uint_as_float(e0[2]), f1 = __uint_as_float(e1[2]);
-            const bool nan0 = __any(f0 != f0), nan1 = __any(f1 != f1);  // uniform
-            // element i: key k0 + 8 (i / 4) + 4 half + i % 4, in the first tile for i < 8
-            if ((k0 + 31 > all_last) | (k0 < all_first) | none0 | none1 | nan0 | nan1) {
+            // factors of the 16-key tiles (the last ones may lie past the last key)
+            float f[2 * G::SUB];
+            bool plain = k0 + 32 * G::SUB - 1 <= all_last && k0 >= all_first;
+#pragma unroll
+            for (int h = 0; h < 2 * G::SUB; h++) {
+                const u32x4_t e = table[(min(k0 + 16 * h, k_end - 1) >> p.log2_page) - page0];
+                f[h] = __uint_as_float(e[2]);  // 0 without a page, or NaN
+                plain = plain && __any(f[h] > 0.0f);
+            }
+            // element i of block u: key k0 + 32 u + 8 (i / 4) + 4 half + i % 4
+            if (!plain) {
                 int key0 = k0 + 4 * half;
                 asm volatile("" : "+v"(key0));  // keeps the compares out of whole tiles
-                const int end0 = none0 ? -1 : mine.last, end1 = none1 ? -1 : mine.last;
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int key = key0 + 8 * (i >> 2) + (i & 3);
-                    const float s = (i < 8 ? nan0 : nan1) ? quant_scale(255) : sc[i];
-                    sc[i] = (key < mine.first) | (key > (i < 8 ? end0 : end1)) ? -INFINITY : s;
+                for (int h = 0; h < 2 * G::SUB; h++) {
+                    const bool none = f[h] == 0.0f, nan = f[h] != f[h];
+                    const int end = none ? -1 : mine.last;
+                    if (none | nan) f[h] = 1.0f;  // the factor goes into the scores themselves
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const int key = key0 + 16 * h + 8 * (i >> 2) + (i & 3);
+                        const float s = nan ? quant_scale(255) : sc[h >> 1][8 * (h & 1) + i];
+                        sc[h >> 1][8 * (h & 1) + i] = (key < mine.first) | (key > end) ? -INFINITY : s;
+                    }
                 }
-                if (nan0) f0 = 1.0f;
-                if (nan1) f1 = 1.0f;
             }
-            float mx0 = sc[0], mx1 = sc[8];
+            float mx = -INFINITY;
 #pragma unroll
-            for (int i = 1; i < 8; i++) {
-                mx0 = fmaxf(mx0, sc[i]);
-                mx1 = fmaxf(mx1, sc[8 + i]);
+            for (int h = 0; h < 2 * G::SUB; h++) {
+                float top = sc[h >> 1][8 * (h & 1)];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top = fmaxf(top, sc[h >> 1][8 * (h & 1) + i]);
+                mx = fmaxf(mx, top * f[h]);
             }
-            float mx = fmaxf(mx0 * f0, mx1 * f1);
             // a row's reference m moves only once its maximum has grown by 2^8
             if (__any(mx > m + 8.0f)) {
                 mx = max_xor32(mx);
@@ -290,41 +314,43 @@ __global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_p
                 m = m_new;
             }
             const float shift = m == -INFINITY ? 0.0f : m;
-            const int v0 = static_cast<int>(e0[3]), v1 = static_cast<int>(e1[3]);
-            const float add0 = static_cast<float>(v0) - shift, add1 = static_cast<float>(v1) - shift;
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[i] = __builtin_amdgcn_exp2f(fmaf(sc[i], i < 8 ? f0 : f1, i < 8 ? add0 : add1));
-            {
-                const float a0 = ((sc[0] + sc[1]) + (sc[2] + sc[3])) + ((sc[4] + sc[5]) + (sc[6] + sc[7]));
-                const float a1 = ((sc[8] + sc[9]) + (sc[10] + sc[11])) + ((sc[12] + sc[13]) + (sc[14] + sc[15]));
-                l += ldexpf(a0, -v0) + ldexpf(a1, -v1);
-            }
-            // contraction slot 8 half + j of step s2: key 16 s2 + 4 half + j (j < 4) or + 8 + j - 4
+            for (int u = 0; u < G::SUB; u++) {
 #pragma unroll
-            for (int s2 = 0; s2 < 2; s2++) {
-                u32x4_t pw[NP];
+                for (int i = 0; i < 16; i++) sc[u][i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], f[2 * u + (i >> 3)], -shift));
+                {
+                    float rs[8];
 #pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    uint32_t part[NP];
-                    split_pair<NP>(sc[8 * s2 + j], sc[8 * s2 + j + 1], part);
-#pragma unroll
-                    for (int c = 0; c < NP; c++) pw[c][j / 2] = part[c];
+                    for (int i = 0; i < 8; i++) rs[i] = sc[u][2 * i] + sc[u][2 * i + 1];
+                    l += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
                 }
-                // ds_read_b64_tr_b16: in each 16-lane group, lane i gets element i % 4 of
-                // the 8-byte pieces addressed by lanes 4 n + i / 4 (n = 0..3)
-                const int i16 = lane & 15;
-                const unsigned char* src = vt + (16 * s2 + 4 * half + (i16 >> 2)) * VP + 2 * (16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
+                // contraction slot 8 half + j of step s2: key 16 s2 + 4 half + j (j < 4) or + 8 + j - 4
 #pragma unroll
-                for (int t = 0; t < DT; t++) {
-                    const unsigned char* s0 = src + 64 * (DT * ds + t);
-                    const short4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (short4_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)s0));
-                    const short4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (short4_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(s0 + 8 * VP)));
-                    const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                for (int s2 = 0; s2 < 2; s2++) {
+                    u32x4_t pw[NP];
 #pragma unroll
-                    for (int c = NP - 1; c >= 0; c--)
-                        acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8_t, pw[c]), acc[t], 0, 0, 0);
+                    for (int j = 0; j < 8; j += 2) {
+                        uint32_t part[NP];
+                        split_pair<NP>(sc[u][8 * s2 + j], sc[u][8 * s2 + j + 1], part);
+#pragma unroll
+                        for (int c = 0; c < NP; c++) pw[c][j / 2] = part[c];
+                    }
+                    // ds_read_b64_tr_b16: in each 16-lane group, lane i gets element i % 4 of
+                    // the 8-byte pieces addressed by lanes 4 n + i / 4 (n = 0..3)
+                    const int i16 = lane & 15;
+                    const unsigned char* src = vt + (32 * u + 16 * s2 + 4 * half + (i16 >> 2)) * VP + 2 * (16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
+#pragma unroll
+                    for (int t = 0; t < DT; t++) {
+                        const unsigned char* s0 = src + 64 * (DT * ds + t);
+                        const short4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (short4_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)s0));
+                        const short4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (short4_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(s0 + 8 * VP)));
+                        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+                        for (int c = NP - 1; c >= 0; c--)
+                            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8_t, pw[c]), acc[t], 0, 0, 0);
+                    }
                 }
             }
         }
@@ -408,6 +434,7 @@ int launch_dim(const QuantAttnArgs& a, hipStream_t stream, Err e) {
     const int64_t rows = static_cast<int64_t>(a.group) * a.p.tokens;
     const int64_t wgs = (rows + 63) / 64 * a.p.batch * a.p.heads;
     const int rw = env_int("SANDY_QUANT_RW", wgs >= 224 ? 2 : 1);
+    if (rw == 4) return launch_rows<T, FORMAT, DP, 4>(a, stream, e);
     if (rw == 2) return launch_rows<T, FORMAT, DP, 2>(a, stream, e);
     return launch_rows<T, FORMAT, DP, 1>(a, stream, e);
 }

@@ -441,31 +441,32 @@ class QuantPagedCache:
         return QuantPagedCache(torch.zeros(shape, dtype=torch.uint8, device=device).view(_QUANT_FORMATS[format][0]),
                                torch.zeros(num_pages, heads, dtype=torch.uint8, device=device))
 
-    def struct(self):
+    def pack(self) -> bytes:
+        """The bytes of the SandyQuantCache describing the cache."""
         pool, scales = self.pool, self.scales
-        if pool.dtype not in _QUANT_CODES:
+        format = _QUANT_CODES.get(pool.dtype)
+        if format is None:
             raise SandyError(1, "quant_paged cache format must be int8 or e4m3")
         if pool.dim() != 4 or not pool.is_contiguous():
             raise SandyError(1, "quant_paged pool must be a contiguous [pages, heads, page_size, dim] tensor")
-        if scales.dtype != torch.uint8 or scales.shape != pool.shape[:2] or not scales.is_contiguous():
-            raise SandyError(1, "quant_paged scales must be a contiguous [pages, heads] uint8 tensor")
         pages, heads, rows, dim = pool.shape
-        return _lib.SandyQuantCache(pool.data_ptr(), scales.data_ptr(), _QUANT_CODES[pool.dtype], 0, rows, heads, dim,
-                                    pages)
+        if scales.dtype != torch.uint8 or scales.shape != (pages, heads) or not scales.is_contiguous():
+            raise SandyError(1, "quant_paged scales must be a contiguous [pages, heads] uint8 tensor")
+        return _lib.pack_quant(pool.data_ptr(), scales.data_ptr(), format, 0, rows, heads, dim, pages)
 
 
-def _quant_call(name, tensors, caches, *args):
-    """An entry point of the quantised cache, on its tensors' own device."""
-    at = caches[0].pool.get_device()
-    for c in caches:
-        if c is not None and (c.pool.get_device() != at or c.scales.get_device() != at):
-            raise SandyError(1, "quant_paged tensors must live on one device")
+def _packed(x):
+    return None if x is None else x.pack() if isinstance(x, QuantPagedCache) else pack(x)
+
+
+def _quant_call(name, at, tensors, *args):
+    """An entry point of the quantised cache, on the device `at` of its tensors."""
     for t in tensors:
         if t is not None and t.get_device() != at:
             raise SandyError(1, "quant_paged tensors must live on one device")
     if at < 0:
         raise SandyError(1, "sandyrt_amd tensors must live on the GPU")
-    if at == torch.cuda.current_device():
+    if at == torch._C._cuda_getDevice():
         call(name, *args, stream=torch._C._cuda_getCurrentRawStream(at))
     else:
         with torch.cuda.device(at):
@@ -493,9 +494,12 @@ def quant_paged_append(k, v, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
     grows.  A write at a page's first row starts its block anew.  `counts` [B]:
     the rows each sequence has of the T, the others are padding.  Sequences of
     one call must not write to the same page."""
-    _quant_call("sandy_hip_quant_paged_append", (k, v, block_table, position_offsets, counts), (k_cache, v_cache),
-                arg(k), arg(v), k_cache.struct(), None if v_cache is None else v_cache.struct(), arg(block_table),
-                arg(position_offsets), arg(counts))
+    kc, vc = _packed(k_cache), _packed(v_cache)
+    tensors = [k, v, block_table, position_offsets, counts, k_cache.scales]
+    if v_cache is not None:
+        tensors += (v_cache.pool, v_cache.scales)
+    _quant_call("sandy_hip_quant_paged_append", k_cache.pool.get_device(), tensors, _packed(k), _packed(v), kc, vc,
+                pack(block_table), pack(position_offsets), _packed(counts))
 
 
 def quant_paged_read(k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_table, position_offsets, tokens: int,
@@ -505,13 +509,16 @@ def quant_paged_read(k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_t
     def output(cache, out):
         if cache is None or out is not None:
             return out
-        return torch.empty(block_table.shape[0], cache.pool.shape[1], tokens, cache.pool.shape[3], dtype=dtype,
-                           device=cache.pool.device)
+        pool = cache.pool
+        return torch.empty((block_table.shape[0], pool.shape[1], tokens, pool.shape[3]), dtype=dtype, device=pool.device)
 
+    kc, vc = _packed(k_cache), _packed(v_cache)
     k_out, v_out = output(k_cache, k_out), output(v_cache, v_out)
-    _quant_call("sandy_hip_quant_paged_read", (k_out, v_out, block_table, position_offsets, counts),
-                (k_cache, v_cache), k_cache.struct(), None if v_cache is None else v_cache.struct(), arg(block_table),
-                arg(position_offsets), arg(counts), arg(k_out), arg(v_out))
+    tensors = [k_out, v_out, block_table, position_offsets, counts, k_cache.scales]
+    if v_cache is not None:
+        tensors += (v_cache.pool, v_cache.scales)
+    _quant_call("sandy_hip_quant_paged_read", k_cache.pool.get_device(), tensors, kc, vc, pack(block_table),
+                pack(position_offsets), _packed(counts), _packed(k_out), _packed(v_out))
     return k_out, v_out
 
 
@@ -521,15 +528,16 @@ def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
     a sequence sees keys up to position_offsets[b] + t (its own, which must have
     been appended).  Queries from counts[b] on give zero."""
     out = torch.empty_like(q) if out is None else out
-    kc, vc, window = k_cache.struct(), v_cache.struct(), int(window)
+    kc, vc, pool, window = k_cache.pack(), v_cache.pack(), k_cache.pool, int(window)
     need, work = 0, None
     if q.dim() == 4 and block_table.dim() == 2:  # else the call says what is wrong
-        need = _quant_workspace(*q.shape, q.dtype, kc.prefix, kc.page_size, block_table.shape[1], window)
+        need = _quant_workspace(*q.shape, q.dtype, pool.shape[1], pool.shape[2], block_table.shape[1], window)
     if need:  # the call's own: calls on other streams and captured graphs share nothing with it
         work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _quant_call("sandy_hip_quant_paged_attention", (q, out, block_table, position_offsets, counts),
-                (k_cache, v_cache), arg(q), kc, vc, arg(block_table), arg(position_offsets), arg(counts), window,
-                float(scale), arg(out), None if work is None else work.data_ptr(), need)
+    tensors = (q, out, block_table, position_offsets, counts, k_cache.scales, v_cache.pool, v_cache.scales)
+    _quant_call("sandy_hip_quant_paged_attention", pool.get_device(), tensors, pack(q), kc, vc, pack(block_table),
+                pack(position_offsets), _packed(counts), window, float(scale), pack(out),
+                None if work is None else work.data_ptr(), need)
     return out
 
 

@@ -366,6 +366,29 @@ def test_not_finite_reaches_its_readers_only(ops, fmt, dtype, T, dim):
     assert not want.any() and torch.isnan(got[0, 1, T - 1]).all() and not torch.isnan(got[0, 1, :T - 1]).any()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("T,dim", [(1, 64), (70, 64), (33, 128), (3, 36)])
+def test_blocks_of_far_scales(ops, fmt, dtype, T, dim):
+    """Blocks of zeros (the smallest scale) and of very small and large numbers
+    beside ordinary ones: their weights count in the sum all the same."""
+    r = rng(33)
+    n = 150
+    table, pages = make_table(r, [n], 16)
+    kc, vc = (empty(ops, pages, 2, 16, dim, fmt, i) for i in (1, 2))
+    k, v = (r.standard_normal((1, 2, n, dim)) for _ in range(2))
+    v[:, :, 16:32] = 0
+    v[:, 0, 64:80] *= 1e-36
+    v[:, 1, 80:96] *= 1e30
+    k[:, :, 96:112] = 0
+    k[:, :, 112:128] *= 1e-37
+    k, v = (from_f32(x.astype(np.float32), dtype) for x in (k, v))
+    ops.quant_paged_append(k, v, kc, vc, cuda(table), cuda(np.zeros(1, np.int64)))
+    assert (vc.scales[int(table[0, 1])] == 1).all() and (kc.scales[int(table[0, 6])] == 1).all()
+    q = from_f32(r.standard_normal((1, 8, T, dim)).astype(np.float32), dtype)
+    check(ops, q, kc, vc, table, [n - T])
+
+
 def test_attention_records(ops):
     from sandyrt_amd._lib import SandyError
     r = rng(41)

@@ -125,13 +125,13 @@ def test_python_refusals():
     with pytest.raises(_lib.SandyError, match="int8 or e4m3"):
         ops.QuantPagedCache.empty(4, 2, 16, 64, "int4", device="cpu")
     with pytest.raises(_lib.SandyError, match="int8 or e4m3"):
-        ops.QuantPagedCache(pool.float(), scales).struct()
+        ops.QuantPagedCache(pool.float(), scales).pack()
     with pytest.raises(_lib.SandyError, match="contiguous"):
-        ops.QuantPagedCache(pool.transpose(1, 2), scales).struct()
+        ops.QuantPagedCache(pool.transpose(1, 2), scales).pack()
     with pytest.raises(_lib.SandyError, match="scales must be"):
-        ops.QuantPagedCache(pool, scales[:3]).struct()
+        ops.QuantPagedCache(pool, scales[:3]).pack()
     with pytest.raises(_lib.SandyError, match="scales must be"):
-        ops.QuantPagedCache(pool, scales.int()).struct()
+        ops.QuantPagedCache(pool, scales.int()).pack()
     c, d = (ops.QuantPagedCache.empty(4, 2, 16, 64, f, device="cpu") for f in ("int8", "e4m3"))
     assert c.pool.dtype == torch.int8 and d.pool.dtype == torch.float8_e4m3fn and not d.pool.float().any()
     x, table, pos = torch.zeros(1, 2, 1, 64), torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)
