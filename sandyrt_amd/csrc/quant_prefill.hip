@@ -2,429 +2,348 @@
 // chunks) over the 8-bit paged cache on v_mfma_f32_32x32x16_bf16.
 //
 // The rows of a kv head are its (query, head of the group) pairs, query major,
-// so a workgroup's rows are a few neighbouring queries of the whole group.
-// S^T = K Q^T (a lane holds the scores of one row), O^T += V^T P^T with P^T as it
-// leaves the softmax.  Payloads become bf16 (exactly) once a workgroup, on their
-// way into LDS; scales never touch them: with K's factor f (scale log2(e) times
-// the block's) and V's scale 2^e, a weight enters as 2^(s f - m + e), which costs
-// the multiply-add that the exponent takes anyway, and the row sum takes the
-// block's partial sum times 2^-e.  bf16 queries' weights enter as two bf16
-// numbers (2^-15), f32 queries and weights as three (exact).
-// A table in LDS holds the blocks' byte offsets and factors, read from the block
-// table and scales once (a segment of kTable pages at a time): a chunk's loads
-// depend on LDS alone.
-// Four waves a workgroup: RW of them own 32 rows each, KW = 4 / RW share the keys
-// of a chunk and are merged at the end; at D 256 twice as many, each with half of
-// the head dims of O.
-#include "quant_attention.h"
+// so a workgroup's 32 CT rows are a few neighbouring queries of the whole group.
+// Its four waves take the key pairs of tiles in turn, each by itself (no barrier
+// in the loop), and are merged at the end.  As in quant_decode.hip payloads go to
+// the matrix unit as they are: S^T = K Q^T straight from 16-byte loads, O^T += V^T
+// P^T with V through the wave's own LDS rows and ds_read_b64_tr_b8; K's scale
+// multiplies the scores in the multiply-add of their exponents, V's the weights
+// (int8) or the conversion (e4m3).  Converted keys serve CT tiles of rows.  bf16
+// queries' weights enter as two bf16 numbers (2^-15), f32 queries and weights as
+// three (exact).
+#include "quant_mfma.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace sandy_hip {
 namespace {
 
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
-typedef short short4_t __attribute__((ext_vector_type(4)));
-typedef float f32x16_t __attribute__((ext_vector_type(16)));
-typedef float f32x4_t __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
-
-constexpr int kTable = 512;              // pages of a segment
-constexpr uint32_t kNoPage = 0xffffffffu;  // upper half of the offset of a page that is not there
-
-struct PrefillQArgs {
+struct PromptArgs {
     QuantAttnArgs a;
     int32_t row_blocks;
-    int32_t table;  // entries of the LDS table: pages of a segment
 };
 
-template <typename T, int FORMAT, int DP, int RW>
-struct QGeo {
+template <typename T, int FORMAT, int DP, int CT>
+struct PromptGeo {
     static constexpr bool kF32 = std::is_same_v<T, F32>;
-    static constexpr int DS = DP == 256 ? 2 : 1;
-    static constexpr int THREADS = 256 * DS;
-    static constexpr int DT = DP / 32 / DS;  // 32-dim tiles of O^T a wave owns
-    static constexpr int KW = 4 / RW;
-    static constexpr int SUB = RW == 4 ? 2 : 1;  // 32-key blocks of a chunk a wave takes
-    static constexpr int CK = 32 * SUB * KW;     // keys of a chunk
-    static constexpr int KP = 2 * DP + 16;   // bytes of a K row in LDS: reads down a column touch every bank once
-    static constexpr int VP = 2 * DP + 64;   // of a V row: 4 rows x 64 bytes a transposing read
-    static constexpr int kBuf = CK * (KP + VP);
-    static constexpr int NB = 2 * kBuf <= 144 * 1024 ? 2 : 1;
-    static constexpr int NPC = CK * DP / 16 / THREADS;  // 16-byte pieces of K (of V) a thread stages
-    static constexpr int kMerge = KW == 1 ? 0 : (KW - 1) * RW * DP * 32 * 4 + 4 * 32 * 8;
-    static constexpr int kBytes = std::max(NB * kBuf, kMerge);
+    static constexpr int KP = DP / 32;  // 16-byte pieces of K a lane holds of a pair of tiles
+    static constexpr int VP = DP + 16;  // bytes of a V row in LDS
+    static constexpr int NV = DP / 64;  // 16-byte pieces of V a lane holds of a tile
+    static constexpr int DT = DP / 32;  // 32-dim tiles of O^T
+    static constexpr int kV = 32 * VP;
+    static constexpr int kMerge = 4 * CT * 16 * 64 * 4;  // one 32-dim tile of every wave
+    static constexpr int kBytes = std::max(4 * kV, kMerge) + 4 * CT * 32 * 8;
+    static constexpr int kWaves = DP == 64 ? (CT == 2 || kF32 ? 2 : 3) : DP == 128 && CT == 1 ? 2 : 1;  // a SIMD
 };
 
-// Four payloads times `scale`, a power of two, as bf16 (exact).
-template <int FORMAT, bool SCALED>
-__device__ __forceinline__ void to_bf16(uint32_t w, float scale, uint32_t& lo, uint32_t& hi) {
-    if constexpr (FORMAT == SANDY_QUANT_E4M3) {
-        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, SCALED ? scale : 1.0f, false));
-        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, SCALED ? scale : 1.0f, true));
-    } else {
-        float v[4];
-        quant_values<FORMAT>(w, v);
-        if constexpr (SCALED)
-#pragma unroll
-            for (int i = 0; i < 4; i++) v[i] *= scale;
-        lo = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x07060302u);
-        hi = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x07060302u);
-    }
-}
-
-// x and y as NS bf16 parts each, packed in pairs: the first ones cut, the last rounded
-template <int NS>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[NS]) {
-#pragma unroll
-    for (int n = 0; n < NS - 1; n++) {
-        const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
-        part[n] = __builtin_amdgcn_perm(yb, xb, 0x07060302u);
-        x -= __uint_as_float(xb & 0xffff0000u);
-        y -= __uint_as_float(yb & 0xffff0000u);
-    }
-    part[NS - 1] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
-}
-
-// Workgroup i's place in the list by falling length: every second round of the
-// 256 CUs backwards, so that the workgroups a CU gets add up to about the same.
-__device__ __forceinline__ int snake(int i, int n) {
-    const int round = i & ~255;
-    return (i & 256) ? round + min(256, n - round) - 1 - (i - round) : i;
-}
-
-template <typename T, int FORMAT, int DP, int RW>
-__global__ __launch_bounds__((QGeo<T, FORMAT, DP, RW>::THREADS), 2) void quant_prefill_kernel(PrefillQArgs pa) {
-    using G = QGeo<T, FORMAT, DP, RW>;
+template <typename T, int FORMAT, int DP, int CT>
+__global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP, CT>::kWaves)) void quant_prompt_kernel(PromptArgs pa) {
+    using G = PromptGeo<T, FORMAT, DP, CT>;
     constexpr bool kF32 = G::kF32;
-    constexpr int KW = G::KW, CK = G::CK, KP = G::KP, VP = G::VP, NPC = G::NPC, DT = G::DT, NB = G::NB;
-    constexpr int NQ = kF32 ? 3 : 1, NP = kF32 ? 3 : 2, KS = DP / 16;  // MFMA steps over the head dim
+    constexpr int NQ = kF32 ? 3 : 1, NP = kF32 ? 3 : 2, KS = DP / 16, DT = G::DT;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const QuantAttnArgs& a = pa.a;
     const QuantPages& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int rw = wave % RW, kw = (wave & 3) / RW, ds = wave >> 2;
     const int col = lane & 31, half = lane >> 5;
     const int D = p.dim;
-    // heads vary fastest (an XCD serves few), the longest row blocks first
+    // heads vary fastest (an XCD serves few), the longest row blocks start first
     const int heads = p.batch * p.heads;
-    const int at = snake(static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
-    const int bh = at % heads;
-    const int rb = pa.row_blocks - 1 - at / heads;
+    const int bh = static_cast<int>(blockIdx.x) % heads;
+    const int rb = pa.row_blocks - 1 - static_cast<int>(blockIdx.x) / heads;
     const int b = bh / p.heads, kh = bh % p.heads;
     const int rows = a.group * p.tokens;
     const int64_t pos = load_index(p.pos, p.pos_dt, b);
     const int count = pos < 0 ? 0 : quant_count(p, b);
     if (pos < 0 && tid == 0) atomicOr(p.errw, static_cast<uint32_t>(SANDY_DEVERR_ATTN_POS));
-    const int r0 = rb * 32 * RW;
-    // the workgroup's keys: those of its first query that is none of the padding to its last
-    int k_begin = 0, k_end = 0;
-    {
-        const int t0 = r0 / a.group, t1 = min(min(rows - 1, r0 + 32 * RW - 1) / a.group, count - 1);
-        if (t0 <= t1) {
-            k_begin = quant_keys(a, pos, t0).first & ~15;
-            k_end = quant_keys(a, pos, t1).last + 1;
-        }
-    }
-    // this lane's row (past the end: the last one, not stored)
-    const int row = r0 + 32 * rw + col;
-    const int rc = min(row, rows - 1);
-    const int qt = rc / a.group, qg = rc - qt * a.group;
-    KeyRange mine = quant_keys(a, pos, qt);
-    if (qt >= count) mine.last = -1;
-    // keys that every row of the wave sees, and keys that some row sees
-    const int t_lo = min(rows - 1, r0 + 32 * rw) / a.group, t_hi = min(rows - 1, r0 + 32 * rw + 31) / a.group;
-    const int any_first = quant_keys(a, pos, t_lo).first;
-    const int any_last = t_lo < count ? quant_keys(a, pos, min(t_hi, count - 1)).last : -1;
+    // the rows' queries, those of the padding aside
+    const int r0 = rb * 32 * CT;
+    const int t_lo = r0 / a.group, t_hi = min(rows - 1, r0 + 32 * CT - 1) / a.group;
+    const int t_end = min(t_hi, count - 1);
+    const int begin = quant_keys(a, pos, t_lo).first & ~15;
+    const int last = t_lo <= t_end ? quant_keys(a, pos, t_end).last : -1;
+    const int pairs = last >= begin ? (last - begin + 32) >> 5 : 0;
+    // keys that every row sees
     const int all_first = quant_keys(a, pos, t_hi).first;
     const int all_last = t_hi < count ? quant_keys(a, pos, t_lo).last : -1;
 
-    // B operands of Q^T: row, dims 16 s + 8 half .. + 7 in step s (past D zeros: so are K's)
-    u32x4_t qv[NQ][KS];
-    {
-        const int64_t q0 = b * a.qs[0] + (kh * a.group + qg) * a.qs[1] + qt * a.qs[2] + 8 * half;
+    // this lane's rows (past the end: the last one, not stored) and their keys
+    int row[CT], qt[CT], qg[CT];
+    KeyRange mine[CT];
+    // B operands of Q^T: row, dims 32 (s / 2) + 16 half + 8 (s & 1) .. + 7 in step s, zeros past D
+    u32x4_t qv[CT][NQ][KS];
+#pragma unroll
+    for (int c = 0; c < CT; c++) {
+        row[c] = r0 + 32 * c + col;
+        const int rc = min(row[c], rows - 1);
+        qt[c] = rc / a.group, qg[c] = rc - qt[c] * a.group;
+        mine[c] = quant_keys(a, pos, qt[c]);
+        if (qt[c] >= count) mine[c].last = -1;
+        const int64_t q0 = b * a.qs[0] + (kh * a.group + qg[c]) * a.qs[1] + qt[c] * a.qs[2];
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            const int64_t from = q0 + (16 * s < D ? 16 * s : 0);
+            const int d = 32 * (s >> 1) + 16 * half + 8 * (s & 1);
             if constexpr (kF32) {
                 float x[8];
-                Vec8<F32>::load(a.q, from, x);
+                Vec8<F32>::load(a.q, q0 + (d < D ? d : 0), x);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     uint32_t part[3];
-                    split_pair<3>(x[2 * i], x[2 * i + 1], part);
+                    split_pair<3>(d < D ? x[2 * i] : 0.0f, d < D ? x[2 * i + 1] : 0.0f, part);
 #pragma unroll
-                    for (int c = 0; c < 3; c++) qv[c][s][i] = part[c];
+                    for (int n = 0; n < 3; n++) qv[c][n][s][i] = part[n];
                 }
             } else {
-                qv[0][s] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + from);
+                qv[c][0][s] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + q0 + (d < D ? d : 0));
+                if (d >= D) qv[c][0][s] = u32x4_t{0, 0, 0, 0};
             }
         }
     }
 
-    u32x4_t* table = reinterpret_cast<u32x4_t*>(lds + G::kBytes);
-    // thread piece i: chunk row prow + i * kRowStep, dims 16 ppc .. + 15
-    constexpr int kRowStep = G::THREADS / (DP / 16);
-    const int prow = tid / (DP / 16), ppc = tid % (DP / 16);
-    const bool in_dim = 16 * ppc < D;
-    const int page_mask = (1 << p.log2_page) - 1;
-    u32x4_t kr[NPC], vr[NPC];
-    bool there[NPC];
-    float vs[NPC];
-    auto load = [&](int c0, int page0) {
+    f32x16_t acc[CT][DT];
+    float m[CT], l[CT];
 #pragma unroll
-        for (int i = 0; i < NPC; i++) {
-            const int key = min(c0 + prow + i * kRowStep, k_end - 1);
-            const u32x4_t e = table[(key >> p.log2_page) - page0];
-            const bool page = e[1] != kNoPage && in_dim;
-            vs[i] = __uint_as_float(e[3]);
-            there[i] = page && c0 + prow + i * kRowStep < k_end;
-            const uint64_t off = page ? (static_cast<uint64_t>(e[1]) << 32 | e[0]) + static_cast<uint32_t>(key & page_mask) * static_cast<uint32_t>(D) + 16 * ppc : 0;
-            kr[i] = *reinterpret_cast<const u32x4_t*>(p.pool[0] + off);
-            vr[i] = *reinterpret_cast<const u32x4_t*>(p.pool[1] + off);
-        }
-    };
-    auto store = [&](int buf) {
-        unsigned char* kt = lds + buf * G::kBuf;
-        unsigned char* vt = kt + CK * KP;
+    for (int c = 0; c < CT; c++) {
+        m[c] = -INFINITY;
+        l[c] = 0.0f;
 #pragma unroll
-        for (int i = 0; i < NPC; i++) {
-            const int r = prow + i * kRowStep;
-            u32x4_t k = kr[i], v = vr[i];
-            // rows past the last key and missing pages: zeros (their weights are 0)
-            if (!there[i]) k = v = u32x4_t{0, 0, 0, 0};
-            u32x4_t o[2];
+        for (int t = 0; t < DT; t++)
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
-                uint32_t lo, hi;
-                to_bf16<FORMAT, false>(k[w], 1.0f, lo, hi);
-                o[w >> 1][2 * (w & 1)] = lo, o[w >> 1][2 * (w & 1) + 1] = hi;
-            }
-            *reinterpret_cast<u32x4_t*>(kt + r * KP + 32 * ppc) = o[0];
-            *reinterpret_cast<u32x4_t*>(kt + r * KP + 32 * ppc + 16) = o[1];
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                uint32_t lo, hi;
-                to_bf16<FORMAT, true>(v[w], vs[i], lo, hi);
-                o[w >> 1][2 * (w & 1)] = lo, o[w >> 1][2 * (w & 1) + 1] = hi;
-            }
-            *reinterpret_cast<u32x4_t*>(vt + r * VP + 32 * ppc) = o[0];
-            *reinterpret_cast<u32x4_t*>(vt + r * VP + 32 * ppc + 16) = o[1];
-        }
-    };
+            for (int i = 0; i < 16; i++) acc[c][t][i] = 0.0f;
+    }
 
-    f32x16_t acc[DT];
+    unsigned char* vrows = lds + wave * G::kV;
+    int k_off[G::KP], v_to[G::NV];
 #pragma unroll
-    for (int t = 0; t < DT; t++)
+    for (int j = 0; j < G::KP; j++) k_off[j] = (lane & 15) * D + (32 * j + 16 * half < D ? 32 * j + 16 * half : 0);
 #pragma unroll
-        for (int i = 0; i < 16; i++) acc[t][i] = 0.0f;
-    float m = -INFINITY, l = 0.0f;
-    int buf = 0;
+    for (int j = 0; j < G::NV; j++) {
+        const int piece = lane + 64 * j, per_row = D / 16;
+        const int r = piece / per_row;
+        v_to[j] = r < 16 ? r * G::VP + 16 * (piece - r * per_row) : DP;  // none: the padding of the first row
+    }
+    // ds_read_b64_tr_b8: lanes 2 n and 2 n + 1 of 16 address row n's 16 bytes, lane i
+    // gets byte i of the 8 rows: keys 4 half + n and 8 + 4 half + n - 4 of a tile
+    const int trow = (lane & 15) >> 1;
+    const unsigned char* v_from = vrows + (trow < 4 ? 4 * half + trow : 8 + 4 * half + trow - 4) * G::VP + 16 * ((lane >> 4) & 1) + 8 * (lane & 1);
 
-    // segments of whole pages that the table holds (k_end at the last)
-    for (int seg = k_begin; seg < k_end;) {
-        const int page0 = seg >> p.log2_page;
-        const int64_t seg_last = (static_cast<int64_t>(page0) + pa.table) << p.log2_page;
-        // chunks start at k_begin + a multiple of CK: a segment ends where one does
-        const int seg_end = seg_last >= k_end ? k_end : k_begin + (static_cast<int>(seg_last) - k_begin) / CK * CK;
-        __syncthreads();  // the segment before has been read
-        for (int i = tid; i < pa.table && page0 + i <= (seg_end - 1) >> p.log2_page; i += G::THREADS) {
-            const int id = quant_block(p, b, page0 + i);
-            u32x4_t e{0, kNoPage, 0, 0};
-            if (id >= 0) {
-                const int64_t block = static_cast<int64_t>(id) * p.heads + kh;
-                const uint64_t off = static_cast<uint64_t>(block << p.log2_page) * D;
-                const int kc = p.scales[0][block], vc = p.scales[1][block];
-                // a NaN block: NaN scores for the rows that see it, V's own factor aside
-                const float f = kc == 255 || vc == 255 ? quant_scale(255) : fmaxf(quant_scale(kc) * a.scale_log2, 0x1p-126f);
-                e = u32x4_t{static_cast<uint32_t>(off), static_cast<uint32_t>(off >> 32), __float_as_uint(f),
-                            __float_as_uint(quant_scale(vc == 255 ? 127 : vc))};
-            }
-            table[i] = e;
+    // a wave takes every fourth pair, 32 of them (64 tiles) a round: lane i holds
+    // tile i & 1 of pair i / 2, its bytes' offset, its rows (none: 0) and factors
+    int bytes_in = 0;
+    uint64_t offset = 0;
+    float kf = 0.0f, vf = 1.0f;
+    u32x4_t kr[G::KP], vr[2][G::NV];
+    auto load = [&](int n) {
+        uint64_t off[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int tile = (2 * n + h) & 63;
+            // rows past the last key and tiles without a page: an empty range reads zeros
+            const int bytes = n < 32 ? __builtin_amdgcn_readlane(bytes_in, tile) : 0;
+            off[h] = static_cast<uint64_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(offset >> 32), tile)) << 32 |
+                     static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<uint32_t>(offset), tile));
+            const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(p.pool[1] + off[h], 0, bytes, kRsrcWord3);
+#pragma unroll
+            for (int j = 0; j < G::NV; j++) vr[h][j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(rv, 16 * (lane + 64 * j), 0, 0));
         }
-        __syncthreads();
-        load(seg, page0);
-        for (int c0 = seg; c0 < seg_end; c0 += CK, buf ^= NB - 1) {
-            if (NB == 1 && c0 > seg) __syncthreads();  // the chunk before has been read
-            store(buf);
-            __syncthreads();
-            if (c0 + CK < seg_end) load(c0 + CK, page0);
-            const int k0 = c0 + 32 * G::SUB * kw;
-            if (k0 > any_last || k0 + 32 * G::SUB - 1 < any_first) continue;  // wave-uniform
-            const unsigned char* kt = lds + buf * G::kBuf + (32 * G::SUB * kw + col) * KP + 16 * half;
-            const unsigned char* vt = lds + buf * G::kBuf + CK * KP + 32 * G::SUB * kw * VP;
-            f32x16_t sc[G::SUB];
+        // K: a lane's key is in the first or the second tile (one without a page: page 0's
+        // bytes, masked)
+        const uint8_t* kp = p.pool[0] + ((lane & 16) ? off[1] : off[0]);
 #pragma unroll
-            for (int u = 0; u < G::SUB; u++) {
+        for (int j = 0; j < G::KP; j++) kr[j] = *reinterpret_cast<const u32x4_t*>(kp + k_off[j]);
+    };
+    auto begin_round = [&](int round0) {
+        const int pair = round0 + 4 * (lane >> 1);
+        const int key0 = begin + 32 * pair + 16 * (lane & 1);
+        const int id = pair < pairs && key0 <= last ? quant_block(p, b, key0 >> p.log2_page) : -1;
+        bytes_in = id < 0 ? 0 : min(16, last - key0 + 1) * D;
+        const int64_t block = static_cast<int64_t>(max(id, 0)) * p.heads + kh;
+        offset = id < 0 ? 0 : static_cast<uint64_t>((block << p.log2_page) + (key0 & ((1 << p.log2_page) - 1))) * D;
+        const int kc = p.scales[0][block], vc = p.scales[1][block];
+        load(0);
+        // a NaN block: NaN scores for whoever sees it, V's own factor aside
+        kf = vc == 255 || kc == 255 ? quant_scale(255) : fmaxf(quant_scale(kc) * a.scale_log2, 0x1p-126f);
+        vf = quant_scale(vc == 255 ? 127 : vc);
+    };
+    auto attend = [&](int round0, int n) {
+        f32x16_t sc[CT];
 #pragma unroll
-                for (int i = 0; i < 16; i++) sc[u][i] = 0.0f;
+        for (int c = 0; c < CT; c++)
 #pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const bf16x8_t ka = *reinterpret_cast<const bf16x8_t*>(kt + 32 * u * KP + 32 * s);
+            for (int i = 0; i < 16; i++) sc[c][i] = 0.0f;
 #pragma unroll
-                    for (int c = NQ - 1; c >= 0; c--)
-                        sc[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][s]), sc[u], 0, 0, 0);
-                }
-            }
-            // factors of the 16-key tiles (the last ones may lie past the last key)
-            float f[2 * G::SUB];
-            bool plain = k0 + 32 * G::SUB - 1 <= all_last && k0 >= all_first;
+        for (int s = 0; s < KS; s++) {
+            const bf16x8_t ka = payload_operand<FORMAT>(kr[s >> 1][2 * (s & 1)], kr[s >> 1][2 * (s & 1) + 1], 1.0f, 1.0f);
 #pragma unroll
-            for (int h = 0; h < 2 * G::SUB; h++) {
-                const u32x4_t e = table[(min(k0 + 16 * h, k_end - 1) >> p.log2_page) - page0];
-                f[h] = __uint_as_float(e[2]);  // 0 without a page, or NaN
-                plain = plain && __any(f[h] > 0.0f);
-            }
-            // element i of block u: key k0 + 32 u + 8 (i / 4) + 4 half + i % 4
-            if (!plain) {
-                int key0 = k0 + 4 * half;
-                asm volatile("" : "+v"(key0));  // keeps the compares out of whole tiles
+            for (int c = 0; c < CT; c++)
 #pragma unroll
-                for (int h = 0; h < 2 * G::SUB; h++) {
-                    const bool none = f[h] == 0.0f, nan = f[h] != f[h];
-                    const int end = none ? -1 : mine.last;
-                    if (none | nan) f[h] = 1.0f;  // the factor goes into the scores themselves
+                for (int i = NQ - 1; i >= 0; i--)
+                    sc[c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[c][i][s]), sc[c], 0, 0, 0);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int j = 0; j < G::NV; j++) *reinterpret_cast<u32x4_t*>(vrows + 16 * h * G::VP + v_to[j]) = vr[h][j];
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        load(n + 1);
+        float f[2], v[2];
+        bool none[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            f[h] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n + h));
+            v[h] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + h));
+            none[h] = __builtin_amdgcn_readlane(bytes_in, 2 * n + h) == 0;
+        }
+        const int k0 = begin + 32 * (round0 + 4 * n);
+        // element i: key k0 + 8 (i / 4) + 4 half + i % 4, in the first tile for i < 8
+        if ((k0 < all_first) | (k0 + 31 > all_last) | none[0] | none[1] | (f[0] != f[0]) | (f[1] != f[1])) {
+            int key0 = k0 + 4 * half;
+            asm volatile("" : "+v"(key0));  // keeps the compares out of whole tiles
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const bool nan = f[h] != f[h];
+                if (nan) f[h] = 1.0f;  // into the scores themselves
+#pragma unroll
+                for (int c = 0; c < CT; c++) {
+                    const int end = none[h] ? -1 : mine[c].last;
 #pragma unroll
                     for (int i = 0; i < 8; i++) {
                         const int key = key0 + 16 * h + 8 * (i >> 2) + (i & 3);
-                        const float s = nan ? quant_scale(255) : sc[h >> 1][8 * (h & 1) + i];
-                        sc[h >> 1][8 * (h & 1) + i] = (key < mine.first) | (key > end) ? -INFINITY : s;
-                    }
-                }
-            }
-            float mx = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 2 * G::SUB; h++) {
-                float top = sc[h >> 1][8 * (h & 1)];
-#pragma unroll
-                for (int i = 1; i < 8; i++) top = fmaxf(top, sc[h >> 1][8 * (h & 1) + i]);
-                mx = fmaxf(mx, top * f[h]);
-            }
-            // a row's reference m moves only once its maximum has grown by 2^8
-            if (__any(mx > m + 8.0f)) {
-                mx = max_xor32(mx);
-                const float m_new = fmaxf(m, mx);
-                const float alpha = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - m_new);
-                l *= alpha;
-#pragma unroll
-                for (int t = 0; t < DT; t++) acc[t] *= alpha;
-                m = m_new;
-            }
-            const float shift = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-            for (int u = 0; u < G::SUB; u++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) sc[u][i] = __builtin_amdgcn_exp2f(fmaf(sc[u][i], f[2 * u + (i >> 3)], -shift));
-                {
-                    float rs[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++) rs[i] = sc[u][2 * i] + sc[u][2 * i + 1];
-                    l += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
-                }
-                // contraction slot 8 half + j of step s2: key 16 s2 + 4 half + j (j < 4) or + 8 + j - 4
-#pragma unroll
-                for (int s2 = 0; s2 < 2; s2++) {
-                    u32x4_t pw[NP];
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        uint32_t part[NP];
-                        split_pair<NP>(sc[u][8 * s2 + j], sc[u][8 * s2 + j + 1], part);
-#pragma unroll
-                        for (int c = 0; c < NP; c++) pw[c][j / 2] = part[c];
-                    }
-                    // ds_read_b64_tr_b16: in each 16-lane group, lane i gets element i % 4 of
-                    // the 8-byte pieces addressed by lanes 4 n + i / 4 (n = 0..3)
-                    const int i16 = lane & 15;
-                    const unsigned char* src = vt + (32 * u + 16 * s2 + 4 * half + (i16 >> 2)) * VP + 2 * (16 * ((lane >> 4) & 1) + 4 * (i16 & 3));
-#pragma unroll
-                    for (int t = 0; t < DT; t++) {
-                        const unsigned char* s0 = src + 64 * (DT * ds + t);
-                        const short4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (short4_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)s0));
-                        const short4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (short4_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(s0 + 8 * VP)));
-                        const bf16x8_t va = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-                        for (int c = NP - 1; c >= 0; c--)
-                            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8_t, pw[c]), acc[t], 0, 0, 0);
+                        const float s = nan ? quant_scale(255) : sc[c][8 * h + i];
+                        sc[c][8 * h + i] = (key < mine[c].first) | (key > end) ? -INFINITY : s;
                     }
                 }
             }
         }
-        seg = seg_end;
+        bf16x8_t pw[CT][2][NP];
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            float top[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                top[h] = sc[c][8 * h];
+#pragma unroll
+                for (int i = 1; i < 8; i++) top[h] = fmaxf(top[h], sc[c][8 * h + i]);
+            }
+            float mx = fmaxf(top[0] * f[0], top[1] * f[1]);
+            // a row's reference m moves only once its maximum has grown by 2^8
+            if (__any(mx > m[c] + 8.0f)) {
+                mx = max_xor32(mx);
+                const float m_new = fmaxf(m[c], mx);
+                const float alpha = m[c] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m[c] - m_new);
+                l[c] *= alpha;
+#pragma unroll
+                for (int t = 0; t < DT; t++) acc[c][t] *= alpha;
+                m[c] = m_new;
+            }
+            const float shift = m[c] == -INFINITY ? 0.0f : m[c];
+            float w[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = __builtin_amdgcn_exp2f(fmaf(sc[c][i], f[i >> 3], -shift));
+            float rs[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) rs[i] = w[2 * i] + w[2 * i + 1];
+            l[c] += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
+            if constexpr (FORMAT == SANDY_QUANT_INT8)
+#pragma unroll
+                for (int i = 0; i < 16; i++) w[i] *= v[i >> 3];
+            // contraction slot 8 half + j of step h: this lane's element 8 h + j
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                u32x4_t parts[NP];
+#pragma unroll
+                for (int j = 0; j < 8; j += 2) {
+                    uint32_t part[NP];
+                    split_pair<NP>(w[8 * h + j], w[8 * h + j + 1], part);
+#pragma unroll
+                    for (int n2 = 0; n2 < NP; n2++) parts[n2][j / 2] = part[n2];
+                }
+#pragma unroll
+                for (int n2 = 0; n2 < NP; n2++) pw[c][h][n2] = __builtin_bit_cast(bf16x8_t, parts[n2]);
+            }
+        }
+        // (dims past D: bytes of earlier tiles, in accumulators that nothing stores)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int t = 0; t < DT; t++) {
+                const i32x2_t eight = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                    (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * h * G::VP + 32 * t)));
+                const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), v[h], v[h]);
+#pragma unroll
+                for (int c = 0; c < CT; c++)
+#pragma unroll
+                    for (int i = NP - 1; i >= 0; i--) acc[c][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pw[c][h][i], acc[c][t], 0, 0, 0);
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    };
+    for (int round0 = wave; round0 < pairs; round0 += 4 * 32) {
+        begin_round(round0);
+        const int n_pairs = min(32, (pairs - round0 + 3) / 4);
+        for (int n = 0; n < n_pairs; n++) attend(round0, n);
     }
 
-    // the two halves of a row's sum; then the key shares of the KW waves
-    l = sum_xor32(l);
-    if constexpr (KW > 1) {
-        __syncthreads();
-        float* red = reinterpret_cast<float*>(lds);
-        float2* ml = reinterpret_cast<float2*>(lds + (KW - 1) * RW * DP * 32 * 4);  // [wave of the first half][32]
-        if (half == 0 && ds == 0) ml[(wave & 3) * 32 + col] = make_float2(m, l);
-        __syncthreads();
-        float mm = -INFINITY;
+    // the four waves' maxima and sums, then their accumulators, 32 dims at a time
+    float2* ml = reinterpret_cast<float2*>(lds + std::max(4 * G::kV, G::kMerge));  // [wave][CT][32]
+    float f[CT], inv[CT];
 #pragma unroll
-        for (int w = 0; w < KW; w++) mm = fmaxf(mm, ml[(w * RW + rw) * 32 + col].x);
-        const float shift = mm == -INFINITY ? 0.0f : mm;
-        l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < KW; w++) {
-            const float2 e = ml[(w * RW + rw) * 32 + col];
-            l += e.y * __builtin_amdgcn_exp2f(e.x - shift);
-        }
-        const float f = __builtin_amdgcn_exp2f(m - shift);
-#pragma unroll
-        for (int t = 0; t < DT; t++) acc[t] *= f;
-        if (kw > 0) {
-#pragma unroll
-            for (int t = 0; t < DT; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) red[(((kw - 1) * RW + rw) * (DP / 2) + 16 * (DT * ds + t) + i) * 64 + lane] = acc[t][i];
-        }
-        __syncthreads();
-        if (kw > 0) return;
-#pragma unroll
-        for (int w = 0; w < KW - 1; w++)
-#pragma unroll
-            for (int t = 0; t < DT; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) acc[t][i] += red[((w * RW + rw) * (DP / 2) + 16 * (DT * ds + t) + i) * 64 + lane];
+    for (int c = 0; c < CT; c++) {
+        l[c] = sum_xor32(l[c]);
+        if (half == 0) ml[(wave * CT + c) * 32 + col] = make_float2(m[c], l[c]);
     }
-    if (row >= rows) return;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t o0 = b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * half;
+    __syncthreads();
 #pragma unroll
-    for (int t = 0; t < DT; t++)
+    for (int c = 0; c < CT; c++) {
+        float mm = -INFINITY, total = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int d = 32 * (DT * ds + t) + 8 * i;
-            if (d >= D) continue;
-            const f32x4_t o = f32x4_t{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]} * inv;
-            if constexpr (kF32) *reinterpret_cast<f32x4_t*>(static_cast<float*>(a.out) + o0 + d) = o;
-            else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + o0 + d) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+        for (int w = 0; w < 4; w++) mm = fmaxf(mm, ml[(w * CT + c) * 32 + col].x);
+        const float shift = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const float2 e = ml[(w * CT + c) * 32 + col];
+            total += e.y * __builtin_amdgcn_exp2f(e.x - shift);
         }
+        f[c] = __builtin_amdgcn_exp2f(m[c] - shift);
+        inv[c] = total == 0.0f ? 0.0f : 1.0f / total;
+    }
+    float* red = reinterpret_cast<float*>(lds);
+#pragma unroll
+    for (int t = 0; t < DT; t++) {
+        if (t > 0) __syncthreads();
+#pragma unroll
+        for (int c = 0; c < CT; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) red[((wave * CT + c) * 16 + i) * 64 + lane] = acc[c][t][i] * f[c];
+        __syncthreads();
+        // this wave's elements 4 wave .. + 3: dims 32 t + 8 wave + 4 half + 0 .. 3
+        const int d = 32 * t + 8 * wave + 4 * half;
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            if (row[c] >= rows || d >= D) continue;
+            f32x4_t o;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float* e = red + (c * 16 + 4 * wave + i) * 64 + lane;
+                o[i] = ((e[0] + e[CT * 1024]) + (e[2 * CT * 1024] + e[3 * CT * 1024])) * inv[c];
+            }
+            store4<T>(a.out, b * a.os[0] + (kh * a.group + qg[c]) * a.os[1] + qt[c] * a.os[2] + d, o);
+        }
+    }
 }
 
-template <typename T, int FORMAT, int DP, int RW>
+template <typename T, int FORMAT, int DP, int CT>
 int launch_rows(const QuantAttnArgs& a, hipStream_t stream, Err e) {
-    using G = QGeo<T, FORMAT, DP, RW>;
-    static_assert(G::kBytes + kTable * 16 <= 160 * 1024 - 256, "LDS of a workgroup");
-    PrefillQArgs pa{};
+    using G = PromptGeo<T, FORMAT, DP, CT>;
+    static_assert(G::kBytes <= 64 * 1024, "LDS of a workgroup");
+    PromptArgs pa{};
     pa.a = a;
     const int64_t rows = static_cast<int64_t>(a.group) * a.p.tokens;
-    pa.row_blocks = static_cast<int32_t>((rows + 32 * RW - 1) / (32 * RW));
-    pa.table = std::min(kTable, a.p.max_blocks);
-    const size_t bytes = G::kBytes + static_cast<size_t>(pa.table) * 16;
-    const void* fn = reinterpret_cast<const void*>(&quant_prefill_kernel<T, FORMAT, DP, RW>);
-    if (bytes > 64 * 1024)
-        SANDY_HIP_TRY(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)), e,
-                      "quant_paged attention launch");
+    pa.row_blocks = static_cast<int32_t>((rows + 32 * CT - 1) / (32 * CT));
     const int64_t wgs = static_cast<int64_t>(pa.row_blocks) * a.p.batch * a.p.heads;
     void* params[] = {&pa};
-    SANDY_HIP_TRY(hipLaunchKernel(fn, dim3(static_cast<unsigned>(wgs)), dim3(G::THREADS), params, bytes, stream), e,
+    SANDY_HIP_TRY(hipLaunchKernel(reinterpret_cast<const void*>(&quant_prompt_kernel<T, FORMAT, DP, CT>),
+                                  dim3(static_cast<unsigned>(wgs)), dim3(256), params, G::kBytes, stream), e,
                   "quant_paged attention launch");
     return ok(e);
 }
@@ -433,9 +352,9 @@ template <typename T, int FORMAT, int DP>
 int launch_dim(const QuantAttnArgs& a, hipStream_t stream, Err e) {
     const int64_t rows = static_cast<int64_t>(a.group) * a.p.tokens;
     const int64_t wgs = (rows + 63) / 64 * a.p.batch * a.p.heads;
-    const int rw = env_int("SANDY_QUANT_RW", wgs >= 224 ? 2 : 1);
-    if (rw == 4) return launch_rows<T, FORMAT, DP, 4>(a, stream, e);
-    if (rw == 2) return launch_rows<T, FORMAT, DP, 2>(a, stream, e);
+    const int ct = env_int("SANDY_QUANT_CT", wgs >= 512 ? 2 : 1);
+    if constexpr (DP <= 128 && !(DP == 128 && std::is_same_v<T, F32>))
+        if (ct == 2) return launch_rows<T, FORMAT, DP, 2>(a, stream, e);
     return launch_rows<T, FORMAT, DP, 1>(a, stream, e);
 }
 
@@ -452,7 +371,7 @@ int launch_format(const QuantAttnArgs& a, hipStream_t stream, Err e) {
 bool quant_prefill_takes(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t max_blocks, bool f32) {
     const int64_t rows = hq / heads * tokens;
     return tokens > 1 && rows >= env_int("SANDY_QUANT_PREFILL_ROWS", 64) && (!f32 || dim <= 128) && max_blocks > 0 &&
-           (rows + 31) / 32 * batch * heads <= UINT32_MAX / 512;
+           (rows + 31) / 32 * batch * heads <= UINT32_MAX / 256;
 }
 
 int launch_quant_prefill(const QuantAttnArgs& a, int32_t format, hipStream_t stream, Err e) {
