@@ -13,21 +13,41 @@ struct QuantAttnArgs {
     int64_t window;
     float scale_log2;      // scale * log2(e)
     int32_t hq, group;     // q heads, of one kv head
+    uint32_t group_magic;  // for divide() by group
     int32_t f32;           // q and out are f32, else bf16
 };
 
-// Keys [first, last] that query t of a sequence at `pos` sees (none: last < first).
+// Keys [first, last] that a query sees (none: last < first).
 struct KeyRange {
     int first, last;
 };
 
-__device__ __forceinline__ KeyRange quant_keys(const QuantAttnArgs& a, int64_t pos, int t) {
-    const int64_t at = min<int64_t>(pos, INT64_MAX - INT32_MAX) + t;
-    const int64_t cap = static_cast<int64_t>(a.p.max_blocks) << a.p.log2_page;
-    KeyRange r;
-    r.last = static_cast<int>(min<int64_t>(at, cap - 1));
-    r.first = a.window > 0 ? static_cast<int>(min<int64_t>(max<int64_t>(at - a.window + 1, 0), cap)) : 0;
-    return r;
+// The positions of a sequence's queries in 32 bits: what lies past the block
+// table (2^30 keys at most) or before the first key is brought to that border.
+struct SeqKeys {
+    int base;   // position of query 0
+    int lower;  // its first key, or below 0
+    int cap;    // keys the block table covers
+
+    __device__ __forceinline__ KeyRange of(int t) const {
+        return KeyRange{min(max(lower + t, 0), cap), min(base + t, cap - 1)};
+    }
+};
+
+__device__ __forceinline__ SeqKeys quant_keys(const QuantAttnArgs& a, int64_t pos) {
+    constexpr int64_t kFar = int64_t{1} << 30;
+    SeqKeys s;
+    s.cap = a.p.max_blocks << a.p.log2_page;
+    s.base = static_cast<int>(min<int64_t>(max<int64_t>(pos, 0), kFar));
+    // window <= INT64_MAX and pos >= 0: no overflow
+    s.lower = a.window > 0 ? static_cast<int>(max<int64_t>(min<int64_t>(max<int64_t>(pos, 0) - a.window, kFar - 1), -kFar) + 1) : -static_cast<int>(kFar);
+    return s;
+}
+
+// n / d with magic = 2^32 / d rounded down (2^32 - 1 for d = 1): at most one short.
+__device__ __forceinline__ int divide(int n, int d, uint32_t magic) {
+    const int q = static_cast<int>(__umulhi(static_cast<uint32_t>(n), magic));
+    return q + (n - q * d >= d ? 1 : 0);
 }
 
 // Few queries a sequence (quant_decode.hip): whether the kernel takes the call,

@@ -33,7 +33,7 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
     const int D = p.dim;
     const int64_t pos = load_index(p.pos, p.pos_dt, b);
     if (pos < 0 && tid == 0) atomicOr(p.errw, static_cast<uint32_t>(SANDY_DEVERR_ATTN_POS));
-    KeyRange keys = quant_keys(a, pos, t);
+    KeyRange keys = quant_keys(a, pos).of(t);
     if (pos < 0 || t >= quant_count(p, b)) keys = KeyRange{0, -1};
     const int64_t q0 = b * a.qs[0] + h * a.qs[1] + t * a.qs[2];
     for (int d = tid; d < D; d += 256) qf[d] = Vec8<T>::load1(a.q, q0 + d * a.qs[3]);
@@ -160,6 +160,7 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     a.scale_log2 = (scale <= 0.0 ? 1.0f / sqrtf(static_cast<float>(a.p.dim)) : static_cast<float>(scale)) * 1.44269504088896341f;
     a.hq = static_cast<int32_t>(q->dims[1]);
     a.group = a.hq / a.p.heads;
+    a.group_magic = a.group == 1 ? UINT32_MAX : static_cast<uint32_t>((uint64_t{1} << 32) / static_cast<uint32_t>(a.group));
     a.f32 = q->dtype == SANDY_F32;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (quant_decode_takes(a)) {

@@ -40,12 +40,12 @@ struct TileKeys {
     int begin, last, pairs, per, active;
 };
 
-__device__ __forceinline__ TileKeys tile_keys(const DecodeArgs& d, int64_t pos, int count, int t_lo, int t_hi) {
+__device__ __forceinline__ TileKeys tile_keys(const DecodeArgs& d, const SeqKeys& seq, int count, int t_lo, int t_hi) {
     TileKeys k{0, -1, 0, kMinPairs, 1};
     t_hi = min(t_hi, count - 1);
-    if (pos >= 0 && t_lo <= t_hi) {
-        k.begin = quant_keys(d.a, pos, t_lo).first & ~15;
-        k.last = quant_keys(d.a, pos, t_hi).last;
+    if (t_lo <= t_hi) {
+        k.begin = seq.of(t_lo).first & ~15;
+        k.last = seq.of(t_hi).last;
         if (k.last >= k.begin) k.pairs = (k.last - k.begin + 32) >> 5;
         k.per = max((k.pairs + d.splits - 1) / d.splits, kMinPairs);
         k.active = max((k.pairs + k.per - 1) / k.per, 1);
@@ -121,7 +121,7 @@ __device__ __forceinline__ void join_splits(const DecodeArgs& da, int64_t first,
                 o += f32x4_t{low(x[s]), high(x[s]), low(y[s]), high(y[s])} * w;
             }
         }
-        const int row = 16 * ct + c, qt = row / a.group, qg = row - qt * a.group;
+        const int row = 16 * ct + c, qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
         if (final_out) {
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
             store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, o * inv);
@@ -169,20 +169,21 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     const int ct = at / da.splits;
     const int rows = a.group * p.tokens;
     const int64_t pos = load_index(p.pos, p.pos_dt, b);
-    const int count = quant_count(p, b);
-    const int t_lo = 16 * ct / a.group, t_hi = min(rows - 1, 16 * ct + 15) / a.group;
-    const TileKeys tk = tile_keys(da, pos, count, t_lo, t_hi);
+    const int count = pos < 0 ? 0 : quant_count(p, b);
+    const SeqKeys seq = quant_keys(a, pos);
+    const int t_lo = divide(16 * ct, a.group, a.group_magic), t_hi = divide(min(rows - 1, 16 * ct + 15), a.group, a.group_magic);
+    const TileKeys tk = tile_keys(da, seq, count, t_lo, t_hi);
     if (split >= tk.active) return;
     if (pos < 0 && tid == 0) atomicOr(p.errw, static_cast<uint32_t>(SANDY_DEVERR_ATTN_POS));
 
     // this lane's column: query qt, head qg of the group (past the rows: the last one, not stored)
     const int row = min(16 * ct + col, rows - 1);
-    const int qt = row / a.group, qg = row - qt * a.group;
-    KeyRange mine = quant_keys(a, pos, qt);
+    const int qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
+    KeyRange mine = seq.of(qt);
     if (qt >= count) mine.last = -1;
     // keys that every column sees
-    const int all_first = quant_keys(a, pos, t_hi).first;
-    const int all_last = t_hi < count ? quant_keys(a, pos, t_lo).last : -1;
+    const int all_first = seq.of(t_hi).first;
+    const int all_last = t_hi < count ? seq.of(t_lo).last : -1;
 
     // B operands of Q^T: column, dims 64 j + 16 g + 8 s .. + 7 in step 2 j + s
     // (past D any of the row's: K is zero there)
@@ -441,9 +442,10 @@ __global__ __launch_bounds__(256) void quant_decode_merge_kernel(DecodeArgs da) 
     const int kh = at % p.heads;
     const int b = at / p.heads;
     const int ct = row >> 4, col = row & 15;
-    const int t_lo = 16 * ct / a.group, t_hi = min(rows - 1, 16 * ct + 15) / a.group;
-    const int qt = row / a.group, qg = row - qt * a.group;
-    const TileKeys tk = tile_keys(da, load_index(p.pos, p.pos_dt, b), quant_count(p, b), t_lo, t_hi);
+    const int t_lo = divide(16 * ct, a.group, a.group_magic), t_hi = divide(min(rows - 1, 16 * ct + 15), a.group, a.group_magic);
+    const int qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
+    const int64_t pos = load_index(p.pos, p.pos_dt, b);
+    const TileKeys tk = tile_keys(da, quant_keys(a, pos), pos < 0 ? 0 : quant_count(p, b), t_lo, t_hi);
     if (tk.active == 1) return;
     const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
     const float* ml = da.part_ml + (unit * da.splits * 16 + col) * 2;

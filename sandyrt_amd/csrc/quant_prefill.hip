@@ -59,14 +59,15 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP, CT>::kWaves)) void q
     if (pos < 0 && tid == 0) atomicOr(p.errw, static_cast<uint32_t>(SANDY_DEVERR_ATTN_POS));
     // the rows' queries, those of the padding aside
     const int r0 = rb * 32 * CT;
-    const int t_lo = r0 / a.group, t_hi = min(rows - 1, r0 + 32 * CT - 1) / a.group;
+    const SeqKeys seq = quant_keys(a, pos);
+    const int t_lo = divide(r0, a.group, a.group_magic), t_hi = divide(min(rows - 1, r0 + 32 * CT - 1), a.group, a.group_magic);
     const int t_end = min(t_hi, count - 1);
-    const int begin = quant_keys(a, pos, t_lo).first & ~15;
-    const int last = t_lo <= t_end ? quant_keys(a, pos, t_end).last : -1;
+    const int begin = seq.of(t_lo).first & ~15;
+    const int last = t_lo <= t_end ? seq.of(t_end).last : -1;
     const int pairs = last >= begin ? (last - begin + 32) >> 5 : 0;
     // keys that every row sees
-    const int all_first = quant_keys(a, pos, t_hi).first;
-    const int all_last = t_hi < count ? quant_keys(a, pos, t_lo).last : -1;
+    const int all_first = seq.of(t_hi).first;
+    const int all_last = t_hi < count ? seq.of(t_lo).last : -1;
 
     // this lane's rows (past the end: the last one, not stored) and their keys
     int row[CT], qt[CT], qg[CT];
@@ -77,8 +78,8 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP, CT>::kWaves)) void q
     for (int c = 0; c < CT; c++) {
         row[c] = r0 + 32 * c + col;
         const int rc = min(row[c], rows - 1);
-        qt[c] = rc / a.group, qg[c] = rc - qt[c] * a.group;
-        mine[c] = quant_keys(a, pos, qt[c]);
+        qt[c] = divide(rc, a.group, a.group_magic), qg[c] = rc - qt[c] * a.group;
+        mine[c] = seq.of(qt[c]);
         if (qt[c] >= count) mine[c].last = -1;
         const int64_t q0 = b * a.qs[0] + (kh * a.group + qg[c]) * a.qs[1] + qt[c] * a.qs[2];
 #pragma unroll
@@ -216,7 +217,19 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP, CT>::kWaves)) void q
                 }
             }
         }
-        bf16x8_t pw[CT][2][NP];
+        // V^T operands (dims past D: bytes of earlier tiles, in accumulators that nothing
+        // stores), kept where they serve two tiles of rows
+        bf16x8_t va[2][DT];
+        auto v_operand = [&](int h, int t) {
+            const i32x2_t eight = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * h * G::VP + 32 * t)));
+            return payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), v[h], v[h]);
+        };
+        if constexpr (CT > 1)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int t = 0; t < DT; t++) va[h][t] = v_operand(h, t);
 #pragma unroll
         for (int c = 0; c < CT; c++) {
             float top[2];
@@ -260,22 +273,14 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP, CT>::kWaves)) void q
                     for (int n2 = 0; n2 < NP; n2++) parts[n2][j / 2] = part[n2];
                 }
 #pragma unroll
-                for (int n2 = 0; n2 < NP; n2++) pw[c][h][n2] = __builtin_bit_cast(bf16x8_t, parts[n2]);
+                for (int t = 0; t < DT; t++) {
+                    if constexpr (CT == 1) va[h][t] = v_operand(h, t);
+#pragma unroll
+                    for (int n2 = NP - 1; n2 >= 0; n2--)
+                        acc[c][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[h][t], __builtin_bit_cast(bf16x8_t, parts[n2]), acc[c][t], 0, 0, 0);
+                }
             }
         }
-        // (dims past D: bytes of earlier tiles, in accumulators that nothing stores)
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int t = 0; t < DT; t++) {
-                const i32x2_t eight = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                    (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * h * G::VP + 32 * t)));
-                const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), v[h], v[h]);
-#pragma unroll
-                for (int c = 0; c < CT; c++)
-#pragma unroll
-                    for (int i = NP - 1; i >= 0; i--) acc[c][t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, pw[c][h][i], acc[c][t], 0, 0, 0);
-            }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     };
     for (int round0 = wave; round0 < pairs; round0 += 4 * 32) {
