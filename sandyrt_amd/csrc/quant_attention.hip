@@ -101,8 +101,10 @@ bool is_prompt(const SandyTensor* q, const SandyQuantCache* kc, const SandyTenso
 }
 
 size_t workspace_of(const SandyTensor* q, const SandyQuantCache* kc, const SandyTensor* table, int64_t window) {
+    const int64_t page = kc->page_size, D = kc->inner;
+    if (D % 16 != 0 || D > 256 || page < 16 || numel(*q) == 0) return 0;
     if (is_prompt(q, kc, table)) return 0;
-    return quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], kc->inner, kc->page_size, table->dims[1], window);
+    return quant_decode_workspace(q->dims[0], q->dims[1], kc->prefix, q->dims[2], D, page, table->dims[1], window);
 }
 
 int check_quant_attention(const SandyTensor* q, const SandyQuantCache* kc, Err e) {
@@ -164,10 +166,10 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     a.f32 = q->dtype == SANDY_F32;
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (quant_decode_takes(a)) {
-        if (is_prompt(q, kc, table)) return launch_quant_prefill(a, kc->format, s, e);
         const size_t need = workspace_of(q, kc, table, window);
         if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
             return fail(e, SANDY_ERR_INVALID, "quant_paged attention needs a 16-byte aligned workspace of %zu bytes", need);
+        if (is_prompt(q, kc, table)) return launch_quant_prefill(a, kc->format, s, e);
         return launch_quant_decode(a, kc->format, workspace, s, e);
     }
     const int64_t wgs = q->dims[0] * q->dims[1] * q->dims[2];

@@ -12,128 +12,10 @@
 //     contraction is free as long as Q has the same);
 //   - V through the wave's own LDS rows, back by ds_read_b64_tr_b8, which gives a
 //     lane one dim of 8 keys -- the A operand of O^T in the order that P leaves S^T.
-#include "quant_mfma.h"
-
-#include <algorithm>
+#include "quant_split.h"
 
 namespace sandy_hip {
 namespace {
-
-constexpr int kMinPairs = 4;            // pairs of tiles a split has at least: one a wave
-
-struct DecodeArgs {
-    QuantAttnArgs a;
-    int32_t col_tiles;  // 16-column tiles of the (query, head) rows of a kv head
-    int32_t splits;     // workgroups a column tile's keys may be split over
-    float* part_o;      // [unit, split][16][D] sums relative to the maximum
-    float* part_ml;     // [unit, split][16][2] maximum and sum of weights
-    uint32_t* arrived;  // [unit][counters_of(splits)] zero between calls, or null: the merge kernel joins the splits
-};
-
-// Splits are joined by the last workgroup to arrive, in groups of 16 and then
-// the groups: a unit's counters are one for the groups (or the only group) and,
-// where there are several, one for each.
-__host__ __device__ constexpr int counters_of(int splits) { return splits <= 16 ? 1 : 1 + (splits + 15) / 16; }
-
-// The keys of one column tile: pairs of 16-key tiles from `begin`, `per` of them a split.
-struct TileKeys {
-    int begin, last, pairs, per, active;
-};
-
-__device__ __forceinline__ TileKeys tile_keys(const DecodeArgs& d, const SeqKeys& seq, int count, int t_lo, int t_hi) {
-    TileKeys k{0, -1, 0, kMinPairs, 1};
-    t_hi = min(t_hi, count - 1);
-    if (t_lo <= t_hi) {
-        k.begin = seq.of(t_lo).first & ~15;
-        k.last = seq.of(t_hi).last;
-        if (k.last >= k.begin) k.pairs = (k.last - k.begin + 32) >> 5;
-        k.per = max((k.pairs + d.splits - 1) / d.splits, kMinPairs);
-        k.active = max((k.pairs + k.per - 1) / k.per, 1);
-    }
-    return k;
-}
-
-// Stores and loads that go through to memory: other XCDs' L2s see them once the
-// storing thread has waited for them.
-__device__ __forceinline__ void put_through(float* to, float x, float y) {
-    const uint64_t v = static_cast<uint64_t>(__float_as_uint(x)) | static_cast<uint64_t>(__float_as_uint(y)) << 32;
-    __hip_atomic_store(reinterpret_cast<uint64_t*>(to), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void put_through(float* to, f32x4_t v) {
-    put_through(to, v[0], v[1]);
-    put_through(to + 2, v[2], v[3]);
-}
-__device__ __forceinline__ uint64_t get_through(const float* from) {
-    return __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float low(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v)); }
-__device__ __forceinline__ float high(uint64_t v) { return __uint_as_float(static_cast<uint32_t>(v >> 32)); }
-
-// Counts this workgroup in once its stores are there; true for the last of n,
-// which leaves the counter zero.
-__device__ __forceinline__ bool last_to_arrive(uint32_t* counter, int n) {
-    __shared__ bool last;
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == static_cast<uint32_t>(n - 1);
-        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
-    __syncthreads();
-    return last;
-}
-
-// Slots first, first + stride, .. (n <= 16) of a column tile joined, in slot
-// order: into the output, or into slot `first`.  A thread per column and 4 dims.
-template <typename T>
-__device__ __forceinline__ void join_splits(const DecodeArgs& da, int64_t first, int stride, int n, int ct, int kh, int b, bool final_out) {
-    __shared__ float2 joined[16];
-    const QuantAttnArgs& a = da.a;
-    const int D = a.p.dim, rows = a.group * a.p.tokens;
-    const int per_col = D / 4;
-    const int cols = min(16, rows - 16 * ct);
-    for (int i = threadIdx.x; i < cols * per_col; i += 256) {
-        const int c = i / per_col, d = 4 * (i - c * per_col);
-        float m = -INFINITY, total = 0.0f;
-        f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = 0; s0 < n; s0 += 8) {
-            uint64_t ml[8], x[8], y[8];
-#pragma unroll
-            for (int s = 0; s < 8; s++) {  // past the last: the last again, unused
-                const int64_t slot = first + static_cast<int64_t>(min(s0 + s, n - 1)) * stride;
-                ml[s] = get_through(da.part_ml + (slot * 16 + c) * 2);
-                x[s] = get_through(da.part_o + (slot * 16 + c) * D + d);
-                y[s] = get_through(da.part_o + (slot * 16 + c) * D + d + 2);
-            }
-            float top = m;
-#pragma unroll
-            for (int s = 0; s < 8; s++) top = fmaxf(top, low(ml[s]));
-            const float shift = top == -INFINITY ? 0.0f : top;
-            const float f = __builtin_amdgcn_exp2f(m - shift);
-            total *= f;
-            o *= f;
-            m = top;
-#pragma unroll
-            for (int s = 0; s < 8; s++) {
-                if (s0 + s >= n) continue;
-                const float w = __builtin_amdgcn_exp2f(low(ml[s]) - shift);
-                total += high(ml[s]) * w;
-                o += f32x4_t{low(x[s]), high(x[s]), low(y[s]), high(y[s])} * w;
-            }
-        }
-        const int row = 16 * ct + c, qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
-        if (final_out) {
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, o * inv);
-        } else {
-            put_through(da.part_o + (first * 16 + c) * D + d, o);
-            if (d == 0) joined[c] = make_float2(m, total);
-        }
-    }
-    if (final_out) return;
-    __syncthreads();  // every thread has read the slot's own maximum and sum
-    if (threadIdx.x < cols) put_through(da.part_ml + (first * 16 + threadIdx.x) * 2, joined[threadIdx.x].x, joined[threadIdx.x].y);
-}
 
 template <typename T, int FORMAT, int DP>
 struct DecodeGeo {
@@ -148,7 +30,7 @@ struct DecodeGeo {
 };
 
 template <typename T, int FORMAT, int DP>
-__global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant_decode_kernel(DecodeArgs da) {
+__global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant_decode_kernel(SplitArgs da) {
     using G = DecodeGeo<T, FORMAT, DP>;
     constexpr bool kF32 = std::is_same_v<T, F32>;
     constexpr int NQ = kF32 ? 3 : 1, NP = kF32 ? 3 : 2, NCH = G::kChunks, NT = DP / 16, RING = G::kRing;
@@ -394,6 +276,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     const bool final_out = tk.active == 1;
     const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
     const int64_t slot = unit * da.splits + split;
+    const Through po(da.part_o + slot * 16 * D);
     const bool stored = 16 * ct + col < rows;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const int64_t o0 = b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2];
@@ -412,103 +295,32 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
             const f32x4_t o = (red[t * 64 + lane] + red[(SET + t) * 64 + lane]) +
                               (red[(2 * SET + t) * 64 + lane] + red[(3 * SET + t) * 64 + lane]);
             if (final_out) store4<T>(a.out, o0 + d, o * inv);
-            else put_through(da.part_o + (slot * 16 + col) * D + d, o);
+            else po.put(col * D + d, o);
         }
     }
     if (final_out) return;
-    if (tid < 16 && stored) put_through(da.part_ml + (slot * 16 + col) * 2, mm, total);
-    if (!da.arrived) return;
-    uint32_t* arrived = da.arrived + unit * counters_of(da.splits);
-    const int groups = (tk.active + 15) / 16, grp = split / 16;
-    const int in_group = min(16, tk.active - 16 * grp);
-    if (!last_to_arrive(arrived + (groups > 1 ? 1 + grp : 0), in_group)) return;
-    join_splits<T>(da, unit * da.splits + 16 * grp, 1, in_group, ct, kh, b, groups == 1);
-    if (groups == 1 || !last_to_arrive(arrived, groups)) return;
-    join_splits<T>(da, unit * da.splits, 16, groups, ct, kh, b, true);
-}
-
-// Joins the splits of one output row: a workgroup per row, every thread 4 dims
-// of every (256 / (D / 4))-th split.
-template <typename T>
-__global__ __launch_bounds__(256) void quant_decode_merge_kernel(DecodeArgs da) {
-    __shared__ f32x4_t sums[256];
-    const QuantAttnArgs& a = da.a;
-    const QuantPages& p = a.p;
-    const int tid = threadIdx.x, D = p.dim;
-    uint32_t at = blockIdx.x;
-    const int rows = a.group * p.tokens;
-    const int row = at % rows;
-    at /= rows;
-    const int kh = at % p.heads;
-    const int b = at / p.heads;
-    const int ct = row >> 4, col = row & 15;
-    const int t_lo = divide(16 * ct, a.group, a.group_magic), t_hi = divide(min(rows - 1, 16 * ct + 15), a.group, a.group_magic);
-    const int qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
-    const int64_t pos = load_index(p.pos, p.pos_dt, b);
-    const TileKeys tk = tile_keys(da, quant_keys(a, pos), pos < 0 ? 0 : quant_count(p, b), t_lo, t_hi);
-    if (tk.active == 1) return;
-    const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
-    const float* ml = da.part_ml + (unit * da.splits * 16 + col) * 2;
-    const float* po = da.part_o + (unit * da.splits * 16 + col) * D;
-    float m = -INFINITY;
-    for (int s = tid & 63; s < tk.active; s += 64) m = fmaxf(m, ml[s * 32]);
-    m = wave_max(m);
-    const float shift = m == -INFINITY ? 0.0f : m;
-    float total = 0.0f;
-    for (int s = tid & 63; s < tk.active; s += 64) total += ml[s * 32 + 1] * __builtin_amdgcn_exp2f(ml[s * 32] - shift);
-    total = wave_sum(total);
-    const int pieces = D / 4, groups = 256 / pieces;
-    const int piece = tid % pieces, grp = tid / pieces;
-    f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
-    if (grp < groups)
-#pragma unroll 4
-        for (int s = grp; s < tk.active; s += groups)
-            o += *reinterpret_cast<const f32x4_t*>(po + static_cast<int64_t>(s) * 16 * D + 4 * piece) * __builtin_amdgcn_exp2f(ml[s * 32] - shift);
-    sums[tid] = o;
-    __syncthreads();
-    if (tid < pieces) {
-        for (int i = 1; i < groups; i++) o += sums[tid + i * pieces];
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * tid, o * inv);
-    }
+    if (tid < 16 && stored) Through(da.part_ml + slot * 32).put(2 * col, mm, total);
+    finish_split<T, 16>(da, unit, split, tk.active, ct, kh, b);
 }
 
 template <typename T, int FORMAT, int DP>
-int launch_dim(const DecodeArgs& d, hipStream_t stream, Err e) {
+int launch_dim(const SplitArgs& d, hipStream_t stream, Err e) {
     using G = DecodeGeo<T, FORMAT, DP>;
-    const void* fn = reinterpret_cast<const void*>(&quant_decode_kernel<T, FORMAT, DP>);
-    if (G::kBytes > 64 * 1024)
-        SANDY_HIP_TRY(hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, G::kBytes), e, "quant_paged attention launch");
-    const QuantPages& p = d.a.p;
-    const int64_t wgs = static_cast<int64_t>(p.batch) * p.heads * d.col_tiles * d.splits;
-    DecodeArgs args = d;
-    void* params[] = {&args};
-    SANDY_HIP_TRY(hipLaunchKernel(fn, dim3(static_cast<unsigned>(wgs)), dim3(256), params, G::kBytes, stream), e,
-                  "quant_paged attention launch");
-    if (d.splits > 1 && !d.arrived) {
-        const int64_t rows = static_cast<int64_t>(p.batch) * d.a.hq * p.tokens;
-        hipLaunchKernelGGL((quant_decode_merge_kernel<T>), dim3(static_cast<unsigned>(rows)), dim3(256), 0, stream, d);
-        SANDY_HIP_TRY(hipGetLastError(), e, "quant_paged attention launch");
-    }
-    return ok(e);
+    static_assert(G::kBytes <= 64 * 1024, "LDS of a workgroup");
+    return launch_split<T, 16>(reinterpret_cast<const void*>(&quant_decode_kernel<T, FORMAT, DP>), d, G::kBytes, stream, e);
 }
 
 template <typename T, int FORMAT>
-int launch_format(const DecodeArgs& d, hipStream_t stream, Err e) {
+int launch_format(const SplitArgs& d, hipStream_t stream, Err e) {
     if (d.a.p.dim <= 64) return launch_dim<T, FORMAT, 64>(d, stream, e);
     if (d.a.p.dim <= 128) return launch_dim<T, FORMAT, 128>(d, stream, e);
     return launch_dim<T, FORMAT, 256>(d, stream, e);
 }
 
-// Splits of a column tile's keys: enough workgroups for the chip, none of less
-// than kMinPairs pairs at the longest context the call can have.
-int decode_splits(int64_t batch, int64_t heads, int64_t col_tiles, int64_t cap, int64_t window, int64_t tokens, int64_t dim) {
-    const int64_t units = batch * heads * col_tiles;
-    const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tokens + 16) : cap;
-    const int64_t most = std::max<int64_t>((keys + 31) / 32 / kMinPairs, 1);
-    const int64_t target = dim > 128 ? 256 : 512;
-    return static_cast<int>(std::clamp<int64_t>(env_int("SANDY_QUANT_SPLITS", static_cast<int>(std::min<int64_t>((target + units - 1) / units, 256))), 1, std::min<int64_t>(most, 256)));
-}
+// Workgroups wanted: us at a target of 256 / 512 / 1024, D 64, 32 sequences 16.6 /
+// 15.2 / 15.3, one of 32749 keys 14.6 / 14.8 / 17.3; D 256, 64 sequences 20.2 / 21.2 /
+// 26.3.
+int64_t target_of(int64_t dim) { return dim > 128 ? 256 : 512; }
 
 } // namespace
 
@@ -525,35 +337,26 @@ bool quant_decode_takes(const QuantAttnArgs& a) {
     if (!aligned(a.out, 4 * es) || ((to[0] | to[1] | to[2]) & 3) || a.os[3] != 1) return false;
     const int64_t rows = static_cast<int64_t>(a.group) * p.tokens;
     const int64_t col_tiles = (rows + 15) / 16;
-    const int64_t wgs = col_tiles * p.batch * p.heads *
-                        decode_splits(p.batch, p.heads, col_tiles, static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens, p.dim);
-    return rows < (1 << 30) && wgs <= UINT32_MAX / 256 && static_cast<int64_t>(p.batch) * a.hq * p.tokens <= UINT32_MAX / 256;
+    // threads of a launch below 2^32, splits (of fewer tiles than wanted) included
+    return rows < (1 << 30) && col_tiles * p.batch * p.heads <= UINT32_MAX / 256 - 2048;
 }
 
 size_t quant_decode_workspace(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t page,
                               int64_t max_blocks, int64_t window) {
-    if (dim % 16 != 0 || dim > 256 || page < 16 || batch == 0 || tokens == 0) return 0;
-    const int64_t cap = max_blocks * page;
-    const int64_t col_tiles = (hq / heads * tokens + 15) / 16;
-    const int64_t splits = decode_splits(batch, heads, col_tiles, cap, window, tokens, dim);
-    return splits == 1 ? 0 : static_cast<size_t>(batch * heads * col_tiles * splits * 16 * (dim + 2)) * sizeof(float);
+    const int64_t units = (hq / heads * tokens + 15) / 16 * batch * heads;
+    const int64_t splits = split_count(units, target_of(dim), max_blocks * page, window, tokens);
+    return splits == 1 ? 0 : static_cast<size_t>(units * splits * 16 * (dim + 2)) * sizeof(float);
 }
 
 int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace, hipStream_t stream, Err e) {
     const QuantPages& p = a.p;
-    DecodeArgs d{};
+    SplitArgs d{};
     d.a = a;
     d.col_tiles = (a.group * p.tokens + 15) / 16;
-    d.splits = decode_splits(p.batch, p.heads, d.col_tiles, static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens, p.dim);
-    const int64_t slots = static_cast<int64_t>(p.batch) * p.heads * d.col_tiles * d.splits;
-    d.part_o = static_cast<float*>(workspace);
-    d.part_ml = d.part_o + slots * 16 * p.dim;
-    if (d.splits > 1 && env_int("SANDY_QUANT_MERGE_KERNEL", 0) == 0) {
-        const size_t words = static_cast<size_t>(slots / d.splits) * counters_of(d.splits);
-        int status = 0;
-        d.arrived = arrival_counters(words, stream, e, &status);
-        if (status) return status;
-    }
+    d.splits = split_count(static_cast<int64_t>(p.batch) * p.heads * d.col_tiles, target_of(p.dim),
+                           static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens);
+    const int status = split_memory<16>(&d, workspace, stream, e);
+    if (status) return status;
     if (format == SANDY_QUANT_INT8)
         return a.f32 ? launch_format<F32, SANDY_QUANT_INT8>(d, stream, e) : launch_format<BF16, SANDY_QUANT_INT8>(d, stream, e);
     return a.f32 ? launch_format<F32, SANDY_QUANT_E4M3>(d, stream, e) : launch_format<BF16, SANDY_QUANT_E4M3>(d, stream, e);
