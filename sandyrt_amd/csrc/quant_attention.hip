@@ -12,9 +12,10 @@ namespace {
 
 constexpr int kMaxDim = 512;
 
-// Any head dim and page size: a workgroup per (sequence, q head, query), 256
-// keys at a time -- a thread scores one key, then owns dims tid and tid + 256.
-template <typename T, int FORMAT>
+// Any head dim, page size and stride: a workgroup per (sequence, q head, query), 256
+// keys at a time.  A thread scores one key, W bytes of it a load; then groups of
+// `lanes` threads (a thread a dim, two past 256 dims) weigh every groups-th key.
+template <typename T, int FORMAT, int W>
 __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnArgs a) {
     constexpr int kDims = kMaxDim / 256;
     __shared__ float qf[kMaxDim];
@@ -38,6 +39,7 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
     const int64_t q0 = b * a.qs[0] + h * a.qs[1] + t * a.qs[2];
     for (int d = tid; d < D; d += 256) qf[d] = Vec8<T>::load1(a.q, q0 + d * a.qs[3]);
     __syncthreads();
+    const int lanes = min(D, 256), groups = 256 / lanes, group = tid / lanes, dim0 = tid - group * lanes;
     float m = -INFINITY, acc[kDims];
     double l = 0.0;
 #pragma unroll
@@ -53,7 +55,17 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
                 const int64_t from = ((block << p.log2_page) + (key & ((1 << p.log2_page) - 1))) * D;
                 const uint8_t* krow = p.pool[0] + from;
                 float dot = 0.0f;
-                for (int d = 0; d < D; d++) dot = fmaf(qf[d], Quant<FORMAT>::template value<0>(krow[d]), dot);
+                if constexpr (W == 4) {
+#pragma unroll 4
+                    for (int d = 0; d < D; d += 4) {
+                        float k[4];
+                        quant_values<FORMAT>(*reinterpret_cast<const uint32_t*>(krow + d), k);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) dot = fmaf(qf[d + j], k[j], dot);
+                    }
+                } else {
+                    for (int d = 0; d < D; d++) dot = fmaf(qf[d], Quant<FORMAT>::template value<0>(krow[d]), dot);
+                }
                 s = dot * quant_scale(p.scales[0][block]) * a.scale_log2;
                 vs = quant_scale(p.scales[1][block]);
                 vrow = p.pool[1] + from;
@@ -75,10 +87,11 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
         const int n = min(256, keys.last - k0 + 1);
 #pragma unroll
         for (int i = 0; i < kDims; i++) {
-            const int d = tid + 256 * i;
-            if (d >= D) continue;
+            const int d = dim0 + 256 * i;
             acc[i] *= alpha;
-            for (int j = 0; j < n; j++)
+            if (group >= groups || d >= D) continue;
+#pragma unroll 4
+            for (int j = group; j < n; j += groups)
                 if (row[j]) acc[i] = fmaf(weight[j], Quant<FORMAT>::template value<0>(row[j][d]), acc[i]);
         }
     }
@@ -88,11 +101,24 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
     const double total = sums[0] + sums[1] + sums[2] + sums[3];
     const float inv = total == 0.0 ? 0.0f : 1.0f / static_cast<float>(total);
     const int64_t o0 = b * a.os[0] + h * a.os[1] + t * a.os[2];
+    if (groups > 1) {  // one dim a thread
+        weight[tid] = acc[0];
+        __syncthreads();
+        if (group == 0)
+            for (int g = 1; g < groups; g++) acc[0] += weight[g * lanes + dim0];
+    }
 #pragma unroll
     for (int i = 0; i < kDims; i++) {
-        const int d = tid + 256 * i;
-        if (d < D) Vec8<T>::store1(a.out, o0 + d * a.os[3], acc[i] * inv);
+        const int d = dim0 + 256 * i;
+        if (group == 0 && d < D) Vec8<T>::store1(a.out, o0 + d * a.os[3], acc[i] * inv);
     }
+}
+
+template <typename T, int FORMAT>
+void launch_general(const QuantAttnArgs& a, unsigned wgs, hipStream_t stream) {
+    const bool words = a.p.dim % 4 == 0 && reinterpret_cast<uintptr_t>(a.p.pool[0]) % 4 == 0;
+    if (words) hipLaunchKernelGGL((quant_attention_general_kernel<T, FORMAT, 4>), dim3(wgs), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((quant_attention_general_kernel<T, FORMAT, 1>), dim3(wgs), dim3(256), 0, stream, a);
 }
 
 // Whether a call of these sizes has rows enough for the prompt kernel.
@@ -150,8 +176,6 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     status = check_quant_pages(kc, vc, table, position_offsets, counts, q->dims[0], q->dims[2], e, &a.p);
     if (status) return status;
     if (numel(*q) == 0) return ok(e);
-    a.p.errw = device_error_word(e, &status);
-    if (status) return status;
     a.q = base_ptr(*q);
     a.out = base_ptr(*out);
     for (int i = 0; i < 4; i++) {
@@ -164,24 +188,22 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     a.group = a.hq / a.p.heads;
     a.group_magic = a.group == 1 ? UINT32_MAX : static_cast<uint32_t>((uint64_t{1} << 32) / static_cast<uint32_t>(a.group));
     a.f32 = q->dtype == SANDY_F32;
+    const bool tiles = quant_decode_takes(a);
+    const size_t need = tiles ? workspace_of(q, kc, table, window) : 0;
+    if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
+        return fail(e, SANDY_ERR_INVALID, "quant_paged attention needs a 16-byte aligned workspace of %zu bytes", need);
+    const int64_t wgs = q->dims[0] * q->dims[1] * q->dims[2];
+    if (!tiles && wgs > UINT32_MAX / 256) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged attention of too many queries");
+    a.p.errw = device_error_word(e, &status);
+    if (status) return status;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (quant_decode_takes(a)) {
-        const size_t need = workspace_of(q, kc, table, window);
-        if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
-            return fail(e, SANDY_ERR_INVALID, "quant_paged attention needs a 16-byte aligned workspace of %zu bytes", need);
+    if (tiles) {
         if (is_prompt(q, kc, table)) return launch_quant_prefill(a, kc->format, s, e);
         return launch_quant_decode(a, kc->format, workspace, s, e);
     }
-    const int64_t wgs = q->dims[0] * q->dims[1] * q->dims[2];
-    if (wgs > UINT32_MAX / 256) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged attention of too many queries");
-    const dim3 grid(static_cast<unsigned>(wgs));
-    if (kc->format == SANDY_QUANT_INT8) {
-        if (a.f32) hipLaunchKernelGGL((quant_attention_general_kernel<F32, SANDY_QUANT_INT8>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((quant_attention_general_kernel<BF16, SANDY_QUANT_INT8>), grid, dim3(256), 0, s, a);
-    } else {
-        if (a.f32) hipLaunchKernelGGL((quant_attention_general_kernel<F32, SANDY_QUANT_E4M3>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((quant_attention_general_kernel<BF16, SANDY_QUANT_E4M3>), grid, dim3(256), 0, s, a);
-    }
+    const unsigned n = static_cast<unsigned>(wgs);
+    if (kc->format == SANDY_QUANT_INT8) a.f32 ? launch_general<F32, SANDY_QUANT_INT8>(a, n, s) : launch_general<BF16, SANDY_QUANT_INT8>(a, n, s);
+    else a.f32 ? launch_general<F32, SANDY_QUANT_E4M3>(a, n, s) : launch_general<BF16, SANDY_QUANT_E4M3>(a, n, s);
     SANDY_HIP_TRY(hipGetLastError(), e, "quant_paged attention launch");
     return ok(e);
 }

@@ -33,8 +33,9 @@ int check_quant_pages(const SandyQuantCache* kc, const SandyQuantCache* vc, cons
             return fail(e, SANDY_ERR_INVALID, "quant_paged cache must have pages, heads and a head dim");
         if (!c->pool || !c->scales) return fail(e, SANDY_ERR_INVALID, "quant_paged cache pool or scales is null");
         if (c->page_size > (int64_t{1} << 30) || c->inner > (int64_t{1} << 30) || c->prefix > (int64_t{1} << 30) ||
-            c->page_size * c->inner > (int64_t{1} << 30) || c->num_pages > INT32_MAX)
-            return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged page of one head above 2^30 elements");
+            c->page_size * c->inner > (int64_t{1} << 30) || c->num_pages > INT32_MAX ||
+            c->num_pages * c->prefix > INT64_MAX / (c->page_size * c->inner))
+            return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged page of one head above 2^30 elements, or too many pages");
     }
     if (vc && (vc->format != kc->format || vc->page_size != kc->page_size || vc->prefix != kc->prefix ||
                vc->inner != kc->inner || vc->num_pages != kc->num_pages))
@@ -296,12 +297,10 @@ __global__ __launch_bounds__(256) void quant_read_kernel(ReadArgs a) {
 bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 template <typename T, int FORMAT>
-int launch_append(const AppendArgs& a, int64_t wgs, bool vec, Err e, hipStream_t stream) {
+int launch_append(const AppendArgs& a, int64_t wgs, bool vec, bool small, Err e, hipStream_t stream) {
     const dim3 grid(static_cast<unsigned>(wgs));
-    // a wave for a block of up to 256 pieces (all held in its registers), else four
-    const int64_t rows = std::min<int64_t>(a.p.tokens, int64_t{1} << a.p.log2_page);
     if (!vec) hipLaunchKernelGGL((quant_append_kernel<T, FORMAT, 1, 256>), grid, dim3(256), 0, stream, a);
-    else if (rows * a.p.dim <= 256 * 8) hipLaunchKernelGGL((quant_append_kernel<T, FORMAT, 8, 64>), grid, dim3(64), 0, stream, a);
+    else if (small) hipLaunchKernelGGL((quant_append_kernel<T, FORMAT, 8, 64>), grid, dim3(64), 0, stream, a);
     else hipLaunchKernelGGL((quant_append_kernel<T, FORMAT, 8, 256>), grid, dim3(256), 0, stream, a);
     SANDY_HIP_TRY(hipGetLastError(), e, "quant_paged append launch");
     return ok(e);
@@ -337,7 +336,12 @@ extern "C" int sandy_hip_quant_paged_append(const SandyTensor* k, const SandyTen
     if (status) return status;
     if (k->dims[1] != kc->prefix || k->dims[3] != kc->inner)
         return fail(e, SANDY_ERR_INVALID, "quant_paged append rows must have the cache's heads and head dim");
-    if (vc && (vc->pool == kc->pool || vc->scales == kc->scales))
+    auto overlap = [](const void* x, const void* y, int64_t bytes) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+        return (a < b ? b - a : a - b) < static_cast<uintptr_t>(bytes);
+    };
+    const int64_t blocks = kc->num_pages * kc->prefix;
+    if (vc && (overlap(kc->pool, vc->pool, blocks * kc->page_size * kc->inner) || overlap(kc->scales, vc->scales, blocks)))
         return fail(e, SANDY_ERR_INVALID, "quant_paged append k and v caches must not share memory");
     if (numel(*k) == 0) return ok(e);
     a.p.errw = device_error_word(e, &status);
@@ -357,14 +361,16 @@ extern "C" int sandy_hip_quant_paged_append(const SandyTensor* k, const SandyTen
     const int64_t page = int64_t{1} << a.p.log2_page;
     const int64_t ordinals = (a.p.tokens + page - 2) / page + 1;
     const int64_t wgs = ordinals * a.p.heads * a.p.batch * (v ? 2 : 1);
-    if (wgs * 256 > UINT32_MAX) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged append of too many blocks");
+    // a wave for a block of up to 256 pieces (all held in its registers), else four
+    const bool small = vec && std::min<int64_t>(a.p.tokens, page) * a.p.dim <= 256 * 8;
+    if (wgs > UINT32_MAX / (small ? 64 : 256)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged append of too many blocks");
     a.ordinals = static_cast<int32_t>(ordinals);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (k->dtype == SANDY_BF16)
-        return kc->format == SANDY_QUANT_INT8 ? launch_append<BF16, SANDY_QUANT_INT8>(a, wgs, vec, e, s)
-                                              : launch_append<BF16, SANDY_QUANT_E4M3>(a, wgs, vec, e, s);
-    return kc->format == SANDY_QUANT_INT8 ? launch_append<F32, SANDY_QUANT_INT8>(a, wgs, vec, e, s)
-                                          : launch_append<F32, SANDY_QUANT_E4M3>(a, wgs, vec, e, s);
+        return kc->format == SANDY_QUANT_INT8 ? launch_append<BF16, SANDY_QUANT_INT8>(a, wgs, vec, small, e, s)
+                                              : launch_append<BF16, SANDY_QUANT_E4M3>(a, wgs, vec, small, e, s);
+    return kc->format == SANDY_QUANT_INT8 ? launch_append<F32, SANDY_QUANT_INT8>(a, wgs, vec, small, e, s)
+                                          : launch_append<F32, SANDY_QUANT_E4M3>(a, wgs, vec, small, e, s);
 }
 
 extern "C" int sandy_hip_quant_paged_read(const SandyQuantCache* kc, const SandyQuantCache* vc,

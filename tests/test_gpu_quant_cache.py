@@ -415,6 +415,86 @@ def test_attention_records(ops):
         check(ops, q, kc, vc, table, [20, 20, 100])
 
 
+@pytest.mark.parametrize("merge_kernel", [0, 1])
+@pytest.mark.parametrize("splits", [1, 2, 5, 17, 40, 256])
+def test_splits(ops, monkeypatch, splits, merge_kernel):
+    """Every number of splits, joined by the last workgroup (in one group of 16 or
+    several) or by the merge kernel; a second call finds the counters as the first."""
+    ops._quant_workspace.cache_clear()
+    monkeypatch.setenv("SANDY_QUANT_SPLITS", str(splits))
+    monkeypatch.setenv("SANDY_QUANT_MERGE_KERNEL", str(merge_kernel))
+    r = rng(splits)
+    ctx = [9000, 3, 1100, 40]
+    for dim, T, dtype in ((64, 1, BF16), (256, 1, BF16), (128, 5, BF16), (64, 2, F32)):
+        table, kc, vc = filled(ops, r, ctx, 2, dim, 16, "int8", 5)
+        q = from_f32(r.standard_normal((4, 8, T, dim)).astype(np.float32), dtype)
+        pos = [max(0, c - T) for c in ctx]
+        first = check(ops, q, kc, vc, table, pos, counts=[T, min(T, 3), T, T])
+        assert torch.equal(first, check(ops, q, kc, vc, table, pos, counts=[T, min(T, 3), T, T]))
+    ops._quant_workspace.cache_clear()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("hq,heads,dim,rows,T,window", [(32, 4, 64, 16, 37, 0), (8, 2, 256, 16, 21, 16), (16, 2, 128, 32, 70, 50),
+                                                        (10, 2, 96, 64, 33, 0), (6, 3, 80, 16, 65, 40), (34, 2, 192, 16, 3, 9),
+                                                        (4, 4, 64, 16, 130, 0), (3, 1, 16, 16, 11, 0)])
+def test_prompt_tiles_of_short_chunks(ops, monkeypatch, hq, heads, dim, rows, T, window, fmt, dtype):
+    """The prompt kernel on rows that do not fill a tile, ragged and windowed."""
+    ops._quant_workspace.cache_clear()
+    monkeypatch.setenv("SANDY_QUANT_PROMPT_WGS", "1")
+    r = rng(T + dim)
+    pos, counts = [0, 3, 100, 257, 40], [T, max(1, T - 5), T, (T + 1) // 2, 0]
+    table, kc, vc = filled(ops, r, [max(p + c, 1) for p, c in zip(pos, counts)], heads, dim, rows, fmt, T)
+    kc.scales[int(table[2, 1])] = 255  # keys the later queries of the third sequence see
+    q = from_f32(r.standard_normal((5, T, hq, dim)).astype(np.float32), dtype).transpose(1, 2)
+    check(ops, q, kc, vc, table, pos, counts, window)
+    ops._quant_workspace.cache_clear()
+
+
+@pytest.mark.parametrize("T,dim", [(1, 64), (300, 64), (3, 128), (2, 36)])
+def test_far_positions_and_windows(ops, T, dim):
+    """Positions past the block table see what it covers, windows of any size."""
+    r = rng(47)
+    table, kc, vc = filled(ops, r, [64, 64], 2, dim, 16, "int8", 3)
+    q = from_f32(r.standard_normal((2, 8, T, dim)).astype(np.float32), BF16)
+    far = 2 ** 63 - 1
+    whole = check(ops, q, kc, vc, table, [63, 64])
+    for pos, window in (([far, far], far), ([far, 70], 0), ([2 ** 31, 2 ** 40], 2 ** 40 + 1), ([63, 64], far), ([70, 64], 2 ** 31)):
+        got = ops.quant_paged_attention(q, kc, vc, cuda(table), cuda(np.array(pos)), window=window)
+        ops.check_device_errors()
+        for b in range(2):
+            for i in sorted({0, T // 2, min(63, T - 1), min(64, T - 1), T - 1}):
+                last = min(pos[b] + i, 63)
+                first = max(0, pos[b] + i + 1 - window) if window else 0
+                if first > last:
+                    assert not got[b, :, i].any()
+                    continue
+                want, slack = R.attention(f64(q)[b:b + 1, :, i:i + 1], R.Cache.of(kc), R.Cache.of(vc), table[b:b + 1], [last], [1],
+                                          last - first + 1, -1.0, WEIGHT)
+                R.assert_attention(got[b:b + 1, :, i:i + 1], want, slack, f"{pos} {window} {b} {i}")
+        if pos == [63, 64]:
+            assert torch.equal(got, whole)
+    # windows that leave the table nothing
+    got = ops.quant_paged_attention(q, kc, vc, cuda(table), cuda(np.array([200, far])), window=100)
+    assert not got.any()
+    ops.check_device_errors()
+
+
+def test_many_sequences(ops):
+    """More row tiles than 2^16."""
+    r = rng(91)
+    B, hq, heads, dim, T = 9000, 16, 8, 64, 9
+    table, kc, vc = filled(ops, r, [T] * 16, heads, dim, 16, "e4m3", 3)
+    gt = cuda(table).repeat(B // 16 + 1, 1)[:B].contiguous()
+    q = torch.randn(B, hq, T, dim, device="cuda", generator=torch.Generator("cuda").manual_seed(1)).to(BF16)
+    got = ops.quant_paged_attention(q, kc, vc, gt, torch.zeros(B, dtype=torch.int32, device="cuda"))
+    ops.check_device_errors()
+    pick = [0, 15, 4097, B - 1]
+    want, slack = R.attention(f64(q[pick]), R.Cache.of(kc), R.Cache.of(vc), table[[b % 16 for b in pick]], [0] * 4, [T] * 4, 0, -1.0, WEIGHT)
+    R.assert_attention(got[pick], want, slack)
+
+
 def test_deterministic(ops):
     r = rng(51)
     table, kc, vc = filled(ops, r, [4000, 900], 4, 64, 16, "e4m3", 3)

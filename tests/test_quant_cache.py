@@ -52,6 +52,8 @@ def test_append_refusals():
         (dict(k=tensor((3, 4, 5, 64))), "the cache's heads and head dim"),
         (dict(k=tensor((3, 2, 5, 32))), "the cache's heads and head dim"),
         (dict(vc=cache()), "must not share memory"),
+        (dict(vc=cache(pool=0x100000 + 8 * 2 * 16 * 64 - 1, scales=0x400000)), "must not share memory"),
+        (dict(vc=cache(pool=0x300000, scales=0x200000 - 15)), "must not share memory"),
         (dict(vc=other(format=1)), "same format and shape"),
         (dict(vc=other(num_pages=9)), "same format and shape"),
         (dict(kc=cache(format=2)), "int8 or e4m3"),
@@ -62,6 +64,7 @@ def test_append_refusals():
         (dict(kc=cache(pool=0)), "pool or scales is null"),
         (dict(kc=cache(scales=0)), "pool or scales is null"),
         (dict(kc=cache(page_size=1 << 25)), "above 2\\^30 elements"),
+        (dict(kc=cache(prefix=1 << 30, num_pages=(1 << 31) - 1)), "too many pages"),
         (dict(table=tensor((2, 4), _lib.I32)), "block table must be"),
         (dict(table=tensor((3, 4), _lib.I64)), "block table must be"),
         (dict(table=tensor((3, 4), _lib.I32, strides=(1, 3))), "block table must be"),
@@ -118,6 +121,30 @@ def test_attention_refusals():
     ]:
         with pytest.raises(_lib.SandyError, match=message):
             attend(**kw)
+
+
+def test_attention_workspace_refusals():
+    """The workspace a call of these sizes needs, and calls that bring less."""
+    need = ctypes.c_size_t(7)
+
+    def query(q, kc=None, table=TABLE):
+        _lib.dcall("sandy_hip_quant_paged_attention_workspace", q, kc or cache(), table, 0, ctypes.byref(need))
+        return need.value
+
+    assert query(tensor((3, 4, 1, 64))) == 0          # 64 keys: one workgroup a head
+    assert query(tensor((3, 4, 0, 64))) == 0
+    wide = tensor((3, 4096), _lib.I32)
+    bytes_ = query(tensor((3, 4, 1, 64)), table=wide)
+    assert bytes_ > 0 and bytes_ % 16 == 0
+    assert query(tensor((3, 4, 1, 20)), cache(inner=20), wide) == 0  # the general kernel needs none
+    for work, size in ((None, 0), (0x10000, bytes_ - 1), (0x10008, bytes_)):
+        with pytest.raises(_lib.SandyError, match=f"workspace of {bytes_} bytes"):
+            _lib.call("sandy_hip_quant_paged_attention", tensor((3, 4, 1, 64)), cache(), other(), wide, POS, None, 0, -1.0,
+                      tensor((3, 4, 1, 64)), work, size, stream=0)
+    with pytest.raises(_lib.SandyError, match="divisible by kv_heads"):
+        query(tensor((3, 5, 1, 64)))
+    with pytest.raises(_lib.SandyError, match="requires a block table"):
+        query(tensor((3, 4, 1, 64)), table=tensor((3,), _lib.I32))
 
 
 def test_python_refusals():
