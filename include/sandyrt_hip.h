@@ -396,8 +396,8 @@ int sandy_hip_paged_attention_noalloc(const SandyTensor* q, const SandyPagedCach
  * starts its block anew.  New values that are not finite (or above 127 * 2^121 for
  * int8, 448 * 2^119 for e4m3, next to 2^128) make the block's scale NaN (c =
  * 255, until it starts anew) with payload 0.  Rows of a page
- * past the last one written are left as they were.  Sequences that write to
- * the same page in one call race on it.  Rows outside the block table are
+ * past the last one written are left as they were.  A page that one call
+ * writes twice (two sequences, or one whose table names it twice) is raced on.  Rows outside the block table are
  * recorded (SANDY_DEVERR_QUANT_ROWS) and that sequence writes nothing.
  */
 int sandy_hip_quant_paged_append(const SandyTensor* k, const SandyTensor* v, const SandyQuantCache* k_cache,

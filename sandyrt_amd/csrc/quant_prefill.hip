@@ -10,6 +10,15 @@
 // multiplies the scores in the multiply-add of their exponents, V's the weights
 // (int8) or the conversion (e4m3).  bf16 queries' weights enter as two bf16 numbers
 // (2^-15), f32 queries and weights as three (exact).
+//
+// 2048 queries of 32 / 4 heads of 64 (e4m3, causal) take 43 to 49 us, 350 to 400
+// TFLOP/s; int8 57 us where e4m3 takes 46 (three instructions convert two payloads, one
+// of e4m3's).  No single unit bounds it: vector instructions issue in 67 % of the
+// cycles, MFMA in 23 %; without the loads it is 13 % faster, without the exponentials
+// 8 %, without the second product 13 %, without the transposing reads 2 %.  Weights in
+// one part would be 5 to 12 % faster, at bf16's own error.  Slower: K in LDS tiles for several waves (52 to 57 us),
+// two row tiles a wave (D 128 34 us against 20), the keys split over workgroups as
+// well (69 against 45).
 #include "quant_mfma.h"
 
 #include <algorithm>
@@ -38,7 +47,9 @@ struct PromptGeo {
 };
 
 // Workgroup i's place in the list by falling length: every second round of the
-// 256 CUs backwards, so that the workgroups a CU gets add up to about the same.
+// 256 CUs backwards, so that the workgroups a CU gets add up to about the same (1024
+// queries 16.5 us so and 18.0 in order, 4 chunks of 700 of D 128 40.7 and 43.8, 8 of
+// 300 behind 100 to 2000 keys 47.5 and 53.5).
 __device__ __forceinline__ uint32_t snake(uint32_t i, uint32_t n) {
     const uint32_t round = i & ~255u;
     return (i & 256) ? round + min(256u, n - round) - 1 - (i - round) : i;

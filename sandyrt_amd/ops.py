@@ -512,6 +512,8 @@ def quant_paged_read(k_cache: QuantPagedCache, v_cache: QuantPagedCache, block_t
         pool = cache.pool
         return torch.empty((block_table.shape[0], pool.shape[1], tokens, pool.shape[3]), dtype=dtype, device=pool.device)
 
+    if k_out is not None and k_out.shape[2:3] != (tokens,):
+        raise SandyError(1, "quant_paged read outputs must have the call's rows")
     kc, vc = _packed(k_cache), _packed(v_cache)
     k_out, v_out = output(k_cache, k_out), output(v_cache, v_out)
     tensors = [k_out, v_out, block_table, position_offsets, counts, k_cache.scales]

@@ -147,6 +147,36 @@ def test_attention_workspace_refusals():
         query(tensor((3, 4, 1, 64)), table=tensor((3,), _lib.I32))
 
 
+def test_sizes_past_the_indices():
+    """Views that repeat memory: counts past 32 bits, products past 64."""
+    big = 1 << 30
+    pos, table = tensor((1,), _lib.I64), tensor((1, 4), _lib.I32)
+    many = 1 << 31
+    for k, kc, tab, at in [
+        (tensor((1, 2, big + 1, 64)), cache(), table, pos),
+        (tensor((many, 2, 1, 64)), cache(), tensor((many, 4), _lib.I32), tensor((many,), _lib.I64)),
+        (tensor((many - 1, 2, big, 64)), cache(), tensor((many - 1, 4), _lib.I32), tensor((many - 1,), _lib.I64)),
+    ]:
+        with pytest.raises(_lib.SandyError, match="too large"):
+            _lib.call("sandy_hip_quant_paged_append", k, None, kc, None, tab, at, None, stream=0)
+        with pytest.raises(_lib.SandyError, match="too large"):
+            _lib.call("sandy_hip_quant_paged_read", kc, None, tab, at, None, k, None, stream=0)
+    need = ctypes.c_size_t(0)
+    for shape in [(1, 2 * big + 2, 1, 64), (1, 4, big + 1, 64), (many, 4, 1, 64), (1 << 30, 1 << 28, 1 << 10, 64)]:
+        q = tensor(shape)
+        with pytest.raises(_lib.SandyError, match="too large"):
+            _lib.dcall("sandy_hip_quant_paged_attention_workspace", q, cache(), table, 0, ctypes.byref(need))
+        with pytest.raises(_lib.SandyError, match="too large"):
+            _lib.call("sandy_hip_quant_paged_attention", q, cache(), other(), table, pos, None, 0, -1.0, q, None, 0, stream=0)
+
+
+def test_read_outputs_of_other_lengths():
+    c = ops.QuantPagedCache.empty(4, 2, 16, 64, device="cpu")
+    table, pos = torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int64)
+    with pytest.raises(_lib.SandyError, match="the call's rows"):
+        ops.quant_paged_read(c, None, table, pos, 3, k_out=torch.zeros(1, 2, 4, 64))
+
+
 def test_python_refusals():
     pool, scales = torch.zeros(4, 2, 16, 64, dtype=torch.int8), torch.zeros(4, 2, dtype=torch.uint8)
     with pytest.raises(_lib.SandyError, match="int8 or e4m3"):
