@@ -42,8 +42,13 @@ struct PromptGeo {
     static constexpr int DT = DP / 32;  // 32-dim tiles of O^T
     static constexpr int kV = 32 * VP;
     static constexpr int kMerge = 4 * 16 * 64 * 4;  // one 32-dim tile of every wave
-    static constexpr int kBytes = std::max(4 * kV, kMerge) + 4 * 32 * 8;
-    static constexpr int kWaves = DP == 64 ? (kF32 ? 3 : 4) : DP == 128 ? 2 : 1;  // a SIMD
+    static constexpr int NQ = kF32 ? 3 : 1, KS = DP / 16;
+    // Q in LDS, once for the four waves: two waves a SIMD then hold the rest in their 256
+    // registers (3000 queries of 8 / 2 heads: 77 us, with Q in one wave's 512 98)
+    static constexpr bool kQLds = DP == 256;
+    static constexpr int kQ = kQLds ? NQ * KS * 64 * 16 : 0;
+    static constexpr int kBytes = std::max(4 * kV, kMerge) + 4 * 32 * 8 + kQ;
+    static constexpr int kWaves = DP == 64 ? (kF32 ? 3 : 4) : 2;  // a SIMD
 };
 
 // Workgroup i's place in the list by falling length: every second round of the
@@ -55,21 +60,22 @@ __device__ __forceinline__ uint32_t snake(uint32_t i, uint32_t n) {
     return (i & 256) ? round + min(256u, n - round) - 1 - (i - round) : i;
 }
 
-template <typename T, int FORMAT, int DP>
+// EXACT: the head dim is DP itself, so that K's addresses are one and constants (D 256:
+// registers again)
+template <typename T, int FORMAT, int DP, bool EXACT>
 __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant_prompt_kernel(PromptArgs pa) {
     using G = PromptGeo<T, FORMAT, DP>;
     constexpr bool kF32 = G::kF32;
-    constexpr int NQ = kF32 ? 3 : 1, NP = kF32 ? 3 : 2, KS = DP / 16, DT = G::DT;
+    constexpr int NQ = G::NQ, NP = kF32 ? 3 : 2, KS = G::KS, DT = G::DT;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const QuantAttnArgs& a = pa.a;
     const QuantPages& p = a.p;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int D = p.dim;
-    // heads vary fastest (an XCD serves few), the longest row blocks come first; where
-    // one workgroup fits a CU the next to end takes the next (D 256: 58 us against 70)
-    uint32_t at = DP == 256 ? blockIdx.x : snake(blockIdx.x, gridDim.x);
+    const int D = EXACT ? DP : p.dim;
+    // heads vary fastest (an XCD serves few), the longest row blocks come first
+    uint32_t at = snake(blockIdx.x, gridDim.x);
     const int kh = at % p.heads;
     at /= p.heads;
     const int b = at % p.batch;
@@ -94,10 +100,10 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
     KeyRange mine = seq.of(qt);
     if (qt >= count) mine.last = -1;
     // B operands of Q^T: row, dims 32 (s / 2) + 16 half + 8 (s & 1) .. + 7 in step s, zeros past D
-    u32x4_t qv[NQ][KS];
+    u32x4_t qv[G::kQLds ? 1 : NQ][G::kQLds ? 1 : KS];
+    u32x4_t* q_lds = reinterpret_cast<u32x4_t*>(lds + G::kBytes - G::kQ);  // [NQ][KS][lane]
     const int64_t q0 = b * a.qs[0] + (kh * a.group + qg) * a.qs[1] + qt * a.qs[2];
-#pragma unroll
-    for (int s = 0; s < KS; s++) {
+    auto query = [&](int s, u32x4_t (&v)[NQ]) {
         const int d = 32 * (s >> 1) + 16 * half + 8 * (s & 1);
         if constexpr (kF32) {
             float x[8];
@@ -107,11 +113,29 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
                 uint32_t part[3];
                 split_pair<3>(d < D ? x[2 * i] : 0.0f, d < D ? x[2 * i + 1] : 0.0f, part);
 #pragma unroll
-                for (int n = 0; n < 3; n++) qv[n][s][i] = part[n];
+                for (int n = 0; n < 3; n++) v[n][i] = part[n];
             }
         } else {
-            qv[0][s] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + q0 + (d < D ? d : 0));
-            if (d >= D) qv[0][s] = u32x4_t{0, 0, 0, 0};
+            v[0] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.q) + q0 + (d < D ? d : 0));
+            if (d >= D) v[0] = u32x4_t{0, 0, 0, 0};
+        }
+    };
+    if constexpr (G::kQLds) {  // the same for the four waves: each fetches a quarter
+#pragma unroll
+        for (int s = 0; s < KS / 4; s++) {
+            u32x4_t v[NQ];
+            query(4 * s + wave, v);
+#pragma unroll
+            for (int n = 0; n < NQ; n++) q_lds[(n * KS + 4 * s + wave) * 64 + lane] = v[n];
+        }
+        __syncthreads();
+    } else {
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            u32x4_t v[NQ];
+            query(s, v);
+#pragma unroll
+            for (int n = 0; n < NQ; n++) qv[n][s] = v[n];
         }
     }
 
@@ -125,7 +149,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
     unsigned char* vrows = lds + wave * G::kV;
     int k_off[G::KP], v_to[G::NV];
 #pragma unroll
-    for (int j = 0; j < G::KP; j++) k_off[j] = (lane & 15) * D + (32 * j + 16 * half < D ? 32 * j + 16 * half : 0);
+    for (int j = 0; j < G::KP; j++) k_off[j] = EXACT || 32 * j + 16 * half < D ? 32 * j : -16 * half;
 #pragma unroll
     for (int j = 0; j < G::NV; j++) {
         const int piece = lane + 64 * j, per_row = D / 16;
@@ -158,7 +182,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         }
         // K: a lane's key is in the first or the second tile (one without a page: page 0's
         // bytes, masked)
-        const uint8_t* kp = p.pool[0] + ((lane & 16) ? off[1] : off[0]);
+        const uint8_t* kp = p.pool[0] + ((lane & 16) ? off[1] : off[0]) + ((lane & 15) * D + 16 * half);
 #pragma unroll
         for (int j = 0; j < G::KP; j++) kr[j] = *reinterpret_cast<const u32x4_t*>(kp + k_off[j]);
     };
@@ -183,8 +207,14 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         for (int s = 0; s < KS; s++) {
             const bf16x8_t ka = payload_operand<FORMAT>(kr[s >> 1][2 * (s & 1)], kr[s >> 1][2 * (s & 1) + 1], 1.0f, 1.0f);
 #pragma unroll
-            for (int i = NQ - 1; i >= 0; i--)
-                sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qv[i][s]), sc, 0, 0, 0);
+            for (int i = NQ - 1; i >= 0; i--) {
+                u32x4_t qi;
+                if constexpr (G::kQLds) qi = q_lds[(i * KS + s) * 64 + lane];
+                else qi = qv[i][s];
+                sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qi), sc, 0, 0, 0);
+            }
+            // int8's conversions all at once would not leave registers for two waves (42 us, 55)
+            if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int h = 0; h < 2; h++)
@@ -267,6 +297,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
 #pragma unroll
                 for (int i = NP - 1; i >= 0; i--)
                     acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8_t, parts[i]), acc[t], 0, 0, 0);
+                if (DP == 256 && t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -319,8 +350,9 @@ int launch_dim(const QuantAttnArgs& a, hipStream_t stream, Err e) {
     pa.row_blocks = static_cast<int32_t>((static_cast<int64_t>(a.group) * a.p.tokens + kRows - 1) / kRows);
     const int64_t wgs = static_cast<int64_t>(pa.row_blocks) * a.p.batch * a.p.heads;
     void* params[] = {&pa};
-    SANDY_HIP_TRY(hipLaunchKernel(reinterpret_cast<const void*>(&quant_prompt_kernel<T, FORMAT, DP>),
-                                  dim3(static_cast<unsigned>(wgs)), dim3(256), params, G::kBytes, stream), e,
+    const void* kernel = a.p.dim == DP ? reinterpret_cast<const void*>(&quant_prompt_kernel<T, FORMAT, DP, true>)
+                                       : reinterpret_cast<const void*>(&quant_prompt_kernel<T, FORMAT, DP, false>);
+    SANDY_HIP_TRY(hipLaunchKernel(kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), params, G::kBytes, stream), e,
                   "quant_paged attention launch");
     return ok(e);
 }
@@ -335,15 +367,15 @@ int launch_format(const QuantAttnArgs& a, hipStream_t stream, Err e) {
 
 } // namespace
 
-// From one workgroup a CU on (D 256, one a CU at a time: a quarter more); fewer leave
-// the chip to the 16-row tiles and their splits.  us, 16-row tiles / here, by the
-// number of workgroups: D 64 128 (behind 4000 keys) 22 / 29, 256 6.4 / 6.9, 512 10.5 /
-// 9.1 and behind 2000 keys 34 / 27, 2048 62 / 43; D 128 256 12.9 / 11.3, 512 55 / 33;
-// D 256 128 12.5 / 19.7, 256 27.5 / 29, 375 47 / 42, 512 68 / 58; f32, D 64, 48 5.5 /
-// 7.1, 120 9.5 / 9.2, 384 17.8 / 16.7.
+// From one workgroup a CU on; fewer leave the chip to the 16-row tiles and their
+// splits.  us, 16-row tiles / here, by the number of workgroups: D 64 128 (behind 4000
+// keys) 22 / 29, 256 6.4 / 6.9, 512 10.5 / 9.1 and behind 2000 keys 34 / 27, 2048 62 /
+// 43; D 128 256 12.9 / 11.3, 512 55 / 33; D 256 104 (2500 keys) 38 / 45, 192 17.5 / 18.5,
+// 256 23.5 / 22.9 and of 2400 keys 50 / 42, 300 47 / 38; f32, D 64, 48 5.5 / 7.1, 120
+// 9.5 / 9.2, 384 17.8 / 16.7.
 bool quant_prefill_takes(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t max_blocks, bool f32) {
     const int64_t wgs = (hq / heads * tokens + kRows - 1) / kRows * batch * heads;
-    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", dim > 128 ? 320 : 256);
+    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", 256);
     return tokens > 1 && wgs >= from && (!f32 || dim <= 128) && max_blocks > 0;
 }
 
