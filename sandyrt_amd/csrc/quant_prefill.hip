@@ -367,15 +367,16 @@ int launch_format(const QuantAttnArgs& a, hipStream_t stream, Err e) {
 
 } // namespace
 
-// From one workgroup a CU on; fewer leave the chip to the 16-row tiles and their
-// splits.  us, 16-row tiles / here, by the number of workgroups: D 64 128 (behind 4000
-// keys) 22 / 29, 256 6.4 / 6.9, 512 10.5 / 9.1 and behind 2000 keys 34 / 27, 2048 62 /
-// 43; D 128 256 12.9 / 11.3, 512 55 / 33; D 256 104 (2500 keys) 38 / 45, 192 17.5 / 18.5,
-// 256 23.5 / 22.9 and of 2400 keys 50 / 42, 300 47 / 38; f32, D 64, 48 5.5 / 7.1, 120
-// 9.5 / 9.2, 384 17.8 / 16.7.
+// From about as many workgroups on as fill half the chip's waves; fewer leave it to the
+// 16-row tiles and their splits.  us, 16-row tiles / here, by the number of workgroups,
+// no / 1000 / 4000 keys before the chunk: D 64 128 5.0 / 5.7, 11.7 / 11.4, 21.7 / 28.5,
+// 192 6.3 / 6.3, 14.3 / 12.4, 28.3 / 29.6, 2048 62 / 43 with none; D 128 96 7.0 / 7.8, 24.2
+// / 15.1, 38.9 / 35.2, 128 11.1 / 8.1, 18.0 / 15.8, 33.7 / 36.9, 160 15.8 / 9.0, 29.6 /
+// 16.6, 49.6 / 37.8; f32 128 12.3 / 10.5, 20.6 / 22.9, 39.5 / 57.8, 192 19.3 / 12.1, 35.5 /
+// 25.0, 57.6 / 60.3; D 256 192 17.5 / 18.5, 256 23.5 / 22.9, of 2400 keys 50 / 42, 300 47 / 38.
 bool quant_prefill_takes(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t max_blocks, bool f32) {
     const int64_t wgs = (hq / heads * tokens + kRows - 1) / kRows * batch * heads;
-    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", 256);
+    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", dim > 128 ? 256 : dim > 64 && !f32 ? 128 : 192);
     return tokens > 1 && wgs >= from && (!f32 || dim <= 128) && max_blocks > 0;
 }
 
