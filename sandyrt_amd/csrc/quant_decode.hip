@@ -48,14 +48,15 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int D = p.dim;
-    // heads vary fastest, then sequences, splits, column tiles
+    // heads vary fastest, then sequences, column tiles, splits: those without keys come last,
+    // not between the others on the same XCDs
     uint32_t at = blockIdx.x;
     const int kh = at % p.heads;
     at /= p.heads;
     const int b = at % p.batch;
     at /= p.batch;
-    const int split = at % da.splits;
-    const int ct = at / da.splits;
+    const int ct = at % da.col_tiles;
+    const int split = at / da.col_tiles;
     const int rows = a.group * p.tokens;
     const int64_t pos = load_index(p.pos, p.pos_dt, b);
     const int count = pos < 0 ? 0 : quant_count(p, b);
@@ -324,11 +325,6 @@ int launch_format(const SplitArgs& d, hipStream_t stream, Err e) {
     return launch_dim<T, FORMAT, 256>(d, stream, e);
 }
 
-// Workgroups wanted: us at a target of 256 / 512 / 1024, D 64, 32 sequences 16.6 /
-// 15.2 / 15.3, one of 32749 keys 14.6 / 14.8 / 17.3; D 256, 64 sequences 20.2 / 21.2 /
-// 26.3.
-int64_t target_of(int64_t dim) { return dim > 128 ? 256 : 512; }
-
 } // namespace
 
 bool quant_decode_takes(const QuantAttnArgs& a) {
@@ -351,8 +347,9 @@ bool quant_decode_takes(const QuantAttnArgs& a) {
 size_t quant_decode_workspace(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t page,
                               int64_t max_blocks, int64_t window) {
     const int64_t units = (hq / heads * tokens + 15) / 16 * batch * heads;
-    const int64_t splits = split_count(units, target_of(dim), max_blocks * page, window, tokens);
-    return splits == 1 ? 0 : static_cast<size_t>(units * splits * 16 * (dim + 2)) * sizeof(float);
+    SplitArgs d{};
+    set_splits(&d, units, dim, max_blocks * page, window, tokens);
+    return d.splits == 1 ? 0 : static_cast<size_t>(units * d.splits * 16 * (dim + 2)) * sizeof(float);
 }
 
 int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace, hipStream_t stream, Err e) {
@@ -360,8 +357,8 @@ int launch_quant_decode(const QuantAttnArgs& a, int32_t format, void* workspace,
     SplitArgs d{};
     d.a = a;
     d.col_tiles = (a.group * p.tokens + 15) / 16;
-    d.splits = split_count(static_cast<int64_t>(p.batch) * p.heads * d.col_tiles, target_of(p.dim),
-                           static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens);
+    set_splits(&d, static_cast<int64_t>(p.batch) * p.heads * d.col_tiles, p.dim,
+               static_cast<int64_t>(p.max_blocks) << p.log2_page, a.window, p.tokens);
     const int status = split_memory<16>(&d, workspace, stream, e);
     if (status) return status;
     if (format == SANDY_QUANT_INT8)

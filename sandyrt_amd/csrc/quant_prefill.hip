@@ -367,16 +367,17 @@ int launch_format(const QuantAttnArgs& a, hipStream_t stream, Err e) {
 
 } // namespace
 
-// From about as many workgroups on as fill half the chip's waves; fewer leave it to the
-// 16-row tiles and their splits.  us, 16-row tiles / here, by the number of workgroups,
-// no / 1000 / 4000 keys before the chunk: D 64 128 5.0 / 5.7, 11.7 / 11.4, 21.7 / 28.5,
-// 192 6.3 / 6.3, 14.3 / 12.4, 28.3 / 29.6, 2048 62 / 43 with none; D 128 96 7.0 / 7.8, 24.2
-// / 15.1, 38.9 / 35.2, 128 11.1 / 8.1, 18.0 / 15.8, 33.7 / 36.9, 160 15.8 / 9.0, 29.6 /
-// 16.6, 49.6 / 37.8; f32 128 12.3 / 10.5, 20.6 / 22.9, 39.5 / 57.8, 192 19.3 / 12.1, 35.5 /
-// 25.0, 57.6 / 60.3; D 256 192 17.5 / 18.5, 256 23.5 / 22.9, of 2400 keys 50 / 42, 300 47 / 38.
+// From more than half a workgroup a CU on; fewer leave the chip to the 16-row tiles and
+// their splits.  us, 16-row tiles / here, by the number of workgroups, no / 1000 / 4000
+// keys before the chunk: D 64 160 5.9 / 6.1, 14.0 / 11.9, 24.6 / 28.9, 192 6.1 / 6.2, 14.4 /
+// 12.1, 27.2 / 28.9, 224 6.3 / 6.3, 15.2 / 12.3, 32.3 / 29.4; D 128 128 7.2 / 8.1, 14.1 / 15.6,
+// 34.7 / 36.1, 160 8.6 / 8.9, 19.7 / 16.6, 46.5 / 38.4; f32 192 10.7 / 11.9, 23.4 / 24.3, 54.2
+// / 58.1, 224 12.1 / 13.3, 24.9 / 26.0, 66.4 / 59.6, of D 64 256 10.5 / 11.3, 24.4 / 19.8,
+// 43.9 / 42.3; D 256 192 17.6 / 18.5, 256 23.3 / 22.2,
+// of 2400 keys 54.5 / 41.1.
 bool quant_prefill_takes(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t max_blocks, bool f32) {
     const int64_t wgs = (hq / heads * tokens + kRows - 1) / kRows * batch * heads;
-    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", dim > 128 ? 256 : dim > 64 && !f32 ? 128 : 192);
+    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", dim > 128 || f32 ? 256 : dim > 64 ? 160 : 192);
     return tokens > 1 && wgs >= from && (!f32 || dim <= 128) && max_blocks > 0;
 }
 

@@ -16,14 +16,19 @@ struct SplitArgs {
     QuantAttnArgs a;
     int32_t col_tiles;  // tiles of COLS columns of the (query, head) rows of a kv head
     int32_t splits;     // workgroups a column tile's keys may be split over
+    int32_t few;        // and are, up to long_pairs each
+    int32_t long_pairs;
     float* part_o;      // [unit, split][COLS][D] sums relative to the maximum
     float* part_ml;     // [unit, split][COLS][2] maximum and sum of weights
-    uint32_t* arrived;  // [unit][counters_of(splits)] zero between calls, or null: the merge kernel joins the splits
+    uint32_t* arrived;  // [unit][counters_of(splits)][kCounterWords] zero between calls, or null: the merge kernel joins the splits
 };
 
 // Splits are joined by the last workgroup to arrive, in groups of 16 and then
 // the groups: a unit's counters are one for the groups (or the only group) and,
-// where there are several, one for each.
+// where there are several, one for each.  Each has 32 bytes of its own: next to each
+// other, one sequence of 32749 keys takes 14.7 us instead of 13.4, 8 of 4000 keys of 16
+// / 2 heads of 128 14.0 instead of 12.1 (64 bytes and more: no further gain).
+constexpr int kCounterWords = 8;
 __host__ __device__ constexpr int counters_of(int splits) { return splits <= 16 ? 1 : 1 + (splits + 15) / 16; }
 
 // The keys of one column tile: pairs of 16-key tiles from `begin`, `per` of them a split.
@@ -39,6 +44,7 @@ __device__ __forceinline__ TileKeys tile_keys(const SplitArgs& d, const SeqKeys&
         k.last = seq.of(t_hi).last;
         if (k.last >= k.begin) k.pairs = (k.last - k.begin + 32) >> 5;
         k.per = max((k.pairs + d.splits - 1) / d.splits, kMinPairs);
+        if (d.few < d.splits) k.per = max(k.per, min((k.pairs + d.few - 1) / d.few, d.long_pairs));
         k.active = max((k.pairs + k.per - 1) / k.per, 1);
     }
     return k;
@@ -140,10 +146,10 @@ __device__ __forceinline__ void join_splits(const SplitArgs& da, int64_t first, 
 template <typename T, int COLS>
 __device__ __forceinline__ void finish_split(const SplitArgs& da, int64_t unit, int split, int active, int ct, int kh, int b) {
     if (!da.arrived) return;
-    uint32_t* arrived = da.arrived + unit * counters_of(da.splits);
+    uint32_t* arrived = da.arrived + unit * counters_of(da.splits) * kCounterWords;
     const int groups = (active + 15) / 16, grp = split / 16;
     const int in_group = min(16, active - 16 * grp);
-    if (!last_to_arrive(arrived + (groups > 1 ? 1 + grp : 0), in_group)) return;
+    if (!last_to_arrive(arrived + (groups > 1 ? 1 + grp : 0) * kCounterWords, in_group)) return;
     join_splits<T, COLS>(da, unit * da.splits + 16 * grp, 1, in_group, ct, kh, b, groups == 1);
     if (groups == 1 || !last_to_arrive(arrived, groups)) return;
     join_splits<T, COLS>(da, unit * da.splits, 16, groups, ct, kh, b, true);
@@ -195,13 +201,25 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
     }
 }
 
-// Splits of a column tile's keys: enough workgroups for the chip, none of less
-// than kMinPairs pairs at the longest context the call can have.
-inline int split_count(int64_t units, int64_t target, int64_t cap, int64_t window, int64_t tokens) {
+// Splits of a column tile's keys: a workgroup a CU, rounded down -- one more to a CU
+// halves nothing and is joined as well (D 128, 188 column tiles of 2000 keys 20.9 us in
+// one piece, 26.0 in two, 29.7 in three; D 256, 80 of them 22.1 in 3, 25.9 in 4).  Where
+// that leaves a tile more than long_pairs pairs, up to four a CU, so that the longest
+// sequences end with the others: 300 tiles of 500 to 6000 keys, D 64 41 -> 35 us, D 128
+// 85 -> 64, D 256 158 -> 112; of 8000 keys each 71 -> 66, 142 -> 118, 271 -> 233.
+// long_pairs 64 (2048 keys), at D 64, whose tiles need least of a CU, 32: 32 sequences
+// of 512 to 4096 keys 16.3 -> 14.9 (D 128 at 32: 150 tiles of 2000 keys 19.4 -> 24.0).
+// None has less than kMinPairs pairs at the longest context the call can have.
+inline void set_splits(SplitArgs* d, int64_t units, int64_t dim, int64_t cap, int64_t window, int64_t tokens) {
     const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tokens + 16) : cap;
     const int64_t most = std::min<int64_t>(std::max<int64_t>((keys + 31) / 32 / kMinPairs, 1), 256);
-    const int64_t want = env_int("SANDY_QUANT_SPLITS", static_cast<int>(std::min<int64_t>((target + units - 1) / units, 256)));
-    return static_cast<int>(std::clamp<int64_t>(want, 1, most));
+    const int forced = env_int("SANDY_QUANT_SPLITS", 0);
+    auto of = [&](int64_t workgroups) {
+        return static_cast<int>(std::clamp<int64_t>(forced > 0 ? forced : workgroups / units, 1, most));
+    };
+    d->long_pairs = dim > 64 ? 64 : 32;
+    d->few = of(256);
+    d->splits = keys > 32 * d->long_pairs * d->few ? of(1024) : d->few;
 }
 
 // Where the parts and counters of a split call are; the splits' launch.
@@ -213,7 +231,7 @@ int split_memory(SplitArgs* d, void* workspace, hipStream_t stream, Err e) {
     d->part_ml = d->part_o + units * d->splits * COLS * p.dim;
     if (d->splits == 1 || env_int("SANDY_QUANT_MERGE_KERNEL", 0) != 0) return SANDY_OK;
     int status = 0;
-    d->arrived = arrival_counters(static_cast<size_t>(units) * counters_of(d->splits), stream, e, &status);
+    d->arrived = arrival_counters(static_cast<size_t>(units) * counters_of(d->splits) * kCounterWords, stream, e, &status);
     return status;
 }
 

@@ -24,7 +24,7 @@ struct Buffer {
 
 constexpr int kStreamRegions = 64;           // streams with arrival counters of their own
 constexpr size_t kRegionWords = 4096;        // of each
-constexpr size_t kCaptureWords = 1u << 20;   // for calls under capture, never given twice
+constexpr size_t kCaptureWords = 1u << 22;   // for calls under capture, never given twice
 
 struct DeviceState {
     uint32_t* error_word = nullptr;
