@@ -14,11 +14,11 @@
 //   - V through the wave's own LDS rows, back by ds_read_b64_tr_b8, which gives a
 //     lane one dim of 8 keys -- the A operand of O^T in the order that P leaves S^T.
 //
-// 32 sequences of 512 to 4096 keys, 32 / 4 heads of 64: 37 MB in 15.2 us (2.5 TB/s; a
-// copy would take 7.2); one sequence of 32749 keys 14.5 us; 64 with a window of 1024,
-// 8 / 2 heads of 256: 19.6 us.  It is bound by latency: a call without keys takes 4.7 us,
-// the chain position, block table, payload to the first pair 5.5 more, the other pairs
-// 6, the join 2.  Workgroups of 8 waves gained nothing.
+// 32 sequences of 512 to 4096 keys, 32 / 4 heads of 64: 37 MB in 14.7 us (2.5 TB/s; a
+// copy would take 7.2); one sequence of 32749 keys 13.4 us; 64 with a window of 1024,
+// 8 / 2 heads of 256: 19.5 us; 32 of 8000 keys 31 us (4.2 TB/s).  Short contexts are
+// latency: a call of up to 128 keys takes 4.6 us, of 600 7.0, the chain position, block
+// table, payload, join.  Workgroups of 8 waves: 15.6 us for the first, 20.3 the third.
 #include "quant_split.h"
 
 namespace sandy_hip {

@@ -1,8 +1,9 @@
 // quant_split.h -- one column tile's keys over several workgroups: which keys each
 // takes, and how their parts are joined, for column tiles of COLS (query, head) rows.
 // The last workgroup to arrive joins them in the same launch: 32 sequences of 512 to
-// 4096 keys 15.5 us, 19.1 with the merge kernel; 64 with a window of 1024 21.3 and 23.9;
-// three short f32 ones 7.3 and 10.7.  The merge kernel is for calls without counters.
+// 4096 keys 14.7 us, 18.4 with the merge kernel; 64 with a window of 1024 19.6 and 22.3;
+// three short f32 ones 6.9 and 9.0; one of 32749 keys 13.4 and 13.0.  The merge kernel
+// is for calls without counters.
 #pragma once
 #include <algorithm>
 
