@@ -481,6 +481,24 @@ def test_far_positions_and_windows(ops, T, dim):
     ops.check_device_errors()
 
 
+@pytest.mark.parametrize("merge_kernel", [0, 1])
+@pytest.mark.parametrize("hq,heads,dim,T,dtype", [(8, 2, 64, 1, BF16), (8, 2, 128, 1, F32), (4, 2, 256, 1, BF16), (16, 2, 64, 2, BF16),
+                                                  (10, 2, 96, 4, F32)])
+def test_splits_of_mixed_contexts(ops, monkeypatch, hq, heads, dim, T, dtype, merge_kernel):
+    """More row tiles than half the CUs: sequences of a piece each beside long ones
+    that take several, at the lengths where their number changes."""
+    monkeypatch.setenv("SANDY_QUANT_MERGE_KERNEL", str(merge_kernel))
+    r = rng(dim + T)
+    long = [1024, 1025, 2048, 2049, 2080, 3073, 4097, 6000]
+    ctx = [long[b // 9] if b % 9 == 0 else int(r.integers(T, 400)) for b in range(72)]
+    table, kc, vc = filled(ops, r, ctx, heads, dim, 16, "e4m3", 5)
+    q = from_f32(r.standard_normal((72, hq, T, dim)).astype(np.float32), dtype)
+    pos = [c - T for c in ctx]
+    first = check(ops, q, kc, vc, table, pos)
+    assert torch.equal(first, check(ops, q, kc, vc, table, pos))
+    check(ops, q, kc, vc, table, pos, window=2500)
+
+
 def test_many_sequences(ops):
     """More row tiles than 2^16."""
     r = rng(91)
