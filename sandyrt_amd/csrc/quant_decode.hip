@@ -4,9 +4,8 @@
 // Both payload types are exact in bf16, so a payload goes to the matrix unit as
 // it is: S^T = K Q^T with K's scale applied to the scores, O^T += V^T P^T with
 // V's applied to the weights (int8) or in the conversion itself (e4m3: exact,
-// the scale is a power of two).  f32 queries enter as three bf16 operands that
-// hold them exactly, and so do their weights; bf16 queries' weights enter as
-// two (2^-15 of each, against the output's 2^-8).  Tiles are 16 keys; a wave takes
+// the scale is a power of two).  f32 queries and all weights enter as three bf16
+// operands that hold them exactly.  Tiles are 16 keys; a wave takes
 // two at a time:
 //   - K straight into the A operand: a lane holds 16 consecutive dims of its key,
 //     the first 8 for one MFMA step and the others for the next (the order of the
@@ -40,7 +39,7 @@ template <typename T, int FORMAT, int DP>
 __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant_decode_kernel(SplitArgs da) {
     using G = DecodeGeo<T, FORMAT, DP>;
     constexpr bool kF32 = std::is_same_v<T, F32>;
-    constexpr int NQ = kF32 ? 3 : 1, NP = kF32 ? 3 : 2, NCH = G::kChunks, NT = DP / 16, RING = G::kRing;
+    constexpr int NQ = kF32 ? 3 : 1, NCH = G::kChunks, NT = DP / 16, RING = G::kRing;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const QuantAttnArgs& a = da.a;
     const QuantPages& p = a.p;
@@ -208,18 +207,18 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
         if constexpr (FORMAT == SANDY_QUANT_INT8)
 #pragma unroll
             for (int i = 0; i < 8; i++) w[i] *= i < 4 ? vf0 : vf1;
-        bf16x8_t pw[NP];
+        bf16x8_t pw[3];
         {
-            u32x4_t parts[NP];
+            u32x4_t parts[3];
 #pragma unroll
             for (int i = 0; i < 8; i += 2) {
-                uint32_t part[NP];
-                split_pair<NP>(w[i], w[i + 1], part);
+                uint32_t part[3];
+                split_pair(w[i], w[i + 1], part);
 #pragma unroll
-                for (int c = 0; c < NP; c++) parts[c][i / 2] = part[c];
+                for (int c = 0; c < 3; c++) parts[c][i / 2] = part[c];
             }
 #pragma unroll
-            for (int c = 0; c < NP; c++) pw[c] = __builtin_bit_cast(bf16x8_t, parts[c]);
+            for (int c = 0; c < 3; c++) pw[c] = __builtin_bit_cast(bf16x8_t, parts[c]);
         }
         // (dims past D: bytes of earlier tiles, in accumulators that nothing stores)
 #pragma unroll
@@ -228,7 +227,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
                 (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * t)));
             const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), vf0, vf1);
 #pragma unroll
-            for (int c = NP - 1; c >= 0; c--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw[c], acc[t], 0, 0, 0);
+            for (int c = 2; c >= 0; c--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw[c], acc[t], 0, 0, 0);
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     };
@@ -243,7 +242,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     uint32_t part[3];
-                    split_pair<3>(__uint_as_float(raw[i >> 1][s][2 * (i & 1)]), __uint_as_float(raw[i >> 1][s][2 * (i & 1) + 1]), part);
+                    split_pair(__uint_as_float(raw[i >> 1][s][2 * (i & 1)]), __uint_as_float(raw[i >> 1][s][2 * (i & 1) + 1]), part);
 #pragma unroll
                     for (int c = 0; c < 3; c++) qv[c][s][i] = part[c];
                 }

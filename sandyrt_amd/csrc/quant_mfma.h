@@ -42,18 +42,17 @@ __device__ __forceinline__ bf16x8_t payload_operand(uint32_t w0, uint32_t w1, fl
     return __builtin_bit_cast(bf16x8_t, r);
 }
 
-// x and y as NS bf16 parts each, packed in pairs: the first ones cut, the last
-// rounded (three hold a finite float exactly, two to 2^-15)
-template <int NS>
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[NS]) {
+// x and y as three bf16 parts each, packed in pairs: 8 of a float's 24 bits a part, so
+// that together they are the float (a finite one)
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t (&part)[3]) {
 #pragma unroll
-    for (int n = 0; n < NS - 1; n++) {
+    for (int n = 0; n < 2; n++) {
         const uint32_t xb = __float_as_uint(x), yb = __float_as_uint(y);
         part[n] = __builtin_amdgcn_perm(yb, xb, 0x07060302u);  // the upper halves
         x -= __uint_as_float(xb & 0xffff0000u);
         y -= __uint_as_float(yb & 0xffff0000u);
     }
-    part[NS - 1] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
+    part[2] = __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(x), static_cast<__bf16>(y)});
 }
 
 template <typename T>

@@ -8,17 +8,14 @@
 // the matrix unit as they are: S^T = K Q^T straight from 16-byte loads, O^T += V^T
 // P^T with V through the wave's own LDS rows and ds_read_b64_tr_b8; K's scale
 // multiplies the scores in the multiply-add of their exponents, V's the weights
-// (int8) or the conversion (e4m3).  bf16 queries' weights enter as two bf16 numbers
-// (2^-15), f32 queries and weights as three (exact).
+// (int8) or the conversion (e4m3).  f32 queries and all weights enter as three bf16
+// numbers (exact).
 //
-// 2048 queries of 32 / 4 heads of 64 (e4m3, causal) take 43 to 49 us, 350 to 400
-// TFLOP/s; int8 57 us where e4m3 takes 46 (three instructions convert two payloads, one
-// of e4m3's).  No single unit bounds it: vector instructions issue in 67 % of the
-// cycles, MFMA in 23 %; without the loads it is 13 % faster, without the exponentials
-// 8 %, without the second product 13 %, without the transposing reads 2 %.  Weights in
-// one part would be 5 to 12 % faster, at bf16's own error.  Slower: K in LDS tiles for several waves (52 to 57 us),
-// two row tiles a wave (D 128 34 us against 20), the keys split over workgroups as
-// well (69 against 45).
+// 2048 queries of 32 / 4 heads of 64 (e4m3, causal) take 47 us, 364 TFLOP/s; int8 is
+// slower (three instructions convert two payloads, one of e4m3's).  Weights in two parts
+// took 40 us, but kept 16 of their 24 bits.  With two, slower still: K in LDS tiles for
+// several waves (52 to 57 us), two row tiles a wave (D 128 34 us against 20), the keys
+// split over workgroups as well (69 against 45).
 #include "quant_mfma.h"
 
 #include <algorithm>
@@ -66,7 +63,7 @@ template <typename T, int FORMAT, int DP, bool EXACT>
 __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant_prompt_kernel(PromptArgs pa) {
     using G = PromptGeo<T, FORMAT, DP>;
     constexpr bool kF32 = G::kF32;
-    constexpr int NQ = G::NQ, NP = kF32 ? 3 : 2, KS = G::KS, DT = G::DT;
+    constexpr int NQ = G::NQ, KS = G::KS, DT = G::DT;
     extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
     const QuantAttnArgs& a = pa.a;
     const QuantPages& p = a.p;
@@ -111,7 +108,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 uint32_t part[3];
-                split_pair<3>(d < D ? x[2 * i] : 0.0f, d < D ? x[2 * i + 1] : 0.0f, part);
+                split_pair(d < D ? x[2 * i] : 0.0f, d < D ? x[2 * i + 1] : 0.0f, part);
 #pragma unroll
                 for (int n = 0; n < 3; n++) v[n][i] = part[n];
             }
@@ -281,13 +278,13 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         // bytes of earlier tiles, in accumulators that nothing stores)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            u32x4_t parts[NP];
+            u32x4_t parts[3];
 #pragma unroll
             for (int j = 0; j < 8; j += 2) {
-                uint32_t part[NP];
-                split_pair<NP>(w[8 * h + j], w[8 * h + j + 1], part);
+                uint32_t part[3];
+                split_pair(w[8 * h + j], w[8 * h + j + 1], part);
 #pragma unroll
-                for (int i = 0; i < NP; i++) parts[i][j / 2] = part[i];
+                for (int i = 0; i < 3; i++) parts[i][j / 2] = part[i];
             }
 #pragma unroll
             for (int t = 0; t < DT; t++) {
@@ -295,7 +292,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
                     (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * h * G::VP + 32 * t)));
                 const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), v[h], v[h]);
 #pragma unroll
-                for (int i = NP - 1; i >= 0; i--)
+                for (int i = 2; i >= 0; i--)
                     acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8_t, parts[i]), acc[t], 0, 0, 0);
                 if (DP == 256 && t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
