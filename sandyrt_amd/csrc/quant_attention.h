@@ -50,6 +50,20 @@ __device__ __forceinline__ int divide(int n, int d, uint32_t magic) {
     return q + (n - q * d >= d ? 1 : 0);
 }
 
+// Sums over V stay finite where V is next to 2^128: from the first block whose scale is
+// 2^80 or more on ("loud"), a sum holds 2^-64 of itself.  A weight is below 2^8 and keys
+// are at most 2^30, so a sum is below 2^126 before and below 2^104 after.  Values that
+// 2^-64 takes below fp32's normal numbers are below 2^-62, 2^-148 of the loud block's
+// largest.  The sum of weights, never negative, carries the mark as its sign.
+constexpr int kLoudCode = 127 + 80;
+constexpr uint32_t kLoudBits = static_cast<uint32_t>(kLoudCode) << 23;  // of such a scale; times 2^-64 none is
+constexpr float kLoudDown = 0x1p-64f, kLoudUp = 0x1p64f;
+__device__ __forceinline__ bool loud_code(int c) { return c >= kLoudCode && c != 255; }
+__device__ __forceinline__ float mark_loud(float total, bool loud) {
+    return __uint_as_float(__float_as_uint(total) | (loud ? 0x80000000u : 0u));
+}
+__device__ __forceinline__ bool is_loud(float total) { return __float_as_uint(total) >> 31; }
+
 // Few queries a sequence (quant_decode.hip): whether the kernel takes the call,
 // its workspace (whatever the call's strides), its launch.
 bool quant_decode_takes(const QuantAttnArgs& a);

@@ -26,6 +26,7 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
     __shared__ float weight[256];
     __shared__ const uint8_t* row[256];
     __shared__ float part[4];
+    __shared__ bool far[4];
     __shared__ double sums[4];
     const QuantPages& p = a.p;
     const int tid = threadIdx.x;
@@ -46,11 +47,13 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
     const int lanes = min(D, 256), groups = 256 / lanes, group = tid / lanes, dim0 = tid - group * lanes;
     float m = -INFINITY, acc[kDims];
     double l = 0.0;
+    bool loud = false;
 #pragma unroll
     for (int i = 0; i < kDims; i++) acc[i] = 0.0f;
     for (int k0 = keys.first; k0 <= keys.last; k0 += 256) {
         const int key = k0 + tid;
-        float s = -INFINITY, vs = 0.0f;
+        float s = -INFINITY;
+        int vc = 0;
         const uint8_t* vrow = nullptr;
         if (key <= keys.last) {
             const int id = quant_block(p, b, key >> p.log2_page);
@@ -71,13 +74,14 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
                     for (int d = 0; d < D; d++) dot = fmaf(qf[d], Quant<FORMAT>::template value<0>(krow[d]), dot);
                 }
                 s = dot * quant_scale(p.scales[0][block]) * a.scale_log2;
-                vs = quant_scale(p.scales[1][block]);
+                vc = p.scales[1][block];
                 vrow = p.pool[1] + from;
             }
         }
         float mx = wave_max(s);
+        const bool any = __any(loud_code(vc));
         __syncthreads();  // the sums over the chunk before have been read
-        if ((tid & 63) == 0) part[tid >> 6] = mx;
+        if ((tid & 63) == 0) part[tid >> 6] = mx, far[tid >> 6] = any;
         __syncthreads();
         mx = fmaxf(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])), m);
         const float shift = mx == -INFINITY ? 0.0f : mx;
@@ -85,7 +89,12 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
         const float w = vrow ? __builtin_amdgcn_exp2f(s - shift) : 0.0f;
         l = l * static_cast<double>(alpha) + static_cast<double>(w);
         m = mx;
-        weight[tid] = vrow ? w * vs : 0.0f;
+        if (!loud && (far[0] || far[1] || far[2] || far[3])) {
+            loud = true;
+#pragma unroll
+            for (int i = 0; i < kDims; i++) acc[i] *= kLoudDown;
+        }
+        weight[tid] = vrow ? w * (quant_scale(vc) * (loud ? kLoudDown : 1.0f)) : 0.0f;
         row[tid] = vrow;
         __syncthreads();
         const int n = min(256, keys.last - k0 + 1);
@@ -114,7 +123,7 @@ __global__ __launch_bounds__(256) void quant_attention_general_kernel(QuantAttnA
 #pragma unroll
     for (int i = 0; i < kDims; i++) {
         const int d = dim0 + 256 * i;
-        if (group == 0 && d < D) Vec8<T>::store1(a.out, o0 + d * a.os[3], acc[i] * inv);
+        if (group == 0 && d < D) Vec8<T>::store1(a.out, o0 + d * a.os[3], acc[i] * inv * (loud ? kLoudUp : 1.0f));
     }
 }
 

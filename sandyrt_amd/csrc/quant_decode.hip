@@ -92,6 +92,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
+    bool loud = false;  // the same for the wave
 
     unsigned char* vrows = lds + wave * G::kV;
     int k_off[NCH], v_to[NCH];  // this lane's bytes of a tile; its V pieces' places in LDS
@@ -114,6 +115,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     int bytes_in = 0;
     uint64_t offset = 0;
     float kf = 0.0f, vf = 1.0f;
+    uint64_t odd = 0;  // the tiles without a page, or that make the sums loud
     u32x4_t kr[RING][2][NCH], vr[RING][2][NCH];
     auto load = [&](int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
 #pragma unroll
@@ -144,7 +146,16 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
         for (int i = 0; i < RING; i++) load(i, kr[i], vr[i]);
         // a NaN block: NaN scores for whoever sees it, V's own factor aside
         kf = quant_scale(vc == 255 ? 255 : kc) * a.scale_log2;
-        vf = quant_scale(vc == 255 ? 127 : vc);
+        vf = quant_scale(vc == 255 || id < 0 ? 127 : vc);
+        if (loud) vf = fmaxf(vf * kLoudDown, 0x1p-126f);
+        odd = __ballot((id < 0) | (__float_as_uint(vf) >= kLoudBits));
+    };
+    // before such a block's values first enter the sums
+    auto get_loud = [&]() {
+        loud = true;
+        vf = fmaxf(vf * kLoudDown, 0x1p-126f);
+#pragma unroll
+        for (int t = 0; t < NT; t++) acc[t] *= kLoudDown;
     };
     auto attend = [&](int round0, int n, u32x4_t (&k)[2][NCH], u32x4_t (&v)[2][NCH]) {
         f32x4_t sc[2];
@@ -169,16 +180,20 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
         load(n + RING, k, v);
         const float kf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n));
         const float kf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n + 1));
-        const float vf0 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n));
-        const float vf1 = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + 1));
-        const bool none0 = __builtin_amdgcn_readlane(bytes_in, 2 * n) == 0;
-        const bool none1 = __builtin_amdgcn_readlane(bytes_in, 2 * n + 1) == 0;
+        uint32_t vf0 = __builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n);
+        uint32_t vf1 = __builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + 1);
         const int k0 = tk.begin + 32 * (round0 + 4 * n);
         sc[0] *= kf0;
         sc[1] *= kf1;
-        if ((k0 < all_first) | (k0 + 31 > all_last) | none0 | none1) {
+        if ((k0 < all_first) | (k0 + 31 > all_last) | ((odd >> (2 * n) & 3) != 0)) {
+            if (max(vf0, vf1) >= kLoudBits) {
+                get_loud();
+                vf0 = __builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n);
+                vf1 = __builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + 1);
+            }
             // element i of tile h: key k0 + 16 h + 4 g + i
-            const int end0 = none0 ? -1 : mine.last, end1 = none1 ? -1 : mine.last;
+            const int end0 = __builtin_amdgcn_readlane(bytes_in, 2 * n) == 0 ? -1 : mine.last;
+            const int end1 = __builtin_amdgcn_readlane(bytes_in, 2 * n + 1) == 0 ? -1 : mine.last;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int key = k0 + 4 * g + i;
@@ -206,7 +221,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
         l += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
         if constexpr (FORMAT == SANDY_QUANT_INT8)
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i] *= i < 4 ? vf0 : vf1;
+            for (int i = 0; i < 8; i++) w[i] *= __uint_as_float(i < 4 ? vf0 : vf1);
         bf16x8_t pw[3];
         {
             u32x4_t parts[3];
@@ -225,7 +240,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
         for (int t = 0; t < NT; t++) {
             const i32x2_t eight = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                 (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * t)));
-            const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), vf0, vf1);
+            const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), __uint_as_float(vf0), __uint_as_float(vf1));
 #pragma unroll
             for (int c = 2; c >= 0; c--) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, pw[c], acc[t], 0, 0, 0);
         }
@@ -269,7 +284,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     float* ml = reinterpret_cast<float*>(lds + std::max(4 * G::kV, G::kMerge));
     if (g == 0) {
         ml[(wave * 16 + col) * 2] = m;
-        ml[(wave * 16 + col) * 2 + 1] = l;
+        ml[(wave * 16 + col) * 2 + 1] = mark_loud(l, loud);
     }
     __syncthreads();
     float mm = -INFINITY, total = 0.0f;
@@ -277,7 +292,11 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     for (int w = 0; w < 4; w++) mm = fmaxf(mm, ml[(w * 16 + col) * 2]);
     const float shift = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-    for (int w = 0; w < 4; w++) total += ml[(w * 16 + col) * 2 + 1] * __builtin_amdgcn_exp2f(ml[(w * 16 + col) * 2] - shift);
+    for (int w = 0; w < 4; w++) total += fabsf(ml[(w * 16 + col) * 2 + 1]) * __builtin_amdgcn_exp2f(ml[(w * 16 + col) * 2] - shift);
+    bool any_loud = false;
+#pragma unroll
+    for (int w = 0; w < 4; w++) any_loud |= is_loud(ml[(w * 16 + col) * 2 + 1]);
+    const float down = any_loud && !loud ? kLoudDown : 1.0f, up = any_loud ? kLoudUp : 1.0f;
     const float f = __builtin_amdgcn_exp2f(m - shift);
     f32x4_t* red = reinterpret_cast<f32x4_t*>(lds);
     const bool final_out = tk.active == 1;
@@ -292,7 +311,7 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
     for (int s0 = 0; s0 < NT; s0 += SET) {
         if (s0 > 0) __syncthreads();
 #pragma unroll
-        for (int t = 0; t < SET; t++) red[(wave * SET + t) * 64 + lane] = acc[s0 + t] * f;
+        for (int t = 0; t < SET; t++) red[(wave * SET + t) * 64 + lane] = acc[s0 + t] * down * f;
         __syncthreads();
 #pragma unroll
         for (int t4 = 0; t4 < SET; t4 += 4) {
@@ -301,12 +320,12 @@ __global__ __launch_bounds__(256, (DecodeGeo<T, FORMAT, DP>::kWaves)) void quant
             if (d >= D || !stored) continue;
             const f32x4_t o = (red[t * 64 + lane] + red[(SET + t) * 64 + lane]) +
                               (red[(2 * SET + t) * 64 + lane] + red[(3 * SET + t) * 64 + lane]);
-            if (final_out) store4<T>(a.out, o0 + d, o * inv);
+            if (final_out) store4<T>(a.out, o0 + d, o * inv * up);
             else po.put(col * D + d, o);
         }
     }
     if (final_out) return;
-    if (tid < 16 && stored) Through(da.part_ml + slot * 32).put(2 * col, mm, total);
+    if (tid < 16 && stored) Through(da.part_ml + slot * 32).put(2 * col, mm, mark_loud(total, any_loud));
     finish_split<T, 16>(da, unit, split, tk.active, ct, kh, b);
 }
 

@@ -138,6 +138,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
 
     f32x16_t acc[DT];
     float m = -INFINITY, l = 0.0f;
+    bool loud = false;  // the same for the wave
 #pragma unroll
     for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -163,6 +164,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
     int bytes_in = 0;
     uint64_t offset = 0;
     float kf = 0.0f, vf = 1.0f;
+    uint64_t odd = 0;  // the tiles without a page, that are NaN, or that make the sums loud
     u32x4_t kr[G::KP], vr[2][G::NV];
     auto load = [&](int n) {
         uint64_t off[2];
@@ -194,7 +196,16 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         load(0);
         // a NaN block: NaN scores for whoever sees it, V's own factor aside
         kf = vc == 255 || kc == 255 ? quant_scale(255) : fmaxf(quant_scale(kc) * a.scale_log2, 0x1p-126f);
-        vf = quant_scale(vc == 255 ? 127 : vc);
+        vf = quant_scale(vc == 255 || id < 0 ? 127 : vc);
+        if (loud) vf = fmaxf(vf * kLoudDown, 0x1p-126f);
+        odd = __ballot((id < 0) | (kf != kf) | (__float_as_uint(vf) >= kLoudBits));
+    };
+    // before such a block's values first enter the sums
+    auto get_loud = [&]() {
+        loud = true;
+        vf = fmaxf(vf * kLoudDown, 0x1p-126f);
+#pragma unroll
+        for (int t = 0; t < DT; t++) acc[t] *= kLoudDown;
     };
     auto attend = [&](int round0, int n) {
         f32x16_t sc;
@@ -219,24 +230,28 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
             for (int j = 0; j < G::NV; j++) *reinterpret_cast<u32x4_t*>(vrows + 16 * h * G::VP + v_to[j]) = vr[h][j];
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         load(n + 1);
-        float f[2], v[2];
-        bool none[2];
+        float f[2];
+        uint32_t v[2];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             f[h] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(kf), 2 * n + h));
-            v[h] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + h));
-            none[h] = __builtin_amdgcn_readlane(bytes_in, 2 * n + h) == 0;
+            v[h] = __builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + h);
         }
         const int k0 = begin + 32 * (round0 + 4 * n);
         // element i: key k0 + 8 (i / 4) + 4 half + i % 4, in the first tile for i < 8
-        if ((k0 < all_first) | (k0 + 31 > all_last) | none[0] | none[1] | (f[0] != f[0]) | (f[1] != f[1])) {
+        if ((k0 < all_first) | (k0 + 31 > all_last) | ((odd >> (2 * n) & 3) != 0)) {
+            if (max(v[0], v[1]) >= kLoudBits) {
+                get_loud();
+#pragma unroll
+                for (int h = 0; h < 2; h++) v[h] = __builtin_amdgcn_readlane(__float_as_uint(vf), 2 * n + h);
+            }
             int key0 = k0 + 4 * half;
             asm volatile("" : "+v"(key0));  // keeps the compares out of whole tiles
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const bool nan = f[h] != f[h];
                 if (nan) f[h] = 1.0f;  // into the scores themselves
-                const int end = none[h] ? -1 : mine.last;
+                const int end = __builtin_amdgcn_readlane(bytes_in, 2 * n + h) == 0 ? -1 : mine.last;
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
                     const int key = key0 + 16 * h + 8 * (i >> 2) + (i & 3);
@@ -273,7 +288,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         l += ((rs[0] + rs[1]) + (rs[2] + rs[3])) + ((rs[4] + rs[5]) + (rs[6] + rs[7]));
         if constexpr (FORMAT == SANDY_QUANT_INT8)
 #pragma unroll
-            for (int i = 0; i < 16; i++) w[i] *= v[i >> 3];
+            for (int i = 0; i < 16; i++) w[i] *= __uint_as_float(v[i >> 3]);
         // contraction slot 8 half + j of step h: this lane's element 8 h + j (dims past D:
         // bytes of earlier tiles, in accumulators that nothing stores)
 #pragma unroll
@@ -290,7 +305,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
             for (int t = 0; t < DT; t++) {
                 const i32x2_t eight = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
                     (i32x2_t __attribute__((address_space(3)))*)((unsigned char __attribute__((address_space(3)))*)(v_from + 16 * h * G::VP + 32 * t)));
-                const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), v[h], v[h]);
+                const bf16x8_t va = payload_operand<FORMAT>(static_cast<uint32_t>(eight[0]), static_cast<uint32_t>(eight[1]), __uint_as_float(v[h]), __uint_as_float(v[h]));
 #pragma unroll
                 for (int i = 2; i >= 0; i--)
                     acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va, __builtin_bit_cast(bf16x8_t, parts[i]), acc[t], 0, 0, 0);
@@ -308,17 +323,20 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
     // the four waves' maxima and sums, then their accumulators, 32 dims at a time
     float2* ml = reinterpret_cast<float2*>(lds + std::max(4 * G::kV, G::kMerge));  // [wave][32]
     l = sum_xor32(l);
-    if (half == 0) ml[wave * 32 + col] = make_float2(m, l);
+    if (half == 0) ml[wave * 32 + col] = make_float2(m, mark_loud(l, loud));
     __syncthreads();
     float mm = -INFINITY, total = 0.0f;
 #pragma unroll
     for (int w = 0; w < 4; w++) mm = fmaxf(mm, ml[w * 32 + col].x);
     const float shift = mm == -INFINITY ? 0.0f : mm;
+    bool any_loud = false;
 #pragma unroll
     for (int w = 0; w < 4; w++) {
         const float2 e = ml[w * 32 + col];
-        total += e.y * __builtin_amdgcn_exp2f(e.x - shift);
+        total += fabsf(e.y) * __builtin_amdgcn_exp2f(e.x - shift);
+        any_loud |= is_loud(e.y);
     }
+    const float down = any_loud && !loud ? kLoudDown : 1.0f, up = any_loud ? kLoudUp : 1.0f;
     const float f = __builtin_amdgcn_exp2f(m - shift);
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
     const int64_t o0 = b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * half;
@@ -328,13 +346,13 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         if (t > 0) __syncthreads();
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            red[(wave * 4 + i) * 64 + lane] = f32x4_t{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]} * f;
+            red[(wave * 4 + i) * 64 + lane] = f32x4_t{acc[t][4 * i], acc[t][4 * i + 1], acc[t][4 * i + 2], acc[t][4 * i + 3]} * down * f;
         __syncthreads();
         // this wave's elements 4 wave .. + 3: dims 32 t + 8 wave + 4 half + 0 .. 3
         const int d = 32 * t + 8 * wave;
         if (r0 + col >= rows || d >= D) continue;
         const f32x4_t o = (red[wave * 64 + lane] + red[(4 + wave) * 64 + lane]) + (red[(8 + wave) * 64 + lane] + red[(12 + wave) * 64 + lane]);
-        store4<T>(a.out, o0 + d, o * inv);
+        store4<T>(a.out, o0 + d, o * inv * up);
     }
 }
 

@@ -102,6 +102,7 @@ __device__ __forceinline__ void join_splits(const SplitArgs& da, int64_t first, 
     for (int i = threadIdx.x; i < cols * per_col; i += 256) {
         const int c = i / per_col, d = 4 * (i - c * per_col);
         float m = -INFINITY, total = 0.0f;
+        bool loud = false;
         f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
         for (int s0 = 0; s0 < n; s0 += 8) {
             float2 ml[8];
@@ -120,21 +121,26 @@ __device__ __forceinline__ void join_splits(const SplitArgs& da, int64_t first, 
             total *= f;
             o *= f;
             m = top;
+            bool any = false;
+#pragma unroll
+            for (int s = 0; s < 8; s++) any |= is_loud(ml[s].y);
+            if (any && !loud) o *= kLoudDown;
+            loud |= any;
 #pragma unroll
             for (int s = 0; s < 8; s++) {
                 if (s0 + s >= n) continue;
                 const float w = __builtin_amdgcn_exp2f(ml[s].x - shift);
-                total += ml[s].y * w;
-                o += x[s] * w;
+                total += fabsf(ml[s].y) * w;
+                o += x[s] * (loud && !is_loud(ml[s].y) ? kLoudDown : 1.0f) * w;
             }
         }
         const int row = COLS * ct + c, qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
         if (final_out) {
             const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, o * inv);
+            store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, o * inv * (loud ? kLoudUp : 1.0f));
         } else {
             po.put(c * D + d, o);
-            if (d == 0) joined[c] = make_float2(m, total);
+            if (d == 0) joined[c] = make_float2(m, mark_loud(total, loud));
         }
     }
     if (final_out) return;
@@ -184,7 +190,12 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
     m = wave_max(m);
     const float shift = m == -INFINITY ? 0.0f : m;
     float total = 0.0f;
-    for (int s = tid & 63; s < tk.active; s += 64) total += ml[s * 2 * COLS + 1] * __builtin_amdgcn_exp2f(ml[s * 2 * COLS] - shift);
+    bool loud = false;
+    for (int s = tid & 63; s < tk.active; s += 64) {
+        total += fabsf(ml[s * 2 * COLS + 1]) * __builtin_amdgcn_exp2f(ml[s * 2 * COLS] - shift);
+        loud |= is_loud(ml[s * 2 * COLS + 1]);
+    }
+    loud = __any(loud);
     total = wave_sum(total);
     const int pieces = D / 4, groups = 256 / pieces;
     const int piece = tid % pieces, grp = tid / pieces;
@@ -192,13 +203,14 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
     if (grp < groups)
 #pragma unroll 4
         for (int s = grp; s < tk.active; s += groups)
-            o += *reinterpret_cast<const f32x4_t*>(po + static_cast<int64_t>(s) * COLS * D + 4 * piece) * __builtin_amdgcn_exp2f(ml[s * 2 * COLS] - shift);
+            o += *reinterpret_cast<const f32x4_t*>(po + static_cast<int64_t>(s) * COLS * D + 4 * piece) *
+                 (loud && !is_loud(ml[s * 2 * COLS + 1]) ? kLoudDown : 1.0f) * __builtin_amdgcn_exp2f(ml[s * 2 * COLS] - shift);
     sums[tid] = o;
     __syncthreads();
     if (tid < pieces) {
         for (int i = 1; i < groups; i++) o += sums[tid + i * pieces];
         const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * tid, o * inv);
+        store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * tid, o * inv * (loud ? kLoudUp : 1.0f));
     }
 }
 

@@ -1,12 +1,12 @@
 """The quantised paged K/V cache on the GPU where it can go wrong: sums that
-cancel."""
+cancel, values next to the largest that a block holds."""
 import numpy as np
 import pytest
 import torch
 
 from tests import quant_reference as R
 from tests.helpers import from_f32, rng
-from tests.test_gpu_quant_cache import BF16, cuda, empty, f64
+from tests.test_gpu_quant_cache import BF16, F32, cuda, empty, f64, filled, make_table
 
 pytestmark = pytest.mark.gpu
 
@@ -54,3 +54,54 @@ def test_weights_keep_24_bits(ops, form, fmt):
     x = np.zeros((B, hq, 2, dim), np.float32)
     x[..., 0] = 0.4 * r.standard_normal(x.shape[:3])
     attend(ops, from_f32(x, BF16), *c, np.zeros((B, 1), np.int32), [1] * B, window=2, scale=0.25)
+
+
+# ------------------------------------------------------------------ values next to the largest
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("T,dim", [(1, 64), (33, 64), (5, 128), (19, 256), (3, 36)])
+def test_values_near_the_largest(ops, form, T, dim, fmt, dtype):
+    """Means of values up to the largest that a block holds are finite, also where
+    the weights' sum times them is not; ordinary and tiny values beside them count."""
+    r = rng(35 + T)
+    n, top = 220, R.LARGEST[fmt] * 2.0 ** (121 if fmt == "int8" else 119)
+    table, pages = make_table(r, [n], 16)
+    k, v = (r.standard_normal((1, 4, n, dim)) for _ in range(2))
+    v[:, 0] = top * r.uniform(0.5, 1, v[:, 0].shape)     # one sign: the mean is as large
+    v[:, 1, 96:160] *= 2.0 ** 118                         # some blocks in the middle
+    v[:, 2, :16] *= 2.0 ** 110                            # of next to no weight
+    k[:, 2, :16] *= 1e-3
+    v[:, 3, 200:] *= 1e-37
+    v[:, 3, 100:112] = top * r.choice([-1, 1], v[:, 3, 100:112].shape)
+    k, v = (from_f32(x.astype(np.float32), dtype) for x in (k, v))
+    if dtype == BF16:  # not rounded past it
+        v = v.clamp(-top, top)
+    kc, vc = (empty(ops, pages, 4, 16, dim, fmt, i) for i in (1, 2))
+    ops.quant_paged_append(k, v, kc, vc, cuda(table), cuda(np.zeros(1, np.int64)))
+    assert (vc.scales[int(table[0, 0]), 0] > 240).all() and not (vc.scales == 255).any()
+    q = r.standard_normal((1, 8, T, dim)).astype(np.float32)
+    for scale in (-1.0, 1.0):  # flat, and one key outweighing the others
+        got = attend(ops, from_f32(q, dtype), kc, vc, table, [n - T], f"scale {scale}", scale=scale)
+        assert torch.isfinite(got).all() and got[0, 0].abs().max() > 2.0 ** 126
+
+
+@pytest.mark.parametrize("merge_kernel", [0, 1])
+@pytest.mark.parametrize("splits,T,dim,dtype", [(1, 1, 64, BF16), (5, 1, 128, F32), (40, 1, 64, BF16), (40, 2, 256, BF16), (17, 9, 64, F32)])
+def test_splits_with_values_near_the_largest(ops, monkeypatch, splits, T, dim, dtype, merge_kernel):
+    """Some splits, and some rounds of a wave's keys, with such values and the others without."""
+    ops._quant_workspace.cache_clear()
+    monkeypatch.setenv("SANDY_QUANT_SPLITS", str(splits))
+    monkeypatch.setenv("SANDY_QUANT_MERGE_KERNEL", str(merge_kernel))
+    r = rng(splits + T)
+    ctx = [9000, 700]
+    table, kc, vc = filled(ops, r, ctx, 2, dim, 16, "int8", 5)
+    for at in (5, 300, 301, 500):  # pages of the first sequence: keys 80.., 4800.., 8000..
+        vc.scales[int(table[0, at]), 0] = 248
+    vc.scales[int(table[1, 20]), 1] = 246
+    q = from_f32(2 * r.standard_normal((2, 8, T, dim)).astype(np.float32), dtype)
+    got = attend(ops, q, kc, vc, table, [c - T for c in ctx])
+    assert torch.isfinite(got).all()
+    assert torch.equal(got, attend(ops, q, kc, vc, table, [c - T for c in ctx]))
+    attend(ops, q, kc, vc, table, [c - T for c in ctx], window=1500)
+    ops._quant_workspace.cache_clear()
