@@ -194,8 +194,10 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
         offset = id < 0 ? 0 : static_cast<uint64_t>((block << p.log2_page) + (key0 & ((1 << p.log2_page) - 1))) * D;
         const int kc = p.scales[0][block], vc = p.scales[1][block];
         load(0);
-        // a NaN block: NaN scores for whoever sees it, V's own factor aside
-        kf = vc == 255 || kc == 255 ? quant_scale(255) : fmaxf(quant_scale(kc) * a.scale_log2, 0x1p-126f);
+        // a NaN block: NaN scores for whoever sees it, V's own factor aside (and none is 0,
+        // which would make masked scores NaN)
+        kf = quant_scale(vc == 255 ? 255 : kc) * a.scale_log2;
+        if (kf == 0.0f) kf = 0x1p-149f;
         vf = quant_scale(vc == 255 || id < 0 ? 127 : vc);
         if (loud) vf = fmaxf(vf * kLoudDown, 0x1p-126f);
         odd = __ballot((id < 0) | (kf != kf) | (__float_as_uint(vf) >= kLoudBits));

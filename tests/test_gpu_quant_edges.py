@@ -1,5 +1,5 @@
 """The quantised paged K/V cache on the GPU where it can go wrong: sums that
-cancel, values next to the largest that a block holds."""
+cancel, values next to the largest and smallest that a block holds."""
 import numpy as np
 import pytest
 import torch
@@ -105,3 +105,16 @@ def test_splits_with_values_near_the_largest(ops, monkeypatch, splits, T, dim, d
     assert torch.equal(got, attend(ops, q, kc, vc, table, [c - T for c in ctx]))
     attend(ops, q, kc, vc, table, [c - T for c in ctx], window=1500)
     ops._quant_workspace.cache_clear()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("form", FORMS, indirect=True)
+@pytest.mark.parametrize("dim", [64, 112])
+def test_keys_of_the_smallest_scale(ops, form, dim, dtype):
+    """Loud queries of the quietest keys: scores of ordinary size."""
+    r = rng(37)
+    table, kc, vc = filled(ops, r, [60], 2, dim, 16, "int8", 3)
+    kc.scales.fill_(1)
+    x = np.zeros((1, 8, 5, dim), np.float32)
+    x[..., 3] = 2.0 ** 120 * r.uniform(-1, 1, x.shape[:3])
+    attend(ops, from_f32(x, dtype), kc, vc, table, [55])
