@@ -531,15 +531,27 @@ def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
     been appended).  Queries from counts[b] on give zero."""
     out = torch.empty_like(q) if out is None else out
     kc, vc, pool, window = k_cache.pack(), v_cache.pack(), k_cache.pool, int(window)
-    need, work = 0, None
+    sizes, need = None, 0
     if q.dim() == 4 and block_table.dim() == 2:  # else the call says what is wrong
-        need = _quant_workspace(*q.shape, q.dtype, pool.shape[1], pool.shape[2], block_table.shape[1], window)
-    if need:  # the call's own: calls on other streams and captured graphs share nothing with it
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+        sizes = (*q.shape, q.dtype, pool.shape[1], pool.shape[2], block_table.shape[1], window)
+        need = _quant_workspace(*sizes)
     tensors = (q, out, block_table, position_offsets, counts, k_cache.scales, v_cache.pool, v_cache.scales)
-    _quant_call("sandy_hip_quant_paged_attention", pool.get_device(), tensors, pack(q), kc, vc, pack(block_table),
-                pack(position_offsets), _packed(counts), window, float(scale), pack(out),
-                None if work is None else work.data_ptr(), need)
+
+    def attend(need):
+        # the workspace is the call's own: calls on other streams and captured graphs share nothing with it
+        work = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        _quant_call("sandy_hip_quant_paged_attention", pool.get_device(), tensors, pack(q), kc, vc, pack(block_table),
+                    pack(position_offsets), _packed(counts), window, float(scale), pack(out),
+                    None if work is None else work.data_ptr(), need)
+
+    try:
+        attend(need)
+    except SandyError:
+        # the size kept may be from before an environment switch that changes it
+        now = need if sizes is None else _quant_workspace.__wrapped__(*sizes)
+        if now <= need:
+            raise
+        attend(now)
     return out
 
 

@@ -118,3 +118,16 @@ def test_keys_of_the_smallest_scale(ops, form, dim, dtype):
     x = np.zeros((1, 8, 5, dim), np.float32)
     x[..., 3] = 2.0 ** 120 * r.uniform(-1, 1, x.shape[:3])
     attend(ops, from_f32(x, dtype), kc, vc, table, [55])
+
+
+# ------------------------------------------------------------------ switches and streams
+def test_switches_between_calls(ops, monkeypatch):
+    """A switch that changes a call's workspace, set after a call of the same sizes."""
+    r = rng(41)
+    table, kc, vc = filled(ops, r, [2000, 900], 2, 64, 16, "int8", 3)
+    q = from_f32(r.standard_normal((2, 8, 3, 64)).astype(np.float32), BF16)
+    ops._quant_workspace.cache_clear()
+    for name, value in (("SANDY_QUANT_SPLITS", "2"), ("SANDY_QUANT_SPLITS", "15"), ("SANDY_QUANT_PROMPT_WGS", "1"),
+                        ("SANDY_QUANT_SPLITS", "1"), ("SANDY_QUANT_PROMPT_WGS", "100000"), ("SANDY_QUANT_SPLITS", "4")):
+        monkeypatch.setenv(name, value)
+        attend(ops, q, kc, vc, table, [1997, 897])
