@@ -120,9 +120,9 @@ void* device_workspace(int slot, size_t bytes, hipStream_t stream, Err e, int* s
 void* device_counters(int slot, size_t bytes, hipStream_t stream, Err e, int* status);
 
 // Zeroed arrival counters that no other work in flight uses, or null where there
-// are none left (the caller then takes a form that needs none): a region for each
-// stream, whose calls follow one another, and for a call under capture words of
-// its graph's own.  The kernels leave them zero.
+// are none (the caller then takes a form that needs none): the legacy stream's, whose
+// calls follow one another, and for a call under capture words that no other call gets,
+// until 2^22 are gone.  The kernels leave them zero.  17 MB a device.
 uint32_t* arrival_counters(size_t words, hipStream_t stream, Err e, int* status);
 
 // ---------------------------------------------------------------- device helpers

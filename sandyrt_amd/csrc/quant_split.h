@@ -1,9 +1,9 @@
 // quant_split.h -- one column tile's keys over several workgroups: which keys each
 // takes, and how their parts are joined, for column tiles of COLS (query, head) rows.
-// The last workgroup to arrive joins them in the same launch: 32 sequences of 512 to
-// 4096 keys 14.7 us, 18.4 with the merge kernel; 64 with a window of 1024 19.6 and 22.3;
-// three short f32 ones 6.9 and 9.0; one of 32749 keys 13.4 and 13.0.  The merge kernel
-// is for calls without counters.
+// The last workgroup to arrive joins them in the same launch (in a graph: 32 sequences
+// of 512 to 4096 keys 15.9 us, 18.4 with the merge kernel; 64 with a window of 1024 20.0
+// and 22.1; three short f32 ones 7.1 and 8.6; one of 32749 keys 14.3 and 14.8).  The
+// merge kernel is for calls without counters and gives the same bits.
 #pragma once
 #include <algorithm>
 
@@ -89,8 +89,60 @@ __device__ __forceinline__ bool last_to_arrive(uint32_t* counter, int n) {
     return last;
 }
 
-// Slots first, first + stride, .. (n <= 16) of a column tile joined, in slot
-// order: into the output, or into slot `first`.  A thread per column and 4 dims.
+// Parts 0 .. n - 1 (n <= 16) of one row and 4 dims joined, in order: `ml` gives a part's
+// maximum and sum of weights, `part` its sums.
+struct Joined {
+    float m, total;
+    bool loud;
+    f32x4_t o;
+};
+
+template <typename ML, typename PART>
+__device__ __forceinline__ Joined join_parts(int n, ML ml, PART part) {
+    Joined j{-INFINITY, 0.0f, false, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (int s0 = 0; s0 < n; s0 += 8) {
+        float2 w[8];
+        f32x4_t x[8];
+#pragma unroll
+        for (int s = 0; s < 8; s++) {  // past the last: the last again, unused
+            w[s] = ml(min(s0 + s, n - 1));
+            x[s] = part(min(s0 + s, n - 1));
+        }
+        float top = j.m;
+        bool any = false;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            top = fmaxf(top, w[s].x);
+            any |= is_loud(w[s].y);
+        }
+        const float shift = top == -INFINITY ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(j.m - shift);
+        j.total *= f;
+        j.o *= f;
+        j.m = top;
+        if (any && !j.loud) j.o *= kLoudDown;
+        j.loud |= any;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            if (s0 + s >= n) continue;
+            const float e = __builtin_amdgcn_exp2f(w[s].x - shift);
+            j.total += fabsf(w[s].y) * e;
+            j.o += x[s] * (j.loud && !is_loud(w[s].y) ? kLoudDown : 1.0f) * e;
+        }
+    }
+    return j;
+}
+
+// Into row `row` of a kv head's rows, dims d .. d + 3.
+template <typename T>
+__device__ __forceinline__ void store_joined(const QuantAttnArgs& a, const Joined& j, int row, int d, int kh, int b) {
+    const int qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
+    const float inv = j.total == 0.0f ? 0.0f : 1.0f / j.total;
+    store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, j.o * inv * (j.loud ? kLoudUp : 1.0f));
+}
+
+// Slots first, first + stride, .. (n <= 16) of a column tile joined: into the output,
+// or into slot `first`.  A thread per column and 4 dims.
 template <typename T, int COLS>
 __device__ __forceinline__ void join_splits(const SplitArgs& da, int64_t first, int stride, int n, int ct, int kh, int b, bool final_out) {
     __shared__ float2 joined[COLS];
@@ -101,46 +153,13 @@ __device__ __forceinline__ void join_splits(const SplitArgs& da, int64_t first, 
     const Through po(da.part_o + first * COLS * D), pm(da.part_ml + first * COLS * 2);
     for (int i = threadIdx.x; i < cols * per_col; i += 256) {
         const int c = i / per_col, d = 4 * (i - c * per_col);
-        float m = -INFINITY, total = 0.0f;
-        bool loud = false;
-        f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = 0; s0 < n; s0 += 8) {
-            float2 ml[8];
-            f32x4_t x[8];
-#pragma unroll
-            for (int s = 0; s < 8; s++) {  // past the last: the last again, unused
-                const int row = min(s0 + s, n - 1) * stride * COLS + c;
-                ml[s] = pm.get2(2 * row);
-                x[s] = po.get4(row * D + d);
-            }
-            float top = m;
-#pragma unroll
-            for (int s = 0; s < 8; s++) top = fmaxf(top, ml[s].x);
-            const float shift = top == -INFINITY ? 0.0f : top;
-            const float f = __builtin_amdgcn_exp2f(m - shift);
-            total *= f;
-            o *= f;
-            m = top;
-            bool any = false;
-#pragma unroll
-            for (int s = 0; s < 8; s++) any |= is_loud(ml[s].y);
-            if (any && !loud) o *= kLoudDown;
-            loud |= any;
-#pragma unroll
-            for (int s = 0; s < 8; s++) {
-                if (s0 + s >= n) continue;
-                const float w = __builtin_amdgcn_exp2f(ml[s].x - shift);
-                total += fabsf(ml[s].y) * w;
-                o += x[s] * (loud && !is_loud(ml[s].y) ? kLoudDown : 1.0f) * w;
-            }
-        }
-        const int row = COLS * ct + c, qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
+        const Joined j = join_parts(n, [&](int s) { return pm.get2(2 * (s * stride * COLS + c)); },
+                                    [&](int s) { return po.get4((s * stride * COLS + c) * D + d); });
         if (final_out) {
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-            store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + d, o * inv * (loud ? kLoudUp : 1.0f));
+            store_joined<T>(a, j, COLS * ct + c, d, kh, b);
         } else {
-            po.put(c * D + d, o);
-            if (d == 0) joined[c] = make_float2(m, mark_loud(total, loud));
+            po.put(c * D + d, j.o);
+            if (d == 0) joined[c] = make_float2(j.m, mark_loud(j.total, j.loud));
         }
     }
     if (final_out) return;
@@ -162,11 +181,12 @@ __device__ __forceinline__ void finish_split(const SplitArgs& da, int64_t unit, 
     join_splits<T, COLS>(da, unit * da.splits, 16, groups, ct, kh, b, true);
 }
 
-// Joins the splits of one output row: a workgroup per row, every thread 4 dims
-// of every (256 / (D / 4))-th split.
+// Joins the splits of one output row, in the order of the last workgroup's join and so
+// to the same bits: a workgroup per row, a thread per 4 dims of a group of 16 splits.
 template <typename T, int COLS>
 __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
-    __shared__ f32x4_t sums[256];
+    __shared__ f32x4_t group_o[16][64];
+    __shared__ float2 group_ml[16];
     const QuantAttnArgs& a = da.a;
     const QuantPages& p = a.p;
     const int tid = threadIdx.x, D = p.dim;
@@ -178,40 +198,30 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
     const int b = at / p.heads;
     const int ct = row / COLS, col = row % COLS;
     const int t_lo = divide(COLS * ct, a.group, a.group_magic), t_hi = divide(min(rows - 1, COLS * ct + COLS - 1), a.group, a.group_magic);
-    const int qt = divide(row, a.group, a.group_magic), qg = row - qt * a.group;
     const int64_t pos = load_index(p.pos, p.pos_dt, b);
     const TileKeys tk = tile_keys(da, quant_keys(a, pos), pos < 0 ? 0 : quant_count(p, b), t_lo, t_hi);
     if (tk.active == 1) return;
     const int64_t unit = (static_cast<int64_t>(ct) * p.batch + b) * p.heads + kh;
     const float* ml = da.part_ml + (unit * da.splits * COLS + col) * 2;
     const float* po = da.part_o + (unit * da.splits * COLS + col) * D;
-    float m = -INFINITY;
-    for (int s = tid & 63; s < tk.active; s += 64) m = fmaxf(m, ml[s * 2 * COLS]);
-    m = wave_max(m);
-    const float shift = m == -INFINITY ? 0.0f : m;
-    float total = 0.0f;
-    bool loud = false;
-    for (int s = tid & 63; s < tk.active; s += 64) {
-        total += fabsf(ml[s * 2 * COLS + 1]) * __builtin_amdgcn_exp2f(ml[s * 2 * COLS] - shift);
-        loud |= is_loud(ml[s * 2 * COLS + 1]);
-    }
-    loud = __any(loud);
-    total = wave_sum(total);
-    const int pieces = D / 4, groups = 256 / pieces;
+    const int pieces = D / 4, at_once = 256 / pieces, groups = (tk.active + 15) / 16;
     const int piece = tid % pieces, grp = tid / pieces;
-    f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
-    if (grp < groups)
-#pragma unroll 4
-        for (int s = grp; s < tk.active; s += groups)
-            o += *reinterpret_cast<const f32x4_t*>(po + static_cast<int64_t>(s) * COLS * D + 4 * piece) *
-                 (loud && !is_loud(ml[s * 2 * COLS + 1]) ? kLoudDown : 1.0f) * __builtin_amdgcn_exp2f(ml[s * 2 * COLS] - shift);
-    sums[tid] = o;
-    __syncthreads();
-    if (tid < pieces) {
-        for (int i = 1; i < groups; i++) o += sums[tid + i * pieces];
-        const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-        store4<T>(a.out, b * a.os[0] + (kh * a.group + qg) * a.os[1] + qt * a.os[2] + 4 * tid, o * inv * (loud ? kLoudUp : 1.0f));
+    for (int g = grp; g < groups && grp < at_once; g += at_once) {
+        const Joined j = join_parts(min(16, tk.active - 16 * g),
+                                    [&](int s) { return *reinterpret_cast<const float2*>(ml + (16 * g + s) * 2 * COLS); },
+                                    [&](int s) { return *reinterpret_cast<const f32x4_t*>(po + (16 * g + s) * COLS * D + 4 * piece); });
+        if (groups == 1) {
+            store_joined<T>(a, j, row, 4 * piece, kh, b);
+            return;
+        }
+        group_o[g][piece] = j.o;
+        if (piece == 0) group_ml[g] = make_float2(j.m, mark_loud(j.total, j.loud));
     }
+    if (groups == 1) return;
+    __syncthreads();
+    if (tid < pieces)
+        store_joined<T>(a, join_parts(groups, [&](int s) { return group_ml[s]; }, [&](int s) { return group_o[s][piece]; }), row,
+                        4 * piece, kh, b);
 }
 
 // Splits of a column tile's keys: a workgroup a CU, rounded down -- one more to a CU

@@ -22,16 +22,13 @@ struct Buffer {
     bool in_graph = false;  // its address was given to work under capture
 };
 
-constexpr int kStreamRegions = 64;           // streams with arrival counters of their own
-constexpr size_t kRegionWords = 4096;        // of each
-constexpr size_t kCaptureWords = 1u << 22;   // for calls under capture, never given twice
+constexpr size_t kEagerWords = 1u << 14;    // arrival counters of the legacy stream's calls
+constexpr size_t kCaptureWords = 1u << 22;  // of calls under capture, never given twice
 
 struct DeviceState {
     uint32_t* error_word = nullptr;
     Buffer ws[kSlots], ctr[kSlots];
     uint32_t* arrivals = nullptr;
-    hipStream_t streams[kStreamRegions];
-    int stream_count = 0;
     size_t captured_words = 0;
 };
 
@@ -45,7 +42,7 @@ DeviceState g_dev[kMaxDevices];
 static __device__ __align__(256) uint32_t error_words[64];
 
 // Arrival counters: zero when the module loads, like the error words.
-static __device__ __align__(256) uint32_t arrival_words[kStreamRegions * kRegionWords + kCaptureWords];
+static __device__ __align__(256) uint32_t arrival_words[kEagerWords + kCaptureWords];
 
 int current_device(Err e, int* dev) {
     hipError_t st = hipGetDevice(dev);
@@ -141,8 +138,10 @@ uint32_t* arrival_counters(size_t words, hipStream_t stream, Err e, int* status)
     int dev = 0;
     *status = current_device(e, &dev);
     if (*status) return nullptr;
-    if (stream == hipStreamPerThread) return nullptr;  // one handle, a stream for each thread
-    const bool captured = capturing(stream);
+    const bool legacy = !stream || stream == hipStreamLegacy, captured = !legacy && capturing(stream);
+    // other streams come and go: one may get the handle of a destroyed one whose calls
+    // are still in flight, and hipStreamPerThread is a stream for each thread
+    if (!legacy && !captured) return nullptr;
     std::lock_guard<std::mutex> lock(g_mu);
     DeviceState& s = g_dev[dev];
     if (!s.arrivals) {
@@ -155,17 +154,13 @@ uint32_t* arrival_counters(size_t words, hipStream_t stream, Err e, int* status)
         s.arrivals = static_cast<uint32_t*>(p);
     }
     if (captured) {
-        if (words > kCaptureWords - s.captured_words) return nullptr;
-        uint32_t* p = s.arrivals + kStreamRegions * kRegionWords + s.captured_words;
+        const size_t most = std::min<size_t>(env_int("SANDY_QUANT_CAPTURE_WORDS", kCaptureWords), kCaptureWords);
+        if (s.captured_words > most || words > most - s.captured_words) return nullptr;
+        uint32_t* p = s.arrivals + kEagerWords + s.captured_words;
         s.captured_words += words;
         return p;
     }
-    if (words > kRegionWords) return nullptr;
-    int i = 0;
-    while (i < s.stream_count && s.streams[i] != stream) i++;
-    if (i == kStreamRegions) return nullptr;
-    if (i == s.stream_count) s.streams[s.stream_count++] = stream;
-    return s.arrivals + i * kRegionWords;
+    return words <= kEagerWords ? s.arrivals : nullptr;
 }
 
 } // namespace sandy_hip

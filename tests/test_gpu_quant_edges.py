@@ -1,5 +1,8 @@
 """The quantised paged K/V cache on the GPU where it can go wrong: sums that
-cancel, values next to the largest and smallest that a block holds."""
+cancel, values next to the largest and smallest that a block holds;
+switches, graphs and streams that come and go."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -131,3 +134,77 @@ def test_switches_between_calls(ops, monkeypatch):
                         ("SANDY_QUANT_SPLITS", "1"), ("SANDY_QUANT_PROMPT_WGS", "100000"), ("SANDY_QUANT_SPLITS", "4")):
         monkeypatch.setenv(name, value)
         attend(ops, q, kc, vc, table, [1997, 897])
+
+
+def split_call(ops, T=1, dim=64):
+    r = rng(43)
+    table, kc, vc = filled(ops, r, [6000, 2000], 4, dim, 16, "int8", 3)
+    q = from_f32(r.standard_normal((2, 32, T, dim)).astype(np.float32), BF16)
+    args = (q, kc, vc, cuda(table), cuda(np.array([6000 - T, 2000 - T])))
+    want, slack = R.attention(f64(q), R.Cache.of(kc), R.Cache.of(vc), table, [6000 - T, 2000 - T], [T, T], 0, -1.0)
+    return args, want, slack
+
+
+@pytest.mark.parametrize("splits", [2, 16, 17, 40, 255])
+@pytest.mark.parametrize("T,dim,dtype", [(1, 64, BF16), (3, 96, F32), (2, 128, BF16), (1, 256, F32)])
+def test_both_joins_give_the_same_bits(ops, monkeypatch, T, dim, dtype, splits):
+    r = rng(splits + dim)
+    table, kc, vc = filled(ops, r, [9000, 3, 1100], 2, dim, 16, "int8", 5)
+    for at in (5, 300, 301):
+        vc.scales[int(table[0, at]), 0] = 248
+    q = from_f32(r.standard_normal((3, 8, T, dim)).astype(np.float32), dtype)
+    args = (q, kc, vc, cuda(table), cuda(np.array([9000 - T, 0, 1100 - T])))
+    monkeypatch.setenv("SANDY_QUANT_SPLITS", str(splits))
+    last = ops.quant_paged_attention(*args)
+    monkeypatch.setenv("SANDY_QUANT_MERGE_KERNEL", "1")
+    assert torch.equal(ops.quant_paged_attention(*args), last)
+    ops.check_device_errors()
+
+
+def test_graphs_without_counters(ops, monkeypatch):
+    """Captured calls past the counters that the library has for them, beside one that
+    has its own and eager calls; every replay checked."""
+    args, want, slack = split_call(ops)
+    first = ops.quant_paged_attention(*args)
+    R.assert_attention(first, want, slack, "eager")
+    graphs = []
+    for limit in (None, "0", "7", None):
+        if limit is not None:
+            monkeypatch.setenv("SANDY_QUANT_CAPTURE_WORDS", limit)
+        else:
+            monkeypatch.delenv("SANDY_QUANT_CAPTURE_WORDS", raising=False)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            out = ops.quant_paged_attention(*args)
+        graphs.append((graph, out, limit))
+    for _ in range(4):
+        for graph, out, limit in graphs:
+            out.zero_()
+            graph.replay()
+            assert torch.equal(ops.quant_paged_attention(*args), first)
+            torch.cuda.synchronize()
+            assert torch.equal(out, first), f"captured with {limit}"
+    ops.check_device_errors()
+
+
+def test_streams_that_come_and_go(ops):
+    """Streams destroyed one after the other, whose handles may be given again."""
+    from sandyrt_amd import _lib
+    hip = _lib.lib()
+    hip.hipStreamCreate.restype = hip.hipStreamDestroy.restype = ctypes.c_int
+    args, want, slack = split_call(ops)
+    first = ops.quant_paged_attention(*args)
+    R.assert_attention(first, want, slack)
+    torch.cuda.synchronize()
+    for i in range(80):
+        handle = ctypes.c_void_p()
+        assert hip.hipStreamCreate(ctypes.byref(handle)) == 0
+        with torch.cuda.stream(torch.cuda.ExternalStream(handle.value)):
+            for _ in range(2):
+                out = ops.quant_paged_attention(*args)
+            torch.cuda.current_stream().synchronize()
+        assert hip.hipStreamDestroy(handle) == 0
+        assert torch.equal(out, first), f"stream {i}"
+    assert torch.equal(ops.quant_paged_attention(*args), first)
+    ops.check_device_errors()
