@@ -424,11 +424,14 @@ int sandy_hip_quant_paged_read(const SandyQuantCache* k_cache, const SandyQuantC
  * 1/sqrt(inner); inner <= 512.  Queries from count on, and queries that see no
  * key, give zero; a negative position is recorded (SANDY_DEVERR_ATTN_POS) and
  * its sequence gives zero.  Scores, softmax and sums are fp32 or wider, for
- * values the cache holds exactly.  (An e4m3 payload that is NaN, which an append
- * never writes, may reach every query of its sequence.)  out has q's shape and type and may be q
- * itself.  `workspace` holds sandy_hip_quant_paged_attention_workspace() bytes
- * (16-byte aligned; NULL where that is 0): the call's alone while it runs, its
- * contents need not be kept or cleared.
+ * values the cache holds exactly, up to the largest.  (A score is summed before
+ * its block's scale is applied: |q| below 2^110.  An infinite q gives NaN, or
+ * zero where it makes every score -inf.  An e4m3 payload that is NaN, which an
+ * append never writes, may reach every query of its sequence.)  out has q's shape
+ * and type, repeats no memory, and is q itself or apart from it.  `workspace`
+ * holds sandy_hip_quant_paged_attention_workspace() bytes (16-byte aligned; NULL
+ * where that is 0): the call's alone while it runs, its contents need not be kept
+ * or cleared.
  */
 int sandy_hip_quant_paged_attention(const SandyTensor* q, const SandyQuantCache* k_cache,
                                     const SandyQuantCache* v_cache, const SandyTensor* block_table,

@@ -186,6 +186,8 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
     if (status) return status;
     if (!vc || !valid_rank(out)) return fail(e, SANDY_ERR_INVALID, "quant_paged attention requires q and caches");
     if (!same_shape(*q, *out) || out->dtype != q->dtype) return fail(e, SANDY_ERR_INVALID, "attention output shape mismatch");
+    for (int i = 0; i < 4; i++)
+        if (out->dims[i] > 1 && out->strides[i] == 0) return fail(e, SANDY_ERR_INVALID, "attention output rows must not share memory");
     if (window < 0) return fail(e, SANDY_ERR_INVALID, "attention window must be >= 0");
     QuantAttnArgs a{};
     status = check_quant_pages(kc, vc, table, position_offsets, counts, q->dims[0], q->dims[2], e, &a.p);
