@@ -1,6 +1,7 @@
 """The quantised paged K/V cache on the GPU where it can go wrong: sums that
-cancel, values next to the largest and smallest that a block holds;
-switches, graphs and streams that come and go."""
+cancel, values next to the largest and smallest that a block holds,
+prompts of several rounds of keys, long appended blocks, switches, graphs, and
+streams that come and go."""
 import ctypes
 
 import numpy as np
@@ -9,7 +10,7 @@ import torch
 
 from tests import quant_reference as R
 from tests.helpers import from_f32, rng
-from tests.test_gpu_quant_cache import BF16, F32, cuda, empty, f64, filled, make_table
+from tests.test_gpu_quant_cache import BF16, F32, assert_same, cuda, empty, f64, filled, loud_rows, make_table
 
 pytestmark = pytest.mark.gpu
 
@@ -121,6 +122,66 @@ def test_keys_of_the_smallest_scale(ops, form, dim, dtype):
     x = np.zeros((1, 8, 5, dim), np.float32)
     x[..., 3] = 2.0 ** 120 * r.uniform(-1, 1, x.shape[:3])
     attend(ops, from_f32(x, dtype), kc, vc, table, [55])
+
+
+# ------------------------------------------------------------------ long prompts and appends
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("form", ["prompt"], indirect=True)
+@pytest.mark.parametrize("hq,heads,dim", [(8, 2, 64), (4, 2, 96), (4, 1, 256)])
+def test_prompts_behind_long_contexts(ops, form, hq, heads, dim, fmt, dtype):
+    """A wave takes 32 pairs of key tiles a round, the four 4096 keys: contexts on
+    both sides of one round and of two, windows that begin in the second, a NaN block
+    and a page that is not there behind the first."""
+    from sandyrt_amd._lib import SandyError
+    r = rng(dim)
+    T = 5
+    ctx = [4095, 4096, 4097, 4128, 8193, 9000]
+    table, kc, vc = filled(ops, r, ctx, heads, dim, 16, fmt, 7)
+    kc.scales[int(table[5, 400]), 0] = 255   # keys 6400 .. 6415
+    vc.scales[int(table[4, 300]), heads - 1] = 255
+    q = from_f32(r.standard_normal((len(ctx), hq, T, dim)).astype(np.float32), dtype)
+    pos = [c - T for c in ctx]
+    attend(ops, q, kc, vc, table, pos)
+    attend(ops, q, kc, vc, table, pos, window=2500)  # from key 6500 of the last
+    attend(ops, q, kc, vc, table, pos, window=4100)
+    missing = table.copy()
+    missing[:, 270] = 10 ** 6   # keys 4320 .. 4335
+    got = ops.quant_paged_attention(q, kc, vc, cuda(missing), cuda(np.array(pos)))
+    with pytest.raises(SandyError, match="block id outside the pool"):
+        ops.check_device_errors()
+    # as if those keys were not there: the same tables without the page
+    for b in (4, 5):
+        less = np.delete(table[b:b + 1], 270, 1)
+        want, slack = R.attention(f64(q[b:b + 1]), R.Cache.of(kc), R.Cache.of(vc), less, [pos[b] - 16], [T], 0, -1.0)
+        R.assert_attention(got[b:b + 1], want, slack, f"sequence {b}")
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("heads,dim,rows,shift,steps", [
+    (2, 100, 16, 0, [3, 20, 40]), (1, 36, 128, 0, [40, 100, 200]), (2, 128, 32, 1, [5, 30, 60]),
+    (1, 256, 64, 0, [20, 64, 100]), (2, 256, 128, 0, [70, 128, 100])])
+def test_appends_of_large_blocks(ops, heads, dim, rows, shift, steps, fmt, dtype):
+    """Blocks of more pieces than a workgroup's registers hold, by element and by
+    eight, written in several calls whose rows get louder: kept rows are rounded
+    again.  (`shift`: rows that are not 16-byte aligned.)"""
+    r = rng(dim + rows)
+    B = 2
+    table, pages = make_table(r, [sum(steps) + 7] * B, rows)
+    kc, vc = empty(ops, pages, heads, rows, dim, fmt, 1), empty(ops, pages, heads, rows, dim, fmt, 2)
+    kr, vr = R.Cache.of(kc), R.Cache.of(vc)
+    pos = np.array([0, 7])
+    for i, n in enumerate(steps):
+        k, v = (torch.zeros(B, heads, n, dim + shift, dtype=dtype, device="cuda")[..., shift:].copy_(
+            loud_rows(r, (B, heads, n, dim), dtype) * 3.0 ** i) for _ in range(2))
+        ops.quant_paged_append(k, v, kc, vc, cuda(table), cuda(pos))
+        kr.append(f64(k), table, pos, [n] * B)
+        vr.append(f64(v), table, pos, [n] * B)
+        pos = pos + n
+        assert_same(kc, kr, f"k, step {i}")
+        assert_same(vc, vr, f"v, step {i}")
+    ops.check_device_errors()
 
 
 # ------------------------------------------------------------------ switches and streams
