@@ -384,18 +384,24 @@ int launch_format(const QuantAttnArgs& a, hipStream_t stream, Err e) {
 
 } // namespace
 
-// From more than half a workgroup a CU on; fewer leave the chip to the 16-row tiles and
-// their splits.  us, 16-row tiles / here, by the number of workgroups, no / 1000 / 4000
-// keys before the chunk: D 64 160 5.9 / 6.1, 14.0 / 11.9, 24.6 / 28.9, 192 6.1 / 6.2, 14.4 /
-// 12.1, 27.2 / 28.9, 224 6.3 / 6.3, 15.2 / 12.3, 32.3 / 29.4; D 128 128 7.2 / 8.1, 14.1 / 15.6,
-// 34.7 / 36.1, 160 8.6 / 8.9, 19.7 / 16.6, 46.5 / 38.4; f32 192 10.7 / 11.9, 23.4 / 24.3, 54.2
-// / 58.1, 224 12.1 / 13.3, 24.9 / 26.0, 66.4 / 59.6, of D 64 256 10.5 / 11.3, 24.4 / 19.8,
-// 43.9 / 42.3; D 256 192 17.6 / 18.5, 256 23.3 / 22.2,
-// of 2400 keys 54.5 / 41.1.
+// Rows for more than one 16-row tile, and about a workgroup a CU; fewer leave the chip to
+// those tiles, which fill with half the rows and split their keys.  us, 16-row tiles / here:
+// - one sequence, no / 1000 / 4000 keys before the chunk, by the number of workgroups: D 64
+//   192 6.4 / 6.6, 14.7 / 13.4, 28.9 / 32.9, 256 6.7 / 6.8, 16.0 / 14.2, 35.6 / 34.7; D 128
+//   160 8.9 / 9.6, 20.8 / 18.5, 48.1 / 43.2, 192 9.7 / 9.7, 21.1 / 18.7, 47.7 / 42.9; D 256
+//   192 19.7 / 21.8, 38.8 / 37.4, 84 / 80, 256 23.3 / 24.6, 41.7 / 40.7, 105 / 89; f32 D 128
+//   192 10.7 / 12.0, 23.1 / 24.0, 55 / 58, 256 12.5 / 13.6, 24.7 / 25.7, 68 / 61.
+// - batches of mixed contexts of 500 to 8000 keys, where one sequence's workgroups take longest:
+//   D 64 of 32 rows 192 50.7 / 76.5, 384 84 / 98, 768 172 / 131; D 128 of 32 to 64 rows 192
+//   76 to 93 / 89 to 91, 384 138 to 162 / 107 to 109; D 256 192 140 / 147, 384 254 / 201.
+// - the same of 16 rows: D 64 192 34 / 58, 384 57 / 82, 768 97 / 116; D 128 384 99 to 108 / 98 to
+//   103, 768 171 to 202 / 200 to 210; D 256 768 371 / 406.  Short contexts: 8.1 / 8.8, 9.5 / 11.1.
 bool quant_prefill_takes(int64_t batch, int64_t hq, int64_t heads, int64_t tokens, int64_t dim, int64_t max_blocks, bool f32) {
-    const int64_t wgs = (hq / heads * tokens + kRows - 1) / kRows * batch * heads;
-    const int64_t from = env_int("SANDY_QUANT_PROMPT_WGS", dim > 128 || f32 ? 256 : dim > 64 ? 160 : 192);
-    return tokens > 1 && wgs >= from && (!f32 || dim <= 128) && max_blocks > 0;
+    const int64_t rows = hq / heads * tokens, wgs = (rows + kRows - 1) / kRows * batch * heads;
+    if (tokens < 2 || (f32 && dim > 128) || max_blocks == 0) return false;
+    const int forced = env_int("SANDY_QUANT_PROMPT_WGS", 0);
+    if (forced > 0) return wgs >= forced;
+    return rows > 16 && wgs >= (dim > 64 && dim <= 128 && !f32 ? 192 : 256);
 }
 
 int launch_quant_prefill(const QuantAttnArgs& a, int32_t format, hipStream_t stream, Err e) {

@@ -158,6 +158,18 @@ def test_prompts_behind_long_contexts(ops, form, hq, heads, dim, fmt, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("T", [2, 3])
+def test_few_queries_of_many_sequences(ops, T, dtype):
+    """Batches on both sides of the choice between the kernels: one and two 16-row tiles
+    a kv head, mixed contexts."""
+    r = rng(T)
+    ctx = [4500 if b == 40 else int(r.integers(T, 300)) for b in range(96)]
+    table, kc, vc = filled(ops, r, ctx, 4, 64, 16, "e4m3", 5)
+    q = from_f32(r.standard_normal((96, 32, T, 64)).astype(np.float32), dtype)
+    attend(ops, q, kc, vc, table, [c - T for c in ctx])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 @pytest.mark.parametrize("heads,dim,rows,shift,steps", [
     (2, 100, 16, 0, [3, 20, 40]), (1, 36, 128, 0, [40, 100, 200]), (2, 128, 32, 1, [5, 30, 60]),

@@ -1,4 +1,6 @@
-"""CPU checks of the quantised paged K/V cache's refusals at its edges."""
+"""CPU checks of the quantised paged K/V cache's refusals at its edges, and its choice between kernels."""
+import ctypes
+
 import pytest
 
 from sandyrt_amd import _lib
@@ -12,3 +14,22 @@ def test_outputs_that_repeat_memory():
         q = tensor(shape, strides=strides)
         with pytest.raises(_lib.SandyError, match="output rows must not share memory"):
             _lib.call("sandy_hip_quant_paged_attention", q, cache(), other(), TABLE, POS, None, 0, -1.0, q, None, 0, stream=0)
+
+
+def test_few_rows_a_sequence_keep_the_tiles_that_split():
+    """A call on 16-row tiles splits a wide table's keys and so needs a workspace; the
+    prompt kernel, which does not, takes many workgroups of more rows than such a tile."""
+    need = ctypes.c_size_t(0)
+
+    def splits(batch, q_heads, tokens, heads, dim=64, dtype=_lib.BF16):
+        _lib.dcall("sandy_hip_quant_paged_attention_workspace", tensor((batch, q_heads, tokens, dim), dtype),
+                   cache(prefix=heads, inner=dim), tensor((batch, 1024), _lib.I32), 0, ctypes.byref(need))
+        return need.value > 0
+
+    for batch, q_heads, tokens, heads in ((48, 32, 2, 4), (96, 32, 2, 4), (120, 32, 2, 4), (40, 12, 16, 12), (64, 16, 4, 4), (20, 12, 2, 12)):
+        assert splits(batch, q_heads, tokens, heads)
+        assert splits(batch, q_heads, tokens, heads, 128)
+    assert splits(63, 32, 3, 4) and not splits(64, 32, 3, 4)              # 252 and 256 workgroups
+    assert splits(47, 32, 3, 4, 128) and not splits(48, 32, 3, 4, 128)    # 188 and 192
+    assert splits(48, 32, 3, 4, 128, _lib.F32) and not splits(64, 32, 3, 4, 128, _lib.F32)
+    assert splits(64, 32, 3, 4, 256, _lib.F32) and not splits(64, 32, 3, 4, 256)
