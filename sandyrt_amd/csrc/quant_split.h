@@ -235,7 +235,8 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
 // None has less than kMinPairs pairs at the longest context the call can have.
 inline void set_splits(SplitArgs* d, int64_t units, int64_t dim, int64_t cap, int64_t window, int64_t tokens) {
     const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tokens + 16) : cap;
-    const int64_t most = std::min<int64_t>(std::max<int64_t>((keys + 31) / 32 / kMinPairs, 1), 256);
+    // (and the threads of a launch stay below 2^32, however many are asked for)
+    const int64_t most = std::clamp<int64_t>((keys + 31) / 32 / kMinPairs, 1, std::clamp<int64_t>((UINT32_MAX / 256) / units, 1, 256));
     const int forced = env_int("SANDY_QUANT_SPLITS", 0);
     auto of = [&](int64_t workgroups) {
         return static_cast<int>(std::clamp<int64_t>(forced > 0 ? forced : workgroups / units, 1, most));

@@ -33,3 +33,15 @@ def test_few_rows_a_sequence_keep_the_tiles_that_split():
     assert splits(47, 32, 3, 4, 128) and not splits(48, 32, 3, 4, 128)    # 188 and 192
     assert splits(48, 32, 3, 4, 128, _lib.F32) and not splits(64, 32, 3, 4, 128, _lib.F32)
     assert splits(64, 32, 3, 4, 256, _lib.F32) and not splits(64, 32, 3, 4, 256)
+
+
+def test_forced_splits_of_many_tiles(monkeypatch):
+    """More workgroups than a launch can have are not asked for."""
+    need = ctypes.c_size_t(0)
+    monkeypatch.setenv("SANDY_QUANT_SPLITS", "256")
+    for batch in (3, 9000, 1 << 20):
+        _lib.dcall("sandy_hip_quant_paged_attention_workspace", tensor((batch, 16, 1, 64)), cache(prefix=8),
+                   tensor((batch, 4096), _lib.I32), 0, ctypes.byref(need))
+        units, part = 8 * batch, 16 * (64 + 2) * 4
+        splits = max(1, need.value // part // units)
+        assert splits == min(256, max(1, (2 ** 32 - 1) // 256 // units))
