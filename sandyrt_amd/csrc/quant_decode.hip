@@ -13,11 +13,12 @@
 //   - V through the wave's own LDS rows, back by ds_read_b64_tr_b8, which gives a
 //     lane one dim of 8 keys -- the A operand of O^T in the order that P leaves S^T.
 //
-// 32 sequences of 512 to 4096 keys, 32 / 4 heads of 64: 37 MB in 14.7 us (2.5 TB/s; a
-// copy would take 7.2); one sequence of 32749 keys 13.4 us; 64 with a window of 1024,
-// 8 / 2 heads of 256: 19.5 us; 32 of 8000 keys 31 us (4.2 TB/s).  Short contexts are
-// latency: a call of up to 128 keys takes 4.6 us, of 600 7.0, the chain position, block
-// table, payload, join.  Workgroups of 8 waves: 15.6 us for the first, 20.3 the third.
+// In a graph, 32 sequences of 512 to 4096 keys, 32 / 4 heads of 64: 37 MB in 15.7 us (2.4
+// TB/s; a copy would take 7.2); one sequence of 32749 keys 13.8 us; 64 with a window of
+// 1024, 8 / 2 heads of 256: 20.2 us; 32 of 8000 keys 32.3 us (4.1 TB/s).  Vector
+// instructions issue in 11 to 20 % of these cycles, MFMA in 2 to 6 %.  Short contexts are
+// latency: a call of up to 128 keys takes 4.7 us, of 600 7.3, the chain position, block
+// table, payload, join.
 #include "quant_split.h"
 
 namespace sandy_hip {
@@ -26,7 +27,7 @@ namespace {
 template <typename T, int FORMAT, int DP>
 struct DecodeGeo {
     static constexpr int kChunks = DP / 64;  // 16-byte pieces a lane holds of a K (V) tile
-    static constexpr int kRing = DP == 256 ? 1 : 2;  // pairs in flight (D 256 with two: 22.5 us to 19.6)
+    static constexpr int kRing = DP == 256 ? 1 : 2;  // pairs in flight (D 256 with two: 38 us to 20)
     static constexpr int kWaves = DP == 64 ? 3 : DP == 256 && std::is_same_v<T, F32> ? 1 : 2;  // a SIMD
     static constexpr int VP = DP + 16;       // bytes of a V row in LDS: column reads spread over the banks
     static constexpr int kV = 32 * VP;       // a wave's V rows

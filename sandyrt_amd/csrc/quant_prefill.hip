@@ -11,11 +11,12 @@
 // (int8) or the conversion (e4m3).  f32 queries and all weights enter as three bf16
 // numbers (exact).
 //
-// 2048 queries of 32 / 4 heads of 64 (e4m3, causal) take 47 us, 364 TFLOP/s; int8 is
-// slower (three instructions convert two payloads, one of e4m3's).  Weights in two parts
-// took 40 us, but kept 16 of their 24 bits.  With two, slower still: K in LDS tiles for
-// several waves (52 to 57 us), two row tiles a wave (D 128 34 us against 20), the keys
-// split over workgroups as well (69 against 45).
+// 2048 queries of 32 / 4 heads of 64 (e4m3, causal) take 48 to 54 us, 318 to 358 TFLOP/s;
+// int8 62 where e4m3 takes 54 (three instructions convert two payloads, one of e4m3's),
+// f32 68.  No single unit bounds it: vector instructions issue in 65 % of the cycles, MFMA
+// in 27 %.  bf16 queries' weights in two parts took 40 to 49 us, but kept 16 of 24 bits;
+// beside those, other layouts were slower: K in LDS tiles for several waves (52 to 57),
+// two row tiles a wave (D 128 34 against 20), the keys split over workgroups (69 against 45).
 #include "quant_mfma.h"
 
 #include <algorithm>
@@ -41,7 +42,7 @@ struct PromptGeo {
     static constexpr int kMerge = 4 * 16 * 64 * 4;  // one 32-dim tile of every wave
     static constexpr int NQ = kF32 ? 3 : 1, KS = DP / 16;
     // Q in LDS, once for the four waves: two waves a SIMD then hold the rest in their 256
-    // registers (3000 queries of 8 / 2 heads: 77 us, with Q in one wave's 512 98)
+    // registers (3000 queries of 8 / 2 heads: 87 us, with Q in one wave's 512 114)
     static constexpr bool kQLds = DP == 256;
     static constexpr int kQ = kQLds ? NQ * KS * 64 * 16 : 0;
     static constexpr int kBytes = std::max(4 * kV, kMerge) + 4 * 32 * 8 + kQ;
@@ -50,8 +51,8 @@ struct PromptGeo {
 
 // Workgroup i's place in the list by falling length: every second round of the
 // 256 CUs backwards, so that the workgroups a CU gets add up to about the same (1024
-// queries 16.5 us so and 18.0 in order, 4 chunks of 700 of D 128 40.7 and 43.8, 8 of
-// 300 behind 100 to 2000 keys 47.5 and 53.5).
+// queries 19.2 us so and 22.3 in order, 8 chunks of 300 of D 128 behind 100 to 2000 keys
+// 62 and 69, 4 of 700 without a context 39 and 37).
 __device__ __forceinline__ uint32_t snake(uint32_t i, uint32_t n) {
     const uint32_t round = i & ~255u;
     return (i & 256) ? round + min(256u, n - round) - 1 - (i - round) : i;
@@ -223,7 +224,7 @@ __global__ __launch_bounds__(256, (PromptGeo<T, FORMAT, DP>::kWaves)) void quant
                 else qi = qv[i][s];
                 sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, __builtin_bit_cast(bf16x8_t, qi), sc, 0, 0, 0);
             }
-            // int8's conversions all at once would not leave registers for two waves (42 us, 55)
+            // int8's conversions all at once would not leave registers for two waves (1500 queries 42 us, 59)
             if (DP == 256 && s % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll

@@ -225,13 +225,13 @@ __global__ __launch_bounds__(256) void quant_merge_kernel(SplitArgs da) {
 }
 
 // Splits of a column tile's keys: a workgroup a CU, rounded down -- one more to a CU
-// halves nothing and is joined as well (D 128, 188 column tiles of 2000 keys 20.9 us in
-// one piece, 26.0 in two, 29.7 in three; D 256, 80 of them 22.1 in 3, 25.9 in 4).  Where
+// halves nothing and is joined as well (D 128, 188 column tiles of 2000 keys 24.0 us in
+// one piece, 26.2 in two, 29.1 in three; D 256, 80 of them 20.9 in 3, 24.6 in 4).  Where
 // that leaves a tile more than long_pairs pairs, up to four a CU, so that the longest
-// sequences end with the others: 300 tiles of 500 to 6000 keys, D 64 41 -> 35 us, D 128
-// 85 -> 64, D 256 158 -> 112; of 8000 keys each 71 -> 66, 142 -> 118, 271 -> 233.
+// sequences end with the others: 300 tiles of 500 to 6000 keys, D 64 43.5 -> 39.0 us,
+// D 128 75 -> 67, D 256 130 -> 115; of 8000 keys each 72 -> 67, 143 -> 125, 270 -> 228.
 // long_pairs 64 (2048 keys), at D 64, whose tiles need least of a CU, 32: 32 sequences
-// of 512 to 4096 keys 16.3 -> 14.9 (D 128 at 32: 150 tiles of 2000 keys 19.4 -> 24.0).
+// of 512 to 4096 keys 16.3 -> 14.9 (D 128 at 32: 150 tiles of 2000 keys 19.4 -> 24.2).
 // None has less than kMinPairs pairs at the longest context the call can have.
 inline void set_splits(SplitArgs* d, int64_t units, int64_t dim, int64_t cap, int64_t window, int64_t tokens) {
     const int64_t keys = window > 0 && window < cap ? std::min(cap, window + tokens + 16) : cap;
