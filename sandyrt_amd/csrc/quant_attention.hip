@@ -6,6 +6,7 @@
 #include "quant_attention.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace sandy_hip {
 namespace {
@@ -200,7 +201,8 @@ extern "C" int sandy_hip_quant_paged_attention(const SandyTensor* q, const Sandy
         a.os[i] = out->strides[i];
     }
     a.window = window;
-    a.scale_log2 = (scale <= 0.0 ? 1.0f / sqrtf(static_cast<float>(a.p.dim)) : static_cast<float>(scale)) * 1.44269504088896341f;
+    // rounded once: what it is off by goes into every exponent times its score
+    a.scale_log2 = static_cast<float>((scale <= 0.0 ? 1.0 / std::sqrt(static_cast<double>(a.p.dim)) : scale) * 1.4426950408889634074);
     a.hq = static_cast<int32_t>(q->dims[1]);
     a.group = a.hq / a.p.heads;
     a.group_magic = a.group == 1 ? UINT32_MAX : static_cast<uint32_t>((uint64_t{1} << 32) / static_cast<uint32_t>(a.group));
