@@ -589,6 +589,57 @@ int sandy_hip_decode_linear(const SandyTensor* x, const SandyTensor* ln_weight, 
                             const SandyTensor* residual, const SandyTensor* out, void* stream, char* err,
                             size_t err_cap);
 
+/* ---------------------------------------------------------------- 8-bit rows and weights */
+
+/*
+ * No counterpart in the reference, whose operands keep the model's type.  A matrix [rows, k] in 8 bits is e4m3
+ * payloads (U8, [.., rows, k], unit inner stride, rows apart by any pitch that keeps them from overlapping) and
+ * scale bytes (U8, contiguous): [.., rows, ceil(k / 128)] with a byte for every 128 columns of a row, or
+ * [.., ceil(rows / 128), ceil(k / 128)] with one for every 128 columns of 128 rows.  Values are
+ * payload * 2^(c - 127) with c the block's byte; c = 255 stands for NaN.  Blocks at the ends may be short.
+ * Ranks 2 or 3.
+ */
+
+/*
+ * x (F32 or BF16, any strides) into payloads of its shape and scales; block_rows 1 or 128.  A block's scale is
+ * the smallest power of two (2^-126 at the least) whose 448-fold holds its largest magnitude, and every value is
+ * rounded once, to the nearest payload, ties to even.  A block with a value that is not finite, or above
+ * 448 * 2^119, gets c = 255 and payloads 0.  Bytes between k and the pitch are left as they were.  Outputs share no
+ * memory with x or one another.
+ */
+int sandy_hip_block_quant(const SandyTensor* x, int64_t block_rows, const SandyTensor* payload,
+                          const SandyTensor* scales, void* stream, char* err, size_t err_cap);
+
+/* What such a matrix stands for: out contiguous, F32 or BF16 (every value exact in either, but for bf16 below
+ * 2^-126). */
+int sandy_hip_block_dequant(const SandyTensor* payload, const SandyTensor* scales, const SandyTensor* out,
+                            void* stream, char* err, size_t err_cap);
+
+/*
+ * Linear over matrices in 8 bits: out[.., m, n] = bias[n] + sum_k x[m, k] * weight[n, k], summed in f32 and
+ * rounded once.  x [.., M, k] with a scale for every row, weight [n, k] with either kind of scales, bias NULL or [n]
+ * of out's type, out F32 or BF16 with unit inner stride.  Rows of x and of weight begin on 16-byte boundaries
+ * (the whole 16-byte pieces of a row are read, what lies past k ignored); rows of x, and of out, are evenly spaced
+ * through all their leading dimensions; out shares no memory with the operands.  A block whose scale byte is 255
+ * makes its row (or its 128 columns) NaN.  For bf16 outputs the matrix instructions drop, of eight neighbouring
+ * products, what lies 13 bits below the largest (less than 2^-10 of the terms' magnitudes in all, far below what the
+ * operands' own rounding changes); f32 outputs are sums of exact products, at half the rate, in which values below
+ * 2^-126 are rounded as bf16 holds them.
+ */
+int sandy_hip_quant_linear(const SandyTensor* x, const SandyTensor* x_scales, const SandyTensor* weight,
+                           const SandyTensor* weight_scales, const SandyTensor* bias, const SandyTensor* out,
+                           void* stream, char* err, size_t err_cap);
+
+/*
+ * The grouped form (sandy_hip_moe_matmul over matrices in 8 bits, weights [E, n, k]): rows expert_offsets[e] ..
+ * expert_offsets[e + 1] - 1 of x [N, k] times weight[e]^T.  expert_offsets E + 1 values (I32 or I64); an expert whose
+ * two are out of order or out of 0..N is recorded (SANDY_DEVERR_OFFSETS) and writes nothing (a row that two others
+ * then both claim holds either's product).  Rows of out that no expert has are left as they were.
+ */
+int sandy_hip_quant_moe_matmul(const SandyTensor* x, const SandyTensor* x_scales, const SandyTensor* expert_offsets,
+                               const SandyTensor* weight, const SandyTensor* weight_scales, const SandyTensor* out,
+                               void* stream, char* err, size_t err_cap);
+
 /* ---------------------------------------------------------------- safetensors weights
  *
  * EagerSafeTensorWeights (src/weight/SafeTensorWeights.h:29-48,

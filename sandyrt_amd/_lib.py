@@ -198,6 +198,10 @@ SIGNATURES = {
     "sandy_hip_quant_paged_read": [*[C.c_void_p] * 7, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_quant_paged_attention": [*[C.c_void_p] * 6, C.c_int64, C.c_double, C.c_void_p, C.c_void_p, C.c_size_t,
                                         C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_block_quant": [C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_block_dequant": [*[C.c_void_p] * 3, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_linear": [*[C.c_void_p] * 6, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_quant_moe_matmul": [*[C.c_void_p] * 6, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_topk": [T, C.c_int64, C.c_int64, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_gather": [T, T, T, C.c_int64, C.c_int64, T, T, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_matmul": [T, T, T, C.c_int32, T, C.c_void_p, ERR, C.c_size_t],
@@ -308,6 +312,14 @@ def pack(t: torch.Tensor) -> bytes:
     if rank > MAX_RANK:
         raise SandyError(1, f"tensor rank {rank} exceeds {MAX_RANK}")
     return _TENSOR_LAYOUT[rank].pack(t.data_ptr(), _TORCH_TO_CODE[t.dtype], rank, *t.shape, *t.stride(), 0)
+
+
+def pack_bytes(t: torch.Tensor) -> bytes:
+    """pack, of a view whose one-byte elements an entry point takes as U8."""
+    rank = t.dim()
+    if rank > MAX_RANK:
+        raise SandyError(1, f"tensor rank {rank} exceeds {MAX_RANK}")
+    return _TENSOR_LAYOUT[rank].pack(t.data_ptr(), U8, rank, *t.shape, *t.stride(), 0)
 
 
 # SandyQuantCache: pool, scales, format, reserved, page_size, prefix, inner, num_pages

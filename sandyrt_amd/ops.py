@@ -460,10 +460,11 @@ def _packed(x):
 
 
 def _quant_call(name, at, tensors, *args):
-    """An entry point of the quantised cache, on the device `at` of its tensors."""
+    """An entry point of the 8-bit operators, on the device `at` of its tensors."""
     for t in tensors:
         if t is not None and t.get_device() != at:
-            raise SandyError(1, "quant_paged tensors must live on one device")
+            raise SandyError(1, "quant_paged tensors must live on one device" if name.startswith("sandy_hip_quant_paged")
+                             else "sandyrt_amd tensors must live on one device")
     if at < 0:
         raise SandyError(1, "sandyrt_amd tensors must live on the GPU")
     if at == torch._C._cuda_getDevice():
@@ -552,6 +553,82 @@ def quant_paged_attention(q, k_cache: QuantPagedCache, v_cache: QuantPagedCache,
         if now <= need:
             raise
         attend(now)
+    return out
+
+
+# ------------------------------------------------------------------ rows and weights in 8 bits
+@dataclass
+class QuantMatrix:
+    """A matrix held in 8 bits: payload [.., rows, k] of float8_e4m3fn (unit inner
+    stride) and scales uint8, contiguous: [.., rows, ceil(k / 128)], a byte for
+    every 128 columns of a row, or [.., ceil(rows / 128), ceil(k / 128)], one
+    for every 128 columns of 128 rows.  Values are payload * 2^(c - 127) with c
+    the block's byte; 255 stands for NaN."""
+
+    payload: torch.Tensor
+    scales: torch.Tensor
+
+    @staticmethod
+    def empty(shape, block_rows: int = 1, device="cuda"):
+        """A matrix without contents, its rows on 16-byte boundaries as the products take them."""
+        *lead, rows, k = shape
+        payload = torch.empty(*lead, rows, (k + 15) // 16 * 16, dtype=torch.float8_e4m3fn, device=device)
+        return QuantMatrix(payload[..., :k] if k % 16 else payload,
+                           torch.empty(*lead, -(-rows // block_rows), -(-k // 128), dtype=torch.uint8, device=device))
+
+    def pack(self):
+        """The bytes of the SandyTensors describing payload and scales."""
+        if self.payload.dtype != torch.float8_e4m3fn:
+            raise SandyError(1, "block_quant payloads must be float8_e4m3fn")
+        if self.scales.dtype != torch.uint8:
+            raise SandyError(1, "block_quant scales must be uint8")
+        return _lib.pack_bytes(self.payload), _lib.pack_bytes(self.scales)
+
+
+def block_quant(x: torch.Tensor, block_rows: int = 1, out: QuantMatrix | None = None) -> QuantMatrix:
+    """x [.., rows, k] (f32 or bf16, any strides) in 8 bits: a power-of-two scale
+    for every 128 columns of a row (block_rows 1: activations) or of 128 rows
+    (128: weights), the smallest that holds the block's largest magnitude.  A
+    block with a value that is not finite stands for NaN."""
+    if out is None:
+        if block_rows not in (1, 128):
+            raise SandyError(1, "block_quant block_rows must be 1 or 128")
+        if x.dim() not in (2, 3):
+            raise SandyError(1, "block_quant x must be f32 or bf16 of rank 2 or 3")
+        out = QuantMatrix.empty(x.shape, block_rows, x.device)
+    _quant_call("sandy_hip_block_quant", x.get_device(), (out.payload, out.scales), pack(x), int(block_rows), *out.pack())
+    return out
+
+
+def block_dequant(q: QuantMatrix, dtype=torch.bfloat16, out=None) -> torch.Tensor:
+    """What a matrix in 8 bits stands for."""
+    out = torch.empty(q.payload.shape, dtype=dtype, device=q.payload.device) if out is None else out
+    _quant_call("sandy_hip_block_dequant", q.payload.get_device(), (q.scales, out), *q.pack(), pack(out))
+    return out
+
+
+def quant_linear(x: QuantMatrix, weight: QuantMatrix, bias=None, dtype=torch.bfloat16, out=None) -> torch.Tensor:
+    """bias + x @ weight^T of two matrices in 8 bits, summed in f32 and rounded once
+    to out's type: x [.., m, k] from block_quant(x), weight [n, k] from
+    block_quant(w, 128) (or 1), bias [n] of out's type or None."""
+    payload = x.payload
+    if out is None:
+        out = torch.empty((*payload.shape[:-1], weight.payload.shape[-2]), dtype=dtype, device=payload.device)
+    _quant_call("sandy_hip_quant_linear", payload.get_device(), (x.scales, weight.payload, weight.scales, bias, out),
+                *x.pack(), *weight.pack(), _packed(bias), pack(out))
+    return out
+
+
+def quant_moe_matmul(x: QuantMatrix, expert_offsets, weight: QuantMatrix, dtype=torch.bfloat16, out=None) -> torch.Tensor:
+    """moe_matmul over matrices in 8 bits: rows expert_offsets[e] ..
+    expert_offsets[e + 1] - 1 of x [n, k] times weight[e]^T, weight [E, m, k].
+    Rows that no expert has are left as they were (without `out`: unset)."""
+    payload = x.payload
+    if out is None:
+        out = torch.empty((*payload.shape[:-1], weight.payload.shape[-2]), dtype=dtype, device=payload.device)
+    _quant_call("sandy_hip_quant_moe_matmul", payload.get_device(),
+                (x.scales, expert_offsets, weight.payload, weight.scales, out), *x.pack(), pack(expert_offsets),
+                *weight.pack(), pack(out))
     return out
 
 

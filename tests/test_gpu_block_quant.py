@@ -1,0 +1,274 @@
+"""Rows and weights in 8 bits on the GPU: block_quant, block_dequant, quant_linear and quant_moe_matmul against plain
+64-bit numpy."""
+import numpy as np
+import pytest
+import torch
+
+from sandyrt_amd import ops
+from tests import block_quant_reference as R
+
+pytestmark = pytest.mark.gpu
+NAN8 = 0x7f
+STEP = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}  # half a step of the type, relative
+
+
+def f64(t):
+    return t.cpu().double().numpy()
+
+
+def loud(rng, shape):
+    """Rows and blocks of very different sizes."""
+    x = rng.standard_normal(shape) * np.exp2(rng.integers(-12, 12, (*shape[:-1], 1)))
+    return x * np.exp2(rng.integers(-3, 4, (shape[-1] + 127) // 128)).repeat(128)[:shape[-1]]
+
+
+# ------------------------------------------------------------------ into 8 bits and back
+@pytest.mark.parametrize("block", [1, 128])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,k", [(1, 1), (1, 7), (1, 2048), (3, 127), (17, 128), (5, 129), (127, 200), (128, 256), (130, 1000), (300, 72)])
+def test_block_quant(rows, k, dtype, block):
+    x = torch.from_numpy(loud(np.random.default_rng(rows * 7 + k), (rows, k))).to(dtype)
+    q = ops.block_quant(x.cuda(), block)
+    payload, code = R.quantise(f64(x), block)
+    np.testing.assert_array_equal(q.scales.cpu().numpy(), code)
+    np.testing.assert_array_equal(f64(q.payload.float()), payload)
+    for out in (torch.float32, torch.bfloat16):
+        back = ops.block_dequant(q, out)
+        assert back.dtype == out
+        np.testing.assert_array_equal(f64(back), R.values(payload, code))  # exact in bf16 too
+
+
+@pytest.mark.parametrize("block", [1, 128])
+def test_block_quant_strides(block):
+    rng = np.random.default_rng(block)
+    base = torch.from_numpy(loud(rng, (2, 211, 403))).float().cuda()
+    for x in (base, base.transpose(1, 2), base[:, 3:, 5:], base[:, :1].expand(2, 40, 403), base[..., ::3], base[1], base[1].t(),
+              base[0, 7:8], base.bfloat16()[:, 1:, 1:]):
+        q = ops.block_quant(x, block)
+        flat = [(x, q.payload, q.scales)] if x.dim() == 2 else list(zip(x, q.payload, q.scales))
+        for part, payload, scales in flat:
+            want, code = R.quantise(f64(part), block)
+            np.testing.assert_array_equal(scales.cpu().numpy(), code)
+            np.testing.assert_array_equal(f64(payload.float()), want)
+
+
+@pytest.mark.parametrize("block", [1, 128])
+def test_block_quant_keeps_what_lies_between_rows(block):
+    x = torch.randn(130, 77, device="cuda")
+    held = torch.full((2, 132, 83), 0x55, dtype=torch.uint8, device="cuda")
+    q = ops.QuantMatrix(held[1, 1:131, 3:80].view(torch.float8_e4m3fn), torch.empty(130 if block == 1 else 2, 1, dtype=torch.uint8, device="cuda"))
+    assert ops.block_quant(x, block, out=q) is q
+    want, _ = R.quantise(f64(x), block)
+    np.testing.assert_array_equal(f64(q.payload.float()), want)
+    held[1, 1:131, 3:80] = 0x55
+    assert bool((held == 0x55).all())
+
+
+def test_block_quant_values_of_all_kinds():
+    tiny, big = 2.0 ** -149, 448.0 * 2.0 ** 119
+    rows = [
+        [0.0] * 130, [-0.0, 0.0], [tiny, -3 * tiny], [2.0 ** -126 * 448, 1e-38], [448.0, 1.0], [448.5, 1.0], [-449.0, 0.3],
+        [big, -1.0], [np.nextafter(np.float32(big), np.float32(np.inf)), 1.0], [3.4e38, 1.0], [np.inf, 1.0], [1.0, -np.inf],
+        [np.nan, 2.0], [1.0, np.nan], [464.0 / 448, 1.0 / 1024], [17.0, 19.0, 21.0, 23.0, 25.0, 448.0],
+        [2.0 ** -9 * 1.5, 2.0 ** -9 * 0.5, 2.0 ** -9 * 2.5, 448.0],
+    ]
+    x = np.zeros((len(rows), 130), np.float32)
+    for i, row in enumerate(rows):
+        x[i, :len(row)] = row
+    x[:, 129] = 5.0  # the second block is of its own
+    q = ops.block_quant(torch.from_numpy(x).cuda())
+    payload, code = R.quantise(x.astype(np.float64), 1)
+    np.testing.assert_array_equal(q.scales.cpu().numpy(), code)
+    assert (code[8:14, 0] == 255).all() and (code[:8, 0] != 255).all() and (code[:, 1] != 255).all()
+    np.testing.assert_array_equal(f64(q.payload.float()), payload)
+    back = ops.block_dequant(q, torch.float32)
+    np.testing.assert_array_equal(f64(back), R.values(payload, code))
+    # a weight's block: one value that is not finite takes its 128 rows and columns along
+    w = torch.randn(200, 300, device="cuda")
+    w[150, 140] = float("nan")
+    lost = torch.isnan(ops.block_dequant(ops.block_quant(w, 128)))
+    want = torch.zeros_like(lost)
+    want[128:, 128:256] = True
+    assert bool((lost == want).all())
+
+
+def test_block_quant_of_nothing():
+    assert ops.block_quant(torch.empty(0, 300, device="cuda")).payload.shape == (0, 300)
+    assert ops.block_dequant(ops.block_quant(torch.empty(4, 0, device="cuda"))).shape == (4, 0)
+
+
+# ------------------------------------------------------------------ products
+def product(x, w, bias=None):
+    y = R.held(x) @ R.held(w).T
+    return y if bias is None else y + f64(bias)
+
+
+def same(got, want, dtype):
+    """Sums that are exact in f32: f32 outputs equal, bf16 ones their nearest value."""
+    torch.testing.assert_close(got.cpu(), torch.from_numpy(want).float().to(dtype), rtol=0, atol=0, equal_nan=True)
+
+
+ROWS = [1, 2, 15, 16, 17, 31, 33, 64, 65, 100, 129, 200, 257, 400]
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 128), (17, 15), (100, 16), (129, 300), (300, 127), (256, 512), (515, 1153), (31, 5600)])
+@pytest.mark.parametrize("rows", ROWS)
+def test_quant_linear_of_whole_numbers(rows, n, k):
+    rng = np.random.default_rng(rows * 1000 + n + k)
+    x, w = R.whole(rng, (rows, k), 1, pad=16 * (rows % 3)), R.whole(rng, (n, k), 128 if (rows + n) % 2 else 1, pad=16 * (n % 2))
+    want = product(x, w)
+    same(ops.quant_linear(x, w, dtype=torch.float32), want, torch.float32)
+    bias = torch.from_numpy(rng.integers(-50, 51, n)).bfloat16().cuda()
+    same(ops.quant_linear(x, w, bias), want + f64(bias), torch.bfloat16)
+
+
+@pytest.mark.parametrize("rows,n,k", [(1, 2048, 2048), (7, 333, 999), (40, 500, 704), (64, 1000, 2048), (150, 700, 1500), (515, 640, 2816),
+                                      (1100, 1030, 640)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quant_linear_of_rows(rows, n, k, dtype):
+    rng = np.random.default_rng(rows + n)
+    x = ops.block_quant(torch.from_numpy(loud(rng, (rows, k))).float().cuda())
+    w = ops.block_quant(torch.from_numpy(rng.standard_normal((n, k)) / k ** 0.5).float().cuda(), 128)
+    got, xv, wv = f64(ops.quant_linear(x, w, dtype=dtype)), R.held(x), R.held(w)
+    want = xv @ wv.T
+    # f32: products are exact, a sum of k of them in any order is off by less than k steps of its terms' magnitudes (2^-23
+    # each, should the adder cut off).  bf16: of eight products the matrix instruction drops what lies 13 bits below
+    # the largest, less than 2^-13 of it for each of the other seven: 2^-10 of the terms' magnitudes at the most.  Then one
+    # rounding to the output's type.
+    sums = k * 2.0 ** -23 if dtype == torch.float32 else 2.0 ** -10
+    bound = sums * (np.abs(xv) @ np.abs(wv).T) + STEP[dtype] * np.abs(want)
+    assert (np.abs(got - want) <= bound * 1.01).all()
+    # and of the whole: f32 sums of k terms whose errors do not line up
+    if dtype == torch.float32:
+        assert np.linalg.norm(got - want) <= (STEP[dtype] + 2.0 ** -24 * k ** 0.5) * np.linalg.norm(want)
+
+
+def test_quant_linear_of_scales_of_all_sizes():
+    rng = np.random.default_rng(5)
+    for low, high in ((1, 30), (100, 160), (215, 246)):
+        x, w = R.whole(rng, (70, 256), 1), R.whole(rng, (40, 256), 1)
+        x.scales.copy_(torch.from_numpy(rng.integers(low, high, (70, 1)).repeat(2, 1)))  # a row's blocks alike: sums stay exact
+        w.scales.fill_(254 - (low + high) // 2 if high > 200 else 127)
+        same(ops.quant_linear(x, w, dtype=torch.float32), product(x, w), torch.float32)
+
+
+@pytest.mark.parametrize("rows", [3, 70, 300])
+def test_quant_linear_of_nan(rows):
+    rng = np.random.default_rng(rows)
+    x, w = R.whole(rng, (rows, 300), 1), R.whole(rng, (200, 300), 128)
+    x.scales[1, 2] = 255
+    w.scales[1, 0] = 255
+    x.payload.view(torch.uint8)[2, 5] = NAN8
+    want = product(x, w)
+    assert np.isnan(want[1]).all() and np.isnan(want[2]).all() and np.isnan(want[:, 128:]).all() and not np.isnan(want[0, :128]).any()
+    same(ops.quant_linear(x, w, dtype=torch.float32), want, torch.float32)
+
+
+@pytest.mark.parametrize("rows", [2, 5, 90])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_quant_linear_layouts(rows, dtype):
+    """[B, M, k] rows, one row of each sequence, a column range of a wider output, outputs that no vector store fits."""
+    rng = np.random.default_rng(rows)
+    x, w = R.whole(rng, (3, rows, 400), 1), R.whole(rng, (150, 400), 128)
+    want = np.stack([product(ops.QuantMatrix(p, s), w) for p, s in zip(x.payload, x.scales)])
+    same(ops.quant_linear(x, w, dtype=dtype), want, dtype)
+    row = ops.QuantMatrix(x.payload[:, 1:2], x.scales[:, 1:2].contiguous())
+    same(ops.quant_linear(row, w, dtype=dtype), want[:, 1:2], dtype)
+    for left, width in ((0, 400), (40, 401), (7, 160), (2, 162)):
+        wide = torch.full((3, rows, width), 7.0, dtype=dtype, device="cuda")
+        out = wide[..., left:left + 150]
+        assert ops.quant_linear(x, w, out=out) is out
+        same(out, want, dtype)
+        out.fill_(7.0)
+        assert bool((wide == 7.0).all())
+    assert ops.quant_linear(ops.QuantMatrix(x.payload[:, :0], x.scales[:, :0].contiguous()), w).shape == (3, 0, 150)
+
+
+def offsets_of(counts, dtype=torch.int64, first=0):
+    return torch.tensor(np.concatenate([[first], first + np.cumsum(counts)]), dtype=dtype).cuda()
+
+
+def grouped(x, counts, w, first=0):
+    y = np.full((x.payload.shape[0], w.payload.shape[1]), np.nan)
+    at = first
+    for e, c in enumerate(counts):
+        if c:
+            y[at:at + c] = product(ops.QuantMatrix(x.payload[at:at + c], x.scales[at:at + c]), ops.QuantMatrix(w.payload[e], w.scales[e]))
+        at += c
+    return y
+
+
+@pytest.mark.parametrize("counts", [[1], [0, 1, 0], [3, 0, 5, 16, 0, 17], [0, 70, 1, 0], [64, 65, 1, 33], [200, 0, 130, 1, 257], [300],
+                                    [9] * 40, [128] * 5, [0] * 30 + [500, 3]])
+@pytest.mark.parametrize("n,k", [(40, 100), (300, 704), (129, 1290)])
+def test_quant_moe_matmul_of_whole_numbers(counts, n, k):
+    rng = np.random.default_rng(sum(counts) + n)
+    x, w = R.whole(rng, (sum(counts), k), 1), R.whole(rng, (len(counts), n, k), 128 if n != 129 else 1, batch_gap=n % 2)
+    want = grouped(x, counts, w)
+    same(ops.quant_moe_matmul(x, offsets_of(counts), w, dtype=torch.float32), want, torch.float32)
+    same(ops.quant_moe_matmul(x, offsets_of(counts, torch.int32), w), want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("scale", [1, 12])
+def test_quant_moe_matmul_leaves_rows_of_no_expert(scale):
+    rng = np.random.default_rng(3)
+    counts = [2 * scale, 0, 5 * scale]
+    x, w = R.whole(rng, (11 * scale, 300), 1), R.whole(rng, (3, 70, 300), 128)
+    want = grouped(x, counts, w, first=scale)
+    out = torch.full((11 * scale, 70), 3.0, dtype=torch.float32, device="cuda")
+    ops.quant_moe_matmul(x, offsets_of(counts, first=scale), w, out=out)
+    want[:scale] = want[8 * scale:] = 3.0
+    same(out, want, torch.float32)
+
+
+@pytest.mark.parametrize("scale", [1, 30])
+def test_quant_moe_matmul_offsets_out_of_order(scale):
+    """Recorded; the experts whose offsets are in order have their rows, the others write nothing."""
+    rng = np.random.default_rng(4)
+    rows = 9 * scale
+    x, w = R.whole(rng, (rows, 200), 1), R.whole(rng, (4, 70, 200), 128)
+    for bad in ([0, 2, 1, 4, 9], [-1, 2, 3, 4, 9], [0, 2, 3, 4, 10], [0, 1 << 40, 3, 4, 9]):
+        offsets = torch.tensor(bad, device="cuda") * scale
+        out = torch.full((rows, 70), 3.0, dtype=torch.float32, device="cuda")
+        ops.quant_moe_matmul(x, offsets, w, out=out)
+        with pytest.raises(ops.SandyError, match="offsets"):
+            ops.check_device_errors()
+        ops.check_device_errors()  # read and cleared
+        want = np.full((rows, 70), 3.0)
+        at = offsets.tolist()
+        claims = np.zeros(rows, int)
+        for e in range(4):
+            a, b = at[e], at[e + 1]
+            if 0 <= a <= b <= rows:
+                claims[a:b] += 1
+                want[a:b] = product(ops.QuantMatrix(x.payload[a:b], x.scales[a:b]), ops.QuantMatrix(w.payload[e], w.scales[e]))
+        once = claims < 2  # a row that two experts claim (0 .. 2 and 1 .. 4) holds either's product
+        same(out[torch.from_numpy(once).cuda()], want[once], torch.float32)
+
+
+def test_products_on_other_streams_and_in_graphs():
+    rng = np.random.default_rng(6)
+    sizes = [(1, 300, 700), (40, 300, 700), (300, 520, 1000)]
+    cases = [(torch.from_numpy(loud(rng, (m, k))).bfloat16().cuda(), ops.block_quant(torch.randn(n, k, device="cuda"), 128)) for m, n, k in sizes]
+
+    def step():
+        return [ops.quant_linear(ops.block_quant(x), w) for x, w in cases]
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for round_ in range(3):
+        for x, _ in cases:
+            x.mul_(1.0 + round_)
+        want_now = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want_now):
+            assert torch.equal(a, b)
+    assert all(torch.equal(a, b) for a, b in zip(other, want))
