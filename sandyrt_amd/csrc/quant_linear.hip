@@ -140,6 +140,8 @@ template <typename T>
 int launch_products(const QuantGemm& a, const char* what, Err e, hipStream_t s) {
     const int64_t rows = a.offsets ? (a.rows + a.groups - 1) / a.groups : a.rows;
     auto grid = [&](int nw) { return dim3(static_cast<unsigned>((a.n + 16 * nw - 1) / (16 * nw)), static_cast<unsigned>(a.groups)); };
+    const int form = env_int("SANDY_QUANT_TILE", rows <= 64 ? -1 : 0);
+    if (form >= 0) return launch_quant_tiles(a, std::is_same_v<T, BF16>, form, e, s);
     if (rows <= 16) hipLaunchKernelGGL((quant_stream_kernel<T, 1, 1, 4, 4>), grid(1), dim3(256), 0, s, a);
     else if (rows <= 32) hipLaunchKernelGGL((quant_stream_kernel<T, 2, 2, 4, 2>), grid(2), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((quant_stream_kernel<T, 4, 2, 4, 2>), grid(2), dim3(256), 0, s, a);
@@ -181,9 +183,9 @@ int check_products(const SandyTensor* x, const SandyTensor* x_scales, const Sand
     if ((wm.rows > 1 && out->strides[r - 1] != 1) || (rows > 1 && a->out_pitch < wm.rows) ||
         (xm.batch > 1 && xm.rows > 1 && bo != xm.rows * ro))
         return fail(e, SANDY_ERR_UNSUPPORTED, "%s rows of out must have unit inner stride and be evenly spaced", what);
-    constexpr int64_t kFar = int64_t{1} << 23;
+    constexpr int64_t kFar = int64_t{1} << 22;
     if (xm.pitch > kFar || a->x_pitch > kFar || wm.pitch > kFar)
-        return fail(e, SANDY_ERR_UNSUPPORTED, "%s payload rows more than 2^23 bytes apart", what);
+        return fail(e, SANDY_ERR_UNSUPPORTED, "%s payload rows more than 2^22 bytes apart", what);
     if (!out->data) return fail(e, SANDY_ERR_INVALID, "%s out is null", what);
     a->x = xm.payload;
     a->xs = xm.scales;

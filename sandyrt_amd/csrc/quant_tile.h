@@ -1,0 +1,343 @@
+// quant_tile.h -- the kernel for many rows of the products of matrices in 8 bits (quant_gemm.h).
+#pragma once
+#include "quant_gemm.h"
+
+namespace sandy_hip {
+
+// Workgroup tile 64 WM x 64 WN of rows x columns, 2 x 2 waves of 32 WM x 32 WN on 32 x 32 instructions, 128 columns
+// of k (a block, a whole 128-byte line of every row) a chunk, STAGES chunks in LDS.
+template <int WM, int WN, int STAGES>
+struct QuantTile {
+    static constexpr int BM = 64 * WM, BN = 64 * WN;
+    static constexpr int kX = BM * 128, kStage = (BM + BN) * 128;
+    static constexpr int kLoads = (BM + BN) / 32;  // 16-byte pieces a thread moves per chunk
+    template <typename T>
+    static constexpr int row_bytes() { return 32 * WN * static_cast<int>(sizeof(typename Vec8<T>::elem)) + 16; }
+    template <typename T>
+    static constexpr int lds() {
+        const int out = 4 * 32 * row_bytes<T>();
+        return STAGES * kStage > out ? STAGES * kStage : out;
+    }
+};
+
+// Four scale bytes j .. j + 3 of a row, those past the last block as 0.
+__device__ __forceinline__ int four_scales(const uint8_t* row, int j, int blocks) {
+    int v = 0;
+    if (__builtin_expect(j + 4 <= blocks, 1)) {
+        __builtin_memcpy(&v, row + j, 4);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 3; i++)
+            if (j + i < blocks) v |= row[j + i] << (8 * i);
+    }
+    return v;
+}
+
+// 16 bytes a lane from a buffer straight into LDS, the wave's 1024 bytes in a row from `lds` on.  In flight until
+// a wait on vmcnt; the compiler does not count it (its own waits only become stricter).  (s_nop: a vector
+// instruction may just have written one of the scalars.)
+__device__ __forceinline__ void copy_to_lds(i32x4_t buffer, int offset, int more, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(buffer), "s"(more)
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <typename T, int WM, int WN, int STAGES>
+__global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
+    using G = QuantTile<WM, WN, STAGES>;
+    constexpr bool kScaled = std::is_same_v<T, BF16>;
+    extern __shared__ __align__(1024) unsigned char lds[];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave & 1, wn = wave >> 1;
+    const int col = lane & 31, half = lane >> 5;
+
+    // workgroups go to the eight XCDs in turn: each takes a run of tiles, eight rows of tiles high, whose operands
+    // its L2 then holds
+    const uint32_t total = static_cast<uint32_t>(m_tiles) * n_tiles, per = (total + 7) / 8;
+    const uint32_t tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if (tile >= total) return;
+    const uint32_t band = tile / (8u * n_tiles), high = min(8u, m_tiles - 8u * band), in = tile - band * 8u * n_tiles;
+    const int m_tile = static_cast<int>(8u * band + in % high), n_tile = static_cast<int>(in / high);
+    int g = 0, r0 = m_tile * G::BM, end = a.rows;
+    if (a.offsets) {
+        // the m_tile-th of the experts' row tiles
+        int before = 0;
+        g = -1;
+        for (int base = 0; base < a.groups; base += 64) {
+            const int e = base + lane;
+            int first = 0, past = 0;
+            if (e < a.groups) {
+                const int64_t b = load_index(a.offsets, a.offsets_dt, e), f = load_index(a.offsets, a.offsets_dt, e + 1);
+                if (b < 0 || f < b || f > a.rows) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_OFFSETS));
+                else first = static_cast<int>(b), past = static_cast<int>(f);
+            }
+            int upto = (past - first + G::BM - 1) / G::BM;
+            const int mine = upto;
+#pragma unroll
+            for (int s = 1; s < 64; s <<= 1) {
+                const int below = __shfl_up(upto, s, 64);
+                if (lane >= s) upto += below;
+            }
+            const uint64_t here = __ballot(before + upto > m_tile);
+            if (here) {
+                const int l = __builtin_ctzll(here);
+                g = base + l;
+                r0 = __shfl(first, l, 64) + (m_tile - before - __shfl(upto - mine, l, 64)) * G::BM;
+                end = __shfl(past, l, 64);
+                break;
+            }
+            before += __shfl(upto, 63, 64);
+        }
+        if (g < 0) return;
+        g = __builtin_amdgcn_readfirstlane(g);
+        r0 = __builtin_amdgcn_readfirstlane(r0);
+        end = __builtin_amdgcn_readfirstlane(end);
+    }
+    const int n0 = n_tile * G::BN;
+    const int xrows = min(G::BM, end - r0), wrows = min(G::BN, a.n - n0);
+
+    // piece i of a thread: 16 bytes of tile row 32 i + tid / 8, x's rows first; rows past the tile's end repeat the last
+    // (never stored).  LDS slot p of row r holds the line's piece p ^ (r / 2) % 8: reads of 16 rows meet no bank twice.
+    const uint8_t* xbase = a.x + r0 * a.x_pitch;
+    const uint8_t* wbase = a.w + g * a.w_group + n0 * a.w_pitch;
+    const int k16 = (a.k + 15) & ~15;
+    auto buffer = [](const uint8_t* p, int64_t bytes) {
+        const uint64_t v = reinterpret_cast<uint64_t>(p);
+        i32x4_t r;
+        r[0] = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
+        r[1] = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32) & 0xffff);
+        r[2] = __builtin_amdgcn_readfirstlane(static_cast<int>(bytes));
+        r[3] = 0x00020000;
+        return r;
+    };
+    const i32x4_t xres = buffer(xbase, (xrows - 1) * a.x_pitch + k16), wres = buffer(wbase, (wrows - 1) * a.w_pitch + k16);
+    const int prow = tid >> 3, slot = tid & 7, piece = slot ^ ((prow >> 1) & 7);
+    int from[G::kLoads];
+#pragma unroll
+    for (int i = 0; i < G::kLoads; i++) {
+        const bool is_x = i < 2 * WM;
+        const int r = 32 * (is_x ? i : i - 2 * WM) + prow;
+        from[i] = static_cast<int>(min(r, (is_x ? xrows : wrows) - 1) * (is_x ? a.x_pitch : a.w_pitch)) + 16 * piece;
+    }
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
+    auto copy = [&](int c, int stage, int i) {
+        copy_to_lds(i < 2 * WM ? xres : wres, from[i], c * 128, lds0 + stage * G::kStage + wave * 1024 + i * 4096);
+    };
+    auto issue = [&](int c, int stage) {
+#pragma unroll
+        for (int i = 0; i < G::kLoads; i++) copy(c, stage, i);
+    };
+    const int sw = (col >> 1) & 7;
+    const int xat = (32 * WM * wm + col) * 128, wat = G::kX + (32 * WN * wn + col) * 128;
+    // half i & 1 of operand i / 2 (the weight's first) of the chunk's columns 64 s ..
+    auto read1 = [&](int stage, int s, int i, i32x4_t (&xf)[WM][2], i32x4_t (&wf)[WN][2]) {
+        const int at = stage * G::kStage + (((4 * s + 2 * half + (i & 1)) ^ sw) << 4);
+        if (i < 2 * WN) wf[i / 2][i & 1] = *reinterpret_cast<const i32x4_t*>(lds + wat + 4096 * (i / 2) + at);
+        else xf[i / 2 - WN][i & 1] = *reinterpret_cast<const i32x4_t*>(lds + xat + 4096 * (i / 2 - WN) + at);
+    };
+    constexpr int kReads = 2 * (WM + WN);
+    auto frags = [&](int stage, int s, i32x4_t (&xf)[WM][2], i32x4_t (&wf)[WN][2]) {
+#pragma unroll
+        for (int i = 0; i < kReads; i++) read1(stage, s, i, xf, wf);
+    };
+    f32x16_t acc[WM][WN];
+#pragma unroll
+    for (int t = 0; t < WM; t++)
+#pragma unroll
+        for (int c = 0; c < WN; c++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[t][c][i] = 0.0f;
+
+    // a lane's scale bytes of four chunks, the next four requested while these are used
+    const uint8_t* xsbase = a.xs + static_cast<int64_t>(r0) * a.blocks;
+    const uint8_t* wsbase = a.ws + static_cast<int64_t>(g) * a.w_scale_rows * a.blocks;
+    uint32_t xso[WM], wso[WN];
+#pragma unroll
+    for (int t = 0; t < WM; t++) xso[t] = min(32 * (WM * wm + t) + col, xrows - 1) * a.blocks;
+#pragma unroll
+    for (int c = 0; c < WN; c++) wso[c] = ((n0 + min(32 * (WN * wn + c) + col, wrows - 1)) >> a.w_shift) * a.blocks;
+    int xs[WM], ws[WN], xs_next[WM], ws_next[WN];
+    auto scales = [&](int j) {
+#pragma unroll
+        for (int t = 0; t < WM; t++) xs_next[t] = four_scales(xsbase + xso[t], j, a.blocks);
+#pragma unroll
+        for (int c = 0; c < WN; c++) ws_next[c] = four_scales(wsbase + wso[c], j, a.blocks);
+    };
+    auto use_scales = [&] {
+#pragma unroll
+        for (int t = 0; t < WM; t++) xs[t] = xs_next[t];
+#pragma unroll
+        for (int c = 0; c < WN; c++) ws[c] = ws_next[c];
+    };
+    // all products of 64 columns, other(i) before the i-th of WM WN
+    auto multiply = [&](const i32x4_t (&xf)[WM][2], const i32x4_t (&wf)[WN][2], auto other) {
+        auto both = [](const i32x4_t (&h)[2]) { return __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7); };
+        if constexpr (kScaled) {
+#pragma unroll
+            for (int c = 0; c < WN; c++)
+#pragma unroll
+                for (int t = 0; t < WM; t++) {
+                    other(c * WM + t);
+                    acc[t][c] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(both(wf[c]), both(xf[t]), acc[t][c], 0, 0, 0, ws[c], 0, xs[t]);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+        } else {
+            Widened xw[WM];
+#pragma unroll
+            for (int t = 0; t < WM; t++) xw[t] = widen(both(xf[t]), quant_scale(xs[t] & 255));
+#pragma unroll
+            for (int c = 0; c < WN; c++) {
+                const Widened ww = widen(both(wf[c]), quant_scale(ws[c] & 255));
+#pragma unroll
+                for (int t = 0; t < WM; t++) other(c * WM + t);
+#pragma unroll
+                for (int s = 0; s < 4; s++)
+#pragma unroll
+                    for (int t = 0; t < WM; t++) acc[t][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ww.v[s], xw[t].v[s], acc[t][c], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    // a point where the scales requested are there: the compiler's wait for them covers every copy in flight (it
+    // does not count those), so it belongs where few are
+    auto scales_arrive = [&] {
+#pragma unroll
+        for (int t = 0; t < WM; t++) asm volatile("" : "+v"(xs_next[t]));
+#pragma unroll
+        for (int c = 0; c < WN; c++) asm volatile("" : "+v"(ws_next[c]));
+    };
+    // what lies between the stages of the pipeline: LDS reads and writes of this wave done, copies but the youngest
+    // `left` arrived, then every wave's
+    auto meet = [&](auto left) {
+        __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+        wait_copies<decltype(left)::value>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    using Left = std::integral_constant<int, (STAGES - 2) * G::kLoads>;
+    using First = std::integral_constant<int, (STAGES - 1) * G::kLoads>;
+
+    // Chunks past the last are the last again, copied and never read: every round waits for the same number.
+    const int chunks = a.k / kQuantBlock, rest = a.k - chunks * kQuantBlock, last = max(chunks - 1, 0);
+    i32x4_t xf[2][WM][2], wf[2][WN][2];
+    if (chunks) {
+#pragma unroll
+        for (int s = 0; s < STAGES - 1; s++) issue(min(s, last), s);
+    }
+    if (rest) {
+        // the last block of a k that is no multiple of 128 goes first, through registers: bytes past k are 0
+        const int left = rest - 16 * piece;
+        i32x4_t v[G::kLoads];
+#pragma unroll
+        for (int i = 0; i < G::kLoads; i++) {
+            v[i] = i32x4_t{0, 0, 0, 0};
+            if (left > 0) v[i] = *reinterpret_cast<const i32x4_t*>((i < 2 * WM ? xbase : wbase) + (static_cast<uint32_t>(from[i]) + chunks * 128));
+        }
+#pragma unroll
+        for (int i = 0; i < G::kLoads; i++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[i][j] &= static_cast<int>(first_bytes(left - 4 * j));
+            *reinterpret_cast<i32x4_t*>(lds + (STAGES - 1) * G::kStage + i * 4096 + tid * 16) = v[i];
+        }
+        scales(chunks);
+        use_scales();
+        __syncthreads();
+        frags(STAGES - 1, 0, xf[0], wf[0]);
+        frags(STAGES - 1, 1, xf[1], wf[1]);
+        multiply(xf[0], wf[0], [](int) {});
+        multiply(xf[1], wf[1], [](int) {});
+        __syncthreads();
+    }
+    if (chunks) {
+        scales(0);
+        use_scales();
+        issue(min(STAGES - 1, last), STAGES - 1);
+        meet(First{});
+        frags(0, 0, xf[0], wf[0]);
+    }
+    for (int c = 0, stage = 0; c < chunks; c++) {
+        const int next = stage + 1 == STAGES ? 0 : stage + 1, then = min(c + STAGES, last);
+        if ((c & 3) == 0) scales(min(c + 4, last));
+        constexpr int kTimes = WM * WN;
+        multiply(xf[0], wf[0], [&](int i) {
+#pragma unroll
+            for (int q = i * kReads / kTimes; q < (i + 1) * kReads / kTimes; q++) read1(stage, 1, q, xf[1], wf[1]);
+        });
+        meet(Left{});  // this chunk is in every wave's registers, the next one in LDS: its place is filled again
+        scales_arrive();
+        multiply(xf[1], wf[1], [&](int i) {
+#pragma unroll
+            for (int q = i * kReads / kTimes; q < (i + 1) * kReads / kTimes; q++) read1(next, 0, q, xf[0], wf[0]);
+#pragma unroll
+            for (int q = i * G::kLoads / kTimes; q < (i + 1) * G::kLoads / kTimes; q++) copy(then, stage, q);
+        });
+        stage = next;
+        if ((c & 3) == 3) {
+            use_scales();
+        } else {
+#pragma unroll
+            for (int t = 0; t < WM; t++) xs[t] = static_cast<int>(static_cast<uint32_t>(xs[t]) >> 8);
+#pragma unroll
+            for (int q = 0; q < WN; q++) ws[q] = static_cast<int>(static_cast<uint32_t>(ws[q]) >> 8);
+        }
+    }
+    wait_copies<0>();  // LDS is used again
+    __syncthreads();
+
+    // acc[t][c][i]: row 32 t + col, column 32 c + 8 (i / 4) + 4 half + i % 4 of the wave's part: 32 rows at a time through
+    // LDS (wave-private) into whole row segments
+    using E = typename Vec8<T>::elem;
+    constexpr int kRow = G::template row_bytes<T>(), kLanes = 32 * WN * static_cast<int>(sizeof(E)) / 16, kEach = 16 / static_cast<int>(sizeof(E));
+    unsigned char* part = lds + wave * 32 * kRow;
+    const int mw = 32 * WM * wm, nw = 32 * WN * wn;
+    E* out = static_cast<E*>(a.out) + r0 * a.out_pitch + n0;
+    const bool whole = ((reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(a.out_pitch * static_cast<int64_t>(sizeof(E)))) & 15) == 0;
+#pragma unroll
+    for (int t = 0; t < WM; t++) {
+        if (mw + 32 * t >= xrows) break;
+#pragma unroll
+        for (int c = 0; c < WN; c++)
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const int at = 32 * c + 8 * q + 4 * half;
+                f32x4_t v{acc[t][c][4 * q], acc[t][c][4 * q + 1], acc[t][c][4 * q + 2], acc[t][c][4 * q + 3]};
+                if (a.bias)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) v[j] += Vec8<T>::load1(a.bias, min(n0 + nw + at + j, a.n - 1));
+                if constexpr (kScaled)
+                    *reinterpret_cast<uint2*>(part + col * kRow + 2 * at) = make_uint2(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]));
+                else
+                    *reinterpret_cast<f32x4_t*>(part + col * kRow + 4 * at) = v;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+        for (int i = 0; i < 32 * kLanes / 64; i++) {
+            const int at = 64 * i + lane, r = mw + 32 * t + at / kLanes, n = nw + kEach * (at % kLanes);
+            const unsigned char* p = part + at / kLanes * kRow + 16 * (at % kLanes);
+            if (r >= xrows || n >= wrows) continue;
+            if (whole && n + kEach <= wrows) {
+                *reinterpret_cast<i32x4_t*>(out + r * a.out_pitch + n) = *reinterpret_cast<const i32x4_t*>(p);
+            } else if (whole) {
+                for (int j = 0; j < kEach && n + j < wrows; j++) out[r * a.out_pitch + n + j] = reinterpret_cast<const E*>(p)[j];
+            }
+        }
+        if (!whole) {
+            // rows of other alignments: neighbouring lanes write neighbouring columns
+            for (int at = lane; at < 32 * 32 * WN; at += 64) {
+                const int r = mw + 32 * t + at / (32 * WN), n = nw + at % (32 * WN);
+                if (r < xrows && n < wrows) out[r * a.out_pitch + n] = *reinterpret_cast<const E*>(part + at / (32 * WN) * kRow + sizeof(E) * (at % (32 * WN)));
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+}
+
+} // namespace sandy_hip
