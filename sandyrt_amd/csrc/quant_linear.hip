@@ -140,7 +140,8 @@ template <typename T>
 int launch_products(const QuantGemm& a, const char* what, Err e, hipStream_t s) {
     const int64_t rows = a.offsets ? (a.rows + a.groups - 1) / a.groups : a.rows;
     auto grid = [&](int nw) { return dim3(static_cast<unsigned>((a.n + 16 * nw - 1) / (16 * nw)), static_cast<unsigned>(a.groups)); };
-    const int form = env_int("SANDY_QUANT_TILE", rows <= 64 ? -1 : 0);
+    auto tiles = [&](int64_t edge) { return (rows + edge - 1) / edge * a.groups * ((a.n + edge - 1) / edge); };
+    const int form = env_int("SANDY_QUANT_TILE", rows <= 32 ? -1 : tiles(256) >= 512 && !a.offsets ? 0 : tiles(128) >= 256 ? 2 : 3);
     if (form >= 0) return launch_quant_tiles(a, std::is_same_v<T, BF16>, form, e, s);
     if (rows <= 16) hipLaunchKernelGGL((quant_stream_kernel<T, 1, 1, 4, 4>), grid(1), dim3(256), 0, s, a);
     else if (rows <= 32) hipLaunchKernelGGL((quant_stream_kernel<T, 2, 2, 4, 2>), grid(2), dim3(256), 0, s, a);

@@ -4,31 +4,34 @@
 
 namespace sandy_hip {
 
-// Workgroup tile 64 WM x 64 WN of rows x columns, 2 x 2 waves of 32 WM x 32 WN on 32 x 32 instructions, 128 columns
+// Workgroup tile 64 WM x 32 PN WN of rows x columns, 2 x PN waves of 32 WM x 32 WN on 32 x 32 instructions, 128 columns
 // of k (a block, a whole 128-byte line of every row) a chunk, STAGES chunks in LDS.
-template <int WM, int WN, int STAGES>
+template <int WM, int WN, int PN, int STAGES>
 struct QuantTile {
-    static constexpr int BM = 64 * WM, BN = 64 * WN;
+    static constexpr int BM = 64 * WM, BN = 32 * PN * WN, kThreads = 128 * PN;
     static constexpr int kX = BM * 128, kStage = (BM + BN) * 128;
-    static constexpr int kLoads = (BM + BN) / 32;  // 16-byte pieces a thread moves per chunk
+    // the scale bytes of 16 blocks of every row, twice, behind the stages
+    static constexpr int kScales = STAGES * kStage, kScaleBytes = (BM + BN) * 16;
+    static constexpr int kStep = kThreads / 8, kXLoads = BM / kStep, kLoads = (BM + BN) / kStep;  // 16-byte pieces a thread moves a chunk
     template <typename T>
     static constexpr int row_bytes() { return 32 * WN * static_cast<int>(sizeof(typename Vec8<T>::elem)) + 16; }
     template <typename T>
     static constexpr int lds() {
-        const int out = 4 * 32 * row_bytes<T>();
-        return STAGES * kStage > out ? STAGES * kStage : out;
+        const int out = kThreads / 64 * 32 * row_bytes<T>();
+        constexpr int loop = kScales + 2 * kScaleBytes;
+        return loop > out ? loop : out;
     }
 };
 
-// Four scale bytes j .. j + 3 of a row, those past the last block as 0.
-__device__ __forceinline__ int four_scales(const uint8_t* row, int j, int blocks) {
-    int v = 0;
-    if (__builtin_expect(j + 4 <= blocks, 1)) {
-        __builtin_memcpy(&v, row + j, 4);
+// Sixteen scale bytes j .. j + 15 of a row, those past the last block as 0.
+__device__ __forceinline__ i32x4_t sixteen_scales(const uint8_t* row, int j, int blocks) {
+    i32x4_t v{0, 0, 0, 0};
+    if (j + 16 <= blocks) {
+        __builtin_memcpy(&v, row + j, 16);
     } else {
 #pragma unroll
-        for (int i = 0; i < 3; i++)
-            if (j + i < blocks) v |= row[j + i] << (8 * i);
+        for (int i = 0; i < 15; i++)
+            if (j + i < blocks) v[i >> 2] |= row[j + i] << (8 * (i & 3));
     }
     return v;
 }
@@ -45,9 +48,9 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <typename T, int WM, int WN, int STAGES>
-__global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
-    using G = QuantTile<WM, WN, STAGES>;
+template <typename T, int WM, int WN, int PN, int STAGES>
+__global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
+    using G = QuantTile<WM, WN, PN, STAGES>;
     constexpr bool kScaled = std::is_same_v<T, BF16>;
     extern __shared__ __align__(1024) unsigned char lds[];
     const int tid = threadIdx.x, lane = tid & 63;
@@ -100,7 +103,7 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
     const int n0 = n_tile * G::BN;
     const int xrows = min(G::BM, end - r0), wrows = min(G::BN, a.n - n0);
 
-    // piece i of a thread: 16 bytes of tile row 32 i + tid / 8, x's rows first; rows past the tile's end repeat the last
+    // piece i of a thread: 16 bytes of tile row kStep i + tid / 8, x's rows first; rows past the tile's end repeat the last
     // (never stored).  LDS slot p of row r holds the line's piece p ^ (r / 2) % 8: reads of 16 rows meet no bank twice.
     const uint8_t* xbase = a.x + r0 * a.x_pitch;
     const uint8_t* wbase = a.w + g * a.w_group + n0 * a.w_pitch;
@@ -119,13 +122,13 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
     int from[G::kLoads];
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
-        const bool is_x = i < 2 * WM;
-        const int r = 32 * (is_x ? i : i - 2 * WM) + prow;
+        const bool is_x = i < G::kXLoads;
+        const int r = G::kStep * (is_x ? i : i - G::kXLoads) + prow;
         from[i] = static_cast<int>(min(r, (is_x ? xrows : wrows) - 1) * (is_x ? a.x_pitch : a.w_pitch)) + 16 * piece;
     }
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
     auto copy = [&](int c, int stage, int i) {
-        copy_to_lds(i < 2 * WM ? xres : wres, from[i], c * 128, lds0 + stage * G::kStage + wave * 1024 + i * 4096);
+        copy_to_lds(i < G::kXLoads ? xres : wres, from[i], c * 128, lds0 + stage * G::kStage + wave * 1024 + i * (16 * G::kThreads));
     };
     auto issue = [&](int c, int stage) {
 #pragma unroll
@@ -152,20 +155,34 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[t][c][i] = 0.0f;
 
-    // a lane's scale bytes of four chunks, the next four requested while these are used
+    // scale bytes come 16 blocks at a time: a row a thread (or two) from memory, half a segment ahead, through LDS to the
+    // lanes that multiply with them
     const uint8_t* xsbase = a.xs + static_cast<int64_t>(r0) * a.blocks;
     const uint8_t* wsbase = a.ws + static_cast<int64_t>(g) * a.w_scale_rows * a.blocks;
-    uint32_t xso[WM], wso[WN];
+    auto scale_row = [&](int r) {
+        return r < G::BM ? xsbase + static_cast<int64_t>(min(r, xrows - 1)) * a.blocks
+                         : wsbase + static_cast<int64_t>((n0 + min(r - G::BM, wrows - 1)) >> a.w_shift) * a.blocks;
+    };
+    constexpr int kScaleRows = (G::BM + G::BN + G::kThreads - 1) / G::kThreads;
+    i32x4_t held[kScaleRows];
+    auto load_scales = [&](int first) {
 #pragma unroll
-    for (int t = 0; t < WM; t++) xso[t] = min(32 * (WM * wm + t) + col, xrows - 1) * a.blocks;
+        for (int u = 0; u < kScaleRows; u++)
+            if (G::kThreads * u + tid < G::BM + G::BN) held[u] = sixteen_scales(scale_row(G::kThreads * u + tid), first, a.blocks);
+    };
+    auto store_scales = [&](int first) {
 #pragma unroll
-    for (int c = 0; c < WN; c++) wso[c] = ((n0 + min(32 * (WN * wn + c) + col, wrows - 1)) >> a.w_shift) * a.blocks;
+        for (int u = 0; u < kScaleRows; u++)
+            if (G::kThreads * u + tid < G::BM + G::BN)
+                *reinterpret_cast<i32x4_t*>(lds + G::kScales + ((first >> 4) & 1) * G::kScaleBytes + (G::kThreads * u + tid) * 16) = held[u];
+    };
     int xs[WM], ws[WN], xs_next[WM], ws_next[WN];
-    auto scales = [&](int j) {
+    auto scales = [&](int c) {  // of chunks c .. c + 3, c a multiple of 4
+        const unsigned char* at = lds + G::kScales + ((c >> 4) & 1) * G::kScaleBytes + (c & 12);
 #pragma unroll
-        for (int t = 0; t < WM; t++) xs_next[t] = four_scales(xsbase + xso[t], j, a.blocks);
+        for (int t = 0; t < WM; t++) xs_next[t] = *reinterpret_cast<const int*>(at + (32 * (WM * wm + t) + col) * 16);
 #pragma unroll
-        for (int c = 0; c < WN; c++) ws_next[c] = four_scales(wsbase + wso[c], j, a.blocks);
+        for (int q = 0; q < WN; q++) ws_next[q] = *reinterpret_cast<const int*>(at + (G::BM + 32 * (WN * wn + q) + col) * 16);
     };
     auto use_scales = [&] {
 #pragma unroll
@@ -202,23 +219,24 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
             }
         }
     };
-    // a point where the scales requested are there: the compiler's wait for them covers every copy in flight (it
-    // does not count those), so it belongs where few are
-    auto scales_arrive = [&] {
-#pragma unroll
-        for (int t = 0; t < WM; t++) asm volatile("" : "+v"(xs_next[t]));
-#pragma unroll
-        for (int c = 0; c < WN; c++) asm volatile("" : "+v"(ws_next[c]));
-    };
-    // what lies between the stages of the pipeline: LDS reads and writes of this wave done, copies but the youngest
-    // `left` arrived, then every wave's
+    // LDS reads and writes of this wave done, copies but the youngest `left` arrived, then every wave's
     auto meet = [&](auto left) {
         __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
         wait_copies<decltype(left)::value>();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    using Left = std::integral_constant<int, (STAGES - 2) * G::kLoads>;
+    // The 2 kTimes products of a chunk c are the clock.  First its second half is read; at kFree it is in every wave's
+    // registers, and copies of chunk c + STAGES into its place begin, spread over what is left; at kLand the next chunk
+    // has to be in LDS, and its first half is read.
+    constexpr int kTimes = WM * WN, kFree = 7 * kTimes / 16, kLand = kTimes + 9 * kTimes / 16;
+    constexpr auto when = [](int q) { return kFree + q * (2 * kTimes - kFree) / G::kLoads; };
+    constexpr int kIssued = [when] {
+        int n = 0;
+        while (n < G::kLoads && when(n) <= kLand) n++;
+        return n;
+    }();
+    using Left = std::integral_constant<int, (STAGES - 2) * G::kLoads + kIssued>;
     using First = std::integral_constant<int, (STAGES - 1) * G::kLoads>;
 
     // Chunks past the last are the last again, copied and never read: every round waits for the same number.
@@ -235,16 +253,18 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
             v[i] = i32x4_t{0, 0, 0, 0};
-            if (left > 0) v[i] = *reinterpret_cast<const i32x4_t*>((i < 2 * WM ? xbase : wbase) + (static_cast<uint32_t>(from[i]) + chunks * 128));
+            if (left > 0) v[i] = *reinterpret_cast<const i32x4_t*>((i < G::kXLoads ? xbase : wbase) + (static_cast<uint32_t>(from[i]) + chunks * 128));
         }
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
 #pragma unroll
             for (int j = 0; j < 4; j++) v[i][j] &= static_cast<int>(first_bytes(left - 4 * j));
-            *reinterpret_cast<i32x4_t*>(lds + (STAGES - 1) * G::kStage + i * 4096 + tid * 16) = v[i];
+            *reinterpret_cast<i32x4_t*>(lds + (STAGES - 1) * G::kStage + i * (16 * G::kThreads) + tid * 16) = v[i];
         }
-        scales(chunks);
-        use_scales();
+#pragma unroll
+        for (int t = 0; t < WM; t++) xs[t] = scale_row(32 * (WM * wm + t) + col)[chunks];
+#pragma unroll
+        for (int c = 0; c < WN; c++) ws[c] = scale_row(G::BM + 32 * (WN * wn + c) + col)[chunks];
         __syncthreads();
         frags(STAGES - 1, 0, xf[0], wf[0]);
         frags(STAGES - 1, 1, xf[1], wf[1]);
@@ -253,28 +273,38 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
         __syncthreads();
     }
     if (chunks) {
-        scales(0);
-        use_scales();
+        load_scales(0);
+        store_scales(0);
         issue(min(STAGES - 1, last), STAGES - 1);
         meet(First{});
         frags(0, 0, xf[0], wf[0]);
+        scales(0);
+        use_scales();
     }
     for (int c = 0, stage = 0; c < chunks; c++) {
         const int next = stage + 1 == STAGES ? 0 : stage + 1, then = min(c + STAGES, last);
-        if ((c & 3) == 0) scales(min(c + 4, last));
-        constexpr int kTimes = WM * WN;
-        multiply(xf[0], wf[0], [&](int i) {
+        auto at_slot = [&](int slot) {
+            constexpr int kRead = (4 * kReads + kTimes - 1) / kTimes;
 #pragma unroll
-            for (int q = i * kReads / kTimes; q < (i + 1) * kReads / kTimes; q++) read1(stage, 1, q, xf[1], wf[1]);
-        });
-        meet(Left{});  // this chunk is in every wave's registers, the next one in LDS: its place is filled again
-        scales_arrive();
-        multiply(xf[1], wf[1], [&](int i) {
+            for (int q = slot * kRead; q < min((slot + 1) * kRead, kReads); q++) read1(stage, 1, q, xf[1], wf[1]);
+            if (slot == kFree) {
+                __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+            }
 #pragma unroll
-            for (int q = i * kReads / kTimes; q < (i + 1) * kReads / kTimes; q++) read1(next, 0, q, xf[0], wf[0]);
+            for (int q = 0; q < G::kLoads; q++)
+                if (when(q) == slot) copy(then, stage, q);
+            if (slot == kLand) meet(Left{});
+            if (slot >= kLand)
 #pragma unroll
-            for (int q = i * G::kLoads / kTimes; q < (i + 1) * G::kLoads / kTimes; q++) copy(then, stage, q);
-        });
+                for (int q = (slot - kLand) * kRead; q < min((slot - kLand + 1) * kRead, kReads); q++) read1(next, 0, q, xf[0], wf[0]);
+        };
+        multiply(xf[0], wf[0], at_slot);
+        if ((c & 15) == 7) store_scales(c + 9);
+        if ((c & 15) == 6) load_scales(c + 10);
+        if ((c & 3) == 3) scales(c + 1);
+        multiply(xf[1], wf[1], [&](int i) { at_slot(kTimes + i); });
         stage = next;
         if ((c & 3) == 3) {
             use_scales();
@@ -322,7 +352,7 @@ __global__ __launch_bounds__(256, 1) void quant_tile_kernel(QuantGemm a, int m_t
             const unsigned char* p = part + at / kLanes * kRow + 16 * (at % kLanes);
             if (r >= xrows || n >= wrows) continue;
             if (whole && n + kEach <= wrows) {
-                *reinterpret_cast<i32x4_t*>(out + r * a.out_pitch + n) = *reinterpret_cast<const i32x4_t*>(p);
+                __builtin_nontemporal_store(*reinterpret_cast<const i32x4_t*>(p), reinterpret_cast<i32x4_t*>(out + r * a.out_pitch + n));
             } else if (whole) {
                 for (int j = 0; j < kEach && n + j < wrows; j++) out[r * a.out_pitch + n + j] = reinterpret_cast<const E*>(p)[j];
             }
