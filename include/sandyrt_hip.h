@@ -59,7 +59,8 @@ enum SandyDeviceError {
     SANDY_DEVERR_BLOCK = 1u << 5,       /* paged block id outside the pool */
     SANDY_DEVERR_ATTN_POS = 1u << 6,    /* attention position_offsets must be non-negative */
     SANDY_DEVERR_QUANT_ROWS = 1u << 7,  /* quant_paged rows before 0 or past the block table */
-    SANDY_DEVERR_QUANT_COUNT = 1u << 8  /* quant_paged count below 0 or above the row count */
+    SANDY_DEVERR_QUANT_COUNT = 1u << 8, /* quant_paged count below 0 or above the row count */
+    SANDY_DEVERR_SAMPLE = 1u << 9       /* sample temperature, top_p, min_p or uniform number out of range */
 };
 
 /* A strided view of device memory (TensorViewDesc, src/device/DeviceTypes.h:25-29). */
@@ -639,6 +640,34 @@ int sandy_hip_quant_linear(const SandyTensor* x, const SandyTensor* x_scales, co
 int sandy_hip_quant_moe_matmul(const SandyTensor* x, const SandyTensor* x_scales, const SandyTensor* expert_offsets,
                                const SandyTensor* weight, const SandyTensor* weight_scales, const SandyTensor* out,
                                void* stream, char* err, size_t err_cap);
+
+/* ---------------------------------------------------------------- sampling */
+
+/*
+ * One token a row of logits [rows, vocab] (F32 or BF16, unit inner stride, rows any distance apart; vocab <= 2^24),
+ * with each row's own settings, all on the device.  The reference picks on the host, greedily among equals by the
+ * lowest id (src/server/Sampler.cpp:69-79,212); here too rank is by logit, then id.  A logit of -inf or NaN is never
+ * drawn.  With w = exp((logit - max) / temperature):
+ *   top_k  keeps the first top_k ranks (0 or less, or not below the tokens there are: all);
+ *   top_p  of those, the ranks before which less than top_p of their summed w lies (1 or more: all; the first always);
+ *   min_p  of those, the tokens with w >= min_p (0 or less: all);
+ * and the token drawn is the one, walking what is left in order of ids, with which the sum of w passes uniforms[row]
+ * (0 <= u < 1, 24 bits) of the whole.  temperature 0 takes the first rank.  temperature, top_p, min_p: [rows] F32 or
+ * NULL (1, 1, 0); top_k [rows] I32 or I64 or NULL; ids [rows] I32 or I64; probs NULL or [rows] F32, the token's share
+ * of w of what is left.  Every w is held as a whole multiple of 2^-s, s = 62 - ceil(log2(vocab)) but 50 at most, sums
+ * and comparisons are exact, so results do not depend on how a call is cut up; what is below 2^-s-1 weighs nothing.
+ * A row without a token gives id -1 and probability 0; so does one with temperature negative or NaN, top_p NaN, min_p
+ * above 1 or NaN, or u out of range, which is recorded (SANDY_DEVERR_SAMPLE).  `workspace` holds
+ * sandy_hip_sample_workspace() bytes (16-byte aligned): the call's alone while it runs, its contents need not be kept or
+ * cleared.
+ */
+int sandy_hip_sample(const SandyTensor* logits, const SandyTensor* temperature, const SandyTensor* top_k,
+                     const SandyTensor* top_p, const SandyTensor* min_p, const SandyTensor* uniforms,
+                     const SandyTensor* ids, const SandyTensor* probs, void* workspace, size_t workspace_bytes,
+                     void* stream, char* err, size_t err_cap);
+
+/* Workspace bytes of a sample call with these logits. */
+int sandy_hip_sample_workspace(const SandyTensor* logits, size_t* bytes, char* err, size_t err_cap);
 
 /* ---------------------------------------------------------------- safetensors weights
  *

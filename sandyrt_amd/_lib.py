@@ -202,6 +202,7 @@ SIGNATURES = {
     "sandy_hip_block_dequant": [*[C.c_void_p] * 3, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_quant_linear": [*[C.c_void_p] * 6, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_quant_moe_matmul": [*[C.c_void_p] * 6, C.c_void_p, ERR, C.c_size_t],
+    "sandy_hip_sample": [*[C.c_void_p] * 8, C.c_void_p, C.c_size_t, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_topk": [T, C.c_int64, C.c_int64, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_gather": [T, T, T, C.c_int64, C.c_int64, T, T, T, T, C.c_void_p, ERR, C.c_size_t],
     "sandy_hip_moe_matmul": [T, T, T, C.c_int32, T, C.c_void_p, ERR, C.c_size_t],
@@ -248,6 +249,7 @@ DEVICE_SIGNATURES = {
     "sandy_hip_device_graph_end": ([DEV, U32P], C.c_int),
     "sandy_hip_device_graph_launch": ([DEV, C.c_uint32], C.c_int),
     "sandy_hip_device_graph_destroy": ([DEV, C.c_uint32], C.c_int),
+    "sandy_hip_sample_workspace": ([T, C.POINTER(C.c_size_t)], C.c_int),
     "sandy_hip_quant_paged_attention_workspace": ([T, Q8, T, C.c_int64, C.POINTER(C.c_size_t)], C.c_int),
 }
 ST = C.c_void_p

@@ -25,19 +25,11 @@ struct BlockArgs {
     uint32_t units;
 };
 
-// Eight elements from element i on, a vector load whatever their alignment.
-template <typename T>
-__device__ __forceinline__ void load8(const void* p, int64_t i, float (&v)[8]) {
-    typename Vec8<T>::raw r;
-    __builtin_memcpy(&r, static_cast<const typename Vec8<T>::elem*>(p) + i, sizeof(r));
-    Vec8<T>::unpack(r, v);
-}
-
 // Columns d .. d + 7 of a row at `at`, those from k on as 0.
 template <typename T, bool UNIT>
 __device__ __forceinline__ void load_piece(const BlockArgs& a, int64_t at, int d, float (&v)[8]) {
     if (UNIT && d + 8 <= a.k) {
-        load8<T>(a.x, at + d, v);
+        load8_unaligned<T>(a.x, at + d, v);
         return;
     }
 #pragma unroll

@@ -237,6 +237,14 @@ struct Vec8<F32> {
     __device__ __forceinline__ static void store1(void* p, int64_t i, float f) { static_cast<float*>(p)[i] = f; }
 };
 
+// Eight elements from element i on by vector loads, whatever their alignment.
+template <typename T>
+__device__ __forceinline__ void load8_unaligned(const void* p, int64_t i, float (&v)[8]) {
+    typename Vec8<T>::raw r;
+    __builtin_memcpy(&r, static_cast<const typename Vec8<T>::elem*>(p) + i, sizeof(r));
+    Vec8<T>::unpack(r, v);
+}
+
 __device__ __forceinline__ float load_any(const void* p, int32_t dt, int64_t i) {
     return dt == SANDY_BF16 ? Vec8<BF16>::load1(p, i) : Vec8<F32>::load1(p, i);
 }

@@ -189,5 +189,6 @@ extern "C" int sandy_hip_take_device_errors(void* stream, uint32_t* flags, char*
     if (host & SANDY_DEVERR_ATTN_POS) return fail(e, SANDY_ERR_INVALID, "attention position_offsets must be non-negative");
     if (host & SANDY_DEVERR_QUANT_ROWS) return fail(e, SANDY_ERR_INVALID, "quant_paged rows outside the block table");
     if (host & SANDY_DEVERR_QUANT_COUNT) return fail(e, SANDY_ERR_INVALID, "quant_paged counts out of range");
+    if (host & SANDY_DEVERR_SAMPLE) return fail(e, SANDY_ERR_INVALID, "sample temperature, top_p, min_p or uniform number out of range");
     return ok(e);
 }

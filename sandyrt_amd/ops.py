@@ -632,6 +632,41 @@ def quant_moe_matmul(x: QuantMatrix, expert_offsets, weight: QuantMatrix, dtype=
     return out
 
 
+# ------------------------------------------------------------------ sampling
+@functools.lru_cache(maxsize=1024)
+def _sample_workspace(rows, vocab):
+    logits, need = _lib.SandyTensor(rank=2, dtype=_lib.F32), C.c_size_t(0)
+    logits.dims[:2] = rows, vocab
+    _lib.dcall("sandy_hip_sample_workspace", logits, C.byref(need))
+    return need.value
+
+
+def sample(logits, uniforms, temperature=None, top_k=None, top_p=None, min_p=None, index_dtype=torch.int64, ids=None,
+           probs=None):
+    """One token a row of logits [rows, vocab], drawn with the given uniform numbers
+    [rows] (f32, 0 <= u < 1); returns (ids [rows], probs [rows]).
+
+    temperature, top_p, min_p (f32) and top_k (i32 or i64) are [rows] tensors,
+    each row's own, or None for off.  Tokens rank by logit, then id; top_k keeps
+    the first ranks, top_p of those the ones before which less than top_p of the
+    weight lies, min_p of those the ones not below min_p of the likeliest, and
+    the draw walks what is left in order of ids.  temperature 0 is greedy.
+    Logits of -inf or NaN are never drawn; a row without any other gives -1.
+    probs: the token's share of what is left."""
+    if logits.dim() != 2:
+        raise SandyError(1, "sample logits must be [rows, vocab] f32 or bf16")
+    rows, device = logits.shape[0], logits.device
+    ids = torch.empty(rows, dtype=index_dtype, device=device) if ids is None else ids
+    probs = torch.empty(rows, dtype=torch.float32, device=device) if probs is None else probs
+    need = _sample_workspace(*logits.shape)
+    # the workspace is the call's own: calls on other streams and captured graphs share nothing with it
+    work = torch.empty(need, dtype=torch.uint8, device=device)
+    settings = (temperature, top_k, top_p, min_p)
+    _quant_call("sandy_hip_sample", logits.get_device(), (*settings, uniforms, ids, probs), pack(logits),
+                *map(_packed, settings), pack(uniforms), pack(ids), pack(probs), work.data_ptr() if need else None, need)
+    return ids, probs
+
+
 # ------------------------------------------------------------------ MoE
 def topk(x, k: int, axis: int = -1, index_dtype=torch.int64, values=None, indices=None):
     """TopKKernelOp: value descending, index ascending on ties (TensorCalc.cpp:1447-1518)."""
