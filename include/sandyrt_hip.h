@@ -658,7 +658,7 @@ int sandy_hip_quant_moe_matmul(const SandyTensor* x, const SandyTensor* x_scales
  * and comparisons are exact, so results do not depend on how a call is cut up; what is below 2^-s-1 weighs nothing.
  * A row without a token gives id -1 and probability 0; so does one with temperature negative or NaN, top_p NaN, min_p
  * above 1 or NaN, or u out of range, which is recorded (SANDY_DEVERR_SAMPLE).  `workspace` holds
- * sandy_hip_sample_workspace() bytes (16-byte aligned): the call's alone while it runs, its contents need not be kept or
+ * sandy_hip_sample_workspace() bytes (16-byte aligned; NULL where that is 0): the call's alone while it runs, its contents need not be kept or
  * cleared.
  */
 int sandy_hip_sample(const SandyTensor* logits, const SandyTensor* temperature, const SandyTensor* top_k,

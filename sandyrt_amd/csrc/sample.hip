@@ -6,15 +6,17 @@
 //   t = u * sum of the weights of P and M's common tokens;  the token where their running sum, in order of ids, passes t
 //
 // Weights are whole numbers: w_i rounded to 2^-s with s = 62 - log2(vocab) (44 bits of a 262144-token vocabulary).
-// Sums of them are exact in any order, so that atomics, chunks and workgroups leave no trace in the result, and every
+// Sums of them are exact in any order, so that atomics, parts and workgroups leave no trace in the result, and every
 // comparison (top_p's and the draw's, whose factors have 24 bits) is exact too, in 128 bits.
 //
 // Ranks are never formed.  Logits fall into 1023 bins of equal width from the maximum down to where weights
-// vanish; counts and weights of the bins say in which the cut of top_k and that of top_p lie, and only the tokens there
-// (a list, or where it is too long the row again) are narrowed down, 1024 bins of (logit, id) at a time.  A small top_k
-// needs counts alone: all it may keep is listed, and top_p looks at the list.  Five launches, the row read three
-// times: peak, bins, cut, gather, draw.  Rows are cut into chunks of 4096 tokens, so that a single row fills many
-// workgroups and the draw looks at one chunk.
+// vanish; counts and weights of the bins say in which the cuts of top_k, top_p and min_p lie, and only the tokens there
+// (a list, or where it is too long all of them again) are narrowed down, 1024 steps of (logit, id) at a time, the
+// last 64 by comparing each with each.  A small top_k needs counts alone: all it may keep is listed, and top_p looks at
+// the list.
+//
+// Up to 65536 tokens a workgroup does a row in one launch, reading it up to four times, mostly from L2.  Longer rows are
+// cut into parts, so that few rows fill the chip, and take five launches: peak, bins, cut, gather, draw.
 #include "common.h"
 
 #include <algorithm>
@@ -23,10 +25,13 @@
 namespace sandy_hip {
 namespace {
 
-constexpr int kChunk = 4096;    // tokens whose kept weight is one number
-constexpr int kBins = 1024;     // the last for tokens without weight
-constexpr int kList = 8192;     // tokens of the bins that hold a cut
-constexpr int kSmall = 4096;    // a top_k whose tokens are all listed
+constexpr int kChunk = 4096;      // a part is a whole number of these
+constexpr int kParts = 64;        // at most, a row
+constexpr int kBins = 1024;       // the last for tokens without weight
+constexpr int kList = 8192;       // listed tokens of a row in parts
+constexpr int kRowList = 2048;    // and of a row that one workgroup does
+constexpr int kRowVocab = 65536;  // the longest such row
+constexpr int kSmall = 1024;      // a top_k whose tokens are all listed
 constexpr int kMaxVocab = 1 << 24;
 
 struct Peak {
@@ -45,18 +50,21 @@ struct Row {
     uint32_t top_k;     // 0: off
     bool greedy, bad;
 
-    // top_k's tokens are all listed
-    __device__ bool small() const { return top_k > 0 && top_k <= kSmall; }
     __device__ bool by_p() const { return top_p < 1.0f; }
+    __device__ bool cuts() const { return top_k || by_p(); }
+    __device__ bool small() const { return top_k > 0 && top_k <= kSmall; }  // top_k's tokens are all listed
 };
 
+// Where a row's cuts lie.  Bins below `sure` are kept; tokens of bins first .. last, m_first .. m_last and k_bin,
+// as far as `limit`, are listed and kept up to the place that narrowing finds, if they are likely enough.
 struct Cut {
-    Row row;
-    // bins below `sure` are kept (as far as min_p goes); tokens of bins first .. last and k_bin are listed
-    int32_t sure, first, last, k_bin;
+    int32_t sure, first, last, m_first, m_last, k_bin, limit;
+    uint32_t rank;      // how many of k_bin's tokens (a small top_k: of the listed ones) are in top_k; 0: all
     uint64_t weight;    // of top_k's tokens in bins below k_bin (k_bin < 0: of all of them)
-    uint32_t rank;      // how many of the listed tokens from the first or k_bin on are in top_k
-    uint32_t pad;
+
+    __device__ bool in_question(int bin) const {
+        return bin <= limit && (bin == k_bin || (bin >= first && bin <= last) || (bin >= m_first && bin <= m_last));
+    }
 };
 
 struct SampleArgs {
@@ -68,16 +76,20 @@ struct SampleArgs {
     uint32_t* errw;
     int64_t stride;
     int32_t top_k_dt, ids_dt;
-    int32_t rows, vocab, chunks, parts, per;  // a part is `per` chunks, one workgroup
-    int32_t bits;                             // s
-    // workspace
-    Peak* peaks;          // [rows, parts]
-    uint64_t* weights;    // [rows, parts, kBins]; after the cut, part 0: weight up to and with each bin
-    uint32_t* counts;     // [rows, parts, kBins]; likewise
+    int32_t rows, vocab;
+    int32_t bits;         // s
+    int32_t parts, per;   // a part is `per` chunks, one workgroup of the bins and gather kernels
+    int32_t peak_parts, peak_per;
+    // workspace of rows in parts
+    Peak* peaks;          // [rows, peak_parts]
+    uint64_t* weights;    // [rows, parts, kBins]
+    uint32_t* counts;     // [rows, parts, kBins]
+    uint64_t* upto;       // [rows, kBins]: the row's weight up to and with each bin
+    Row* settings;        // [rows]
     Cut* cuts;            // [rows]
     uint32_t* listed;     // [rows]
     uint64_t* list;       // [rows, kList]
-    uint64_t* kept;       // [rows, chunks]
+    uint64_t* kept;       // [rows, parts]: kept weight of bins below the cuts
 };
 
 __device__ __forceinline__ bool token(float l) { return l > -__builtin_inff(); }  // not masked, not NaN
@@ -91,45 +103,73 @@ __device__ __forceinline__ float key_logit(uint32_t k) { return __uint_as_float(
 // (logit, id) in rank order
 __device__ __forceinline__ uint64_t place_of(float l, uint32_t id) { return static_cast<uint64_t>(rank_key(l)) << 24 | id; }
 
-// Row parameters from its parts' peaks; every thread of the workgroup gets them.
-__device__ __forceinline__ Row row_of(const SampleArgs& a, int row, Row* shared) {
-    if (threadIdx.x < 64) {
-        float mx = -__builtin_inff(), mn = __builtin_inff();
-        int arg = INT32_MAX;
-        const int p = threadIdx.x;  // at most 64 parts
-        if (p < a.parts) {
-            const Peak k = a.peaks[static_cast<int64_t>(row) * a.parts + p];
-            mx = k.max, arg = k.arg, mn = k.min;
-        }
-        Row r;
-        const float t = a.temperature ? a.temperature[row] : 1.0f;
-        r.top_p = a.top_p ? a.top_p[row] : 1.0f;
-        r.least = a.min_p ? a.min_p[row] : 0.0f;
-        r.uniform = a.uniforms[row];
-        const int64_t k = a.top_k ? load_index(a.top_k, a.top_k_dt, row) : 0;
-#pragma unroll
-        for (int m = 32; m >= 1; m >>= 1) {
-            const float ox = __shfl_xor(mx, m, 64);
-            const int oa = __shfl_xor(arg, m, 64);
-            if (ox > mx || (ox == mx && oa < arg)) mx = ox, arg = oa;
-            mn = fminf(mn, __shfl_xor(mn, m, 64));
-        }
-        if (threadIdx.x == 0) {
-            r.max = mx;
-            r.arg = arg;
-            r.bits = a.bits;
-            r.top_k = k > 0 && k < a.vocab ? static_cast<uint32_t>(k) : 0;
-            r.greedy = t == 0.0f;
-            r.bad = !(t >= 0.0f) || r.top_p != r.top_p || !(r.least <= 1.0f) || !(r.uniform >= 0.0f && r.uniform < 1.0f);
-            r.rate = 1.4426950408889634074 / static_cast<double>(t);
-            // bins reach to where weights vanish (2^-bits-1, and a little on), or to the lowest logit where that is nearer
-            const double width = fmin(static_cast<double>(mx) - static_cast<double>(mn), (a.bits + 1.5) / r.rate);
-            r.scale = width > 0.0 ? static_cast<float>(fmin((kBins - 2) / width, 3.0e38)) : 0.0f;
-            *shared = r;
-        }
-    }
+// ------------------------------------------------------------------ sums over waves and workgroups
+// The value `CTRL` names of another lane of the wave, 0 where there is none.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lane_move(uint32_t v) {
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t lane_move(uint64_t v) {
+    return static_cast<uint64_t>(lane_move<CTRL, ROWS>(static_cast<uint32_t>(v >> 32))) << 32 | lane_move<CTRL, ROWS>(static_cast<uint32_t>(v));
+}
+// Inclusive sums over a wave by DPP moves: within rows of 16 lanes, then each row's last lane to the next rows.
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v += lane_move<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += lane_move<0x112, 0xf>(v);
+    v += lane_move<0x114, 0xf>(v);
+    v += lane_move<0x118, 0xf>(v);
+    v += lane_move<0x142, 0xa>(v);  // row_bcast 15 to rows 1 and 3
+    v += lane_move<0x143, 0xc>(v);  // row_bcast 31 to rows 2 and 3
+    return v;
+}
+// Inclusive sums over a workgroup of WAVES waves; `waves` holds WAVES values, *total all of them.
+template <int WAVES, typename V>
+__device__ __forceinline__ V block_scan(V v, V* waves, V* total) {
+    const int wave = threadIdx.x >> 6;
+    v = wave_scan(v);
+    __syncthreads();  // the last use of `waves` is over
+    if ((threadIdx.x & 63) == 63) waves[wave] = v;
     __syncthreads();
-    return *shared;
+    V before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        if (w < wave) before += waves[w];
+        all += waves[w];
+    }
+    *total = all;
+    return before + v;
+}
+
+// ------------------------------------------------------------------ a row's settings
+__device__ __forceinline__ void better_peak(float& mx, int& arg, float& mn, float ox, int oa, float on) {
+    if (ox > mx || (ox == mx && oa < arg)) mx = ox, arg = oa;
+    mn = fminf(mn, on);
+}
+__device__ __forceinline__ void wave_peak(float& mx, int& arg, float& mn) {
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) better_peak(mx, arg, mn, __shfl_xor(mx, m, 64), __shfl_xor(arg, m, 64), __shfl_xor(mn, m, 64));
+}
+
+__device__ __forceinline__ Row make_row(const SampleArgs& a, int row, float mx, int arg, float mn) {
+    Row r;
+    const float t = a.temperature ? a.temperature[row] : 1.0f;
+    const int64_t k = a.top_k ? load_index(a.top_k, a.top_k_dt, row) : 0;
+    r.top_p = a.top_p ? a.top_p[row] : 1.0f;
+    r.least = a.min_p ? a.min_p[row] : 0.0f;
+    r.uniform = a.uniforms[row];
+    r.max = mx;
+    r.arg = arg;
+    r.bits = a.bits;
+    r.top_k = k > 0 && k < a.vocab ? static_cast<uint32_t>(k) : 0;
+    r.greedy = t == 0.0f;
+    r.bad = !(t >= 0.0f) || r.top_p != r.top_p || !(r.least <= 1.0f) || !(r.uniform >= 0.0f && r.uniform < 1.0f);
+    r.rate = 1.4426950408889634074 / static_cast<double>(t);
+    // bins reach to where weights vanish (2^-bits-1, and a little on), or to the lowest logit where that is nearer
+    const double width = fmin(static_cast<double>(mx) - static_cast<double>(mn), (a.bits + 1.5) / r.rate);
+    r.scale = width > 0.0 ? static_cast<float>(fmin((kBins - 2) / width, 3.0e38)) : 0.0f;
+    return r;
 }
 
 // exp((l - max) / T) = 2^f 2^k, 1 at the maximum: f in -1/2 .. 1/2 by the Taylor series of e^(f ln 2) to the 11th
@@ -162,6 +202,7 @@ __device__ __forceinline__ uint64_t weight_of(const Row& r, const Ratio& ratio) 
     const double unit = __longlong_as_double(static_cast<long long>(1023 + r.bits + ratio.k) << 52);
     return static_cast<uint64_t>(__double_as_longlong(fma(ratio.p, unit, 4503599627370496.0))) - 0x4330000000000000ull;
 }
+__device__ __forceinline__ uint64_t weight_of(const Row& r, float l) { return weight_of(r, ratio_of(r, l)); }
 __device__ __forceinline__ bool likely(const Row& r, const Ratio& ratio) {
     return r.least <= 0.0f || ratio.value() >= static_cast<double>(r.least);
 }
@@ -182,6 +223,8 @@ __device__ __forceinline__ uint64_t part_of(float p, uint64_t w, bool up) {
     const uint64_t q = static_cast<uint64_t>(prod >> shift);
     return q + (up && (prod & ((static_cast<unsigned __int128>(1) << shift) - 1)) != 0 ? 1 : 0);
 }
+// top_p's part of a weight, at least; 0 where it is that of the first token alone
+__device__ __forceinline__ uint64_t nucleus(const Row& r, uint64_t weight) { return r.top_p > 0.0f ? part_of(r.top_p, weight, true) : 0; }
 
 // Eight tokens from id `first` on of a row, what lies past the vocabulary as masked.
 template <typename T>
@@ -194,12 +237,395 @@ __device__ __forceinline__ void load_tokens(const SampleArgs& a, int64_t at, int
     for (int j = 0; j < 8; j++) v[j] = first + j < a.vocab ? Vec8<T>::load1(a.logits, at + first + j) : -__builtin_inff();
 }
 
-// ------------------------------------------------------------------ peak
+__device__ __forceinline__ void store_token(const SampleArgs& a, int row, int64_t id, float prob) {
+    store_index(a.ids, a.ids_dt, row, id);
+    if (a.probs) a.probs[row] = prob;
+}
+// Rows that need no draw: bad settings (recorded), no token, or greedy.
+__device__ __forceinline__ bool drawn(const SampleArgs& a, const Row& r, int row) {
+    const bool none = r.bad || r.arg == INT32_MAX;
+    if (!none && !r.greedy) return false;
+    if (threadIdx.x == 0) {
+        if (r.bad) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_SAMPLE));
+        store_token(a, row, none ? -1 : r.arg, none ? 0.0f : 1.0f);
+    }
+    return true;
+}
+
+// ------------------------------------------------------------------ where the cuts lie
+struct CutShared {
+    uint64_t waves64[16], low, high;
+    uint32_t waves32[16], rank;
+    int k_bin, k_last, p_first, p_last;
+};
+
+// Cuts of a row from its bins' counts and weights, one bin a thread of 1024; *up_to: the weight up to and with the bin.
+__device__ __forceinline__ Cut find_cuts(const Row& r, uint32_t c, uint64_t w, CutShared& sh, uint64_t* up_to) {
+    const int bin = threadIdx.x;
+    uint64_t all = 0, w_to = 0;
+    uint32_t tokens = 0, c_to = 0;
+    if (!r.small()) w_to = block_scan<16>(w, sh.waves64, &all);
+    if (r.top_k) c_to = block_scan<16>(c, sh.waves32, &tokens);
+    *up_to = w_to;
+    if (bin == 0) sh.k_bin = -1, sh.k_last = sh.p_first = sh.p_last = kBins, sh.low = sh.high = all, sh.rank = 0;
+    __syncthreads();
+    const uint32_t k = r.top_k;
+    // the bin where top_k ends, if it ends inside one whose tokens weigh anything
+    if (k && k < tokens && c_to >= k && c_to - c < k) {
+        sh.k_last = bin;
+        if (c_to == k || bin == kBins - 1) {
+            sh.low = sh.high = w_to;
+        } else {
+            sh.k_bin = bin;
+            sh.low = w_to - w;
+            sh.high = w_to;
+            sh.rank = k - (c_to - c);
+        }
+    }
+    __syncthreads();
+    Cut cut{};
+    cut.limit = sh.k_last;
+    cut.k_bin = -1;
+    cut.first = cut.m_first = kBins;
+    cut.last = cut.m_last = -1;
+    if (r.small()) {
+        // all that top_k may keep: to its last bin, or every token that weighs anything
+        cut.first = 0;
+        cut.last = min(sh.k_last, kBins - 2);
+        cut.rank = k < tokens && sh.k_last < kBins - 1 ? k : 0;
+        return cut;
+    }
+    cut.weight = sh.low;
+    if (r.by_p()) {
+        // top_p's cut lies where the sums reach its part of top_k's weight, which is between low and high
+        const uint64_t from = nucleus(r, sh.low), to = nucleus(r, sh.high), before = w_to - w;
+        if (w_to >= from && (bin == 0 || before < from)) sh.p_first = bin;
+        if (w_to >= to && (bin == 0 || before < to)) sh.p_last = bin;
+    }
+    __syncthreads();
+    const int k_bin = sh.k_bin;
+    cut.sure = k_bin >= 0 ? k_bin : sh.k_last < kBins ? sh.k_last + 1 : kBins;
+    int p_first = kBins;
+    if (r.by_p()) cut.sure = min(cut.sure, p_first = sh.p_first);
+    if (r.least > 0.0f) {
+        // min_p's cut is at a logit: within a bin of where that falls
+        const double at = -log2(static_cast<double>(r.least)) / r.rate * static_cast<double>(r.scale);
+        if (at < kBins) {
+            cut.m_first = max(static_cast<int>(at) - 1, 0);
+            cut.m_last = static_cast<int>(at) + 1;
+            cut.sure = min(cut.sure, cut.m_first);
+            if (cut.m_last < p_first && cut.m_last < (k_bin >= 0 ? k_bin : kBins)) return cut;  // nothing else cuts
+        }
+    }
+    if (r.by_p()) {
+        cut.first = p_first;
+        cut.last = sh.p_last;
+    }
+    if (k_bin >= 0) {
+        cut.k_bin = k_bin;
+        cut.rank = sh.rank;
+    }
+    return cut;
+}
+
+// ------------------------------------------------------------------ narrowing down
+struct NarrowShared {
+    uint64_t bin_weights[kBins], waves64[16], lows[16], highs[16], places[64], weights[64];
+    uint64_t lo, hi, weight_before;
+    uint32_t bin_counts[kBins], waves32[16], count_before, n;
+};
+
+// Of the tokens that each(f) names as f(place, weight), in rank order: the place of the one with which they become `rank`,
+// or (rank 0) with which their weights reach `weight`, the first token reaching 0; the last of all if they never do.
+// sh.weight_before is then the sum up to and with it.  1024 threads.
+template <typename Each>
+__device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint64_t weight, Each each) {
+    const int tid = threadIdx.x;
+    uint64_t low = ~uint64_t{0}, high = 0;
+    uint32_t n = 0;
+    each([&](uint64_t place, uint64_t) {
+        low = min(low, place);
+        high = max(high, place);
+        n++;
+    });
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) {
+        low = min(low, static_cast<uint64_t>(__shfl_xor(low, m, 64)));
+        high = max(high, static_cast<uint64_t>(__shfl_xor(high, m, 64)));
+    }
+    if ((tid & 63) == 0) sh.lows[tid >> 6] = low, sh.highs[tid >> 6] = high;
+    uint32_t tokens;
+    block_scan<16>(n, sh.waves32, &tokens);
+    if (tid < 64) {
+        low = sh.lows[tid & 15];
+        high = sh.highs[tid & 15];
+#pragma unroll
+        for (int m = 8; m >= 1; m >>= 1) {
+            low = min(low, static_cast<uint64_t>(__shfl_xor(low, m, 64)));
+            high = max(high, static_cast<uint64_t>(__shfl_xor(high, m, 64)));
+        }
+        if (tid == 0) sh.lo = low, sh.hi = high, sh.weight_before = 0, sh.count_before = 0, sh.n = tokens;
+    }
+    __syncthreads();
+    while (sh.n > 64) {  // each round is among fewer than before: a step of 1024
+        const uint64_t from = sh.lo, to = sh.hi;
+        const int shift = max(0, 54 - __builtin_clzll((to - from) | 1));
+        sh.bin_weights[tid] = 0;
+        sh.bin_counts[tid] = 0;
+        __syncthreads();
+        each([&](uint64_t place, uint64_t w) {
+            if (place < from || place > to) return;
+            const int q = static_cast<int>((place - from) >> shift);
+            atomicAdd(&sh.bin_counts[q], 1u);
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bin_weights[q]), static_cast<unsigned long long>(w));
+        });
+        __syncthreads();
+        const uint64_t w = sh.bin_weights[tid];
+        const uint32_t c = sh.bin_counts[tid];
+        uint64_t all;
+        const uint64_t w_to = sh.weight_before + block_scan<16>(w, sh.waves64, &all);
+        const uint32_t c_to = sh.count_before + block_scan<16>(c, sh.waves32, &tokens);
+        const bool here = c != 0 && (rank ? c_to >= rank && c_to - c < rank : w_to >= weight && (w_to - w < weight || c_to == c));
+        if (!__syncthreads_or(here)) {
+            if (tid == 0) sh.weight_before += all;
+            __syncthreads();
+            return to;
+        }
+        if (here) {
+            sh.lo = from + (static_cast<uint64_t>(tid) << shift);
+            sh.hi = min(to, from + ((static_cast<uint64_t>(tid) + 1) << shift) - 1);
+            sh.weight_before = w_to - w;
+            sh.count_before = c_to - c;
+            sh.n = c;
+        }
+        __syncthreads();
+    }
+    // the last few: each with each
+    const uint64_t from = sh.lo, to = sh.hi;
+    const uint32_t few = sh.n;
+    __syncthreads();
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    each([&](uint64_t place, uint64_t w) {
+        if (place < from || place > to) return;
+        const uint32_t i = atomicAdd(&sh.n, 1u);
+        sh.places[i] = place;
+        sh.weights[i] = w;
+    });
+    __syncthreads();
+    if (tid < 64) {
+        const bool in = tid < few;
+        const uint64_t place = in ? sh.places[tid] : ~uint64_t{0}, w = in ? sh.weights[tid] : 0;
+        uint64_t w_to = sh.weight_before + w, all = sh.weight_before;
+        uint32_t c_to = sh.count_before + 1;
+        for (uint32_t i = 0; i < few; i++) {
+            const uint64_t other = sh.weights[i];
+            const bool before = sh.places[i] < place;
+            w_to += before ? other : 0;
+            c_to += before ? 1 : 0;
+            all += other;
+        }
+        const bool here = in && (rank ? c_to == rank : w_to >= weight && (w_to - w < weight || c_to == 1));
+        const uint64_t found = __ballot(here);
+        if (here) sh.lo = place, sh.weight_before = w_to;
+        if (!found && tid == 0) sh.lo = to, sh.weight_before = all;
+    }
+    __syncthreads();
+    return sh.lo;
+}
+
+// The last place that top_k and top_p keep: ~0 where no listed token is cut by them.  each(b0, b1, f) names the listed
+// tokens of bins b0 .. b1; up_to(bin): the row's weight up to and with a bin.
+template <typename Each, typename UpTo>
+__device__ __forceinline__ uint64_t last_place(const Row& r, const Cut& cut, NarrowShared& sh, Each each, UpTo up_to) {
+    uint64_t last = ~uint64_t{0}, kept = cut.weight;  // top_k's
+    const bool small = r.small();
+#pragma unroll 1
+    for (int step = 0; step < 2; step++) {
+        // first where top_k ends (a small one with room for all: their weight), then where top_p does
+        int b0 = 0, b1 = kBins;
+        uint32_t rank = 0;
+        uint64_t weight = 0;
+        if (step == 0) {
+            if (small ? !cut.rank && !r.by_p() : cut.k_bin < 0) continue;
+            rank = cut.rank ? cut.rank : UINT32_MAX;
+            if (!small) b0 = b1 = cut.k_bin;
+        } else {
+            if (small ? !r.by_p() : cut.last < 0) continue;
+            weight = nucleus(r, kept);
+            if (!small) {
+                int bin = cut.first;
+                while (bin < cut.last && up_to(bin) < weight) bin++;
+                const uint64_t before = bin > 0 ? up_to(bin - 1) : 0;
+                weight = weight > before ? weight - before : 0;
+                b0 = b1 = bin;
+            }
+        }
+        const uint64_t place = narrow(sh, rank, weight, [&](auto f) { each(b0, b1, f); });
+        last = min(last, place);
+        if (step == 0) kept += sh.weight_before;
+        __syncthreads();
+    }
+    return last;
+}
+
+// ------------------------------------------------------------------ a row a workgroup
+constexpr int kBlock = 8192;  // tokens a workgroup of 1024 takes at a time
+
+struct RowShared {
+    uint64_t weights[kBins], up_to[kBins];
+    uint32_t counts[kBins];
+    uint64_t places[kRowList], held[kRowList];
+    NarrowShared narrow;
+    uint64_t sums[kRowVocab / kBlock][16];
+    Peak peaks[16];
+    CutShared cuts;
+    Row row;
+    uint32_t listed;
+};
+
+// f(logits, first id) for this thread's eight tokens of each block of a row, the next eight requested meanwhile.
+template <typename T, typename F>
+__device__ __forceinline__ void row_tokens(const SampleArgs& a, int64_t at, F f) {
+    float next[8];
+    load_tokens<T>(a, at, static_cast<int>(threadIdx.x) * 8, next);
+#pragma unroll 1
+    for (int first = threadIdx.x * 8; first - static_cast<int>(threadIdx.x) * 8 < a.vocab; first += kBlock) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = next[j];
+        load_tokens<T>(a, at, first + kBlock, next);
+        f(v, first);
+    }
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a) {
+    __shared__ RowShared sh;
+    const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t at = row * a.stride;
+    float mx = -__builtin_inff(), mn = __builtin_inff();
+    int arg = INT32_MAX;
+    sh.weights[tid] = 0;
+    sh.counts[tid] = 0;
+    if (tid == 0) sh.listed = 0;
+    row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (token(v[j])) better_peak(mx, arg, mn, v[j], first + j, v[j]);
+    });
+    wave_peak(mx, arg, mn);
+    if (lane == 0) sh.peaks[wave] = Peak{mx, mn, arg, 0};
+    __syncthreads();
+    if (wave == 0) {
+        const Peak p = sh.peaks[lane & 15];
+        mx = p.max, arg = p.arg, mn = p.min;
+        wave_peak(mx, arg, mn);
+        if (lane == 0) sh.row = make_row(a, row, mx, arg, mn);
+    }
+    __syncthreads();
+    const Row r = sh.row;
+    if (drawn(a, r, row)) return;
+    Cut cut{};
+    cut.sure = cut.limit = kBins;
+    cut.k_bin = cut.last = cut.m_last = -1;
+    uint64_t last = ~uint64_t{0};
+    if (r.cuts()) {
+        const bool count = r.top_k != 0, weigh = !r.small();
+        row_tokens<T>(a, at, [&](const float (&v)[8], int) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (!token(v[j])) continue;
+                const int b = bin_of(r, v[j]);
+                if (count) atomicAdd(&sh.counts[b], 1u);
+                if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.weights[b]), static_cast<unsigned long long>(weight_of(r, v[j])));
+            }
+        });
+        __syncthreads();
+        uint64_t up_to;
+        cut = find_cuts(r, sh.counts[tid], sh.weights[tid], sh.cuts, &up_to);
+        sh.up_to[tid] = up_to;
+        row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (!token(v[j]) || !cut.in_question(bin_of(r, v[j]))) continue;
+                const uint32_t i = atomicAdd(&sh.listed, 1u);
+                if (i < kRowList) sh.places[i] = place_of(v[j], first + j);
+            }
+        });
+        __syncthreads();
+        const uint32_t listed = sh.listed;
+        if (listed <= kRowList)
+            for (uint32_t i = tid; i < listed; i += 1024) sh.held[i] = weight_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
+        __syncthreads();
+        auto each = [&](int b0, int b1, auto f) {
+            if (listed <= kRowList) {
+                for (uint32_t i = tid; i < listed; i += 1024) {
+                    const int b = bin_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
+                    if (b >= b0 && b <= b1) f(sh.places[i], sh.held[i]);
+                }
+                return;
+            }
+            row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (!token(v[j])) continue;
+                    const int b = bin_of(r, v[j]);
+                    if (b >= b0 && b <= b1 && cut.in_question(b)) f(place_of(v[j], first + j), weight_of(r, v[j]));
+                }
+            });
+        };
+        last = last_place(r, cut, sh.narrow, each, [&](int bin) { return sh.up_to[bin]; });
+    }
+    // a token's kept weight, and the sums over each wave's tokens of a block
+    auto kept = [&](float l, int id) -> uint64_t {
+        if (!token(l)) return 0;
+        const int b = bin_of(r, l);
+        if (b >= cut.sure && !(cut.in_question(b) && place_of(l, id) <= last)) return 0;
+        const Ratio ratio = ratio_of(r, l);
+        return likely(r, ratio) ? weight_of(r, ratio) : 0;
+    };
+    row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
+        uint64_t mine = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) mine += kept(v[j], first + j);
+        mine = wave_scan(mine);
+        if (lane == 63) sh.sums[first / kBlock][wave] = mine;
+    });
+    __syncthreads();
+    const int blocks = (a.vocab + kBlock - 1) / kBlock;
+    uint64_t total = 0;
+    for (int i = 0; i < blocks * 16; i++) total += sh.sums[i >> 4][i & 15];
+    const uint64_t target = part_of(r.uniform, total, false);
+    // the block's wave in which the sum passes the target
+    uint64_t run = 0;
+    for (int i = 0; i < blocks * 16; i++) {
+        const uint64_t w = sh.sums[i >> 4][i & 15];
+        if (run <= target && run + w > target && (i & 15) == wave) {
+            float v[8];
+            uint64_t w8[8], mine = 0;
+            const int first = (i >> 4) * kBlock + tid * 8;
+            load_tokens<T>(a, at, first, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) mine += w8[j] = kept(v[j], first + j);
+            uint64_t to = run + wave_scan(mine) - mine;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (to <= target && to + w8[j] > target)
+                    store_token(a, row, first + j, static_cast<float>(static_cast<double>(w8[j]) / static_cast<double>(total)));
+                to += w8[j];
+            }
+        }
+        run += w;
+    }
+}
+
+// ------------------------------------------------------------------ rows in parts
 template <typename T>
 __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
-    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const int row = blockIdx.x / a.peak_parts, part = blockIdx.x - row * a.peak_parts;
     const int64_t at = row * a.stride;
-    const int begin = part * a.per * kChunk, end = min(begin + a.per * kChunk, a.vocab);
+    const int begin = part * a.peak_per * kChunk, end = min(begin + a.peak_per * kChunk, a.vocab);
     float mx = -__builtin_inff(), mn = __builtin_inff();
     int arg = INT32_MAX;
     for (int chunk = begin; chunk < end; chunk += kChunk) {
@@ -210,446 +636,272 @@ __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
         for (int h = 0; h < kChunk / 2048; h++)
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (token(v[h][j])) {
-                    if (v[h][j] > mx || arg == INT32_MAX) mx = v[h][j], arg = chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8 + j;
-                    mn = fminf(mn, v[h][j]);
-                }
+                if (token(v[h][j])) better_peak(mx, arg, mn, v[h][j], chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8 + j, v[h][j]);
     }
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        const float ox = __shfl_xor(mx, m, 64);
-        const int oa = __shfl_xor(arg, m, 64);
-        if (ox > mx || (ox == mx && oa < arg)) mx = ox, arg = oa;
-        mn = fminf(mn, __shfl_xor(mn, m, 64));
-    }
+    wave_peak(mx, arg, mn);
     __shared__ Peak waves[4];
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = Peak{mx, mn, arg, 0};
     __syncthreads();
     if (threadIdx.x == 0) {
-        Peak p = waves[0];
 #pragma unroll
-        for (int w = 1; w < 4; w++) {
-            if (waves[w].max > p.max || (waves[w].max == p.max && waves[w].arg < p.arg)) p.max = waves[w].max, p.arg = waves[w].arg;
-            p.min = fminf(p.min, waves[w].min);
-        }
-        a.peaks[blockIdx.x] = p;
+        for (int w = 1; w < 4; w++) better_peak(mx, arg, mn, waves[w].max, waves[w].arg, waves[w].min);
+        a.peaks[blockIdx.x] = Peak{mx, mn, arg, 0};
     }
 }
 
-// ------------------------------------------------------------------ bins
-// Counts where top_k asks for them, weights where top_p does and top_k's tokens are not all listed.
+// Settings from the parts' peaks; every thread of the workgroup gets them.
+__device__ __forceinline__ Row row_of(const SampleArgs& a, int row, Row* shared) {
+    if (threadIdx.x < 64) {
+        float mx = -__builtin_inff(), mn = __builtin_inff();
+        int arg = INT32_MAX;
+        if (static_cast<int>(threadIdx.x) < a.peak_parts) {
+            const Peak p = a.peaks[static_cast<int64_t>(row) * a.peak_parts + threadIdx.x];
+            mx = p.max, arg = p.arg, mn = p.min;
+        }
+        wave_peak(mx, arg, mn);
+        if (threadIdx.x == 0) *shared = make_row(a, row, mx, arg, mn);
+    }
+    __syncthreads();
+    return *shared;
+}
+
+// Counts where top_k asks for them, weights unless all of top_k's tokens are listed; the part's weight of rows that
+// nothing cuts but min_p.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
-    __shared__ uint64_t weights[kBins];
+    __shared__ uint64_t weights[kBins], waves[4];
     __shared__ uint32_t counts[kBins];
     __shared__ Row shared;
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     for (int i = threadIdx.x; i < kBins; i += 256) weights[i] = 0, counts[i] = 0;
     const Row r = row_of(a, row, &shared);
-    if (r.greedy || r.bad || !(r.top_k || r.by_p())) return;
+    if (r.greedy || r.bad) return;
     const int64_t at = row * a.stride;
     const int begin = part * a.per * kChunk, end = min(begin + a.per * kChunk, a.vocab);
-    auto fill = [&](auto count, auto weigh) {
+    auto tokens = [&](auto f) {
         for (int i = begin + threadIdx.x * 8; i < end; i += 2048) {
             float v[8];
             load_tokens<T>(a, at, i, v);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (!token(v[j])) continue;
-                const int b = bin_of(r, v[j]);
-                if constexpr (decltype(count)::value) atomicAdd(&counts[b], 1u);
-                if constexpr (decltype(weigh)::value)
-                    atomicAdd(reinterpret_cast<unsigned long long*>(&weights[b]), static_cast<unsigned long long>(weight_of(r, ratio_of(r, v[j]))));
-            }
+            for (int j = 0; j < 8; j++)
+                if (token(v[j])) f(v[j]);
         }
     };
-    const bool weigh = r.by_p() && !r.small();
-    if (!weigh) fill(std::true_type{}, std::false_type{});
-    else if (r.top_k) fill(std::true_type{}, std::true_type{});
-    else fill(std::false_type{}, std::true_type{});
+    auto count = [&](float l) { atomicAdd(&counts[bin_of(r, l)], 1u); };
+    auto weigh = [&](float l) { atomicAdd(reinterpret_cast<unsigned long long*>(&weights[bin_of(r, l)]), static_cast<unsigned long long>(weight_of(r, l))); };
+    if (!r.cuts()) {
+        uint64_t sum = 0, total;
+        tokens([&](float l) {
+            const Ratio ratio = ratio_of(r, l);
+            if (likely(r, ratio)) sum += weight_of(r, ratio);
+        });
+        block_scan<4>(sum, waves, &total);
+        if (threadIdx.x == 0) a.kept[blockIdx.x] = total;
+        return;
+    }
+    if (r.small()) tokens(count);
+    else if (r.top_k) tokens([&](float l) { count(l), weigh(l); });
+    else tokens(weigh);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += 256) {
-        a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i] = weights[i];
-        a.counts[static_cast<int64_t>(blockIdx.x) * kBins + i] = counts[i];
+        if (!r.small()) a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i] = weights[i];
+        if (r.top_k) a.counts[static_cast<int64_t>(blockIdx.x) * kBins + i] = counts[i];
     }
 }
 
-// ------------------------------------------------------------------ sums over a workgroup of 1024
-// Inclusive sums of v over the threads; `waves` holds 16 values, `total` all of them.
-template <typename V>
-__device__ __forceinline__ V block_scan(V v, V* waves, V* total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const V o = __shfl_up(v, s, 64);
-        if (lane >= s) v += o;
-    }
-    __syncthreads();  // the last use of `waves` is over
-    if (lane == 63) waves[wave] = v;
-    __syncthreads();
-    V before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < 16; w++) {
-        if (w < wave) before += waves[w];
-        all += waves[w];
-    }
-    *total = all;
-    return before + v;
-}
-
-// ------------------------------------------------------------------ cut
 __global__ __launch_bounds__(1024) void sample_cut_kernel(SampleArgs a) {
     __shared__ Row shared;
-    __shared__ uint64_t waves64[16];
-    __shared__ uint32_t waves32[16];
-    __shared__ int k_bin, k_last, p_first, p_last;
-    __shared__ uint64_t low, high;
-    __shared__ uint32_t rank;
+    __shared__ CutShared sh;
     const int row = blockIdx.x, bin = threadIdx.x;
     const Row r = row_of(a, row, &shared);
-    uint64_t w = 0, w_to = 0, all = 0;
-    uint32_t c = 0, c_to = 0, tokens = 0;
-    const bool cuts = !r.greedy && !r.bad && (r.top_k || r.by_p());
-    if (cuts) {
+    Cut cut{};
+    cut.sure = cut.limit = kBins;
+    cut.k_bin = cut.last = cut.m_last = -1;
+    if (!drawn(a, r, row) && r.cuts()) {
+        uint64_t w = 0, up_to;
+        uint32_t c = 0;
         const int64_t first = static_cast<int64_t>(row) * a.parts * kBins + bin;
+        if (!r.small())
 #pragma unroll 8
-        for (int p = 0; p < a.parts; p++) {
-            w += a.weights[first + p * kBins];
-            c += a.counts[first + p * kBins];
-        }
-        w_to = block_scan(w, waves64, &all);
-        c_to = block_scan(c, waves32, &tokens);
-        a.weights[first] = w_to;  // part 0's, which no one else reads before the draw
+            for (int p = 0; p < a.parts; p++) w += a.weights[first + p * kBins];
+        if (r.top_k)
+#pragma unroll 8
+            for (int p = 0; p < a.parts; p++) c += a.counts[first + p * kBins];
+        cut = find_cuts(r, c, w, sh, &up_to);
+        a.upto[static_cast<int64_t>(row) * kBins + bin] = up_to;
     }
-    if (bin == 0) k_bin = -1, k_last = p_first = p_last = kBins, low = high = all, rank = 0;
-    __syncthreads();
-    const uint32_t k = r.top_k;
-    // the bin where top_k ends, if it ends inside one whose tokens weigh anything
-    if (cuts && k && k < tokens && c_to >= k && c_to - c < k) {
-        k_last = bin;
-        if (c_to == k || bin == kBins - 1) {
-            low = high = w_to;
-        } else {
-            k_bin = bin;
-            low = w_to - w;
-            high = w_to;
-            rank = k - (c_to - c);
-        }
-    }
-    __syncthreads();
-    if (cuts && r.by_p() && !r.small()) {
-        // top_p's cut lies where the sums reach its part of top_k's weight, which is between low and high
-        const uint64_t from = r.top_p > 0.0f ? part_of(r.top_p, low, true) : 0, to = r.top_p > 0.0f ? part_of(r.top_p, high, true) : 0;
-        const uint64_t before = w_to - w;
-        if (w_to >= from && (bin == 0 || before < from)) p_first = bin;
-        if (w_to >= to && (bin == 0 || before < to)) p_last = bin;
-    }
-    __syncthreads();
     if (bin == 0) {
-        if (r.bad) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_SAMPLE));
-        a.listed[row] = 0;
-        Cut cut;
-        cut.row = r;
-        cut.weight = low;
-        cut.rank = rank;
-        cut.pad = 0;
-        cut.k_bin = k_bin;
-        cut.first = kBins;
-        cut.last = -1;
-        const int by_k = k_bin >= 0 ? k_bin : k_last < kBins ? k_last + 1 : kBins;
-        cut.sure = by_k;
-        if (cuts && r.small()) {
-            // all that top_k may keep: to its last bin, or every token that weighs anything
-            cut.sure = cut.first = 0;
-            cut.last = min(k_last, kBins - 2);
-            cut.rank = k < tokens && k_last < kBins - 1 ? k : 0;
-        } else if (cuts && r.by_p()) {
-            cut.first = p_first;
-            cut.last = p_last;
-            cut.sure = min(p_first, by_k);
-        }
+        a.settings[row] = r;
         a.cuts[row] = cut;
+        a.listed[row] = 0;
     }
 }
 
-__device__ __forceinline__ bool in_question(const Cut& c, int bin) { return bin == c.k_bin || (bin >= c.first && bin <= c.last); }
-
-// ------------------------------------------------------------------ gather
+// Lists the tokens in question, and sums up what a part keeps for sure from its bins.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
     __shared__ uint64_t waves[4], places[kChunk];
     __shared__ uint32_t found, to;
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
+    const Row r = a.settings[row];
+    if (r.greedy || r.bad || !r.cuts()) return;
     const Cut cut = a.cuts[row];
-    const Row& r = cut.row;
-    if (r.greedy || r.bad) return;
     const int64_t at = row * a.stride;
-    for (int chunk = part * a.per; chunk < min((part + 1) * a.per, a.chunks); chunk++) {
-        if (threadIdx.x == 0) found = 0;
-        __syncthreads();
-        uint64_t sum = 0;
+    uint64_t sum = 0, total;
+    for (int i = threadIdx.x; i < cut.sure && i < kBins; i += 256) sum += a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i];
+    block_scan<4>(sum, waves, &total);
+    if (threadIdx.x == 0) a.kept[blockIdx.x] = total, found = 0;
+    __syncthreads();
+    for (int chunk = part * a.per * kChunk; chunk < min((part + 1) * a.per * kChunk, a.vocab); chunk += kChunk) {
         float v[kChunk / 2048][8];
 #pragma unroll
-        for (int h = 0; h < kChunk / 2048; h++) load_tokens<T>(a, at, chunk * kChunk + h * 2048 + static_cast<int>(threadIdx.x) * 8, v[h]);
+        for (int h = 0; h < kChunk / 2048; h++) load_tokens<T>(a, at, chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8, v[h]);
 #pragma unroll
         for (int h = 0; h < kChunk / 2048; h++)
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                if (!token(v[h][j])) continue;
-                const int b = bin_of(r, v[h][j]);
-                if (b < cut.sure) {
-                    const Ratio ratio = ratio_of(r, v[h][j]);
-                    if (likely(r, ratio)) sum += weight_of(r, ratio);
-                } else if (in_question(cut, b)) {
-                    places[atomicAdd(&found, 1u)] = place_of(v[h][j], chunk * kChunk + h * 2048 + static_cast<int>(threadIdx.x) * 8 + j);
-                }
+                if (!token(v[h][j]) || !cut.in_question(bin_of(r, v[h][j]))) continue;
+                places[atomicAdd(&found, 1u)] = place_of(v[h][j], chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8 + j);
             }
-        sum = wave_sum(sum);
-        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = sum;
         __syncthreads();
-        if (threadIdx.x == 0) {
-            a.kept[static_cast<int64_t>(row) * a.chunks + chunk] = waves[0] + waves[1] + waves[2] + waves[3];
-            if (found) to = atomicAdd(&a.listed[row], found);
-        }
+        if (found == 0) continue;  // the same for all
+        if (threadIdx.x == 0) to = atomicAdd(&a.listed[row], found);
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < found && to + i < kList; i += 256) a.list[static_cast<int64_t>(row) * kList + to + i] = places[i];
         __syncthreads();
+        if (threadIdx.x == 0) found = 0;
+        __syncthreads();
     }
 }
 
-// ------------------------------------------------------------------ draw
-// What the draw of a row keeps in LDS.
 struct DrawShared {
     uint64_t places[kList], weights[kList];
-    uint64_t bin_weights[kBins], waves64[16], lows[16], highs[16];
-    uint32_t bin_counts[kBins], waves32[16];
-    uint64_t lo, hi, weight_before;
-    uint32_t count_before;
+    NarrowShared narrow;
+    uint64_t waves64[16], sums[kParts], before;
     int chosen;
 };
-
-// f(place, weight, bin) for every listed token, or (whole) every token of the row.
-template <typename T, typename F>
-__device__ __forceinline__ void each_token(const SampleArgs& a, const Row& r, const DrawShared& sh, int row, uint32_t listed, F f) {
-    if (listed <= kList) {
-        for (uint32_t i = threadIdx.x; i < listed; i += 1024) f(sh.places[i], sh.weights[i], bin_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24))));
-        return;
-    }
-    for (int i = threadIdx.x * 8; i < a.vocab; i += 8192) {
-        float v[8];
-        load_tokens<T>(a, row * a.stride, i, v);
-#pragma unroll 1
-        for (int j = 0; j < 8; j++) {
-            float l = v[0];
-#pragma unroll
-            for (int q = 1; q < 8; q++) l = j == q ? v[q] : l;
-            if (token(l)) f(place_of(l, i + j), weight_of(r, ratio_of(r, l)), bin_of(r, l));
-        }
-    }
-}
-
-// Of the tokens of bins b0 .. b1, in rank order: the place of the one with which they become `rank`, or (rank 0) with
-// which their weights reach `weight`; weight_before is then the sum up to and with it.  Places are told apart 1024
-// equal steps at a time, each time among fewer than before.
-template <typename T>
-__device__ __attribute__((noinline)) uint64_t narrow(const SampleArgs& a, const Row& r, DrawShared& sh, int row, uint32_t listed, int b0, int b1,
-                                                     uint32_t rank, uint64_t weight) {
-    const int tid = threadIdx.x;
-    // from the first to the last of them
-    uint64_t low = ~uint64_t{0}, high = 0;
-    each_token<T>(a, r, sh, row, listed, [&](uint64_t place, uint64_t, int b) {
-        if (b < b0 || b > b1) return;
-        low = min(low, place);
-        high = max(high, place);
-    });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        low = min(low, static_cast<uint64_t>(__shfl_xor(low, m, 64)));
-        high = max(high, static_cast<uint64_t>(__shfl_xor(high, m, 64)));
-    }
-    if ((tid & 63) == 0) sh.lows[tid >> 6] = low, sh.highs[tid >> 6] = high;
-    __syncthreads();
-    if (tid == 0) {
-        for (int w = 1; w < 16; w++) low = min(low, sh.lows[w]), high = max(high, sh.highs[w]);
-        sh.lo = low;
-        sh.hi = high;
-        sh.weight_before = 0;
-        sh.count_before = 0;
-    }
-    __syncthreads();
-    for (;;) {
-        const uint64_t from = sh.lo, to = sh.hi;
-        const int shift = max(0, 54 - __builtin_clzll((to - from) | 1));  // at most 1024 steps
-        sh.bin_weights[tid] = 0;
-        sh.bin_counts[tid] = 0;
-        __syncthreads();
-        each_token<T>(a, r, sh, row, listed, [&](uint64_t place, uint64_t w, int b) {
-            if (b < b0 || b > b1 || place < from || place > to) return;
-            const int q = static_cast<int>((place - from) >> shift);
-            atomicAdd(&sh.bin_counts[q], 1u);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bin_weights[q]), static_cast<unsigned long long>(w));
-        });
-        __syncthreads();
-        const uint64_t w = sh.bin_weights[tid];
-        const uint32_t c = sh.bin_counts[tid];
-        uint64_t all;
-        uint32_t tokens;
-        const uint64_t w_to = sh.weight_before + block_scan(w, sh.waves64, &all);
-        const uint32_t c_to = sh.count_before + block_scan(c, sh.waves32, &tokens);
-        // (a weight of 0 is reached by the first token)
-        const bool here = c != 0 && (rank ? c_to >= rank && c_to - c < rank : w_to >= weight && (w_to - w < weight || c_to == c));
-        if (!__syncthreads_or(here)) {  // fewer tokens, or less weight, than asked for: all of them
-            if (tid == 0) sh.lo = to, sh.weight_before += all;
-            __syncthreads();
-            break;
-        }
-        if (here) {
-            sh.lo = from + (static_cast<uint64_t>(tid) << shift);
-            sh.hi = min(to, from + ((static_cast<uint64_t>(tid) + 1) << shift) - 1);
-            sh.weight_before = shift == 0 ? w_to : w_to - w;
-            sh.count_before = c_to - c;
-        }
-        __syncthreads();
-        if (shift == 0) break;
-    }
-    return sh.lo;
-}
 
 template <typename T>
 __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     __shared__ DrawShared sh;
     const int tid = threadIdx.x, row = blockIdx.x;
+    const Row r = a.settings[row];
+    if (r.bad || r.greedy || r.arg == INT32_MAX) return;  // the cut kernel has stored those
     const Cut cut = a.cuts[row];
-    const Row& r = cut.row;
-    if (r.bad || r.greedy || r.arg == INT32_MAX) {
-        if (tid == 0) {
-            store_index(a.ids, a.ids_dt, row, r.bad || r.arg == INT32_MAX ? -1 : r.arg);
-            if (a.probs) a.probs[row] = r.bad || r.arg == INT32_MAX ? 0.0f : 1.0f;
+    const int64_t at = row * a.stride;
+    if (tid < a.parts) sh.sums[tid] = a.kept[static_cast<int64_t>(row) * a.parts + tid];
+    uint64_t last = ~uint64_t{0};
+    if (r.cuts()) {
+        const uint32_t listed = a.listed[row];  // above kList: the list does not hold them, the row again
+        if (listed <= kList)
+            for (uint32_t i = tid; i < listed; i += 1024) {
+                const uint64_t place = a.list[static_cast<int64_t>(row) * kList + i];
+                sh.places[i] = place;
+                sh.weights[i] = weight_of(r, key_logit(static_cast<uint32_t>(place >> 24)));
+            }
+        __syncthreads();
+        auto each = [&](int b0, int b1, auto f) {
+            if (listed <= kList) {
+                for (uint32_t i = tid; i < listed; i += 1024) {
+                    const int b = bin_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
+                    if (b >= b0 && b <= b1) f(sh.places[i], sh.weights[i]);
+                }
+                return;
+            }
+            for (int i = tid * 8; i < a.vocab; i += 8192) {
+                float v[8];
+                load_tokens<T>(a, at, i, v);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (!token(v[j])) continue;
+                    const int b = bin_of(r, v[j]);
+                    if (b >= b0 && b <= b1 && cut.in_question(b)) f(place_of(v[j], i + j), weight_of(r, v[j]));
+                }
+            }
+        };
+        last = last_place(r, cut, sh.narrow, each, [&](int bin) { return a.upto[static_cast<int64_t>(row) * kBins + bin]; });
+        // the listed tokens that are kept join their parts' weights
+        each(cut.sure, kBins, [&](uint64_t place, uint64_t w) {
+            if (place > last || w == 0 || !likely(r, ratio_of(r, key_logit(static_cast<uint32_t>(place >> 24))))) return;
+            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[(place & 0xffffff) / (a.per * kChunk)]), static_cast<unsigned long long>(w));
+        });
+    }
+    __syncthreads();
+    if (tid < 64) {
+        const uint64_t w = tid < a.parts ? sh.sums[tid] : 0;
+        const uint64_t to = wave_scan(w), total = __shfl(to, 63, 64);
+        const uint64_t target = part_of(r.uniform, total, false);
+        if (to > target && to - w <= target) sh.chosen = tid, sh.before = to - w;
+        if (tid == 0) sh.waves64[0] = total;
+    }
+    __syncthreads();
+    const uint64_t total = sh.waves64[0], target = part_of(r.uniform, total, false);
+    const int part = sh.chosen;
+    uint64_t run = sh.before;
+    __syncthreads();
+    // the tokens of the part in which the sum passes the target, four a thread at a time
+    for (int chunk = part * a.per * kChunk; chunk < min((part + 1) * a.per * kChunk, a.vocab); chunk += kChunk) {
+        uint64_t w4[4], sum = 0;
+        const int id0 = chunk + tid * 4;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float l = id0 + j < a.vocab ? Vec8<T>::load1(a.logits, at + id0 + j) : -__builtin_inff();
+            w4[j] = 0;
+            if (token(l)) {
+                const int b = bin_of(r, l);
+                if (b < cut.sure || (cut.in_question(b) && place_of(l, id0 + j) <= last)) {
+                    const Ratio ratio = ratio_of(r, l);
+                    if (likely(r, ratio)) w4[j] = weight_of(r, ratio);
+                }
+            }
+            sum += w4[j];
+        }
+        uint64_t all;
+        uint64_t to = run + block_scan<16>(sum, sh.waves64, &all) - sum;
+        run += all;
+        if (run <= target) continue;  // the same for all
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (to + w4[j] > target && to <= target) store_token(a, row, id0 + j, static_cast<float>(static_cast<double>(w4[j]) / static_cast<double>(total)));
+            to += w4[j];
         }
         return;
     }
-    const uint32_t listed = a.listed[row];  // above kList: the list does not hold them, the row again
-    const int64_t at = row * a.stride;
-    if (listed <= kList)
-        for (uint32_t i = tid; i < listed; i += 1024) {
-            const uint64_t place = a.list[static_cast<int64_t>(row) * kList + i];
-            sh.places[i] = place;
-            sh.weights[i] = weight_of(r, ratio_of(r, key_logit(static_cast<uint32_t>(place >> 24))));
-        }
-    __syncthreads();
-    uint64_t last = ~uint64_t{0};  // the last place kept
-    if (r.small()) {
-        // ranks and weights from the first token on
-        uint64_t kept = 0;
-        if (cut.rank) {
-            last = narrow<T>(a, r, sh, row, listed, 0, cut.last, cut.rank, 0);
-            kept = sh.weight_before;
-            __syncthreads();
-        } else if (r.by_p()) {
-            uint64_t mine = 0;
-            each_token<T>(a, r, sh, row, listed, [&](uint64_t, uint64_t w, int b) { mine += b <= cut.last ? w : 0; });
-            block_scan(mine, sh.waves64, &kept);
-        }
-        if (r.by_p()) {
-            last = min(last, narrow<T>(a, r, sh, row, listed, 0, cut.last, 0, r.top_p > 0.0f ? part_of(r.top_p, kept, true) : 0));
-            __syncthreads();
-        }
-    } else {
-        uint64_t kept = cut.weight;  // top_k's
-        if (cut.k_bin >= 0) {
-            last = narrow<T>(a, r, sh, row, listed, cut.k_bin, cut.k_bin, cut.rank, 0);
-            kept += sh.weight_before;
-            __syncthreads();
-        }
-        if (cut.last >= 0) {
-            const uint64_t upto = r.top_p > 0.0f ? part_of(r.top_p, kept, true) : 0;
-            const uint64_t* to = a.weights + static_cast<int64_t>(row) * a.parts * kBins;
-            int bin = cut.first;
-            while (bin < cut.last && to[bin] < upto) bin++;
-            const uint64_t before = bin > 0 ? to[bin - 1] : 0;
-            last = min(last, narrow<T>(a, r, sh, row, listed, bin, bin, 0, upto > before ? upto - before : 0));
-            __syncthreads();
-        }
-    }
-    // the kept weight of each chunk: that of the bins below the cuts, and of the listed tokens up to `last`
-    uint64_t* chunk_sums = a.kept + static_cast<int64_t>(row) * a.chunks;
-    if (listed) {
-        each_token<T>(a, r, sh, row, listed, [&](uint64_t place, uint64_t w, int b) {
-            if (b < cut.sure || !in_question(cut, b) || place > last || w == 0) return;
-            if (!likely(r, ratio_of(r, key_logit(static_cast<uint32_t>(place >> 24))))) return;
-            atomicAdd(reinterpret_cast<unsigned long long*>(&chunk_sums[(place & 0xffffff) / kChunk]), static_cast<unsigned long long>(w));
-        });
-        __threadfence();
-        __syncthreads();
-    }
-    auto chunk_sum = [&](int c) -> uint64_t { return __hip_atomic_load(&chunk_sums[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-    uint64_t total = 0, mine = 0;
-    for (int c = tid; c < a.chunks; c += 1024) mine += chunk_sum(c);
-    block_scan(mine, sh.waves64, &total);
-    const uint64_t target = part_of(r.uniform, total, false);
-    uint64_t base = 0;
-    if (tid == 0) sh.chosen = 0;
-    __syncthreads();
-    for (int c0 = 0; c0 < a.chunks; c0 += 1024) {
-        const uint64_t w = c0 + tid < a.chunks ? chunk_sum(c0 + tid) : 0;
-        uint64_t all;
-        const uint64_t to = base + block_scan(w, sh.waves64, &all);
-        if (to > target && to - w <= target) sh.chosen = c0 + tid, sh.weight_before = to - w;
-        base += all;
-    }
-    __syncthreads();
-    // the tokens of the chunk in which the sum passes the target, four a thread
-    uint64_t w4[4], sum = 0;
-    const int id0 = sh.chosen * kChunk + tid * 4;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const float l = id0 + j < a.vocab ? Vec8<T>::load1(a.logits, at + id0 + j) : -__builtin_inff();
-        w4[j] = 0;
-        if (token(l)) {
-            const Ratio ratio = ratio_of(r, l);
-            const int b = bin_of(r, l);
-            if ((b < cut.sure || (in_question(cut, b) && place_of(l, id0 + j) <= last)) && likely(r, ratio)) w4[j] = weight_of(r, ratio);
-        }
-        sum += w4[j];
-    }
-    uint64_t all;
-    uint64_t to = sh.weight_before + block_scan(sum, sh.waves64, &all) - sum;
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-        if (to + w4[j] > target && to <= target) {
-            store_index(a.ids, a.ids_dt, row, id0 + j);
-            if (a.probs) a.probs[row] = static_cast<float>(static_cast<double>(w4[j]) / static_cast<double>(total));
-        }
-        to += w4[j];
-    }
 }
 
-// How a call's rows are cut, and its workspace.
+// How a call's rows are cut, and its workspace; rows that a workgroup does need none.
 struct Plan {
-    int32_t chunks, parts, per;
-    int64_t peaks, weights, counts, cuts, listed, list, kept, bytes;
+    int32_t parts, per, peak_parts, peak_per;
+    int64_t peaks, weights, counts, upto, settings, cuts, listed, list, kept, bytes;
 };
 
 Plan plan_of(int64_t rows, int64_t vocab) {
     Plan p{};
-    p.chunks = static_cast<int32_t>((vocab + kChunk - 1) / kChunk);
-    // about four workgroups a CU, of at least two chunks, and no more parts than the cut sums up quickly
-    const int64_t want = std::min<int64_t>({std::max<int64_t>((1024 + rows - 1) / rows, 1), (p.chunks + 1) / 2, 64});
-    p.per = static_cast<int32_t>((p.chunks + want - 1) / want);
-    p.parts = (p.chunks + p.per - 1) / p.per;
+    if (vocab <= kRowVocab) return p;
+    const int64_t chunks = (vocab + kChunk - 1) / kChunk;
+    auto split = [&](int64_t most, int32_t* parts, int32_t* per) {
+        const int64_t want = std::max<int64_t>(std::min<int64_t>({most, chunks, kParts}), 1);
+        *per = static_cast<int32_t>((chunks + want - 1) / want);
+        *parts = static_cast<int32_t>((chunks + *per - 1) / *per);
+    };
+    // peaks: as many workgroups as there may be; bins: about four a CU, since each leaves 12 KB behind
+    split(kParts, &p.peak_parts, &p.peak_per);
+    split((1024 + rows - 1) / rows, &p.parts, &p.per);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.peaks = take(rows * p.parts * static_cast<int64_t>(sizeof(Peak)));
+    p.peaks = take(rows * p.peak_parts * static_cast<int64_t>(sizeof(Peak)));
     p.weights = take(rows * p.parts * kBins * 8);
     p.counts = take(rows * p.parts * kBins * 4);
+    p.upto = take(rows * kBins * 8);
+    p.settings = take(rows * static_cast<int64_t>(sizeof(Row)));
     p.cuts = take(rows * static_cast<int64_t>(sizeof(Cut)));
     p.listed = take(rows * 4);
     p.list = take(rows * kList * 8);
-    p.kept = take(rows * p.chunks * 8);
+    p.kept = take(rows * p.parts * 8);
     p.bytes = at;
     return p;
 }
@@ -659,18 +911,23 @@ int check_logits(const SandyTensor* logits, Err e) {
         return fail(e, SANDY_ERR_INVALID, "sample logits must be [rows, vocab] f32 or bf16");
     if (logits->dims[0] > 0 && logits->dims[1] < 1) return fail(e, SANDY_ERR_INVALID, "sample logits must have a vocabulary");
     if (logits->dims[1] > kMaxVocab) return fail(e, SANDY_ERR_UNSUPPORTED, "sample vocabulary above 2^24 tokens");
-    if (logits->dims[0] > (1 << 20)) return fail(e, SANDY_ERR_UNSUPPORTED, "sample of more than 2^20 rows");
+    if (logits->dims[0] > (1 << 17)) return fail(e, SANDY_ERR_UNSUPPORTED, "sample of more than 2^17 rows");
     return SANDY_OK;
 }
 
 template <typename T>
 int launch_sample(const SampleArgs& a, Err e, hipStream_t s) {
-    const dim3 parts(static_cast<unsigned>(a.rows) * a.parts), rows(static_cast<unsigned>(a.rows));
-    hipLaunchKernelGGL(sample_peak_kernel<T>, parts, dim3(256), 0, s, a);
-    hipLaunchKernelGGL(sample_bins_kernel<T>, parts, dim3(256), 0, s, a);
-    hipLaunchKernelGGL(sample_cut_kernel, rows, dim3(1024), 0, s, a);
-    hipLaunchKernelGGL(sample_gather_kernel<T>, parts, dim3(256), 0, s, a);
-    hipLaunchKernelGGL(sample_draw_kernel<T>, rows, dim3(1024), 0, s, a);
+    const dim3 rows(static_cast<unsigned>(a.rows));
+    if (a.vocab <= kRowVocab) {
+        hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(1024), 0, s, a);
+    } else {
+        const dim3 parts(static_cast<unsigned>(a.rows) * a.parts), peaks(static_cast<unsigned>(a.rows) * a.peak_parts);
+        hipLaunchKernelGGL(sample_peak_kernel<T>, peaks, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(sample_bins_kernel<T>, parts, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(sample_cut_kernel, rows, dim3(1024), 0, s, a);
+        hipLaunchKernelGGL(sample_gather_kernel<T>, parts, dim3(256), 0, s, a);
+        hipLaunchKernelGGL(sample_draw_kernel<T>, rows, dim3(1024), 0, s, a);
+    }
     SANDY_HIP_TRY(hipGetLastError(), e, "sample launch");
     return ok(e);
 }
@@ -709,8 +966,7 @@ extern "C" int sandy_hip_sample(const SandyTensor* logits, const SandyTensor* te
     if (rows == 0) return ok(e);
     if (!logits->data) return fail(e, SANDY_ERR_INVALID, "sample logits are null");
     const Plan p = plan_of(rows, vocab);
-    if (rows * p.parts > (int64_t{1} << 23)) return fail(e, SANDY_ERR_UNSUPPORTED, "sample of too many rows");
-    if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < static_cast<size_t>(p.bytes))
+    if (p.bytes && (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < static_cast<size_t>(p.bytes)))
         return fail(e, SANDY_ERR_INVALID, "sample needs a workspace of %lld bytes, 16-byte aligned", static_cast<long long>(p.bytes));
     SampleArgs a{};
     int status = 0;
@@ -730,15 +986,18 @@ extern "C" int sandy_hip_sample(const SandyTensor* logits, const SandyTensor* te
     a.probs = probs ? static_cast<float*>(base_ptr(*probs)) : nullptr;
     a.rows = static_cast<int32_t>(rows);
     a.vocab = static_cast<int32_t>(vocab);
-    a.chunks = p.chunks;
     a.parts = p.parts;
     a.per = p.per;
+    a.peak_parts = p.peak_parts;
+    a.peak_per = p.peak_per;
     a.bits = 62 - (vocab > 1 ? 64 - __builtin_clzll(static_cast<uint64_t>(vocab - 1)) : 0);
     if (a.bits > 50) a.bits = 50;
     char* w = static_cast<char*>(workspace);
     a.peaks = reinterpret_cast<Peak*>(w + p.peaks);
     a.weights = reinterpret_cast<uint64_t*>(w + p.weights);
     a.counts = reinterpret_cast<uint32_t*>(w + p.counts);
+    a.upto = reinterpret_cast<uint64_t*>(w + p.upto);
+    a.settings = reinterpret_cast<Row*>(w + p.settings);
     a.cuts = reinterpret_cast<Cut*>(w + p.cuts);
     a.listed = reinterpret_cast<uint32_t*>(w + p.listed);
     a.list = reinterpret_cast<uint64_t*>(w + p.list);

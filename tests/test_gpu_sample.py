@@ -42,7 +42,7 @@ def settings(rng, rows):
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 2), (7, 100), (4, 2047), (3, 4095), (5, 4096), (3, 4097), (6, 8193), (8, 32000),
-                                        (4, 50257), (3, 131075), (200, 1000)])
+                                        (4, 50257), (2, 65536), (2, 65537), (3, 131075), (200, 1000)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_settings(rows, vocab, dtype):
     rng = np.random.default_rng(vocab + rows)
@@ -71,7 +71,7 @@ def test_edges_of_the_settings():
         check(model_logits(rng, 8, 300, torch.float32), [u] * 8, k=k, p=[0.0, 1e-30, 0.5, last] * 2, least=[0.0, 1.0, 0.1, 0.2] * 2)
 
 
-@pytest.mark.parametrize("vocab", [5, 5000, 20000])
+@pytest.mark.parametrize("vocab", [5, 5000, 20000, 70000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_equal_logits(vocab, dtype):
     """Cuts inside runs of equals, more of them than a list holds: the lowest ids stay."""
@@ -91,7 +91,7 @@ def test_equal_logits(vocab, dtype):
         assert ids.tolist() == list(range(n)) and torch.equal(probs, torch.full_like(probs, 1 / n))
 
 
-@pytest.mark.parametrize("vocab", [4, 4100, 30000])
+@pytest.mark.parametrize("vocab", [4, 4100, 30000, 66000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_masks(vocab, dtype):
     rng = np.random.default_rng(vocab + 1)

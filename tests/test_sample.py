@@ -21,6 +21,7 @@ def workspace(logits):
 
 def test_refusals():
     f, i = tensor((3,), F32), tensor((3,), I64)
+    big = tensor((3, 100000))
     default = dict(logits=tensor((3, 1000)), temperature=f, top_k=i, top_p=f, min_p=f, uniforms=f, ids=i, probs=f, work=0x100000,
                    bytes=1 << 40)
     for kw, message in [
@@ -29,7 +30,7 @@ def test_refusals():
         (dict(logits=tensor((3, 1000), I32)), "logits must be"),
         (dict(logits=tensor((3, 0))), "must have a vocabulary"),
         (dict(logits=tensor((3, (1 << 24) + 1))), "above 2\\^24"),
-        (dict(logits=tensor(((1 << 20) + 1, 2))), "more than 2\\^20 rows"),
+        (dict(logits=tensor(((1 << 17) + 1, 2))), "more than 2\\^17 rows"),
         (dict(logits=tensor((3, 1000), strides=[1000, 2])), "unit inner stride"),
         (dict(logits=tensor((3, 1000), data=0)), "null"),
         (dict(temperature=i), "contiguous f32"),
@@ -45,16 +46,16 @@ def test_refusals():
         (dict(ids=f), "ids must be"),
         (dict(ids=None), "ids must be"),
         (dict(probs=i), "probs must be"),
-        (dict(work=None), "needs a workspace"),
-        (dict(work=0x100008), "16-byte aligned"),
-        (dict(bytes=workspace(tensor((3, 1000))) - 1), "needs a workspace"),
+        (dict(logits=big, work=None), "needs a workspace"),
+        (dict(logits=big, work=0x100008), "16-byte aligned"),
+        (dict(logits=big, bytes=workspace(big) - 1), "needs a workspace"),
     ]:
         with pytest.raises(_lib.SandyError, match=message):
             _lib.call("sandy_hip_sample", *{**default, **kw}.values(), stream=0)
     e = tensor((0,), F32)
     _lib.call("sandy_hip_sample", tensor((0, 1000)), None, None, None, None, e, tensor((0,), I64), None, None, 0, stream=0)
     assert workspace(tensor((0, 1000))) == 0
-    assert 0 < workspace(tensor((1, 1))) < workspace(tensor((64, 262144), F32))
+    assert 0 == workspace(tensor((1, 1))) < workspace(tensor((64, 262144), F32))
 
 
 def test_python_refusals():
