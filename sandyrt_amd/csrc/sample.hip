@@ -25,14 +25,17 @@
 namespace sandy_hip {
 namespace {
 
-constexpr int kChunk = 4096;      // a part is a whole number of these
+constexpr int kChunk = 2048;      // a part is a whole number of these
 constexpr int kParts = 64;        // at most, a row
 constexpr int kBins = 1024;       // the last for tokens without weight
 constexpr int kList = 8192;       // listed tokens of a row in parts
 constexpr int kRowList = 2048;    // and of a row that one workgroup does
+constexpr int kPartList = 1024;   // and of a part's
 constexpr int kRowVocab = 65536;  // the longest such row
 constexpr int kSmall = 1024;      // a top_k whose tokens are all listed
 constexpr int kMaxVocab = 1 << 24;
+// The cut, draw and whole-row kernels: 256 registers a thread, which 1024 threads would not have.  A thread has two bins.
+constexpr int kThreads = 512, kWaves = kThreads / 64, kPer = kBins / kThreads;
 
 struct Peak {
     float max, min;  // of the logits above -inf
@@ -63,9 +66,19 @@ struct Cut {
     uint64_t weight;    // of top_k's tokens in bins below k_bin (k_bin < 0: of all of them)
 
     __device__ bool in_question(int bin) const {
-        return bin <= limit && (bin == k_bin || (bin >= first && bin <= last) || (bin >= m_first && bin <= m_last));
+        return (bin <= limit) & ((bin == k_bin) | ((bin >= first) & (bin <= last)) | ((bin >= m_first) & (bin <= m_last)));
     }
+    __device__ bool listed_in(int bin, int b0, int b1) const { return (bin >= b0) & (bin <= b1) & in_question(bin); }
+    // whether a token of this bin and place stays, as far as top_k and top_p go
+    __device__ bool keeps(int bin, uint64_t place, uint64_t last_place) const { return (bin < sure) | (in_question(bin) & (place <= last_place)); }
 };
+
+__device__ __forceinline__ Cut no_cut() {
+    Cut cut{};
+    cut.sure = cut.limit = cut.first = cut.m_first = kBins;
+    cut.last = cut.m_last = cut.k_bin = -1;
+    return cut;
+}
 
 struct SampleArgs {
     const void* logits;
@@ -172,46 +185,54 @@ __device__ __forceinline__ Row make_row(const SampleArgs& a, int row, float mx, 
     return r;
 }
 
-// exp((l - max) / T) = 2^f 2^k, 1 at the maximum: f in -1/2 .. 1/2 by the Taylor series of e^(f ln 2) to the 11th
-// power (the next term is below 7e-15 of the sum).  Below 2^-200 it stays there, which weighs nothing.
-struct Ratio {
-    double p;
-    int k;
-    __device__ double value() const { return p * __longlong_as_double(static_cast<long long>(1023 + k) << 52); }
-};
-__device__ __forceinline__ Ratio ratio_of(const Row& r, float l) {
-    if (l == r.max) return Ratio{1.0, 0};
-    const double x = fmax((static_cast<double>(l) - static_cast<double>(r.max)) * r.rate, -200.0);  // (inf less inf: -200 too)
-    const double k = __builtin_rint(x), f = x - k;
-    double p = 4.44553827187081162e-10;  // (ln 2)^11 / 11!
-    p = fma(p, f, 7.05491162080112336e-09);
-    p = fma(p, f, 1.01780860092396999e-07);
-    p = fma(p, f, 1.32154867901443095e-06);
-    p = fma(p, f, 1.52527338040598411e-05);
-    p = fma(p, f, 1.54035303933816088e-04);
-    p = fma(p, f, 1.33335581464284433e-03);
-    p = fma(p, f, 9.61812910762847688e-03);
-    p = fma(p, f, 5.55041086648215831e-02);
-    p = fma(p, f, 2.40226506959100722e-01);
-    p = fma(p, f, 6.93147180559945286e-01);
-    p = fma(p, f, 1.0);
-    return Ratio{p, static_cast<int>(k)};
+// (ln 2)^n / n!, n = 11 .. 0
+__device__ constexpr double kSeries[12] = {
+    4.44553827187081162e-10, 7.05491162080112336e-09, 1.01780860092396999e-07,
+    1.32154867901443095e-06, 1.52527338040598411e-05, 1.54035303933816088e-04,
+    1.33335581464284433e-03, 9.61812910762847688e-03, 5.55041086648215831e-02,
+    2.40226506959100722e-01, 6.93147180559945286e-01, 1.0};
+// Weights of N logits at once, so that their series interleave: exp((l - max) / T) = 2^f 2^k, 1 at the maximum, f in
+// -1/2 .. 1/2 by the Taylor series of e^(f ln 2) to the 11th power (the next term is below 7e-15 of the sum), rounded to
+// the nearest multiple of 2^-bits, 52 bits of which lie behind 2^52.  Below 2^-200 it stays there, which weighs nothing.
+// `all` false: 0 for those that min_p leaves out.  Masked logits weigh 0.
+template <int N>
+__device__ __forceinline__ void weigh(const Row& r, const float (&l)[N], bool all, uint64_t (&w)[N]) {
+    double f[N], p[N];
+    int k[N];
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const double d = l[j] == r.max ? 0.0 : static_cast<double>(l[j]) - static_cast<double>(r.max);
+        const double x = fmax(d * r.rate, -200.0), whole = __builtin_rint(x);  // (inf less inf: -200 too)
+        f[j] = x - whole;
+        k[j] = static_cast<int>(whole);
+        p[j] = kSeries[0];
+    }
+#pragma unroll
+    for (int n = 1; n < 12; n++)
+#pragma unroll
+        for (int j = 0; j < N; j++) p[j] = fma(p[j], f[j], kSeries[n]);
+    auto two_to = [](int e) { return __longlong_as_double(static_cast<long long>(1023 + e) << 52); };
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        w[j] = static_cast<uint64_t>(__double_as_longlong(fma(p[j], two_to(r.bits + k[j]), 4503599627370496.0))) - 0x4330000000000000ull;
+        w[j] = token(l[j]) ? w[j] : 0;
+    }
+    if (__builtin_amdgcn_readfirstlane(!all & (r.least > 0.0f)))  // a row's own, the same for all
+#pragma unroll
+        for (int j = 0; j < N; j++) w[j] = p[j] * two_to(k[j]) >= static_cast<double>(r.least) ? w[j] : 0;
 }
-// to the nearest whole multiple of 2^-bits: 52 bits hold it behind 2^52
-__device__ __forceinline__ uint64_t weight_of(const Row& r, const Ratio& ratio) {
-    const double unit = __longlong_as_double(static_cast<long long>(1023 + r.bits + ratio.k) << 52);
-    return static_cast<uint64_t>(__double_as_longlong(fma(ratio.p, unit, 4503599627370496.0))) - 0x4330000000000000ull;
-}
-__device__ __forceinline__ uint64_t weight_of(const Row& r, float l) { return weight_of(r, ratio_of(r, l)); }
-__device__ __forceinline__ bool likely(const Row& r, const Ratio& ratio) {
-    return r.least <= 0.0f || ratio.value() >= static_cast<double>(r.least);
+__device__ __forceinline__ uint64_t weight_of(const Row& r, float l, bool all = true) {
+    const float v[1] = {l};
+    uint64_t w[1];
+    weigh(r, v, all, w);
+    return w[0];
 }
 // Non-decreasing as logits fall; the last bin holds no token that weighs anything (those end a ninetieth before it, or
 // the lowest logit ends at kBins - 2).
 __device__ __forceinline__ int bin_of(const Row& r, float l) {
-    if (l == r.max) return 0;
-    const float at = (r.max - l) * r.scale;
-    return at >= static_cast<float>(kBins - 1) ? kBins - 1 : static_cast<int>(fminf(at, static_cast<float>(kBins - 2)));
+    const float at = l == r.max ? 0.0f : (r.max - l) * r.scale;
+    const int bin = static_cast<int>(fminf(at, static_cast<float>(kBins - 2)));
+    return at >= static_cast<float>(kBins - 1) ? kBins - 1 : bin;
 }
 
 // p * w rounded up or down, exactly; 0 <= p < 1
@@ -237,6 +258,25 @@ __device__ __forceinline__ void load_tokens(const SampleArgs& a, int64_t at, int
     for (int j = 0; j < 8; j++) v[j] = first + j < a.vocab ? Vec8<T>::load1(a.logits, at + first + j) : -__builtin_inff();
 }
 
+// f(logits, first id) for a thread's eights of a part's chunks, N loads at a time without a guard where they are whole.
+template <typename T, int N, typename F>
+__device__ __forceinline__ void part_tokens(const SampleArgs& a, int64_t at, int begin, int end, F f) {
+    const int mine = static_cast<int>(threadIdx.x) * 8;
+    for (; begin + N * kChunk <= end; begin += N * kChunk) {
+        float v[N][8];
+#pragma unroll
+        for (int n = 0; n < N; n++) load8_unaligned<T>(a.logits, at + begin + n * kChunk + mine, v[n]);
+#pragma unroll
+        for (int n = 0; n < N; n++) f(v[n], begin + n * kChunk + mine);
+    }
+#pragma unroll 1
+    for (; begin < end; begin += kChunk) {
+        float v[8];
+        load_tokens<T>(a, at, begin + mine, v);
+        f(v, begin + mine);
+    }
+}
+
 __device__ __forceinline__ void store_token(const SampleArgs& a, int row, int64_t id, float prob) {
     store_index(a.ids, a.ids_dt, row, id);
     if (a.probs) a.probs[row] = prob;
@@ -254,40 +294,49 @@ __device__ __forceinline__ bool drawn(const SampleArgs& a, const Row& r, int row
 
 // ------------------------------------------------------------------ where the cuts lie
 struct CutShared {
-    uint64_t waves64[16], low, high;
-    uint32_t waves32[16], rank;
+    uint64_t waves64[kWaves], low, high;
+    uint32_t waves32[kWaves], rank;
     int k_bin, k_last, p_first, p_last;
 };
 
-// Cuts of a row from its bins' counts and weights, one bin a thread of 1024; *up_to: the weight up to and with the bin.
-__device__ __forceinline__ Cut find_cuts(const Row& r, uint32_t c, uint64_t w, CutShared& sh, uint64_t* up_to) {
-    const int bin = threadIdx.x;
-    uint64_t all = 0, w_to = 0;
-    uint32_t tokens = 0, c_to = 0;
-    if (!r.small()) w_to = block_scan<16>(w, sh.waves64, &all);
-    if (r.top_k) c_to = block_scan<16>(c, sh.waves32, &tokens);
-    *up_to = w_to;
-    if (bin == 0) sh.k_bin = -1, sh.k_last = sh.p_first = sh.p_last = kBins, sh.low = sh.high = all, sh.rank = 0;
+// Cuts of a row from its bins' counts and weights, bins kPer threadIdx .. of a thread; up_to: the weight up to and with each.
+__device__ __forceinline__ Cut find_cuts(const Row& r, const uint32_t (&c)[kPer], const uint64_t (&w)[kPer], CutShared& sh, uint64_t (&up_to)[kPer]) {
+    uint64_t all = 0, mine = 0;
+    uint32_t tokens = 0, c_to[kPer], mine_c = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) up_to[i] = mine += w[i], c_to[i] = mine_c += c[i];
+    if (!r.small()) {
+        const uint64_t before = block_scan<kWaves>(mine, sh.waves64, &all) - mine;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) up_to[i] += before;
+    }
+    if (r.top_k) {
+        const uint32_t before = block_scan<kWaves>(mine_c, sh.waves32, &tokens) - mine_c;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) c_to[i] += before;
+    }
+    if (threadIdx.x == 0) sh.k_bin = -1, sh.k_last = sh.p_first = sh.p_last = kBins, sh.low = sh.high = all, sh.rank = 0;
     __syncthreads();
     const uint32_t k = r.top_k;
     // the bin where top_k ends, if it ends inside one whose tokens weigh anything
-    if (k && k < tokens && c_to >= k && c_to - c < k) {
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+        const int bin = kPer * threadIdx.x + i;
+        if (!(k && k < tokens && c_to[i] >= k && c_to[i] - c[i] < k)) continue;
         sh.k_last = bin;
-        if (c_to == k || bin == kBins - 1) {
-            sh.low = sh.high = w_to;
+        if (c_to[i] == k || bin == kBins - 1) {
+            sh.low = sh.high = up_to[i];
         } else {
             sh.k_bin = bin;
-            sh.low = w_to - w;
-            sh.high = w_to;
-            sh.rank = k - (c_to - c);
+            sh.low = up_to[i] - w[i];
+            sh.high = up_to[i];
+            sh.rank = k - (c_to[i] - c[i]);
         }
     }
     __syncthreads();
-    Cut cut{};
+    Cut cut = no_cut();
+    cut.sure = 0;
     cut.limit = sh.k_last;
-    cut.k_bin = -1;
-    cut.first = cut.m_first = kBins;
-    cut.last = cut.m_last = -1;
     if (r.small()) {
         // all that top_k may keep: to its last bin, or every token that weighs anything
         cut.first = 0;
@@ -298,9 +347,14 @@ __device__ __forceinline__ Cut find_cuts(const Row& r, uint32_t c, uint64_t w, C
     cut.weight = sh.low;
     if (r.by_p()) {
         // top_p's cut lies where the sums reach its part of top_k's weight, which is between low and high
-        const uint64_t from = nucleus(r, sh.low), to = nucleus(r, sh.high), before = w_to - w;
-        if (w_to >= from && (bin == 0 || before < from)) sh.p_first = bin;
-        if (w_to >= to && (bin == 0 || before < to)) sh.p_last = bin;
+        const uint64_t from = nucleus(r, sh.low), to = nucleus(r, sh.high);
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            const int bin = kPer * threadIdx.x + i;
+            const uint64_t before = up_to[i] - w[i];
+            if (up_to[i] >= from && (bin == 0 || before < from)) sh.p_first = bin;
+            if (up_to[i] >= to && (bin == 0 || before < to)) sh.p_last = bin;
+        }
     }
     __syncthreads();
     const int k_bin = sh.k_bin;
@@ -330,14 +384,14 @@ __device__ __forceinline__ Cut find_cuts(const Row& r, uint32_t c, uint64_t w, C
 
 // ------------------------------------------------------------------ narrowing down
 struct NarrowShared {
-    uint64_t bin_weights[kBins], waves64[16], lows[16], highs[16], places[64], weights[64];
+    uint64_t bin_weights[kBins], waves64[kWaves], lows[kWaves], highs[kWaves], places[64], weights[64];
     uint64_t lo, hi, weight_before;
-    uint32_t bin_counts[kBins], waves32[16], count_before, n;
+    uint32_t bin_counts[kBins], waves32[kWaves], count_before, n;
 };
 
 // Of the tokens that each(f) names as f(place, weight), in rank order: the place of the one with which they become `rank`,
 // or (rank 0) with which their weights reach `weight`, the first token reaching 0; the last of all if they never do.
-// sh.weight_before is then the sum up to and with it.  1024 threads.
+// sh.weight_before is then the sum up to and with it.
 template <typename Each>
 __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint64_t weight, Each each) {
     const int tid = threadIdx.x;
@@ -355,12 +409,12 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
     }
     if ((tid & 63) == 0) sh.lows[tid >> 6] = low, sh.highs[tid >> 6] = high;
     uint32_t tokens;
-    block_scan<16>(n, sh.waves32, &tokens);
+    block_scan<kWaves>(n, sh.waves32, &tokens);
     if (tid < 64) {
-        low = sh.lows[tid & 15];
-        high = sh.highs[tid & 15];
+        low = sh.lows[tid & (kWaves - 1)];
+        high = sh.highs[tid & (kWaves - 1)];
 #pragma unroll
-        for (int m = 8; m >= 1; m >>= 1) {
+        for (int m = kWaves / 2; m >= 1; m >>= 1) {
             low = min(low, static_cast<uint64_t>(__shfl_xor(low, m, 64)));
             high = max(high, static_cast<uint64_t>(__shfl_xor(high, m, 64)));
         }
@@ -370,8 +424,8 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
     while (sh.n > 64) {  // each round is among fewer than before: a step of 1024
         const uint64_t from = sh.lo, to = sh.hi;
         const int shift = max(0, 54 - __builtin_clzll((to - from) | 1));
-        sh.bin_weights[tid] = 0;
-        sh.bin_counts[tid] = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) sh.bin_weights[kPer * tid + i] = 0, sh.bin_counts[kPer * tid + i] = 0;
         __syncthreads();
         each([&](uint64_t place, uint64_t w) {
             if (place < from || place > to) return;
@@ -380,24 +434,37 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
             atomicAdd(reinterpret_cast<unsigned long long*>(&sh.bin_weights[q]), static_cast<unsigned long long>(w));
         });
         __syncthreads();
-        const uint64_t w = sh.bin_weights[tid];
-        const uint32_t c = sh.bin_counts[tid];
-        uint64_t all;
-        const uint64_t w_to = sh.weight_before + block_scan<16>(w, sh.waves64, &all);
-        const uint32_t c_to = sh.count_before + block_scan<16>(c, sh.waves32, &tokens);
-        const bool here = c != 0 && (rank ? c_to >= rank && c_to - c < rank : w_to >= weight && (w_to - w < weight || c_to == c));
-        if (!__syncthreads_or(here)) {
+        uint64_t w[kPer], w_to[kPer], mine = 0, all;
+        uint32_t c[kPer], c_to[kPer], mine_c = 0;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            w_to[i] = mine += w[i] = sh.bin_weights[kPer * tid + i];
+            c_to[i] = mine_c += c[i] = sh.bin_counts[kPer * tid + i];
+        }
+        const uint64_t w_before = sh.weight_before + block_scan<kWaves>(mine, sh.waves64, &all) - mine;
+        const uint32_t c_before = sh.count_before + block_scan<kWaves>(mine_c, sh.waves32, &tokens) - mine_c;
+        int here = -1;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) {
+            w_to[i] += w_before;
+            c_to[i] += c_before;
+            if (c[i] != 0 && (rank ? c_to[i] >= rank && c_to[i] - c[i] < rank : w_to[i] >= weight && (w_to[i] - w[i] < weight || c_to[i] == c[i]))) here = i;
+        }
+        if (!__syncthreads_or(here >= 0)) {
             if (tid == 0) sh.weight_before += all;
             __syncthreads();
             return to;
         }
-        if (here) {
-            sh.lo = from + (static_cast<uint64_t>(tid) << shift);
-            sh.hi = min(to, from + ((static_cast<uint64_t>(tid) + 1) << shift) - 1);
-            sh.weight_before = w_to - w;
-            sh.count_before = c_to - c;
-            sh.n = c;
-        }
+#pragma unroll
+        for (int i = 0; i < kPer; i++)
+            if (here == i) {
+                const uint64_t step = kPer * tid + i;
+                sh.lo = from + (step << shift);
+                sh.hi = min(to, from + ((step + 1) << shift) - 1);
+                sh.weight_before = w_to[i] - w[i];
+                sh.count_before = c_to[i] - c[i];
+                sh.n = c[i];
+            }
         __syncthreads();
     }
     // the last few: each with each
@@ -415,10 +482,13 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
     __syncthreads();
     if (tid < 64) {
         const bool in = tid < few;
-        const uint64_t place = in ? sh.places[tid] : ~uint64_t{0}, w = in ? sh.weights[tid] : 0;
+        if (!in) sh.places[tid] = ~uint64_t{0}, sh.weights[tid] = 0;
+        const uint64_t place = sh.places[tid], w = sh.weights[tid];
         uint64_t w_to = sh.weight_before + w, all = sh.weight_before;
         uint32_t c_to = sh.count_before + 1;
-        for (uint32_t i = 0; i < few; i++) {
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 8
+        for (uint32_t i = 0; i < (few + 7 & ~7u); i++) {
             const uint64_t other = sh.weights[i];
             const bool before = sh.places[i] < place;
             w_to += before ? other : 0;
@@ -469,18 +539,29 @@ __device__ __forceinline__ uint64_t last_place(const Row& r, const Cut& cut, Nar
     return last;
 }
 
+// The tokens in question of bins b0 .. b1, from the row itself: for lists that are too long.
+template <typename T, typename F>
+__device__ __forceinline__ void each_of_row(const SampleArgs& a, int64_t at, const Row& r, const Cut& cut, int b0, int b1, F f) {
+#pragma unroll 1
+    for (int i = threadIdx.x; i < a.vocab; i += kThreads) {
+        const float l = Vec8<T>::load1(a.logits, at + i);
+        if (token(l) && cut.listed_in(bin_of(r, l), b0, b1)) f(place_of(l, i), weight_of(r, l));
+    }
+}
+
 // ------------------------------------------------------------------ a row a workgroup
-constexpr int kBlock = 8192;  // tokens a workgroup of 1024 takes at a time
+constexpr int kBlock = 8 * kThreads;  // tokens a workgroup takes at a time
 
 struct RowShared {
     uint64_t weights[kBins], up_to[kBins];
     uint32_t counts[kBins];
     uint64_t places[kRowList], held[kRowList];
     NarrowShared narrow;
-    uint64_t sums[kRowVocab / kBlock][16];
-    Peak peaks[16];
+    uint64_t sums[kRowVocab / kBlock * kWaves];  // of each wave's tokens of each block
+    Peak peaks[kWaves];
     CutShared cuts;
     Row row;
+    Cut cut;
     uint32_t listed;
 };
 
@@ -500,14 +581,14 @@ __device__ __forceinline__ void row_tokens(const SampleArgs& a, int64_t at, F f)
 }
 
 template <typename T>
-__global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     __shared__ RowShared sh;
     const int tid = threadIdx.x, row = blockIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t at = row * a.stride;
     float mx = -__builtin_inff(), mn = __builtin_inff();
     int arg = INT32_MAX;
-    sh.weights[tid] = 0;
-    sh.counts[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) sh.weights[kPer * tid + i] = 0, sh.counts[kPer * tid + i] = 0;
     if (tid == 0) sh.listed = 0;
     row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
 #pragma unroll
@@ -518,33 +599,41 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a) {
     if (lane == 0) sh.peaks[wave] = Peak{mx, mn, arg, 0};
     __syncthreads();
     if (wave == 0) {
-        const Peak p = sh.peaks[lane & 15];
+        const Peak p = sh.peaks[lane & (kWaves - 1)];
         mx = p.max, arg = p.arg, mn = p.min;
         wave_peak(mx, arg, mn);
         if (lane == 0) sh.row = make_row(a, row, mx, arg, mn);
     }
     __syncthreads();
-    const Row r = sh.row;
+    const Row& r = sh.row;
     if (drawn(a, r, row)) return;
-    Cut cut{};
-    cut.sure = cut.limit = kBins;
-    cut.k_bin = cut.last = cut.m_last = -1;
+    const Cut& cut = sh.cut;
+    if (tid == 0) sh.cut = no_cut();
+    __syncthreads();
     uint64_t last = ~uint64_t{0};
     if (r.cuts()) {
-        const bool count = r.top_k != 0, weigh = !r.small();
+        const bool count = r.top_k != 0, weighed = !r.small();
         row_tokens<T>(a, at, [&](const float (&v)[8], int) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (!token(v[j])) continue;
-                const int b = bin_of(r, v[j]);
-                if (count) atomicAdd(&sh.counts[b], 1u);
-                if (weigh) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.weights[b]), static_cast<unsigned long long>(weight_of(r, v[j])));
-            }
+            for (int j = 0; j < 8; j++)
+                if (count && token(v[j])) atomicAdd(&sh.counts[bin_of(r, v[j])], 1u);
+            if (!weighed) return;
+            uint64_t w[8];
+            weigh(r, v, true, w);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (w[j]) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.weights[bin_of(r, v[j])]), static_cast<unsigned long long>(w[j]));
         });
         __syncthreads();
-        uint64_t up_to;
-        cut = find_cuts(r, sh.counts[tid], sh.weights[tid], sh.cuts, &up_to);
-        sh.up_to[tid] = up_to;
+        uint64_t w[kPer], up_to[kPer];
+        uint32_t c[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; i++) w[i] = sh.weights[kPer * tid + i], c[i] = sh.counts[kPer * tid + i];
+        const Cut found = find_cuts(r, c, w, sh.cuts, up_to);
+        if (tid == 0) sh.cut = found;
+#pragma unroll
+        for (int i = 0; i < kPer; i++) sh.up_to[kPer * tid + i] = up_to[i];
+        __syncthreads();
         row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -556,67 +645,73 @@ __global__ __launch_bounds__(1024) void sample_row_kernel(SampleArgs a) {
         __syncthreads();
         const uint32_t listed = sh.listed;
         if (listed <= kRowList)
-            for (uint32_t i = tid; i < listed; i += 1024) sh.held[i] = weight_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
+            for (uint32_t i = tid; i < listed; i += kThreads) sh.held[i] = weight_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
         __syncthreads();
         auto each = [&](int b0, int b1, auto f) {
             if (listed <= kRowList) {
-                for (uint32_t i = tid; i < listed; i += 1024) {
+                for (uint32_t i = tid; i < listed; i += kThreads) {
                     const int b = bin_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
                     if (b >= b0 && b <= b1) f(sh.places[i], sh.held[i]);
                 }
                 return;
             }
-            row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (!token(v[j])) continue;
-                    const int b = bin_of(r, v[j]);
-                    if (b >= b0 && b <= b1 && cut.in_question(b)) f(place_of(v[j], first + j), weight_of(r, v[j]));
-                }
-            });
+            each_of_row<T>(a, at, r, cut, b0, b1, f);
         };
         last = last_place(r, cut, sh.narrow, each, [&](int bin) { return sh.up_to[bin]; });
     }
-    // a token's kept weight, and the sums over each wave's tokens of a block
-    auto kept = [&](float l, int id) -> uint64_t {
-        if (!token(l)) return 0;
-        const int b = bin_of(r, l);
-        if (b >= cut.sure && !(cut.in_question(b) && place_of(l, id) <= last)) return 0;
-        const Ratio ratio = ratio_of(r, l);
-        return likely(r, ratio) ? weight_of(r, ratio) : 0;
+    // kept weights of eight tokens, and their sums over each wave's part of a block
+    auto kept = [&](const float (&v)[8], int first, uint64_t (&w)[8]) {
+        bool keep[8], any = false;
+#pragma unroll
+        for (int j = 0; j < 8; j++) any |= keep[j] = cut.keeps(bin_of(r, v[j]), place_of(v[j], first + j), last);  // (masked ones weigh 0)
+        if (__any(any)) {
+            weigh(r, v, false, w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = keep[j] ? w[j] : 0;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = 0;
+        }
+        return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
     };
     row_tokens<T>(a, at, [&](const float (&v)[8], int first) {
-        uint64_t mine = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) mine += kept(v[j], first + j);
-        mine = wave_scan(mine);
-        if (lane == 63) sh.sums[first / kBlock][wave] = mine;
+        uint64_t w[8];
+        const uint64_t sum = wave_scan(kept(v, first, w));
+        if (lane == 63) sh.sums[first / kBlock * kWaves + wave] = sum;
     });
     __syncthreads();
-    const int blocks = (a.vocab + kBlock - 1) / kBlock;
-    uint64_t total = 0;
-    for (int i = 0; i < blocks * 16; i++) total += sh.sums[i >> 4][i & 15];
+    // the block and wave in which the sum of all passes the target: each wave looks, that one goes on
+    const int parts = (a.vocab + kBlock - 1) / kBlock * kWaves;
+    constexpr int kRounds = kRowVocab / kBlock * kWaves / 64;
+    uint64_t part_w[kRounds], total = 0;
+#pragma unroll
+    for (int q = 0; q < kRounds; q++) {
+        const int i = 64 * q + lane;
+        part_w[q] = i < parts ? sh.sums[i] : 0;
+        total += __shfl(wave_scan(part_w[q]), 63, 64);
+    }
     const uint64_t target = part_of(r.uniform, total, false);
-    // the block's wave in which the sum passes the target
     uint64_t run = 0;
-    for (int i = 0; i < blocks * 16; i++) {
-        const uint64_t w = sh.sums[i >> 4][i & 15];
-        if (run <= target && run + w > target && (i & 15) == wave) {
-            float v[8];
-            uint64_t w8[8], mine = 0;
-            const int first = (i >> 4) * kBlock + tid * 8;
-            load_tokens<T>(a, at, first, v);
 #pragma unroll
-            for (int j = 0; j < 8; j++) mine += w8[j] = kept(v[j], first + j);
-            uint64_t to = run + wave_scan(mine) - mine;
+    for (int q = 0; q < kRounds; q++) {
+        const uint64_t to = run + wave_scan(part_w[q]);
+        const uint64_t here = __ballot(to > target && to - part_w[q] <= target);
+        run = __shfl(to, 63, 64);
+        if (!here) continue;
+        const int l = __builtin_ctzll(here), part = 64 * q + l;
+        if (part % kWaves != wave) continue;
+        float v[8];
+        uint64_t w[8];
+        const int first = part / kWaves * kBlock + tid * 8;
+        load_tokens<T>(a, at, first, v);
+        const uint64_t mine = kept(v, first, w);
+        uint64_t upto = __shfl(to - part_w[q], l, 64) + wave_scan(mine) - mine;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (to <= target && to + w8[j] > target)
-                    store_token(a, row, first + j, static_cast<float>(static_cast<double>(w8[j]) / static_cast<double>(total)));
-                to += w8[j];
-            }
+        for (int j = 0; j < 8; j++) {
+            if (upto <= target && upto + w[j] > target)
+                store_token(a, row, first + j, static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total)));
+            upto += w[j];
         }
-        run += w;
     }
 }
 
@@ -627,16 +722,22 @@ __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
     const int64_t at = row * a.stride;
     const int begin = part * a.peak_per * kChunk, end = min(begin + a.peak_per * kChunk, a.vocab);
     float mx = -__builtin_inff(), mn = __builtin_inff();
-    int arg = INT32_MAX;
-    for (int chunk = begin; chunk < end; chunk += kChunk) {
-        float v[kChunk / 2048][8];  // requested together
+    int eight = -1, arg = INT32_MAX;  // the first eight that hold the maximum, looked at again for its id
+    part_tokens<T, 4>(a, at, begin, end, [&](const float (&v)[8], int i) {
+        float top = -__builtin_inff();
 #pragma unroll
-        for (int h = 0; h < kChunk / 2048; h++) load_tokens<T>(a, at, chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8, v[h]);
+        for (int j = 0; j < 8; j++) {
+            top = fmaxf(top, v[j]);  // (the number, of a number and NaN)
+            mn = fminf(mn, token(v[j]) ? v[j] : __builtin_inff());
+        }
+        eight = top > mx ? i : eight;
+        mx = fmaxf(mx, top);
+    });
+    if (eight >= 0) {
+        float v[8];
+        load_tokens<T>(a, at, eight, v);
 #pragma unroll
-        for (int h = 0; h < kChunk / 2048; h++)
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (token(v[h][j])) better_peak(mx, arg, mn, v[h][j], chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8 + j, v[h][j]);
+        for (int j = 7; j >= 0; j--) arg = v[j] == mx ? eight + j : arg;
     }
     wave_peak(mx, arg, mn);
     __shared__ Peak waves[4];
@@ -675,33 +776,33 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     for (int i = threadIdx.x; i < kBins; i += 256) weights[i] = 0, counts[i] = 0;
     const Row r = row_of(a, row, &shared);
+    if (part == 0 && threadIdx.x == 0) a.settings[row] = r;
     if (r.greedy || r.bad) return;
     const int64_t at = row * a.stride;
     const int begin = part * a.per * kChunk, end = min(begin + a.per * kChunk, a.vocab);
-    auto tokens = [&](auto f) {
-        for (int i = begin + threadIdx.x * 8; i < end; i += 2048) {
-            float v[8];
-            load_tokens<T>(a, at, i, v);
+    const bool cuts = r.cuts(), count = r.top_k != 0, weighed = !r.small();
+    uint64_t sum = 0;
+    part_tokens<T, 1>(a, at, begin, end, [&](const float (&v)[8], int) {
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (token(v[j])) f(v[j]);
+        for (int j = 0; j < 8; j++)
+            if (count && token(v[j])) atomicAdd(&counts[bin_of(r, v[j])], 1u);
+        if (!weighed) return;
+        uint64_t w[8];
+        weigh(r, v, cuts, w);
+        if (!cuts) {
+            sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            return;
         }
-    };
-    auto count = [&](float l) { atomicAdd(&counts[bin_of(r, l)], 1u); };
-    auto weigh = [&](float l) { atomicAdd(reinterpret_cast<unsigned long long*>(&weights[bin_of(r, l)]), static_cast<unsigned long long>(weight_of(r, l))); };
-    if (!r.cuts()) {
-        uint64_t sum = 0, total;
-        tokens([&](float l) {
-            const Ratio ratio = ratio_of(r, l);
-            if (likely(r, ratio)) sum += weight_of(r, ratio);
-        });
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (w[j]) atomicAdd(reinterpret_cast<unsigned long long*>(&weights[bin_of(r, v[j])]), static_cast<unsigned long long>(w[j]));
+    });
+    if (!cuts) {
+        uint64_t total;
         block_scan<4>(sum, waves, &total);
         if (threadIdx.x == 0) a.kept[blockIdx.x] = total;
         return;
     }
-    if (r.small()) tokens(count);
-    else if (r.top_k) tokens([&](float l) { count(l), weigh(l); });
-    else tokens(weigh);
     __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += 256) {
         if (!r.small()) a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i] = weights[i];
@@ -709,92 +810,118 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
     }
 }
 
-__global__ __launch_bounds__(1024) void sample_cut_kernel(SampleArgs a) {
-    __shared__ Row shared;
+__global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleArgs a) {
     __shared__ CutShared sh;
-    const int row = blockIdx.x, bin = threadIdx.x;
-    const Row r = row_of(a, row, &shared);
-    Cut cut{};
-    cut.sure = cut.limit = kBins;
-    cut.k_bin = cut.last = cut.m_last = -1;
+    const int row = blockIdx.x, bin = kPer * threadIdx.x;
+    const Row r = a.settings[row];
+    Cut cut = no_cut();
     if (!drawn(a, r, row) && r.cuts()) {
-        uint64_t w = 0, up_to;
-        uint32_t c = 0;
+        uint64_t w[kPer] = {}, up_to[kPer];
+        uint32_t c[kPer] = {};
         const int64_t first = static_cast<int64_t>(row) * a.parts * kBins + bin;
         if (!r.small())
 #pragma unroll 8
-            for (int p = 0; p < a.parts; p++) w += a.weights[first + p * kBins];
+            for (int p = 0; p < a.parts; p++)
+#pragma unroll
+                for (int i = 0; i < kPer; i++) w[i] += a.weights[first + p * kBins + i];
         if (r.top_k)
 #pragma unroll 8
-            for (int p = 0; p < a.parts; p++) c += a.counts[first + p * kBins];
-        cut = find_cuts(r, c, w, sh, &up_to);
-        a.upto[static_cast<int64_t>(row) * kBins + bin] = up_to;
+            for (int p = 0; p < a.parts; p++)
+#pragma unroll
+                for (int i = 0; i < kPer; i++) c[i] += a.counts[first + p * kBins + i];
+        cut = find_cuts(r, c, w, sh, up_to);
+#pragma unroll
+        for (int i = 0; i < kPer; i++) a.upto[static_cast<int64_t>(row) * kBins + bin + i] = up_to[i];
     }
     if (bin == 0) {
-        a.settings[row] = r;
         a.cuts[row] = cut;
         a.listed[row] = 0;
     }
 }
 
-// Lists the tokens in question, and sums up what a part keeps for sure from its bins.
+// The logits between which all tokens in question lie, a little widened: bins are rounded.
+__device__ __forceinline__ void logits_in_question(const Row& r, const Cut& cut, float* low, float* high) {
+    int b0 = kBins, b1 = -1;
+    if (cut.k_bin >= 0) b0 = b1 = cut.k_bin;
+    if (cut.first <= cut.last) b0 = min(b0, cut.first), b1 = max(b1, cut.last);
+    if (cut.m_first <= cut.m_last) b0 = min(b0, cut.m_first), b1 = max(b1, cut.m_last);
+    b1 = min(b1, cut.limit);
+    const double most = r.max, wide = 1.0 / r.scale, edge = 1e-6 * fabs(most);  // (no scale: all tokens)
+    const bool finite = fabs(most) < 3.0e38;
+    *high = b0 <= 0 || !finite ? __builtin_inff() : static_cast<float>(most - b0 * wide * (1 - 1e-6) + edge);
+    *low = b1 >= kBins - 2 || !finite || r.scale == 0.0f ? -__builtin_inff()
+                                                                       : static_cast<float>(most - (b1 + 1) * wide * (1 + 1e-6) - edge);
+}
+
+// Lists the tokens in question, and sums up what a part keeps for sure from its bins.  A part lists its tokens in LDS,
+// takes as many places of the row's list at once and copies them there; what LDS has no room for goes there by itself.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
-    __shared__ uint64_t waves[4], places[kChunk];
+    __shared__ uint64_t waves[4], places[kPartList];
     __shared__ uint32_t found, to;
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const Row r = a.settings[row];
     if (r.greedy || r.bad || !r.cuts()) return;
     const Cut cut = a.cuts[row];
     const int64_t at = row * a.stride;
+    uint64_t* const list = a.list + static_cast<int64_t>(row) * kList;
     uint64_t sum = 0, total;
-    for (int i = threadIdx.x; i < cut.sure && i < kBins; i += 256) sum += a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i];
+    for (int i = threadIdx.x; i < min(cut.sure, kBins); i += 256) sum += a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i];
+    if (threadIdx.x == 0) found = 0;
+    float low, high;
+    logits_in_question(r, cut, &low, &high);
     block_scan<4>(sum, waves, &total);
-    if (threadIdx.x == 0) a.kept[blockIdx.x] = total, found = 0;
-    __syncthreads();
-    for (int chunk = part * a.per * kChunk; chunk < min((part + 1) * a.per * kChunk, a.vocab); chunk += kChunk) {
-        float v[kChunk / 2048][8];
+    part_tokens<T, 4>(a, at, part * a.per * kChunk, min((part + 1) * a.per * kChunk, a.vocab), [&](const float (&v)[8], int first) {
 #pragma unroll
-        for (int h = 0; h < kChunk / 2048; h++) load_tokens<T>(a, at, chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8, v[h]);
-#pragma unroll
-        for (int h = 0; h < kChunk / 2048; h++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (!token(v[h][j]) || !cut.in_question(bin_of(r, v[h][j]))) continue;
-                places[atomicAdd(&found, 1u)] = place_of(v[h][j], chunk + h * 2048 + static_cast<int>(threadIdx.x) * 8 + j);
+        for (int j = 0; j < 8; j++)
+            if (v[j] >= low && v[j] <= high && token(v[j]) && cut.in_question(bin_of(r, v[j]))) {
+                const uint64_t place = place_of(v[j], first + j);
+                const uint32_t i = atomicAdd(&found, 1u);
+                if (i < kPartList) {
+                    places[i] = place;
+                } else {
+                    const uint32_t next = atomicAdd(&a.listed[row], 1u);
+                    if (next < kList) list[next] = place;
+                }
             }
-        __syncthreads();
-        if (found == 0) continue;  // the same for all
-        if (threadIdx.x == 0) to = atomicAdd(&a.listed[row], found);
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < found && to + i < kList; i += 256) a.list[static_cast<int64_t>(row) * kList + to + i] = places[i];
-        __syncthreads();
-        if (threadIdx.x == 0) found = 0;
-        __syncthreads();
+    });
+    __syncthreads();
+    const uint32_t held = min(found, static_cast<uint32_t>(kPartList));
+    if (threadIdx.x == 0) {
+        a.kept[blockIdx.x] = total;
+        to = held ? atomicAdd(&a.listed[row], held) : 0;
     }
+    __syncthreads();
+    const uint32_t next = to;
+    for (uint32_t i = threadIdx.x; i < held; i += 256)
+        if (next + i < kList) list[next + i] = places[i];
 }
 
 struct DrawShared {
     uint64_t places[kList], weights[kList];
     NarrowShared narrow;
-    uint64_t waves64[16], sums[kParts], before;
+    Row row;
+    Cut cut;
+    uint64_t waves64[kWaves], sums[kParts], before;
     int chosen;
 };
 
 template <typename T>
-__global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     __shared__ DrawShared sh;
     const int tid = threadIdx.x, row = blockIdx.x;
-    const Row r = a.settings[row];
+    if (tid == 0) sh.row = a.settings[row], sh.cut = a.cuts[row];
+    __syncthreads();
+    const Row& r = sh.row;
+    const Cut& cut = sh.cut;
     if (r.bad || r.greedy || r.arg == INT32_MAX) return;  // the cut kernel has stored those
-    const Cut cut = a.cuts[row];
     const int64_t at = row * a.stride;
     if (tid < a.parts) sh.sums[tid] = a.kept[static_cast<int64_t>(row) * a.parts + tid];
     uint64_t last = ~uint64_t{0};
     if (r.cuts()) {
         const uint32_t listed = a.listed[row];  // above kList: the list does not hold them, the row again
         if (listed <= kList)
-            for (uint32_t i = tid; i < listed; i += 1024) {
+            for (uint32_t i = tid; i < listed; i += kThreads) {
                 const uint64_t place = a.list[static_cast<int64_t>(row) * kList + i];
                 sh.places[i] = place;
                 sh.weights[i] = weight_of(r, key_logit(static_cast<uint32_t>(place >> 24)));
@@ -802,28 +929,20 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
         __syncthreads();
         auto each = [&](int b0, int b1, auto f) {
             if (listed <= kList) {
-                for (uint32_t i = tid; i < listed; i += 1024) {
+                for (uint32_t i = tid; i < listed; i += kThreads) {
                     const int b = bin_of(r, key_logit(static_cast<uint32_t>(sh.places[i] >> 24)));
                     if (b >= b0 && b <= b1) f(sh.places[i], sh.weights[i]);
                 }
                 return;
             }
-            for (int i = tid * 8; i < a.vocab; i += 8192) {
-                float v[8];
-                load_tokens<T>(a, at, i, v);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (!token(v[j])) continue;
-                    const int b = bin_of(r, v[j]);
-                    if (b >= b0 && b <= b1 && cut.in_question(b)) f(place_of(v[j], i + j), weight_of(r, v[j]));
-                }
-            }
+            each_of_row<T>(a, at, r, cut, b0, b1, f);
         };
         last = last_place(r, cut, sh.narrow, each, [&](int bin) { return a.upto[static_cast<int64_t>(row) * kBins + bin]; });
         // the listed tokens that are kept join their parts' weights
         each(cut.sure, kBins, [&](uint64_t place, uint64_t w) {
-            if (place > last || w == 0 || !likely(r, ratio_of(r, key_logit(static_cast<uint32_t>(place >> 24))))) return;
-            atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[(place & 0xffffff) / (a.per * kChunk)]), static_cast<unsigned long long>(w));
+            if (place > last) return;
+            if (r.least > 0.0f) w = weight_of(r, key_logit(static_cast<uint32_t>(place >> 24)), false);
+            if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.sums[(place & 0xffffff) / (a.per * kChunk)]), static_cast<unsigned long long>(w));
         });
     }
     __syncthreads();
@@ -839,31 +958,29 @@ __global__ __launch_bounds__(1024) void sample_draw_kernel(SampleArgs a) {
     const int part = sh.chosen;
     uint64_t run = sh.before;
     __syncthreads();
-    // the tokens of the part in which the sum passes the target, four a thread at a time
-    for (int chunk = part * a.per * kChunk; chunk < min((part + 1) * a.per * kChunk, a.vocab); chunk += kChunk) {
-        uint64_t w4[4], sum = 0;
-        const int id0 = chunk + tid * 4;
+    // the tokens of the part in which the sum passes the target, eight a thread at a time
+    const int end = min((part + 1) * a.per * kChunk, a.vocab);
+    for (int begin = part * a.per * kChunk; begin < end; begin += 8 * kThreads) {
+        const int first = begin + tid * 8;
+        float v[8];
+        uint64_t w[8], sum = 0;
+        load_tokens<T>(a, at, first, v);
+        weigh(r, v, false, w);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float l = id0 + j < a.vocab ? Vec8<T>::load1(a.logits, at + id0 + j) : -__builtin_inff();
-            w4[j] = 0;
-            if (token(l)) {
-                const int b = bin_of(r, l);
-                if (b < cut.sure || (cut.in_question(b) && place_of(l, id0 + j) <= last)) {
-                    const Ratio ratio = ratio_of(r, l);
-                    if (likely(r, ratio)) w4[j] = weight_of(r, ratio);
-                }
-            }
-            sum += w4[j];
+        for (int j = 0; j < 8; j++) {
+            // (a select of values: zeroed in branches, elements of this array kept their old values with hipcc 7.2)
+            const bool in = (first + j < end) & cut.keeps(bin_of(r, v[j]), place_of(v[j], first + j), last);
+            w[j] = in ? w[j] : 0;
+            sum += w[j];
         }
         uint64_t all;
-        uint64_t to = run + block_scan<16>(sum, sh.waves64, &all) - sum;
+        uint64_t to = run + block_scan<kWaves>(sum, sh.waves64, &all) - sum;
         run += all;
         if (run <= target) continue;  // the same for all
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            if (to + w4[j] > target && to <= target) store_token(a, row, id0 + j, static_cast<float>(static_cast<double>(w4[j]) / static_cast<double>(total)));
-            to += w4[j];
+        for (int j = 0; j < 8; j++) {
+            if (to + w[j] > target && to <= target) store_token(a, row, first + j, static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total)));
+            to += w[j];
         }
         return;
     }
@@ -875,9 +992,12 @@ struct Plan {
     int64_t peaks, weights, counts, upto, settings, cuts, listed, list, kept, bytes;
 };
 
+// A workgroup a row where that fills the chip, or a row is one block.
+bool by_rows(int64_t rows, int64_t vocab) { return vocab <= kRowVocab && (rows >= env_int("SANDY_SAMPLE_ROWS", 256) || vocab <= kBlock); }
+
 Plan plan_of(int64_t rows, int64_t vocab) {
     Plan p{};
-    if (vocab <= kRowVocab) return p;
+    if (by_rows(rows, vocab)) return p;
     const int64_t chunks = (vocab + kChunk - 1) / kChunk;
     auto split = [&](int64_t most, int32_t* parts, int32_t* per) {
         const int64_t want = std::max<int64_t>(std::min<int64_t>({most, chunks, kParts}), 1);
@@ -918,15 +1038,15 @@ int check_logits(const SandyTensor* logits, Err e) {
 template <typename T>
 int launch_sample(const SampleArgs& a, Err e, hipStream_t s) {
     const dim3 rows(static_cast<unsigned>(a.rows));
-    if (a.vocab <= kRowVocab) {
-        hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(1024), 0, s, a);
+    if (by_rows(a.rows, a.vocab)) {
+        hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(kThreads), 0, s, a);
     } else {
         const dim3 parts(static_cast<unsigned>(a.rows) * a.parts), peaks(static_cast<unsigned>(a.rows) * a.peak_parts);
         hipLaunchKernelGGL(sample_peak_kernel<T>, peaks, dim3(256), 0, s, a);
         hipLaunchKernelGGL(sample_bins_kernel<T>, parts, dim3(256), 0, s, a);
-        hipLaunchKernelGGL(sample_cut_kernel, rows, dim3(1024), 0, s, a);
+        hipLaunchKernelGGL(sample_cut_kernel, rows, dim3(kThreads), 0, s, a);
         hipLaunchKernelGGL(sample_gather_kernel<T>, parts, dim3(256), 0, s, a);
-        hipLaunchKernelGGL(sample_draw_kernel<T>, rows, dim3(1024), 0, s, a);
+        hipLaunchKernelGGL(sample_draw_kernel<T>, rows, dim3(kThreads), 0, s, a);
     }
     SANDY_HIP_TRY(hipGetLastError(), e, "sample launch");
     return ok(e);
