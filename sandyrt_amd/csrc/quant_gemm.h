@@ -62,8 +62,9 @@ __device__ __forceinline__ void quant_group_rows(const QuantGemm& a, int g, int*
     *end = static_cast<int>(e);
 }
 
-// The kernel for many rows (quant_tile.h), in one of its tile forms.
-int launch_quant_tiles(const QuantGemm& a, bool bf16, int form, Err e, hipStream_t s);
+// The kernel for few rows (quant_linear.hip), or that for many (quant_tile.h) in one of its tile forms.
+enum class QuantForm { kStream, k64x64Split, k64x128Split, k128x128Split, k64x128, k128x128, k256x256 };
+int launch_quant_tiles(const QuantGemm& a, bool bf16, QuantForm form, Err e, hipStream_t s);
 
 // The bits of a dword that hold the first n bytes.
 __device__ __forceinline__ uint32_t first_bytes(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }

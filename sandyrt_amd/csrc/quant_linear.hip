@@ -18,29 +18,23 @@
 namespace sandy_hip {
 namespace {
 
-// Few rows: a stream of the weight.  A workgroup takes 16 NW weight rows and every WAVES-th block of 128 columns
-// per wave; a lane loads 32 bytes of its weight row (16 rows of whole 128-byte lines a wave) and of its x
-// row straight into the operand registers, DEPTH blocks ahead.  The waves' sums meet in LDS, in their order.
-// More than 16 RT rows go round again, the weights then coming from L2.
-template <typename T, int RT, int NW, int WAVES, int DEPTH>
+// Few rows: a stream of the weight.  A workgroup takes 16 weight rows, a wave every WAVES-th block of 128 columns; a lane
+// loads 32 bytes of its weight row (16 rows of whole 128-byte lines a wave) and of its x row straight into the operand
+// registers, DEPTH blocks ahead.  The waves' sums meet in LDS, in their order.  More than 16 rows go round again, the
+// weights then coming from L2.
+template <typename T, int WAVES, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
-    constexpr bool kScaled = std::is_same_v<T, BF16>;
-    __shared__ float red[WAVES][RT * NW][4][64];
+    __shared__ float red[WAVES][4][64];
     const int lane = threadIdx.x & 63, row = lane & 15, quarter = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const int g = blockIdx.y, n0 = static_cast<int>(blockIdx.x) * 16 * NW;
+    const int g = blockIdx.y, n0 = static_cast<int>(blockIdx.x) * 16;
     int begin, end;
     quant_group_rows(a, g, &begin, &end);
     if (begin >= end) return;
     const int last = a.blocks - 1, rest = a.k - last * kQuantBlock;  // columns of the last block
-    const uint8_t* wp[NW];
-    const uint8_t* wsp[NW];
-#pragma unroll
-    for (int c = 0; c < NW; c++) {
-        const int n = min(n0 + 16 * c + row, a.n - 1);
-        wp[c] = a.w + g * a.w_group + n * a.w_pitch + 32 * quarter;
-        wsp[c] = a.ws + (static_cast<int64_t>(g) * a.w_scale_rows + (n >> a.w_shift)) * a.blocks;
-    }
+    const int n = min(n0 + row, a.n - 1);
+    const uint8_t* wp = a.w + g * a.w_group + n * a.w_pitch + 32 * quarter;
+    const uint8_t* wsp = a.ws + (static_cast<int64_t>(g) * a.w_scale_rows + (n >> a.w_shift)) * a.blocks;
     // a block's 32 bytes of a row, those past k as 0 (a piece that begins there is not read)
     auto load = [&](const uint8_t* p, int j) -> i32x8_t {
         const uint8_t* at = p + static_cast<int64_t>(j) * kQuantBlock;
@@ -61,28 +55,17 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
         }
         return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     };
-    for (int r0 = begin; r0 < end; r0 += 16 * RT) {
-        const uint8_t* xp[RT];
-        const uint8_t* xsp[RT];
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
-            const int r = min(r0 + 16 * t + row, end - 1);
-            xp[t] = a.x + r * a.x_pitch + 32 * quarter;
-            xsp[t] = a.xs + static_cast<int64_t>(r) * a.blocks;
-        }
-        i32x8_t wf[DEPTH][NW], xf[DEPTH][RT];
-        int wsf[DEPTH][NW], xsf[DEPTH][RT];
+    for (int r0 = begin; r0 < end; r0 += 16) {
+        const int r = min(r0 + row, end - 1);
+        const uint8_t* xp = a.x + r * a.x_pitch + 32 * quarter;
+        const uint8_t* xsp = a.xs + static_cast<int64_t>(r) * a.blocks;
+        i32x8_t wf[DEPTH], xf[DEPTH];
+        int wsf[DEPTH], xsf[DEPTH];
         auto request = [&](int d, int j) {
-#pragma unroll
-            for (int c = 0; c < NW; c++) wf[d][c] = load(wp[c], j), wsf[d][c] = wsp[c][j];
-#pragma unroll
-            for (int t = 0; t < RT; t++) xf[d][t] = load(xp[t], j), xsf[d][t] = xsp[t][j];
+            wf[d] = load(wp, j), wsf[d] = wsp[j];
+            xf[d] = load(xp, j), xsf[d] = xsp[j];
         };
-        f32x4_t acc[RT][NW];
-#pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-            for (int c = 0; c < NW; c++) acc[t][c] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4_t acc{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int d = 0; d < DEPTH; d++)
             if (wave + d * WAVES <= last) request(d, wave + d * WAVES);
@@ -91,61 +74,72 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
             for (int d = 0; d < DEPTH; d++) {
                 const int j = j0 + d * WAVES;
                 if (j > last) break;
+                if constexpr (std::is_same_v<T, BF16>) {
+                    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[d], xf[d], acc, 0, 0, 0, wsf[d], 0, xsf[d]);
+                } else {
+                    const Widened xw = widen(xf[d], quant_scale(xsf[d])), ww = widen(wf[d], quant_scale(wsf[d]));
 #pragma unroll
-                for (int c = 0; c < NW; c++)
-#pragma unroll
-                    for (int t = 0; t < RT && kScaled; t++)
-                        acc[t][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wf[d][c], xf[d][t], acc[t][c], 0, 0, 0, wsf[d][c],
-                                                                                    0, xsf[d][t]);
-                if constexpr (!kScaled) {
-                    Widened xw[RT];
-#pragma unroll
-                    for (int t = 0; t < RT; t++) xw[t] = widen(xf[d][t], quant_scale(xsf[d][t]));
-#pragma unroll
-                    for (int c = 0; c < NW; c++) {
-                        const Widened ww = widen(wf[d][c], quant_scale(wsf[d][c]));
-#pragma unroll
-                        for (int s = 0; s < 4; s++)
-#pragma unroll
-                            for (int t = 0; t < RT; t++)
-                                acc[t][c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww.v[s], xw[t].v[s], acc[t][c], 0, 0, 0);
-                    }
+                    for (int s = 0; s < 4; s++) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ww.v[s], xw.v[s], acc, 0, 0, 0);
                 }
                 if (j + DEPTH * WAVES <= last) request(d, j + DEPTH * WAVES);
             }
         }
-        // acc[t][c][i]: x row 16 t + lane % 16, column 16 c + 4 (lane / 16) + i
+        // acc[i]: x row lane % 16, column 4 (lane / 16) + i
 #pragma unroll
-        for (int t = 0; t < RT; t++)
-#pragma unroll
-            for (int c = 0; c < NW; c++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) red[wave][t * NW + c][i][lane] = acc[t][c][i];
+        for (int i = 0; i < 4; i++) red[wave][i][lane] = acc[i];
         __syncthreads();
-        for (int q = wave; q < RT * NW; q += WAVES) {
-            const int t = q / NW, c = q % NW;
+        if (wave == 0) {
             f32x4_t v{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < WAVES; s++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) v[i] += red[s][q][i][lane];
-            const int r = r0 + 16 * t + row;
-            if (r < end) store_columns<T>(a, r, n0 + 16 * c + 4 * quarter, v);
+                for (int i = 0; i < 4; i++) v[i] += red[s][i][lane];
+            if (r0 + row < end) store_columns<T>(a, r0 + row, n0 + 4 * quarter, v);
         }
         __syncthreads();
     }
 }
 
+// Which kernel, from how many tiles there are for 256 CUs (us, bf16 outputs, rows x columns x k).  One workgroup a CU leaves
+// most of it idle, so few tiles are made smaller and their k is split between two groups of waves:
+//   333 x 1999 x 5617    64 x 64 split 15.8, 64 x 128 whole 26, 128 x 128 whole 34, 256 x 256 84
+//   128 x 11264 x 2048   64 x 128 split 11.9, whole 13.5, 64 x 64 split 14
+//   1024 x 4096 x 4096   128 x 128 split 23.5, whole 27, 256 x 256 46
+// Many tiles: 256 x 256 has half the traffic of 128 x 128, which two a CU come in smaller rounds:
+//   1024 x 11264 x 2048  29.5 against 35   2048 x 11264 x 2048  59 against 52   4096 x 4096 x 4096  57 against 69
+//   4096 x 8192 x 8192   202 against 262
+// Few rows: the stream of the weight.  Every workgroup reads x for 16 columns, so that more rows and many columns are for tiles:
+//   1 x 11264 x 2048     7.2, 64 x 64 split 8.7      16 x 4096 x 4096   7.8 against 10.6    16 x 8192 x 8192  24 against 26
+//   1 x 28672 x 8192     52, 64 x 128 split 62       4 x 16384 x 4096   19 against 17       1 x 32000 x 2048  18.3, 64 x 128 15.2
+// Many columns for a row of tiles, split where k is long: 64 x 128 split and whole
+//   8 x 65536 x 2048     32 and 28                   8 x 152064 x 4096  116 and 138
+// Experts have uneven rows, a tile more than they fill; by the rows of each on average, 128 experts of 1408 x 2816 and
+// 2816 x 704:
+//   1 row     stream 71 and 55, 64 x 128 79 and 58       4 rows    stream 108 and 95, 64 x 128 95 and 73
+//   64 rows   64 x 128 153 and 127, 128 x 128 149 and 117
+QuantForm form_of(const QuantGemm& a) {
+    const int64_t rows = a.offsets ? (a.rows + a.groups - 1) / a.groups : a.rows;
+    auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * a.groups * ((a.n + n - 1) / n); };
+    const int64_t least = tiles(64, 64);
+    if (rows <= (a.offsets ? 1 : least <= 128 ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0)) return QuantForm::kStream;
+    if (least <= 256) return QuantForm::k64x64Split;
+    if (a.offsets) return rows > 32 && tiles(128, 128) >= 512 ? QuantForm::k128x128 : QuantForm::k64x128;
+    if (tiles(64, 128) <= 256 || (rows <= 64 && a.blocks >= 32)) return QuantForm::k64x128Split;
+    if (rows <= 64) return QuantForm::k64x128;
+    if (tiles(128, 128) <= 256) return QuantForm::k128x128Split;
+    // a round of 256 tiles of 256 x 256 takes 1.6 to 1.7 times one of 512 of 128 x 128 (57 and 35 at k = 4096)
+    const double large = 1.7 * static_cast<double>((tiles(256, 256) + 255) / 256), small = static_cast<double>((tiles(128, 128) + 511) / 512);
+    return large < small ? QuantForm::k256x256 : QuantForm::k128x128;
+}
+
 template <typename T>
 int launch_products(const QuantGemm& a, const char* what, Err e, hipStream_t s) {
-    const int64_t rows = a.offsets ? (a.rows + a.groups - 1) / a.groups : a.rows;
-    auto grid = [&](int nw) { return dim3(static_cast<unsigned>((a.n + 16 * nw - 1) / (16 * nw)), static_cast<unsigned>(a.groups)); };
-    auto tiles = [&](int64_t edge) { return (rows + edge - 1) / edge * a.groups * ((a.n + edge - 1) / edge); };
-    const int form = env_int("SANDY_QUANT_TILE", rows <= 32 ? -1 : tiles(256) >= 512 && !a.offsets ? 0 : tiles(128) >= 256 ? 2 : 3);
-    if (form >= 0) return launch_quant_tiles(a, std::is_same_v<T, BF16>, form, e, s);
-    if (rows <= 16) hipLaunchKernelGGL((quant_stream_kernel<T, 1, 1, 4, 4>), grid(1), dim3(256), 0, s, a);
-    else if (rows <= 32) hipLaunchKernelGGL((quant_stream_kernel<T, 2, 2, 4, 2>), grid(2), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((quant_stream_kernel<T, 4, 2, 4, 2>), grid(2), dim3(256), 0, s, a);
+    const QuantForm form = static_cast<QuantForm>(env_int("SANDY_QUANT_FORM", static_cast<int>(form_of(a))));
+    if (form != QuantForm::kStream) return launch_quant_tiles(a, std::is_same_v<T, BF16>, form, e, s);
+    const dim3 grid(static_cast<unsigned>((a.n + 15) / 16), static_cast<unsigned>(a.groups));
+    // eight waves where each still has four blocks (1 x 1024 x 8192: 7.6 us against 11.1; 1 x 11264 x 2048: 8.2 against 7.3)
+    if (a.blocks >= 32) hipLaunchKernelGGL((quant_stream_kernel<T, 8, 2>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((quant_stream_kernel<T, 4, 4>), grid, dim3(256), 0, s, a);
     SANDY_HIP_TRY(hipGetLastError(), e, what);
     return ok(e);
 }

@@ -2,11 +2,20 @@
 #pragma once
 #include "quant_gemm.h"
 
+#include <algorithm>
+
 namespace sandy_hip {
 
 // Workgroup tile 64 WM x 32 PN WN of rows x columns, 2 x PN waves of 32 WM x 32 WN on 32 x 32 instructions, 128 columns
-// of k (a block, a whole 128-byte line of every row) a chunk, STAGES chunks in LDS.
-template <int WM, int WN, int PN, int STAGES>
+// of k (a block, a whole 128-byte line of every row) a chunk, STAGES chunks in LDS.  SPLIT groups of so many waves share the
+// chunks, a run each, and add up their sums at the end.
+//
+// What it is up against: a CU's copies into LDS move 64 bytes a cycle, which a 64 x 64 tile needs for 256 cycles a chunk and
+// its products for 64 a wave, so that small tiles are bound by the copies and the two meetings of a chunk (about 490 ns with
+// four waves, whether 2, 4 or 8 chunks are under way: 333 x 1999 x 5617 in 22 us each time) and gain from SPLIT, which has
+// twice the waves between the same meetings (15.8); a third and fourth group gained nothing (17.7).  A 256 x 256 tile needs
+// 1024 cycles of copies for 2048 of products: 2720 TFLOP/s at 4096 x 8192 x 8192 and 2402 at 4096 x 4096 x 4096.
+template <int WM, int WN, int PN, int STAGES, int SPLIT>
 struct QuantTile {
     static constexpr int BM = 64 * WM, BN = 32 * PN * WN, kThreads = 128 * PN;
     static constexpr int kX = BM * 128, kStage = (BM + BN) * 128;
@@ -16,22 +25,23 @@ struct QuantTile {
     template <typename T>
     static constexpr int row_bytes() { return 32 * WN * static_cast<int>(sizeof(typename Vec8<T>::elem)) + 16; }
     template <typename T>
-    static constexpr int lds() {
+    static constexpr int group_lds() {
         const int out = kThreads / 64 * 32 * row_bytes<T>();
-        constexpr int loop = kScales + 2 * kScaleBytes;
-        return loop > out ? loop : out;
+        constexpr int loop = kScales + 2 * kScaleBytes, sums = SPLIT > 1 ? BM * BN * 4 : 0;
+        return std::max({loop, sums, (out + 1023) / 1024 * 1024});
     }
+    template <typename T>
+    static constexpr int lds() { return SPLIT * group_lds<T>(); }
 };
 
-// Sixteen scale bytes j .. j + 15 of a row, those past the last block as 0.
+// Sixteen scale bytes j .. j + 15 of a row, the last for those past it.
 __device__ __forceinline__ i32x4_t sixteen_scales(const uint8_t* row, int j, int blocks) {
     i32x4_t v{0, 0, 0, 0};
     if (j + 16 <= blocks) {
         __builtin_memcpy(&v, row + j, 16);
-    } else {
+    } else {  // (all at once: loads under a condition each would wait for one another)
 #pragma unroll
-        for (int i = 0; i < 15; i++)
-            if (j + i < blocks) v[i >> 2] |= row[j + i] << (8 * (i & 3));
+        for (int i = 0; i < 16; i++) v[i >> 2] |= row[min(j + i, blocks - 1)] << (8 * (i & 3));
     }
     return v;
 }
@@ -48,13 +58,14 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <typename T, int WM, int WN, int PN, int STAGES>
-__global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
-    using G = QuantTile<WM, WN, PN, STAGES>;
+template <typename T, int WM, int WN, int PN, int STAGES, int SPLIT>
+__global__ __launch_bounds__(128 * PN * SPLIT, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
+    using G = QuantTile<WM, WN, PN, STAGES, SPLIT>;
     constexpr bool kScaled = std::is_same_v<T, BF16>;
-    extern __shared__ __align__(1024) unsigned char lds[];
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    extern __shared__ __align__(1024) unsigned char all_lds[];
+    const int lane = threadIdx.x & 63, waves = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int group = waves / (2 * PN), wave = waves - group * 2 * PN, tid = 64 * wave + lane;
+    unsigned char* const lds = all_lds + group * G::template group_lds<T>();
     const int wm = wave & 1, wn = wave >> 1;
     const int col = lane & 31, half = lane >> 5;
 
@@ -67,19 +78,29 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
     const int m_tile = static_cast<int>(8u * band + in % high), n_tile = static_cast<int>(in / high);
     int g = 0, r0 = m_tile * G::BM, end = a.rows;
     if (a.offsets) {
-        // the m_tile-th of the experts' row tiles
+        // the m_tile-th of the experts' row tiles; a lane takes four experts at a time
         int before = 0;
         g = -1;
-        for (int base = 0; base < a.groups; base += 64) {
-            const int e = base + lane;
-            int first = 0, past = 0;
-            if (e < a.groups) {
-                const int64_t b = load_index(a.offsets, a.offsets_dt, e), f = load_index(a.offsets, a.offsets_dt, e + 1);
-                if (b < 0 || f < b || f > a.rows) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_OFFSETS));
-                else first = static_cast<int>(b), past = static_cast<int>(f);
+        for (int base = 0; base < a.groups && g < 0; base += 256) {
+            const int e0 = base + 4 * lane;
+            int64_t edge[5];
+            if (a.offsets_dt == SANDY_I32) {
+#pragma unroll
+                for (int i = 0; i < 5; i++) edge[i] = static_cast<const int32_t*>(a.offsets)[min(e0 + i, a.groups)];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 5; i++) edge[i] = static_cast<const int64_t*>(a.offsets)[min(e0 + i, a.groups)];
             }
-            int upto = (past - first + G::BM - 1) / G::BM;
-            const int mine = upto;
+            int tiles[4], mine = 0;
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const bool in_order = edge[i] >= 0 && edge[i + 1] >= edge[i] && edge[i + 1] <= a.rows;
+                bad |= !in_order;
+                mine += tiles[i] = in_order ? static_cast<int>((edge[i + 1] - edge[i] + G::BM - 1) / G::BM) : 0;
+            }
+            if (bad) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_OFFSETS));
+            int upto = mine;
 #pragma unroll
             for (int s = 1; s < 64; s <<= 1) {
                 const int below = __shfl_up(upto, s, 64);
@@ -88,10 +109,18 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
             const uint64_t here = __ballot(before + upto > m_tile);
             if (here) {
                 const int l = __builtin_ctzll(here);
-                g = base + l;
-                r0 = __shfl(first, l, 64) + (m_tile - before - __shfl(upto - mine, l, 64)) * G::BM;
+                int at = before + upto - mine, found = 0, first = 0, past = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool in = m_tile >= at && m_tile < at + tiles[i];
+                    found = in ? e0 + i : found;
+                    first = in ? static_cast<int>(edge[i]) + (m_tile - at) * G::BM : first;
+                    past = in ? static_cast<int>(edge[i + 1]) : past;
+                    at += tiles[i];
+                }
+                g = __shfl(found, l, 64);
+                r0 = __shfl(first, l, 64);
                 end = __shfl(past, l, 64);
-                break;
             }
             before += __shfl(upto, 63, 64);
         }
@@ -130,9 +159,14 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
     auto copy = [&](int c, int stage, int i) {
         copy_to_lds(i < G::kXLoads ? xres : wres, from[i], c * 128, lds0 + stage * G::kStage + wave * 1024 + i * (16 * G::kThreads));
     };
+    // The group's whole blocks are first .. first + mine - 1, of all groups' `turns` turns; those past the last are the last
+    // again, copied and never read: every round waits for the same number.
+    const int chunks = a.k / kQuantBlock, rest = a.k - chunks * kQuantBlock;
+    const int turns = (chunks + SPLIT - 1) / SPLIT, first = min(group * turns, max(chunks - 1, 0));
+    const int mine = min(turns, chunks - group * turns), last = max(first + mine - 1, first);
     auto issue = [&](int c, int stage) {
 #pragma unroll
-        for (int i = 0; i < G::kLoads; i++) copy(c, stage, i);
+        for (int i = 0; i < G::kLoads; i++) copy(min(first + c, last), stage, i);
     };
     const int sw = (col >> 1) & 7;
     const int xat = (32 * WM * wm + col) * 128, wat = G::kX + (32 * WN * wn + col) * 128;
@@ -165,16 +199,16 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
     };
     constexpr int kScaleRows = (G::BM + G::BN + G::kThreads - 1) / G::kThreads;
     i32x4_t held[kScaleRows];
-    auto load_scales = [&](int first) {
+    auto load_scales = [&](int at) {
 #pragma unroll
         for (int u = 0; u < kScaleRows; u++)
-            if (G::kThreads * u + tid < G::BM + G::BN) held[u] = sixteen_scales(scale_row(G::kThreads * u + tid), first, a.blocks);
+            if (G::kThreads * u + tid < G::BM + G::BN) held[u] = sixteen_scales(scale_row(G::kThreads * u + tid), first + at, a.blocks);
     };
-    auto store_scales = [&](int first) {
+    auto store_scales = [&](int at) {
 #pragma unroll
         for (int u = 0; u < kScaleRows; u++)
             if (G::kThreads * u + tid < G::BM + G::BN)
-                *reinterpret_cast<i32x4_t*>(lds + G::kScales + ((first >> 4) & 1) * G::kScaleBytes + (G::kThreads * u + tid) * 16) = held[u];
+                *reinterpret_cast<i32x4_t*>(lds + G::kScales + ((at >> 4) & 1) * G::kScaleBytes + (G::kThreads * u + tid) * 16) = held[u];
     };
     int xs[WM], ws[WN], xs_next[WM], ws_next[WN];
     auto scales = [&](int c) {  // of chunks c .. c + 3, c a multiple of 4
@@ -239,16 +273,15 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
     using Left = std::integral_constant<int, (STAGES - 2) * G::kLoads + kIssued>;
     using First = std::integral_constant<int, (STAGES - 1) * G::kLoads>;
 
-    // Chunks past the last are the last again, copied and never read: every round waits for the same number.
-    const int chunks = a.k / kQuantBlock, rest = a.k - chunks * kQuantBlock, last = max(chunks - 1, 0);
     i32x4_t xf[2][WM][2], wf[2][WN][2];
     if (chunks) {
 #pragma unroll
-        for (int s = 0; s < STAGES - 1; s++) issue(min(s, last), s);
+        for (int s = 0; s < STAGES - 1; s++) issue(s, s);
     }
     if (rest) {
-        // the last block of a k that is no multiple of 128 goes first, through registers: bytes past k are 0
-        const int left = rest - 16 * piece;
+        // the last block of a k that is no multiple of 128 goes first, through registers: bytes past k are 0 (all of them
+        // for groups but the first)
+        const int left = (group ? 0 : rest) - 16 * piece;
         i32x4_t v[G::kLoads];
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
@@ -275,14 +308,14 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
     if (chunks) {
         load_scales(0);
         store_scales(0);
-        issue(min(STAGES - 1, last), STAGES - 1);
+        issue(STAGES - 1, STAGES - 1);
         meet(First{});
         frags(0, 0, xf[0], wf[0]);
         scales(0);
         use_scales();
     }
-    for (int c = 0, stage = 0; c < chunks; c++) {
-        const int next = stage + 1 == STAGES ? 0 : stage + 1, then = min(c + STAGES, last);
+    for (int c = 0, stage = 0; c < mine; c++) {
+        const int next = stage + 1 == STAGES ? 0 : stage + 1, then = min(first + c + STAGES, last);
         auto at_slot = [&](int slot) {
             constexpr int kRead = (4 * kReads + kTimes - 1) / kTimes;
 #pragma unroll
@@ -302,7 +335,7 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
         };
         multiply(xf[0], wf[0], at_slot);
         if ((c & 15) == 7) store_scales(c + 9);
-        if ((c & 15) == 6) load_scales(c + 10);
+        if ((c & 15) == 6 && first + c + 10 <= last) load_scales(c + 10);
         if ((c & 3) == 3) scales(c + 1);
         multiply(xf[1], wf[1], [&](int i) { at_slot(kTimes + i); });
         stage = next;
@@ -315,8 +348,38 @@ __global__ __launch_bounds__(128 * PN, 1) void quant_tile_kernel(QuantGemm a, in
             for (int q = 0; q < WN; q++) ws[q] = static_cast<int>(static_cast<uint32_t>(ws[q]) >> 8);
         }
     }
+    for (int c = max(mine, 0); c < turns; c++) {  // the other groups' meetings
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_s_barrier();
+    }
     wait_copies<0>();  // LDS is used again
     __syncthreads();
+    if constexpr (SPLIT > 1) {
+        // the groups' sums, in their order
+        auto at = [&](int g, int t, int c, int q) {
+            return reinterpret_cast<f32x4_t*>(all_lds + g * G::template group_lds<T>()) + ((wave * WM + t) * WN + c) * 256 + 64 * q + lane;
+        };
+#pragma unroll
+        for (int t = 0; t < WM && group; t++)
+#pragma unroll
+            for (int c = 0; c < WN; c++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) *at(group, t, c, q) = f32x4_t{acc[t][c][4 * q], acc[t][c][4 * q + 1], acc[t][c][4 * q + 2], acc[t][c][4 * q + 3]};
+        __syncthreads();
+        if (group) return;
+#pragma unroll
+        for (int g = 1; g < SPLIT; g++)
+#pragma unroll
+            for (int t = 0; t < WM; t++)
+#pragma unroll
+                for (int c = 0; c < WN; c++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const f32x4_t v = *at(g, t, c, q);
+#pragma unroll
+                        for (int i = 0; i < 4; i++) acc[t][c][4 * q + i] += v[i];
+                    }
+    }
 
     // acc[t][c][i]: row 32 t + col, column 32 c + 8 (i / 4) + 4 half + i % 4 of the wave's part: 32 rows at a time through
     // LDS (wave-private) into whole row segments

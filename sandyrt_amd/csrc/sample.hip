@@ -15,7 +15,7 @@
 // last 64 by comparing each with each.  A small top_k needs counts alone: all it may keep is listed, and top_p looks at
 // the list.
 //
-// Up to 65536 tokens a workgroup does a row in one launch, reading it up to four times, mostly from L2.  Longer rows are
+// Up to 8192 tokens a workgroup does a row in one launch, reading it up to four times, mostly from L2.  Longer rows are
 // cut into parts, so that few rows fill the chip, and take five launches: peak, bins, cut, gather, draw.
 #include "common.h"
 
@@ -31,7 +31,7 @@ constexpr int kBins = 1024;       // the last for tokens without weight
 constexpr int kList = 8192;       // listed tokens of a row in parts
 constexpr int kRowList = 2048;    // and of a row that one workgroup does
 constexpr int kPartList = 1024;   // and of a part's
-constexpr int kRowVocab = 65536;  // the longest such row
+constexpr int kRowVocab = 8192;   // the longest such row
 constexpr int kSmall = 1024;      // a top_k whose tokens are all listed
 constexpr int kMaxVocab = 1 << 24;
 // The cut, draw and whole-row kernels: 256 registers a thread, which 1024 threads would not have.  A thread has two bins.
@@ -681,37 +681,24 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     });
     __syncthreads();
     // the block and wave in which the sum of all passes the target: each wave looks, that one goes on
-    const int parts = (a.vocab + kBlock - 1) / kBlock * kWaves;
-    constexpr int kRounds = kRowVocab / kBlock * kWaves / 64;
-    uint64_t part_w[kRounds], total = 0;
+    constexpr int kSums = kRowVocab / kBlock * kWaves;
+    static_assert(kSums <= 64);
+    const uint64_t part_w = lane < (a.vocab + kBlock - 1) / kBlock * kWaves ? sh.sums[lane & (kSums - 1)] : 0, to = wave_scan(part_w);
+    const uint64_t total = __shfl(to, 63, 64), target = part_of(r.uniform, total, false);
+    const int part = __builtin_ctzll(__ballot(to > target));  // (the total is above the target)
+    if (part % kWaves != wave) return;
+    const uint64_t before = __shfl(to - part_w, part, 64);
+    float v[8];
+    uint64_t w[8];
+    const int first = part / kWaves * kBlock + tid * 8;
+    load_tokens<T>(a, at, first, v);
+    const uint64_t mine = kept(v, first, w);
+    uint64_t upto = before + wave_scan(mine) - mine;
 #pragma unroll
-    for (int q = 0; q < kRounds; q++) {
-        const int i = 64 * q + lane;
-        part_w[q] = i < parts ? sh.sums[i] : 0;
-        total += __shfl(wave_scan(part_w[q]), 63, 64);
-    }
-    const uint64_t target = part_of(r.uniform, total, false);
-    uint64_t run = 0;
-#pragma unroll
-    for (int q = 0; q < kRounds; q++) {
-        const uint64_t to = run + wave_scan(part_w[q]);
-        const uint64_t here = __ballot(to > target && to - part_w[q] <= target);
-        run = __shfl(to, 63, 64);
-        if (!here) continue;
-        const int l = __builtin_ctzll(here), part = 64 * q + l;
-        if (part % kWaves != wave) continue;
-        float v[8];
-        uint64_t w[8];
-        const int first = part / kWaves * kBlock + tid * 8;
-        load_tokens<T>(a, at, first, v);
-        const uint64_t mine = kept(v, first, w);
-        uint64_t upto = __shfl(to - part_w[q], l, 64) + wave_scan(mine) - mine;
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            if (upto <= target && upto + w[j] > target)
-                store_token(a, row, first + j, static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total)));
-            upto += w[j];
-        }
+    for (int j = 0; j < 8; j++) {
+        if (upto <= target && upto + w[j] > target)
+            store_token(a, row, first + j, static_cast<float>(static_cast<double>(w[j]) / static_cast<double>(total)));
+        upto += w[j];
     }
 }
 
@@ -992,12 +979,14 @@ struct Plan {
     int64_t peaks, weights, counts, upto, settings, cuts, listed, list, kept, bytes;
 };
 
-// A workgroup a row where that fills the chip, or a row is one block.
-bool by_rows(int64_t rows, int64_t vocab) { return vocab <= kRowVocab && (rows >= env_int("SANDY_SAMPLE_ROWS", 256) || vocab <= kBlock); }
+// A workgroup a row where a row is two blocks at most: 512 rows of 8000 bf16 tokens 24 to 46 us, in parts 30 to 48; 16 rows
+// 14 to 25, 18 to 27.  Longer ones are better in parts, also where workgroups of whole rows would fill the chip: 512 rows of
+// 32000 61 to 121 us, in parts 63 to 91; 16 rows 31 to 62, 18 to 31 (weights alone, and top-p).
+bool by_rows(int64_t vocab) { return vocab <= kRowVocab; }
 
 Plan plan_of(int64_t rows, int64_t vocab) {
     Plan p{};
-    if (by_rows(rows, vocab)) return p;
+    if (by_rows(vocab)) return p;
     const int64_t chunks = (vocab + kChunk - 1) / kChunk;
     auto split = [&](int64_t most, int32_t* parts, int32_t* per) {
         const int64_t want = std::max<int64_t>(std::min<int64_t>({most, chunks, kParts}), 1);
@@ -1038,7 +1027,7 @@ int check_logits(const SandyTensor* logits, Err e) {
 template <typename T>
 int launch_sample(const SampleArgs& a, Err e, hipStream_t s) {
     const dim3 rows(static_cast<unsigned>(a.rows));
-    if (by_rows(a.rows, a.vocab)) {
+    if (by_rows(a.vocab)) {
         hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(kThreads), 0, s, a);
     } else {
         const dim3 parts(static_cast<unsigned>(a.rows) * a.parts), peaks(static_cast<unsigned>(a.rows) * a.peak_parts);
