@@ -258,14 +258,24 @@ __device__ __forceinline__ void load_tokens(const SampleArgs& a, int64_t at, int
     for (int j = 0; j < 8; j++) v[j] = first + j < a.vocab ? Vec8<T>::load1(a.logits, at + first + j) : -__builtin_inff();
 }
 
-// f(logits, first id) for a thread's eights of a part's chunks, N loads at a time without a guard where they are whole.
+// f(logits, first id) for a thread's eights of a part's chunks, N loads at a time without a guard where they are whole, the
+// next requested meanwhile.
 template <typename T, int N, typename F>
 __device__ __forceinline__ void part_tokens(const SampleArgs& a, int64_t at, int begin, int end, F f) {
     const int mine = static_cast<int>(threadIdx.x) * 8;
+    float next[N][8];
+    auto request = [&](int first) {
+#pragma unroll
+        for (int n = 0; n < N; n++) load8_unaligned<T>(a.logits, at + first + n * kChunk + mine, next[n]);
+    };
+    if (begin + N * kChunk <= end) request(begin);
     for (; begin + N * kChunk <= end; begin += N * kChunk) {
         float v[N][8];
 #pragma unroll
-        for (int n = 0; n < N; n++) load8_unaligned<T>(a.logits, at + begin + n * kChunk + mine, v[n]);
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[n][j] = next[n][j];
+        request(min(begin + N * kChunk, end - N * kChunk));  // (past the last whole ones: tokens of before, not used)
 #pragma unroll
         for (int n = 0; n < N; n++) f(v[n], begin + n * kChunk + mine);
     }
@@ -945,13 +955,17 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     const int part = sh.chosen;
     uint64_t run = sh.before;
     __syncthreads();
-    // the tokens of the part in which the sum passes the target, eight a thread at a time
+    // the tokens of the part in which the sum passes the target, eight a thread at a time, the next eight requested meanwhile
     const int end = min((part + 1) * a.per * kChunk, a.vocab);
-    for (int begin = part * a.per * kChunk; begin < end; begin += 8 * kThreads) {
+    float next[8];
+    load_tokens<T>(a, at, part * a.per * kChunk + tid * 8, next);
+    for (int begin = part * a.per * kChunk; begin < end; begin += kBlock) {
         const int first = begin + tid * 8;
         float v[8];
         uint64_t w[8], sum = 0;
-        load_tokens<T>(a, at, first, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = next[j];
+        load_tokens<T>(a, at, first + kBlock, next);
         weigh(r, v, false, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
