@@ -113,17 +113,23 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 //   1 x 28672 x 8192     52, 64 x 128 split 62       4 x 16384 x 4096   19 against 17       1 x 32000 x 2048  18.3, 64 x 128 15.2
 // Many columns for a row of tiles, split where k is long: 64 x 128 split and whole
 //   8 x 65536 x 2048     32 and 28                   8 x 152064 x 4096  116 and 138
-// Experts have uneven rows, a tile more than they fill; by the rows of each on average, 128 experts of 1408 x 2816 and
-// 2816 x 704:
-//   1 row     stream 71 and 55, 64 x 128 79 and 58       4 rows    stream 108 and 95, 64 x 128 95 and 73
-//   64 rows   64 x 128 153 and 127, 128 x 128 149 and 117
+// Experts: as if the rows were spread evenly over as many as may have one, but that their unevenness wants room for more
+// tiles.  A stream has workgroups for the empty ones as well, which cost it from some thousands on (us, experts x columns x k):
+//   2 rows, 8 x 1024 x 4096     stream 6.9, 64 x 64 split 12.4     8 rows, 256 x 2048 x 256    16.7 against 6.7
+//   8 rows, 128 x 2816 x 704    stream 18.6, 64 x 128 11           128 rows, 128 x 2816 x 704  58 against 40
+//   64 rows, 8 x 14336 x 4096   64 x 128 split 102, whole 117      2 times 64 rows, 8 x 4096 x 1024  split 18.7, whole 13.8
+//   64 rows each, 128 x 1408 x 2816 and 2816 x 704   64 x 128 142 and 110, 128 x 128 138 and 98
 QuantForm form_of(const QuantGemm& a) {
-    const int64_t rows = a.offsets ? (a.rows + a.groups - 1) / a.groups : a.rows;
-    auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * a.groups * ((a.n + n - 1) / n); };
-    const int64_t least = tiles(64, 64);
-    if (rows <= (a.offsets ? 1 : least <= 128 ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0)) return QuantForm::kStream;
+    const int64_t some = std::min<int64_t>(a.groups, a.rows), rows = (a.rows + some - 1) / some;
+    auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * some * ((a.n + n - 1) / n); };
+    const int64_t least = tiles(64, 64), streams = int64_t{a.groups} * ((a.n + 15) / 16);
+    const int64_t few = a.offsets ? (streams <= 4096 ? 2 : 0) : least <= 128 ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0;
+    if (rows <= few) return QuantForm::kStream;
     if (least <= 256) return QuantForm::k64x64Split;
-    if (a.offsets) return rows > 32 && tiles(128, 128) >= 512 ? QuantForm::k128x128 : QuantForm::k64x128;
+    if (a.offsets) {
+        if (rows > 32 && tiles(128, 128) >= 512) return QuantForm::k128x128;
+        return tiles(64, 128) <= 128 || a.blocks >= 32 ? QuantForm::k64x128Split : QuantForm::k64x128;
+    }
     if (tiles(64, 128) <= 256 || (rows <= 64 && a.blocks >= 32)) return QuantForm::k64x128Split;
     if (rows <= 64) return QuantForm::k64x128;
     if (tiles(128, 128) <= 256) return QuantForm::k128x128Split;

@@ -10,11 +10,11 @@ namespace sandy_hip {
 // of k (a block, a whole 128-byte line of every row) a chunk, STAGES chunks in LDS.  SPLIT groups of so many waves share the
 // chunks, a run each, and add up their sums at the end.
 //
-// What it is up against: a CU's copies into LDS move 64 bytes a cycle, which a 64 x 64 tile needs for 256 cycles a chunk and
-// its products for 64 a wave, so that small tiles are bound by the copies and the two meetings of a chunk (about 490 ns with
-// four waves, whether 2, 4 or 8 chunks are under way: 333 x 1999 x 5617 in 22 us each time) and gain from SPLIT, which has
-// twice the waves between the same meetings (15.8); a third and fourth group gained nothing (17.7).  A 256 x 256 tile needs
-// 1024 cycles of copies for 2048 of products: 2720 TFLOP/s at 4096 x 8192 x 8192 and 2402 at 4096 x 4096 x 4096.
+// What it is up against: a CU's copies into LDS came to no more than 35 bytes a cycle (83 KB/us) in any form, also with 4 and
+// 8 chunks under way and one meeting a chunk in place of two.  A chunk of a 64 x 64 tile takes them 480 cycles for 64 a wave
+// of products, one of 128 x 128 960 for 512 of two workgroups, one of 256 x 256 1900 for 2048, so that large tiles are bound
+// by both (2720 TFLOP/s at 4096 x 8192 x 8192) and small ones by copies: 333 x 1999 x 5617 in 22 us, where each workgroup
+// waits at every meeting, and 15.8 with SPLIT, whose groups wait for each other's copies; a third and fourth gain nothing.
 template <int WM, int WN, int PN, int STAGES, int SPLIT>
 struct QuantTile {
     static constexpr int BM = 64 * WM, BN = 32 * PN * WN, kThreads = 128 * PN;
@@ -69,51 +69,66 @@ __global__ __launch_bounds__(128 * PN * SPLIT, 1) void quant_tile_kernel(QuantGe
     const int wm = wave & 1, wn = wave >> 1;
     const int col = lane & 31, half = lane >> 5;
 
+    // experts' row tiles: a lane takes four experts from `base` on, up to whose end there are `upto` more than before base
+    int64_t edge[5];
+    int tiles[4], mine_tiles = 0;
+    auto count = [&](int base) {
+        const int e0 = base + 4 * lane;
+        if (a.offsets_dt == SANDY_I32) {
+#pragma unroll
+            for (int i = 0; i < 5; i++) edge[i] = static_cast<const int32_t*>(a.offsets)[min(e0 + i, a.groups)];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 5; i++) edge[i] = static_cast<const int64_t*>(a.offsets)[min(e0 + i, a.groups)];
+        }
+        bool bad = false;
+        mine_tiles = 0;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool in_order = edge[i] >= 0 && edge[i + 1] >= edge[i] && edge[i + 1] <= a.rows;
+            bad |= !in_order;
+            mine_tiles += tiles[i] = in_order ? static_cast<int>((edge[i + 1] - edge[i] + G::BM - 1) / G::BM) : 0;
+        }
+        if (bad) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_OFFSETS));
+        int upto = mine_tiles;
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int below = __shfl_up(upto, s, 64);
+            if (lane >= s) upto += below;
+        }
+        return upto;
+    };
+    int upto = 0;
+    if (a.offsets) {
+        // the grid has room for the most there can be; the XCDs share what there is (1024 tokens to 8 of 128 experts of
+        // 2816 x 704: 118 us where the last XCDs had the empty ones, 98 so)
+        int all = 0;
+        for (int base = 0; base < a.groups; base += 256) all += __shfl(upto = count(base), 63, 64);
+        m_tiles = min(__builtin_amdgcn_readfirstlane(all), m_tiles);
+        if (m_tiles <= 0) return;
+    }
     // workgroups go to the eight XCDs in turn: each takes a run of tiles, eight rows of tiles high, whose operands
     // its L2 then holds
     const uint32_t total = static_cast<uint32_t>(m_tiles) * n_tiles, per = (total + 7) / 8;
     const uint32_t tile = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if (tile >= total) return;
+    if (blockIdx.x >> 3 >= per || tile >= total) return;
     const uint32_t band = tile / (8u * n_tiles), high = min(8u, m_tiles - 8u * band), in = tile - band * 8u * n_tiles;
     const int m_tile = static_cast<int>(8u * band + in % high), n_tile = static_cast<int>(in / high);
     int g = 0, r0 = m_tile * G::BM, end = a.rows;
     if (a.offsets) {
-        // the m_tile-th of the experts' row tiles; a lane takes four experts at a time
+        // the expert of the m_tile-th
         int before = 0;
         g = -1;
         for (int base = 0; base < a.groups && g < 0; base += 256) {
-            const int e0 = base + 4 * lane;
-            int64_t edge[5];
-            if (a.offsets_dt == SANDY_I32) {
-#pragma unroll
-                for (int i = 0; i < 5; i++) edge[i] = static_cast<const int32_t*>(a.offsets)[min(e0 + i, a.groups)];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 5; i++) edge[i] = static_cast<const int64_t*>(a.offsets)[min(e0 + i, a.groups)];
-            }
-            int tiles[4], mine = 0;
-            bool bad = false;
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const bool in_order = edge[i] >= 0 && edge[i + 1] >= edge[i] && edge[i + 1] <= a.rows;
-                bad |= !in_order;
-                mine += tiles[i] = in_order ? static_cast<int>((edge[i + 1] - edge[i] + G::BM - 1) / G::BM) : 0;
-            }
-            if (bad) atomicOr(a.errw, static_cast<uint32_t>(SANDY_DEVERR_OFFSETS));
-            int upto = mine;
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const int below = __shfl_up(upto, s, 64);
-                if (lane >= s) upto += below;
-            }
+            if (a.groups > 256) upto = count(base);
             const uint64_t here = __ballot(before + upto > m_tile);
             if (here) {
                 const int l = __builtin_ctzll(here);
-                int at = before + upto - mine, found = 0, first = 0, past = 0;
+                int at = before + upto - mine_tiles, found = 0, first = 0, past = 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const bool in = m_tile >= at && m_tile < at + tiles[i];
-                    found = in ? e0 + i : found;
+                    found = in ? base + 4 * lane + i : found;
                     first = in ? static_cast<int>(edge[i]) + (m_tile - at) * G::BM : first;
                     past = in ? static_cast<int>(edge[i + 1]) : past;
                     at += tiles[i];
@@ -124,7 +139,7 @@ __global__ __launch_bounds__(128 * PN * SPLIT, 1) void quant_tile_kernel(QuantGe
             }
             before += __shfl(upto, 63, 64);
         }
-        if (g < 0) return;
+        if (g < 0 || r0 < 0 || r0 >= end) return;  // (the latter where offsets are out of order)
         g = __builtin_amdgcn_readfirstlane(g);
         r0 = __builtin_amdgcn_readfirstlane(r0);
         end = __builtin_amdgcn_readfirstlane(end);

@@ -1,6 +1,8 @@
 // quant_tile.hip -- launches of the kernel for many rows of the products of matrices in 8 bits.
 #include "quant_tile.h"
 
+#include <algorithm>
+
 namespace sandy_hip {
 
 namespace {
@@ -9,8 +11,9 @@ template <typename T, int WM, int WN, int PN, int STAGES, int SPLIT>
 int launch(const QuantGemm& a, Err e, hipStream_t s) {
     using G = QuantTile<WM, WN, PN, STAGES, SPLIT>;
     constexpr int kBytes = G::template lds<T>();
-    // row tiles: those of the experts are not known here, at most one more each than their rows fill
-    const int64_t m = (a.rows + G::BM - 1) / G::BM + (a.offsets ? a.groups - 1 : 0), n = (a.n + G::BN - 1) / G::BN;
+    // row tiles: of the experts, not known here, at most one each that has a row and one more for every BM further rows
+    const int64_t some = std::min<int64_t>(a.rows, a.groups), n = (a.n + G::BN - 1) / G::BN;
+    const int64_t m = a.offsets ? some + (a.rows - some) / G::BM : (a.rows + G::BM - 1) / G::BM;
     if (m * n > (int64_t{1} << 28)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
     const auto kernel = quant_tile_kernel<T, WM, WN, PN, STAGES, SPLIT>;
     SANDY_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes), e, "quant tile");
