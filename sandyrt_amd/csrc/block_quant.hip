@@ -208,7 +208,7 @@ extern "C" int sandy_hip_block_quant(const SandyTensor* x, int64_t block_rows, c
     if (numel(*x) == 0) return ok(e);
     if (!x->data) return fail(e, SANDY_ERR_INVALID, "block_quant x is null");
     const int64_t units = m.batch * scale_rows * m.blocks;
-    if (units > UINT32_MAX / 256) return fail(e, SANDY_ERR_UNSUPPORTED, "block_quant of too many blocks");
+    if (units > UINT32_MAX / (block_rows == 1 ? 16 : 256)) return fail(e, SANDY_ERR_UNSUPPORTED, "block_quant of too many blocks");
     BlockArgs a = block_args(m);
     a.x = base_ptr(*x);
     const int r = x->rank;
@@ -232,7 +232,7 @@ extern "C" int sandy_hip_block_dequant(const SandyTensor* payload, const SandyTe
     if (numel(*out) == 0) return ok(e);
     if (!out->data) return fail(e, SANDY_ERR_INVALID, "block_dequant out is null");
     const int64_t units = m.batch * m.rows * m.blocks;
-    if (units > UINT32_MAX / 256) return fail(e, SANDY_ERR_UNSUPPORTED, "block_dequant of too many blocks");
+    if (units > UINT32_MAX / 16) return fail(e, SANDY_ERR_UNSUPPORTED, "block_dequant of too many blocks");
     BlockArgs a = block_args(m);
     a.out = base_ptr(*out);
     a.units = static_cast<uint32_t>(units);

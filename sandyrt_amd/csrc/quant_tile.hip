@@ -14,7 +14,7 @@ int launch(const QuantGemm& a, Err e, hipStream_t s) {
     // row tiles: of the experts, not known here, at most one each that has a row and one more for every BM further rows
     const int64_t some = std::min<int64_t>(a.rows, a.groups), n = (a.n + G::BN - 1) / G::BN;
     const int64_t m = a.offsets ? some + (a.rows - some) / G::BM : (a.rows + G::BM - 1) / G::BM;
-    if (m * n > (int64_t{1} << 28)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
+    if (m * n > (int64_t{1} << 22)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
     const auto kernel = quant_tile_kernel<T, WM, WN, PN, STAGES, SPLIT>;
     SANDY_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes), e, "quant tile");
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((m * n + 7) / 8 * 8)), dim3(SPLIT * G::kThreads), kBytes, s, a, static_cast<int>(m), static_cast<int>(n));

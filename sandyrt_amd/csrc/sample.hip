@@ -998,9 +998,13 @@ struct Plan {
 // 32000 61 to 121 us, in parts 63 to 91; 16 rows 31 to 62, 18 to 31 (weights alone, and top-p).
 bool by_rows(int64_t vocab) { return vocab <= kRowVocab; }
 
+// Rows in parts are done so many at a time, which fill the chip, and the workspace is that of no more.
+constexpr int64_t kSlab = 1024;
+
 Plan plan_of(int64_t rows, int64_t vocab) {
     Plan p{};
     if (by_rows(vocab)) return p;
+    rows = std::min(rows, kSlab);
     const int64_t chunks = (vocab + kChunk - 1) / kChunk;
     auto split = [&](int64_t most, int32_t* parts, int32_t* per) {
         const int64_t want = std::max<int64_t>(std::min<int64_t>({most, chunks, kParts}), 1);
@@ -1039,17 +1043,30 @@ int check_logits(const SandyTensor* logits, Err e) {
 }
 
 template <typename T>
-int launch_sample(const SampleArgs& a, Err e, hipStream_t s) {
-    const dim3 rows(static_cast<unsigned>(a.rows));
-    if (by_rows(a.vocab)) {
-        hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(kThreads), 0, s, a);
-    } else {
+int launch_sample(SampleArgs a, Err e, hipStream_t s) {
+    const int64_t all = a.rows, slab = by_rows(a.vocab) ? all : kSlab;
+    for (int64_t first = 0; first < all; first += slab) {
+        a.rows = static_cast<int32_t>(std::min(slab, all - first));
+        const dim3 rows(static_cast<unsigned>(a.rows));
+        if (by_rows(a.vocab)) {
+            hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(kThreads), 0, s, a);
+            continue;
+        }
         const dim3 parts(static_cast<unsigned>(a.rows) * a.parts), peaks(static_cast<unsigned>(a.rows) * a.peak_parts);
         hipLaunchKernelGGL(sample_peak_kernel<T>, peaks, dim3(256), 0, s, a);
         hipLaunchKernelGGL(sample_bins_kernel<T>, parts, dim3(256), 0, s, a);
         hipLaunchKernelGGL(sample_cut_kernel, rows, dim3(kThreads), 0, s, a);
         hipLaunchKernelGGL(sample_gather_kernel<T>, parts, dim3(256), 0, s, a);
         hipLaunchKernelGGL(sample_draw_kernel<T>, rows, dim3(kThreads), 0, s, a);
+        auto next = [](auto*& p, int64_t bytes) {
+            if (p) p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(reinterpret_cast<uintptr_t>(p) + bytes);
+        };
+        auto index = [](int32_t dt) { return dt == SANDY_I32 ? 4 : 8; };
+        next(a.logits, slab * a.stride * static_cast<int64_t>(sizeof(typename Vec8<T>::elem)));
+        for (const float** p : {&a.temperature, &a.top_p, &a.min_p, &a.uniforms}) next(*p, slab * 4);
+        next(a.top_k, slab * index(a.top_k_dt));
+        next(a.ids, slab * index(a.ids_dt));
+        next(a.probs, slab * 4);
     }
     SANDY_HIP_TRY(hipGetLastError(), e, "sample launch");
     return ok(e);

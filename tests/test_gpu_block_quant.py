@@ -272,3 +272,49 @@ def test_products_on_other_streams_and_in_graphs():
         for a, b in zip(got, want_now):
             assert torch.equal(a, b)
     assert all(torch.equal(a, b) for a, b in zip(other, want))
+
+
+# the kernel for few rows, and the tile forms of the one for many
+@pytest.mark.parametrize("form", range(7))
+def test_every_form(form, monkeypatch):
+    monkeypatch.setenv("SANDY_QUANT_FORM", str(form))
+    rng = np.random.default_rng(form)
+    for rows, n, k in ((1, 1, 1), (5, 70, 129), (70, 200, 1000), (130, 300, 128 * 17), (260, 257, 128 * 33 + 5), (300, 520, 40)):
+        x, w = R.whole(rng, (rows, k), 1), R.whole(rng, (n, k), 128)
+        want = product(x, w)
+        same(ops.quant_linear(x, w, dtype=torch.float32), want, torch.float32)
+        same(ops.quant_linear(x, w), want, torch.bfloat16)
+    for counts in ([0, 3, 0, 1], [70, 0, 1, 300], [2] * 300, [0] * 270 + [65, 0, 130, 1]):
+        x, w = R.whole(rng, (sum(counts), 300), 1), R.whole(rng, (len(counts), 70, 300), 128)
+        want = grouped(x, counts, w)
+        same(ops.quant_moe_matmul(x, offsets_of(counts), w, dtype=torch.float32), want, torch.float32)
+        same(ops.quant_moe_matmul(x, offsets_of(counts, torch.int32), w), want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("form", range(7))
+def test_offsets_past_32_bits(form, monkeypatch):
+    """Rows of x, of the weight and of out so far apart that theirs pass 2^32."""
+    monkeypatch.setenv("SANDY_QUANT_FORM", str(form))
+    rng = np.random.default_rng(form + 10)
+    rows, n, k, far = 1100, 1200, 200, 1 << 22
+    near, held = R.whole(rng, (rows, k), 1), R.whole(rng, (n, k), 128)
+
+    def apart(q):
+        wide = torch.empty(q.payload.shape[0], far, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[:, :k]
+        wide.view(torch.uint8).copy_(q.payload.view(torch.uint8))
+        return ops.QuantMatrix(wide, q.scales)
+
+    out = torch.empty(rows, far, dtype=torch.bfloat16, device="cuda")[:, :n]
+    ops.quant_linear(apart(near), apart(held), out=out)
+    same(out, product(near, held), torch.bfloat16)
+
+
+def test_more_than_2_24_blocks():
+    x = torch.randn((1 << 24) + 5, 1, device="cuda")
+    q = ops.block_quant(x)
+    back = ops.block_dequant(q, torch.float32)
+    for a in range(0, x.shape[0], 1 << 22):
+        part = ops.block_quant(x[a:a + (1 << 22)])
+        assert torch.equal(q.payload[a:a + (1 << 22)].view(torch.uint8), part.payload.view(torch.uint8))
+        assert torch.equal(q.scales[a:a + (1 << 22)], part.scales)
+        assert torch.equal(back[a:a + (1 << 22)], ops.block_dequant(part, torch.float32))

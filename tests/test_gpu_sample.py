@@ -176,3 +176,25 @@ def test_streams_and_graphs():
             torch.cuda.synchronize()
             assert torch.equal(out[0], now[0]) and torch.equal(out[1], now[1])
     assert torch.equal(other[0], want[0]) and torch.equal(other[1], want[1])
+
+
+def test_more_rows_than_are_done_at_a_time():
+    rng = np.random.default_rng(7)
+    rows, vocab = 2100, 9000
+    x = torch.full((rows, vocab + 3), -np.inf)
+    for r in range(rows):
+        x[r, rng.integers(0, vocab, 12)] = torch.from_numpy(3 * rng.standard_normal(12)).float()
+    s = settings(rng, rows)
+    for index in (torch.int32, torch.int64):
+        check(x.cuda()[:, :vocab], rng.random(rows, np.float32), **s, k_dtype=index, index_dtype=index)
+
+
+def test_largest_vocabulary():
+    """Ids of 24 bits, at either end and where parts meet."""
+    vocab = 1 << 24
+    at = torch.tensor([0, 1, 262143, 262144, 1 << 23, vocab - 2, vocab - 1])
+    for dtype in (torch.float32, torch.bfloat16):
+        x = torch.full((2, vocab), -np.inf, dtype=dtype)
+        x[:, at] = torch.tensor([1.0, 0.5, 0.5, -1.0, 1.0, 0.25, 1.0], dtype=dtype)
+        for u in (0.0, 0.4, 0.7, 1 - 2.0 ** -24):
+            check(x.cuda(), [u] * 2, k=[0, 5], p=[1.0, 0.9])
