@@ -69,6 +69,8 @@ struct Cut {
         return (bin <= limit) & ((bin == k_bin) | ((bin >= first) & (bin <= last)) | ((bin >= m_first) & (bin <= m_last)));
     }
     __device__ bool listed_in(int bin, int b0, int b1) const { return (bin >= b0) & (bin <= b1) & in_question(bin); }
+    // the logits between which all listed ones lie
+    __device__ void logits(const Row& r, float* low, float* high) const;
     // whether a token of this bin and place stays, as far as top_k and top_p go
     __device__ bool keeps(int bin, uint64_t place, uint64_t last_place) const { return (bin < sure) | (in_question(bin) & (place <= last_place)); }
 };
@@ -235,6 +237,22 @@ __device__ __forceinline__ int bin_of(const Row& r, float l) {
     return at >= static_cast<float>(kBins - 1) ? kBins - 1 : bin;
 }
 
+// The logits between which all tokens of bins b0 .. b1 lie, a little widened: bins are rounded.
+__device__ __forceinline__ void logits_of_bins(const Row& r, int b0, int b1, float* low, float* high) {
+    const double most = r.max, wide = 1.0 / r.scale, edge = 1e-6 * fabs(most);
+    const bool all = !(fabs(most) < 3.0e38) || r.scale == 0.0f;
+    *high = b0 <= 0 || all ? r.max : static_cast<float>(most - b0 * wide * (1 - 1e-6) + edge);
+    *low = b1 >= kBins - 2 || all ? -__builtin_inff() : static_cast<float>(most - (b1 + 1) * wide * (1 + 1e-6) - edge);
+}
+
+__device__ __forceinline__ void Cut::logits(const Row& r, float* low, float* high) const {
+    int b0 = kBins, b1 = -1;
+    if (k_bin >= 0) b0 = b1 = k_bin;
+    if (first <= last) b0 = min(b0, first), b1 = max(b1, last);
+    if (m_first <= m_last) b0 = min(b0, m_first), b1 = max(b1, m_last);
+    logits_of_bins(r, b0, min(b1, limit), low, high);
+}
+
 // p * w rounded up or down, exactly; 0 <= p < 1
 __device__ __forceinline__ uint64_t part_of(float p, uint64_t w, bool up) {
     const uint32_t u = __float_as_uint(p), e = u >> 23, m = e ? (u & 0x7fffffu) | 0x800000u : u & 0x7fffffu;
@@ -394,44 +412,21 @@ __device__ __forceinline__ Cut find_cuts(const Row& r, const uint32_t (&c)[kPer]
 
 // ------------------------------------------------------------------ narrowing down
 struct NarrowShared {
-    uint64_t bin_weights[kBins], waves64[kWaves], lows[kWaves], highs[kWaves], places[64], weights[64];
+    uint64_t bin_weights[kBins], waves64[kWaves], places[64], weights[64];
     uint64_t lo, hi, weight_before;
     uint32_t bin_counts[kBins], waves32[kWaves], count_before, n;
 };
 
-// Of the tokens that each(f) names as f(place, weight), in rank order: the place of the one with which they become `rank`,
-// or (rank 0) with which their weights reach `weight`, the first token reaching 0; the last of all if they never do.
-// sh.weight_before is then the sum up to and with it.
+// Of the tokens that each(f) names as f(place, weight), at most `most` and from `low` to `high`, in rank order: the place of
+// the one with which they become `rank`, or (rank 0) with which their weights reach `weight`, the first token reaching 0;
+// no less than the last of all if they never do.  sh.weight_before is then the sum up to and with it.
 template <typename Each>
-__device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint64_t weight, Each each) {
+__device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint64_t weight, uint32_t most, uint64_t low, uint64_t high, Each each) {
     const int tid = threadIdx.x;
-    uint64_t low = ~uint64_t{0}, high = 0;
-    uint32_t n = 0;
-    each([&](uint64_t place, uint64_t) {
-        low = min(low, place);
-        high = max(high, place);
-        n++;
-    });
-#pragma unroll
-    for (int m = 32; m >= 1; m >>= 1) {
-        low = min(low, static_cast<uint64_t>(__shfl_xor(low, m, 64)));
-        high = max(high, static_cast<uint64_t>(__shfl_xor(high, m, 64)));
-    }
-    if ((tid & 63) == 0) sh.lows[tid >> 6] = low, sh.highs[tid >> 6] = high;
     uint32_t tokens;
-    block_scan<kWaves>(n, sh.waves32, &tokens);
-    if (tid < 64) {
-        low = sh.lows[tid & (kWaves - 1)];
-        high = sh.highs[tid & (kWaves - 1)];
-#pragma unroll
-        for (int m = kWaves / 2; m >= 1; m >>= 1) {
-            low = min(low, static_cast<uint64_t>(__shfl_xor(low, m, 64)));
-            high = max(high, static_cast<uint64_t>(__shfl_xor(high, m, 64)));
-        }
-        if (tid == 0) sh.lo = low, sh.hi = high, sh.weight_before = 0, sh.count_before = 0, sh.n = tokens;
-    }
+    if (tid == 0) sh.lo = low, sh.hi = high, sh.weight_before = 0, sh.count_before = 0, sh.n = most;
     __syncthreads();
-    while (sh.n > 64) {  // each round is among fewer than before: a step of 1024
+    while (sh.n > 64) {  // a step of 1024 of the last one
         const uint64_t from = sh.lo, to = sh.hi;
         const int shift = max(0, 54 - __builtin_clzll((to - from) | 1));
 #pragma unroll
@@ -479,7 +474,6 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
     }
     // the last few: each with each
     const uint64_t from = sh.lo, to = sh.hi;
-    const uint32_t few = sh.n;
     __syncthreads();
     if (tid == 0) sh.n = 0;
     __syncthreads();
@@ -490,6 +484,7 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
         sh.weights[i] = w;
     });
     __syncthreads();
+    const uint32_t few = sh.n;
     if (tid < 64) {
         const bool in = tid < few;
         if (!in) sh.places[tid] = ~uint64_t{0}, sh.weights[tid] = 0;
@@ -515,9 +510,9 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
 }
 
 // The last place that top_k and top_p keep: ~0 where no listed token is cut by them.  each(b0, b1, f) names the listed
-// tokens of bins b0 .. b1; up_to(bin): the row's weight up to and with a bin.
+// tokens of bins b0 .. b1, `most` of all; up_to(bin): the row's weight up to and with a bin.
 template <typename Each, typename UpTo>
-__device__ __forceinline__ uint64_t last_place(const Row& r, const Cut& cut, NarrowShared& sh, Each each, UpTo up_to) {
+__device__ __forceinline__ uint64_t last_place(const Row& r, const Cut& cut, NarrowShared& sh, uint32_t most, Each each, UpTo up_to) {
     uint64_t last = ~uint64_t{0}, kept = cut.weight;  // top_k's
     const bool small = r.small();
 #pragma unroll 1
@@ -541,7 +536,9 @@ __device__ __forceinline__ uint64_t last_place(const Row& r, const Cut& cut, Nar
                 b0 = b1 = bin;
             }
         }
-        const uint64_t place = narrow(sh, rank, weight, [&](auto f) { each(b0, b1, f); });
+        float low, high;
+        logits_of_bins(r, b0, min(b1, cut.limit), &low, &high);
+        const uint64_t place = narrow(sh, rank, weight, most, place_of(high, 0), place_of(low, 0xffffff), [&](auto f) { each(b0, b1, f); });
         last = min(last, place);
         if (step == 0) kept += sh.weight_before;
         __syncthreads();
@@ -667,7 +664,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
             }
             each_of_row<T>(a, at, r, cut, b0, b1, f);
         };
-        last = last_place(r, cut, sh.narrow, each, [&](int bin) { return sh.up_to[bin]; });
+        last = last_place(r, cut, sh.narrow, listed, each, [&](int bin) { return sh.up_to[bin]; });
     }
     // kept weights of eight tokens, and their sums over each wave's part of a block
     auto kept = [&](const float (&v)[8], int first, uint64_t (&w)[8]) {
@@ -836,20 +833,6 @@ __global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleArgs a) {
     }
 }
 
-// The logits between which all tokens in question lie, a little widened: bins are rounded.
-__device__ __forceinline__ void logits_in_question(const Row& r, const Cut& cut, float* low, float* high) {
-    int b0 = kBins, b1 = -1;
-    if (cut.k_bin >= 0) b0 = b1 = cut.k_bin;
-    if (cut.first <= cut.last) b0 = min(b0, cut.first), b1 = max(b1, cut.last);
-    if (cut.m_first <= cut.m_last) b0 = min(b0, cut.m_first), b1 = max(b1, cut.m_last);
-    b1 = min(b1, cut.limit);
-    const double most = r.max, wide = 1.0 / r.scale, edge = 1e-6 * fabs(most);  // (no scale: all tokens)
-    const bool finite = fabs(most) < 3.0e38;
-    *high = b0 <= 0 || !finite ? __builtin_inff() : static_cast<float>(most - b0 * wide * (1 - 1e-6) + edge);
-    *low = b1 >= kBins - 2 || !finite || r.scale == 0.0f ? -__builtin_inff()
-                                                                       : static_cast<float>(most - (b1 + 1) * wide * (1 + 1e-6) - edge);
-}
-
 // Lists the tokens in question, and sums up what a part keeps for sure from its bins.  A part lists its tokens in LDS,
 // takes as many places of the row's list at once and copies them there; what LDS has no room for goes there by itself.
 template <typename T>
@@ -866,7 +849,7 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
     for (int i = threadIdx.x; i < min(cut.sure, kBins); i += 256) sum += a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i];
     if (threadIdx.x == 0) found = 0;
     float low, high;
-    logits_in_question(r, cut, &low, &high);
+    cut.logits(r, &low, &high);
     block_scan<4>(sum, waves, &total);
     part_tokens<T, 4>(a, at, part * a.per * kChunk, min((part + 1) * a.per * kChunk, a.vocab), [&](const float (&v)[8], int first) {
 #pragma unroll
@@ -934,7 +917,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
             }
             each_of_row<T>(a, at, r, cut, b0, b1, f);
         };
-        last = last_place(r, cut, sh.narrow, each, [&](int bin) { return a.upto[static_cast<int64_t>(row) * kBins + bin]; });
+        last = last_place(r, cut, sh.narrow, listed, each, [&](int bin) { return a.upto[static_cast<int64_t>(row) * kBins + bin]; });
         // the listed tokens that are kept join their parts' weights
         each(cut.sure, kBins, [&](uint64_t place, uint64_t w) {
             if (place > last) return;
@@ -966,13 +949,20 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] = next[j];
         load_tokens<T>(a, at, first + kBlock, next);
-        weigh(r, v, false, w);
+        bool in[8], any = false;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            // (a select of values: zeroed in branches, elements of this array kept their old values with hipcc 7.2)
-            const bool in = (first + j < end) & cut.keeps(bin_of(r, v[j]), place_of(v[j], first + j), last);
-            w[j] = in ? w[j] : 0;
-            sum += w[j];
+        for (int j = 0; j < 8; j++) any |= in[j] = (first + j < end) & cut.keeps(bin_of(r, v[j]), place_of(v[j], first + j), last);
+        if (__any(any)) {
+            weigh(r, v, false, w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                // (a select of values: zeroed in branches, elements of this array kept their old values with hipcc 7.2)
+                w[j] = in[j] ? w[j] : 0;
+                sum += w[j];
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = 0;
         }
         uint64_t all;
         uint64_t to = run + block_scan<kWaves>(sum, sh.waves64, &all) - sum;
