@@ -101,7 +101,9 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 }
 
 // Which kernel, from how many tiles there are for 256 CUs (us, bf16 outputs, rows x columns x k).  One workgroup a CU leaves
-// most of it idle, so few tiles are made smaller and their k is split between two groups of waves:
+// most of it idle, so few tiles are made smaller and their k is split between two groups of waves, or four:
+//   64 x 4096 x 4096     32 x 32 split 8.2, 64 x 64 split 11     64 x 1024 x 8192  10.5 against 18    64 x 2048 x 5632  9.1, 14
+//   128 x 4096 x 4096    32 x 32 split 10.8, 64 x 64 split 11.2  16 x 11264 x 2048  9.3 against 8.8   64 x 11264 x 2048  14.5, 9.6
 //   333 x 1999 x 5617    64 x 64 split 15.8, 64 x 128 whole 26, 128 x 128 whole 34, 256 x 256 84
 //   128 x 11264 x 2048   64 x 128 split 11.9, whole 13.5, 64 x 64 split 14
 //   1024 x 4096 x 4096   128 x 128 split 23.5, whole 27, 256 x 256 46
@@ -109,7 +111,7 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 //   1024 x 11264 x 2048  29.5 against 35   2048 x 11264 x 2048  59 against 52   4096 x 4096 x 4096  57 against 69
 //   4096 x 8192 x 8192   202 against 262
 // Few rows: the stream of the weight.  Every workgroup reads x for 16 columns, so that more rows and many columns are for tiles:
-//   1 x 11264 x 2048     7.2, 64 x 64 split 8.7      16 x 4096 x 4096   7.8 against 10.6    16 x 8192 x 8192  24 against 26
+//   1 x 11264 x 2048     7.2, 64 x 64 split 8.7      16 x 2048 x 2048  5.4, 32 x 32 split 5.9    16 x 8192 x 8192  24 against 16
 //   1 x 28672 x 8192     52, 64 x 128 split 62       4 x 16384 x 4096   19 against 17       1 x 32000 x 2048  18.3, 64 x 128 15.2
 // Many columns for a row of tiles, split where k is long: 64 x 128 split and whole
 //   8 x 65536 x 2048     32 and 28                   8 x 152064 x 4096  116 and 138
@@ -123,8 +125,10 @@ QuantForm form_of(const QuantGemm& a) {
     const int64_t some = std::min<int64_t>(a.groups, a.rows), rows = (a.rows + some - 1) / some;
     auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * some * ((a.n + n - 1) / n); };
     const int64_t least = tiles(64, 64), streams = int64_t{a.groups} * ((a.n + 15) / 16);
-    const int64_t few = a.offsets ? (streams <= 4096 ? 2 : 0) : least <= 128 ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0;
+    const int64_t alone = least <= 128 && a.blocks < 64 ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0;
+    const int64_t few = a.offsets ? (streams <= 4096 ? 2 : 0) : alone;
     if (rows <= few) return QuantForm::kStream;
+    if (tiles(32, 32) <= (a.blocks >= 32 ? 512 : 256)) return QuantForm::k32x32Split;
     if (least <= 256) return QuantForm::k64x64Split;
     if (a.offsets) {
         if (rows > 32 && tiles(128, 128) >= 512) return QuantForm::k128x128;

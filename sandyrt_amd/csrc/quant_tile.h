@@ -6,7 +6,7 @@
 
 namespace sandy_hip {
 
-// Workgroup tile 64 WM x 32 PN WN of rows x columns, 2 x PN waves of 32 WM x 32 WN on 32 x 32 instructions, 128 columns
+// Workgroup tile 32 PM WM x 32 PN WN of rows x columns, PM x PN waves of 32 WM x 32 WN on 32 x 32 instructions, 128 columns
 // of k (a block, a whole 128-byte line of every row) a chunk, STAGES chunks in LDS.  SPLIT groups of so many waves share the
 // chunks, a run each, and add up their sums at the end.
 //
@@ -14,10 +14,10 @@ namespace sandy_hip {
 // 8 chunks under way and one meeting a chunk in place of two.  A chunk of a 64 x 64 tile takes them 480 cycles for 64 a wave
 // of products, one of 128 x 128 960 for 512 of two workgroups, one of 256 x 256 1900 for 2048, so that large tiles are bound
 // by both (2720 TFLOP/s at 4096 x 8192 x 8192) and small ones by copies: 333 x 1999 x 5617 in 22 us, where each workgroup
-// waits at every meeting, and 15.8 with SPLIT, whose groups wait for each other's copies; a third and fourth gain nothing.
-template <int WM, int WN, int PN, int STAGES, int SPLIT>
+// waits at every meeting, and 15.8 with SPLIT 2, whose groups wait for each other's copies; 4 gain nothing there.
+template <int WM, int WN, int PM, int PN, int STAGES, int SPLIT>
 struct QuantTile {
-    static constexpr int BM = 64 * WM, BN = 32 * PN * WN, kThreads = 128 * PN;
+    static constexpr int BM = 32 * PM * WM, BN = 32 * PN * WN, kThreads = 64 * PM * PN;
     static constexpr int kX = BM * 128, kStage = (BM + BN) * 128;
     // the scale bytes of 16 blocks of every row, twice, behind the stages
     static constexpr int kScales = STAGES * kStage, kScaleBytes = (BM + BN) * 16;
@@ -58,15 +58,15 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <typename T, int WM, int WN, int PN, int STAGES, int SPLIT>
-__global__ __launch_bounds__(128 * PN * SPLIT, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
-    using G = QuantTile<WM, WN, PN, STAGES, SPLIT>;
+template <typename T, int WM, int WN, int PM, int PN, int STAGES, int SPLIT>
+__global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
+    using G = QuantTile<WM, WN, PM, PN, STAGES, SPLIT>;
     constexpr bool kScaled = std::is_same_v<T, BF16>;
     extern __shared__ __align__(1024) unsigned char all_lds[];
     const int lane = threadIdx.x & 63, waves = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    const int group = waves / (2 * PN), wave = waves - group * 2 * PN, tid = 64 * wave + lane;
+    const int group = waves / (PM * PN), wave = waves - group * PM * PN, tid = 64 * wave + lane;
     unsigned char* const lds = all_lds + group * G::template group_lds<T>();
-    const int wm = wave & 1, wn = wave >> 1;
+    const int wm = wave % PM, wn = wave / PM;
     const int col = lane & 31, half = lane >> 5;
 
     // experts' row tiles: a lane takes four experts from `base` on, up to whose end there are `upto` more than before base
@@ -162,17 +162,19 @@ __global__ __launch_bounds__(128 * PN * SPLIT, 1) void quant_tile_kernel(QuantGe
         return r;
     };
     const i32x4_t xres = buffer(xbase, (xrows - 1) * a.x_pitch + k16), wres = buffer(wbase, (wrows - 1) * a.w_pitch + k16);
-    const int prow = tid >> 3, slot = tid & 7, piece = slot ^ ((prow >> 1) & 7);
+    const int prow = tid >> 3, slot = tid & 7;
+    auto piece = [&](int i) { return slot ^ (((G::kStep * i + prow) >> 1) & 7); };  // (the same for all i from 16 rows a step on)
     int from[G::kLoads];
 #pragma unroll
     for (int i = 0; i < G::kLoads; i++) {
         const bool is_x = i < G::kXLoads;
         const int r = G::kStep * (is_x ? i : i - G::kXLoads) + prow;
-        from[i] = static_cast<int>(min(r, (is_x ? xrows : wrows) - 1) * (is_x ? a.x_pitch : a.w_pitch)) + 16 * piece;
+        from[i] = static_cast<int>(min(r, (is_x ? xrows : wrows) - 1) * (is_x ? a.x_pitch : a.w_pitch)) + 16 * piece(i);
     }
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) unsigned char*)lds));
     auto copy = [&](int c, int stage, int i) {
-        copy_to_lds(i < G::kXLoads ? xres : wres, from[i], c * 128, lds0 + stage * G::kStage + wave * 1024 + i * (16 * G::kThreads));
+        const uint32_t to = lds0 + stage * G::kStage + wave * 1024 + i * (16 * G::kThreads);
+        copy_to_lds(i < G::kXLoads ? xres : wres, from[i], __builtin_amdgcn_readfirstlane(c * 128), __builtin_amdgcn_readfirstlane(to));
     };
     // The group's whole blocks are first .. first + mine - 1, of all groups' `turns` turns; those past the last are the last
     // again, copied and never read: every round waits for the same number.
@@ -296,17 +298,17 @@ __global__ __launch_bounds__(128 * PN * SPLIT, 1) void quant_tile_kernel(QuantGe
     if (rest) {
         // the last block of a k that is no multiple of 128 goes first, through registers: bytes past k are 0 (all of them
         // for groups but the first)
-        const int left = (group ? 0 : rest) - 16 * piece;
+        const int left = group ? 0 : rest;
         i32x4_t v[G::kLoads];
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
             v[i] = i32x4_t{0, 0, 0, 0};
-            if (left > 0) v[i] = *reinterpret_cast<const i32x4_t*>((i < G::kXLoads ? xbase : wbase) + (static_cast<uint32_t>(from[i]) + chunks * 128));
+            if (left > 16 * piece(i)) v[i] = *reinterpret_cast<const i32x4_t*>((i < G::kXLoads ? xbase : wbase) + (static_cast<uint32_t>(from[i]) + chunks * 128));
         }
 #pragma unroll
         for (int i = 0; i < G::kLoads; i++) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[i][j] &= static_cast<int>(first_bytes(left - 4 * j));
+            for (int j = 0; j < 4; j++) v[i][j] &= static_cast<int>(first_bytes(left - 16 * piece(i) - 4 * j));
             *reinterpret_cast<i32x4_t*>(lds + (STAGES - 1) * G::kStage + i * (16 * G::kThreads) + tid * 16) = v[i];
         }
 #pragma unroll

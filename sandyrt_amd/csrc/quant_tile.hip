@@ -7,15 +7,15 @@ namespace sandy_hip {
 
 namespace {
 
-template <typename T, int WM, int WN, int PN, int STAGES, int SPLIT>
+template <typename T, int WM, int WN, int PM, int PN, int STAGES, int SPLIT>
 int launch(const QuantGemm& a, Err e, hipStream_t s) {
-    using G = QuantTile<WM, WN, PN, STAGES, SPLIT>;
+    using G = QuantTile<WM, WN, PM, PN, STAGES, SPLIT>;
     constexpr int kBytes = G::template lds<T>();
     // row tiles: of the experts, not known here, at most one each that has a row and one more for every BM further rows
     const int64_t some = std::min<int64_t>(a.rows, a.groups), n = (a.n + G::BN - 1) / G::BN;
     const int64_t m = a.offsets ? some + (a.rows - some) / G::BM : (a.rows + G::BM - 1) / G::BM;
     if (m * n > (int64_t{1} << 22)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
-    const auto kernel = quant_tile_kernel<T, WM, WN, PN, STAGES, SPLIT>;
+    const auto kernel = quant_tile_kernel<T, WM, WN, PM, PN, STAGES, SPLIT>;
     SANDY_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes), e, "quant tile");
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((m * n + 7) / 8 * 8)), dim3(SPLIT * G::kThreads), kBytes, s, a, static_cast<int>(m), static_cast<int>(n));
     SANDY_HIP_TRY(hipGetLastError(), e, "quant tile launch");
@@ -25,12 +25,13 @@ int launch(const QuantGemm& a, Err e, hipStream_t s) {
 template <typename T>
 int launch(const QuantGemm& a, QuantForm form, Err e, hipStream_t s) {
     switch (form) {
-        case QuantForm::k64x64Split: return launch<T, 1, 1, 2, 2, 2>(a, e, s);
-        case QuantForm::k64x128Split: return launch<T, 1, 2, 2, 2, 2>(a, e, s);
-        case QuantForm::k128x128Split: return launch<T, 2, 2, 2, 2, 2>(a, e, s);
-        case QuantForm::k64x128: return launch<T, 1, 2, 2, 2, 1>(a, e, s);
-        case QuantForm::k128x128: return launch<T, 2, 2, 2, 2, 1>(a, e, s);
-        default: return launch<T, 4, 4, 2, 2, 1>(a, e, s);
+        case QuantForm::k32x32Split: return launch<T, 1, 1, 1, 1, 2, 4>(a, e, s);
+        case QuantForm::k64x64Split: return launch<T, 1, 1, 2, 2, 2, 2>(a, e, s);
+        case QuantForm::k64x128Split: return launch<T, 1, 2, 2, 2, 2, 2>(a, e, s);
+        case QuantForm::k128x128Split: return launch<T, 2, 2, 2, 2, 2, 2>(a, e, s);
+        case QuantForm::k64x128: return launch<T, 1, 2, 2, 2, 2, 1>(a, e, s);
+        case QuantForm::k128x128: return launch<T, 2, 2, 2, 2, 2, 1>(a, e, s);
+        default: return launch<T, 4, 4, 2, 2, 2, 1>(a, e, s);
     }
 }
 
