@@ -118,9 +118,10 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 // Experts: as if the rows were spread evenly over as many as may have one, but that their unevenness wants room for more
 // tiles.  A stream has workgroups for the empty ones as well, which cost it from some thousands on (us, experts x columns x k):
 //   2 rows, 8 x 1024 x 4096     stream 6.9, 64 x 64 split 12.4     8 rows, 256 x 2048 x 256    16.7 against 6.7
-//   8 rows, 128 x 2816 x 704    stream 18.6, 64 x 128 11           128 rows, 128 x 2816 x 704  58 against 40
-//   64 rows, 8 x 14336 x 4096   64 x 128 split 102, whole 117      2 times 64 rows, 8 x 4096 x 1024  split 18.7, whole 13.8
-//   64 rows each, 128 x 1408 x 2816 and 2816 x 704   64 x 128 142 and 110, 128 x 128 138 and 98
+//   8 rows, 128 x 2816 x 704    stream 18.6, 64 x 128 11           128 rows, 128 x 2816 x 704  58 against 31
+//   64 rows, 8 x 14336 x 4096   64 x 128 split 106, whole 116      2 times 64 rows, 8 x 4096 x 1024  split 18.7, whole 13.8
+//   64 rows each, 128 x 1408 x 2816 and 2816 x 704   64 x 128 136 and 95, 128 x 128 140 and 97
+//   256 rows each, the same     64 x 128 262 and 224, 128 x 128 232 and 196
 QuantForm form_of(const QuantGemm& a) {
     const int64_t some = std::min<int64_t>(a.groups, a.rows), rows = (a.rows + some - 1) / some;
     auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * some * ((a.n + n - 1) / n); };
@@ -131,7 +132,7 @@ QuantForm form_of(const QuantGemm& a) {
     if (tiles(32, 32) <= (a.blocks >= 32 ? 512 : 256)) return QuantForm::k32x32Split;
     if (least <= 256) return QuantForm::k64x64Split;
     if (a.offsets) {
-        if (rows > 32 && tiles(128, 128) >= 512) return QuantForm::k128x128;
+        if (rows > 64 && tiles(128, 128) >= 512) return QuantForm::k128x128;
         return tiles(64, 128) <= 128 || a.blocks >= 32 ? QuantForm::k64x128Split : QuantForm::k64x128;
     }
     if (tiles(64, 128) <= 256 || (rows <= 64 && a.blocks >= 32)) return QuantForm::k64x128Split;

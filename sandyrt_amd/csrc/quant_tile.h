@@ -19,8 +19,9 @@ template <int WM, int WN, int PM, int PN, int STAGES, int SPLIT>
 struct QuantTile {
     static constexpr int BM = 32 * PM * WM, BN = 32 * PN * WN, kThreads = 64 * PM * PN;
     static constexpr int kX = BM * 128, kStage = (BM + BN) * 128;
-    // the scale bytes of 16 blocks of every row, twice, behind the stages
-    static constexpr int kScales = STAGES * kStage, kScaleBytes = (BM + BN) * 16;
+    // the scale bytes of kRun blocks of every row, twice, behind the stages: 8 for small tiles, so that three workgroups of
+    // 64 x 128 fit a CU (128 rows of 128 experts of 1408 x 2816: 62 us to 53), 16 for large ones (4096 x 8192 x 8192: 212 to 203)
+    static constexpr int kRun = WM * WN < 16 ? 8 : 16, kScales = STAGES * kStage, kScaleBytes = (BM + BN) * kRun;
     static constexpr int kStep = kThreads / 8, kXLoads = BM / kStep, kLoads = (BM + BN) / kStep;  // 16-byte pieces a thread moves a chunk
     template <typename T>
     static constexpr int row_bytes() { return 32 * WN * static_cast<int>(sizeof(typename Vec8<T>::elem)) + 16; }
@@ -34,14 +35,15 @@ struct QuantTile {
     static constexpr int lds() { return SPLIT * group_lds<T>(); }
 };
 
-// Sixteen scale bytes j .. j + 15 of a row, the last for those past it.
-__device__ __forceinline__ i32x4_t sixteen_scales(const uint8_t* row, int j, int blocks) {
-    i32x4_t v{0, 0, 0, 0};
-    if (j + 16 <= blocks) {
-        __builtin_memcpy(&v, row + j, 16);
+// N scale bytes from j on of a row, the last for those past it.
+template <int N>
+__device__ __forceinline__ auto some_scales(const uint8_t* row, int j, int blocks) {
+    int32_t __attribute__((ext_vector_type(N / 4))) v = 0;
+    if (j + N <= blocks) {
+        __builtin_memcpy(&v, row + j, N);
     } else {  // (all at once: loads under a condition each would wait for one another)
 #pragma unroll
-        for (int i = 0; i < 16; i++) v[i >> 2] |= row[min(j + i, blocks - 1)] << (8 * (i & 3));
+        for (int i = 0; i < N; i++) v[i >> 2] |= row[min(j + i, blocks - 1)] << (8 * (i & 3));
     }
     return v;
 }
@@ -206,7 +208,7 @@ __global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(Qua
 #pragma unroll
             for (int i = 0; i < 16; i++) acc[t][c][i] = 0.0f;
 
-    // scale bytes come 16 blocks at a time: a row a thread (or two) from memory, half a segment ahead, through LDS to the
+    // scale bytes come a run of blocks at a time: a row a thread (or two) from memory, half a segment ahead, through LDS to the
     // lanes that multiply with them
     const uint8_t* xsbase = a.xs + static_cast<int64_t>(r0) * a.blocks;
     const uint8_t* wsbase = a.ws + static_cast<int64_t>(g) * a.w_scale_rows * a.blocks;
@@ -215,25 +217,26 @@ __global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(Qua
                          : wsbase + static_cast<int64_t>((n0 + min(r - G::BM, wrows - 1)) >> a.w_shift) * a.blocks;
     };
     constexpr int kScaleRows = (G::BM + G::BN + G::kThreads - 1) / G::kThreads;
-    i32x4_t held[kScaleRows];
+    constexpr int kRun = G::kRun;
+    decltype(some_scales<kRun>(nullptr, 0, 0)) held[kScaleRows];
     auto load_scales = [&](int at) {
 #pragma unroll
         for (int u = 0; u < kScaleRows; u++)
-            if (G::kThreads * u + tid < G::BM + G::BN) held[u] = sixteen_scales(scale_row(G::kThreads * u + tid), first + at, a.blocks);
+            if (G::kThreads * u + tid < G::BM + G::BN) held[u] = some_scales<kRun>(scale_row(G::kThreads * u + tid), first + at, a.blocks);
     };
     auto store_scales = [&](int at) {
 #pragma unroll
         for (int u = 0; u < kScaleRows; u++)
             if (G::kThreads * u + tid < G::BM + G::BN)
-                *reinterpret_cast<i32x4_t*>(lds + G::kScales + ((at >> 4) & 1) * G::kScaleBytes + (G::kThreads * u + tid) * 16) = held[u];
+                *reinterpret_cast<decltype(&held[0])>(lds + G::kScales + (at / kRun & 1) * G::kScaleBytes + (G::kThreads * u + tid) * kRun) = held[u];
     };
     int xs[WM], ws[WN], xs_next[WM], ws_next[WN];
     auto scales = [&](int c) {  // of chunks c .. c + 3, c a multiple of 4
-        const unsigned char* at = lds + G::kScales + ((c >> 4) & 1) * G::kScaleBytes + (c & 12);
+        const unsigned char* at = lds + G::kScales + (c / kRun & 1) * G::kScaleBytes + (c & (kRun - 4));
 #pragma unroll
-        for (int t = 0; t < WM; t++) xs_next[t] = *reinterpret_cast<const int*>(at + (32 * (WM * wm + t) + col) * 16);
+        for (int t = 0; t < WM; t++) xs_next[t] = *reinterpret_cast<const int*>(at + (32 * (WM * wm + t) + col) * kRun);
 #pragma unroll
-        for (int q = 0; q < WN; q++) ws_next[q] = *reinterpret_cast<const int*>(at + (G::BM + 32 * (WN * wn + q) + col) * 16);
+        for (int q = 0; q < WN; q++) ws_next[q] = *reinterpret_cast<const int*>(at + (G::BM + 32 * (WN * wn + q) + col) * kRun);
     };
     auto use_scales = [&] {
 #pragma unroll
@@ -351,8 +354,9 @@ __global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(Qua
                 for (int q = (slot - kLand) * kRead; q < min((slot - kLand + 1) * kRead, kReads); q++) read1(next, 0, q, xf[0], wf[0]);
         };
         multiply(xf[0], wf[0], at_slot);
-        if ((c & 15) == 7) store_scales(c + 9);
-        if ((c & 15) == 6 && first + c + 10 <= last) load_scales(c + 10);
+        constexpr int kLoad = kRun == 8 ? 1 : 6, kStore = kRun == 8 ? 5 : 7;
+        if ((c & (kRun - 1)) == kStore) store_scales(c + kRun - kStore);
+        if ((c & (kRun - 1)) == kLoad && first + c + kRun - kLoad <= last) load_scales(c + kRun - kLoad);
         if ((c & 3) == 3) scales(c + 1);
         multiply(xf[1], wf[1], [&](int i) { at_slot(kTimes + i); });
         stage = next;
