@@ -63,7 +63,7 @@ __device__ __forceinline__ void quant_group_rows(const QuantGemm& a, int g, int*
 }
 
 // The kernel for few rows (quant_linear.hip), or that for many (quant_tile.h) in one of its tile forms.
-enum class QuantForm { kStream, k32x32Split, k64x64Split, k64x128Split, k128x128Split, k64x128, k128x128, k256x256 };
+enum class QuantForm { kStream, k32x32Split, k64x64Split, k64x128Split, k128x128Split, k64x128, k128x128, k192x256, k256x256 };
 int launch_quant_tiles(const QuantGemm& a, bool bf16, QuantForm form, Err e, hipStream_t s);
 
 // The bits of a dword that hold the first n bytes.

@@ -107,9 +107,11 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 //   333 x 1999 x 5617    64 x 64 split 15.8, 64 x 128 whole 26, 128 x 128 whole 34, 256 x 256 84
 //   128 x 11264 x 2048   64 x 128 split 11.9, whole 13.5, 64 x 64 split 14
 //   1024 x 4096 x 4096   128 x 128 split 23.5, whole 27, 256 x 256 46
-// Many tiles: 256 x 256 has half the traffic of 128 x 128, which two a CU come in smaller rounds:
-//   1024 x 11264 x 2048  29.5 against 35   2048 x 11264 x 2048  59 against 52   4096 x 4096 x 4096  57 against 69
-//   4096 x 8192 x 8192   202 against 262
+// Many tiles: 256 x 256 has half the traffic of 128 x 128, which two a CU come in smaller rounds; 192 x 256 (bf16 outputs,
+// for f32's double products it gains nothing) fills rounds that 256 x 256 does not:
+//   128 x 128, 192 x 256, 256 x 256    1024 x 11264 x 2048  36, 48, 30      2048 x 11264 x 2048  55, 52, 60
+//   4096 x 2560 x 2048   31, 26, 30    8192 x 2816 x 2816   71, 65, 77      4096 x 11264 x 2048  99, 102, 96
+//   1500 x 8192 x 4096   61, 47, 50    4096 x 4096 x 4096   70, 81, 57      4096 x 8192 x 8192   266, 237, 204
 // Few rows: the stream of the weight.  Every workgroup reads x for 16 columns, so that more rows and many columns are for tiles:
 //   1 x 11264 x 2048     7.2, 64 x 64 split 8.7      16 x 2048 x 2048  5.4, 32 x 32 split 5.9    16 x 8192 x 8192  24 against 16
 //   1 x 28672 x 8192     52, 64 x 128 split 62       4 x 16384 x 4096   19 against 17       1 x 32000 x 2048  18.3, 64 x 128 15.2
@@ -122,7 +124,7 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 //   64 rows, 8 x 14336 x 4096   64 x 128 split 106, whole 116      2 times 64 rows, 8 x 4096 x 1024  split 18.7, whole 13.8
 //   64 rows each, 128 x 1408 x 2816 and 2816 x 704   64 x 128 136 and 95, 128 x 128 140 and 97
 //   256 rows each, the same     64 x 128 262 and 224, 128 x 128 232 and 196
-QuantForm form_of(const QuantGemm& a) {
+QuantForm form_of(const QuantGemm& a, bool bf16) {
     const int64_t some = std::min<int64_t>(a.groups, a.rows), rows = (a.rows + some - 1) / some;
     auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * some * ((a.n + n - 1) / n); };
     const int64_t least = tiles(64, 64), streams = int64_t{a.groups} * ((a.n + 15) / 16);
@@ -138,14 +140,16 @@ QuantForm form_of(const QuantGemm& a) {
     if (tiles(64, 128) <= 256 || (rows <= 64 && a.blocks >= 32)) return QuantForm::k64x128Split;
     if (rows <= 64) return QuantForm::k64x128;
     if (tiles(128, 128) <= 256) return QuantForm::k128x128Split;
-    // a round of 256 tiles of 256 x 256 takes 1.6 to 1.7 times one of 512 of 128 x 128 (57 and 35 at k = 4096)
-    const double large = 1.7 * static_cast<double>((tiles(256, 256) + 255) / 256), small = static_cast<double>((tiles(128, 128) + 511) / 512);
+    // rounds, of 512 tiles of 128 x 128 and 256 larger ones, in times of the former (36, 47 and 57 us at k = 4096)
+    auto rounds = [&](int64_t count, int64_t at_once) { return static_cast<double>((count + at_once - 1) / at_once); };
+    const double small = rounds(tiles(128, 128), 512), middle = 1.35 * rounds(tiles(192, 256), 256), large = 1.63 * rounds(tiles(256, 256), 256);
+    if (bf16 && middle < std::min(small, large)) return QuantForm::k192x256;
     return large < small ? QuantForm::k256x256 : QuantForm::k128x128;
 }
 
 template <typename T>
 int launch_products(const QuantGemm& a, const char* what, Err e, hipStream_t s) {
-    const QuantForm form = static_cast<QuantForm>(env_int("SANDY_QUANT_FORM", static_cast<int>(form_of(a))));
+    const QuantForm form = static_cast<QuantForm>(env_int("SANDY_QUANT_FORM", static_cast<int>(form_of(a, std::is_same_v<T, BF16>))));
     if (form != QuantForm::kStream) return launch_quant_tiles(a, std::is_same_v<T, BF16>, form, e, s);
     const dim3 grid(static_cast<unsigned>((a.n + 15) / 16), static_cast<unsigned>(a.groups));
     // eight waves where each still has four blocks (1 x 1024 x 8192: 7.6 us against 11.1; 1 x 11264 x 2048: 8.2 against 7.3)

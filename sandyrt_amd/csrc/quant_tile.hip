@@ -31,6 +31,9 @@ int launch(const QuantGemm& a, QuantForm form, Err e, hipStream_t s) {
         case QuantForm::k128x128Split: return launch<T, 2, 2, 2, 2, 2, 2>(a, e, s);
         case QuantForm::k64x128: return launch<T, 1, 2, 2, 2, 2, 1>(a, e, s);
         case QuantForm::k128x128: return launch<T, 2, 2, 2, 2, 2, 1>(a, e, s);
+        case QuantForm::k192x256:
+            if constexpr (std::is_same_v<T, BF16>) return launch<T, 3, 4, 2, 2, 2, 1>(a, e, s);
+            [[fallthrough]];
         default: return launch<T, 4, 4, 2, 2, 2, 1>(a, e, s);
     }
 }

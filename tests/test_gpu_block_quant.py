@@ -275,7 +275,7 @@ def test_products_on_other_streams_and_in_graphs():
 
 
 # the kernel for few rows, and the tile forms of the one for many
-@pytest.mark.parametrize("form", range(8))
+@pytest.mark.parametrize("form", range(9))
 def test_every_form(form, monkeypatch):
     monkeypatch.setenv("SANDY_QUANT_FORM", str(form))
     rng = np.random.default_rng(form)
@@ -291,7 +291,7 @@ def test_every_form(form, monkeypatch):
         same(ops.quant_moe_matmul(x, offsets_of(counts, torch.int32), w), want, torch.bfloat16)
 
 
-@pytest.mark.parametrize("form", range(8))
+@pytest.mark.parametrize("form", range(9))
 def test_offsets_past_32_bits(form, monkeypatch):
     """Rows of x, of the weight and of out so far apart that theirs pass 2^32."""
     monkeypatch.setenv("SANDY_QUANT_FORM", str(form))
