@@ -93,10 +93,9 @@ struct SampleArgs {
     int32_t top_k_dt, ids_dt;
     int32_t rows, vocab;
     int32_t bits;         // s
-    int32_t parts, per;   // a part is `per` chunks, one workgroup of the bins and gather kernels
-    int32_t peak_parts, peak_per;
+    int32_t parts, per;   // a part is `per` chunks, one workgroup of the peak, bins and gather kernels
     // workspace of rows in parts
-    Peak* peaks;          // [rows, peak_parts]
+    Peak* peaks;          // [rows, parts]
     uint64_t* weights;    // [rows, parts, kBins]
     uint32_t* counts;     // [rows, parts, kBins]
     uint64_t* upto;       // [rows, kBins]: the row's weight up to and with each bin
@@ -155,6 +154,27 @@ __device__ __forceinline__ V block_scan(V v, V* waves, V* total) {
     }
     *total = all;
     return before + v;
+}
+
+// Two at once.
+template <int WAVES>
+__device__ __forceinline__ void block_scan(uint64_t& a, uint32_t& b, uint64_t* waves_a, uint32_t* waves_b, uint64_t* total_a) {
+    const int wave = threadIdx.x >> 6;
+    a = wave_scan(a);
+    b = wave_scan(b);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 63) waves_a[wave] = a, waves_b[wave] = b;
+    __syncthreads();
+    uint64_t before_a = 0, all = 0;
+    uint32_t before_b = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        if (w < wave) before_a += waves_a[w], before_b += waves_b[w];
+        all += waves_a[w];
+    }
+    a += before_a;
+    b += before_b;
+    *total_a = all;
 }
 
 // ------------------------------------------------------------------ a row's settings
@@ -423,7 +443,6 @@ struct NarrowShared {
 template <typename Each>
 __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint64_t weight, uint32_t most, uint64_t low, uint64_t high, Each each) {
     const int tid = threadIdx.x;
-    uint32_t tokens;
     if (tid == 0) sh.lo = low, sh.hi = high, sh.weight_before = 0, sh.count_before = 0, sh.n = most;
     __syncthreads();
     while (sh.n > 64) {  // a step of 1024 of the last one
@@ -446,8 +465,11 @@ __device__ __forceinline__ uint64_t narrow(NarrowShared& sh, uint32_t rank, uint
             w_to[i] = mine += w[i] = sh.bin_weights[kPer * tid + i];
             c_to[i] = mine_c += c[i] = sh.bin_counts[kPer * tid + i];
         }
-        const uint64_t w_before = sh.weight_before + block_scan<kWaves>(mine, sh.waves64, &all) - mine;
-        const uint32_t c_before = sh.count_before + block_scan<kWaves>(mine_c, sh.waves32, &tokens) - mine_c;
+        uint64_t w_before = mine;
+        uint32_t c_before = mine_c;
+        block_scan<kWaves>(w_before, c_before, sh.waves64, sh.waves32, &all);
+        w_before += sh.weight_before - mine;
+        c_before += sh.count_before - mine_c;
         int here = -1;
 #pragma unroll
         for (int i = 0; i < kPer; i++) {
@@ -712,9 +734,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
 // ------------------------------------------------------------------ rows in parts
 template <typename T>
 __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
-    const int row = blockIdx.x / a.peak_parts, part = blockIdx.x - row * a.peak_parts;
+    const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
     const int64_t at = row * a.stride;
-    const int begin = part * a.peak_per * kChunk, end = min(begin + a.peak_per * kChunk, a.vocab);
+    const int begin = part * a.per * kChunk, end = min(begin + a.per * kChunk, a.vocab);
     float mx = -__builtin_inff(), mn = __builtin_inff();
     int eight = -1, arg = INT32_MAX;  // the first eight that hold the maximum, looked at again for its id
     part_tokens<T, 4>(a, at, begin, end, [&](const float (&v)[8], int i) {
@@ -749,8 +771,8 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int row, Row* shared)
     if (threadIdx.x < 64) {
         float mx = -__builtin_inff(), mn = __builtin_inff();
         int arg = INT32_MAX;
-        if (static_cast<int>(threadIdx.x) < a.peak_parts) {
-            const Peak p = a.peaks[static_cast<int64_t>(row) * a.peak_parts + threadIdx.x];
+        if (static_cast<int>(threadIdx.x) < a.parts) {
+            const Peak p = a.peaks[static_cast<int64_t>(row) * a.parts + threadIdx.x];
             mx = p.max, arg = p.arg, mn = p.min;
         }
         wave_peak(mx, arg, mn);
@@ -979,7 +1001,7 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
 
 // How a call's rows are cut, and its workspace; rows that a workgroup does need none.
 struct Plan {
-    int32_t parts, per, peak_parts, peak_per;
+    int32_t parts, per;
     int64_t peaks, weights, counts, upto, settings, cuts, listed, list, kept, bytes;
 };
 
@@ -996,21 +1018,18 @@ Plan plan_of(int64_t rows, int64_t vocab) {
     if (by_rows(vocab)) return p;
     rows = std::min(rows, kSlab);
     const int64_t chunks = (vocab + kChunk - 1) / kChunk;
-    auto split = [&](int64_t most, int32_t* parts, int32_t* per) {
-        const int64_t want = std::max<int64_t>(std::min<int64_t>({most, chunks, kParts}), 1);
-        *per = static_cast<int32_t>((chunks + want - 1) / want);
-        *parts = static_cast<int32_t>((chunks + *per - 1) / *per);
-    };
-    // peaks: as many workgroups as there may be; bins: about four a CU, since each leaves 12 KB behind
-    split(kParts, &p.peak_parts, &p.peak_per);
-    split((1024 + rows - 1) / rows, &p.parts, &p.per);
+    // about four workgroups a CU, since each leaves 12 KB of bins behind (64 rows of 262144, top-p 0.9: 76 us; with eight 82,
+    // with two 90; the peaks alone in as many parts as there may be: 78)
+    const int64_t want = std::max<int64_t>(std::min<int64_t>({(1024 + rows - 1) / rows, chunks, kParts}), 1);
+    p.per = static_cast<int32_t>((chunks + want - 1) / want);
+    p.parts = static_cast<int32_t>((chunks + p.per - 1) / p.per);
     int64_t at = 0;
     auto take = [&](int64_t bytes) {
         const int64_t here = at;
         at += (bytes + 255) / 256 * 256;
         return here;
     };
-    p.peaks = take(rows * p.peak_parts * static_cast<int64_t>(sizeof(Peak)));
+    p.peaks = take(rows * p.parts * static_cast<int64_t>(sizeof(Peak)));
     p.weights = take(rows * p.parts * kBins * 8);
     p.counts = take(rows * p.parts * kBins * 4);
     p.upto = take(rows * kBins * 8);
@@ -1042,8 +1061,8 @@ int launch_sample(SampleArgs a, Err e, hipStream_t s) {
             hipLaunchKernelGGL(sample_row_kernel<T>, rows, dim3(kThreads), 0, s, a);
             continue;
         }
-        const dim3 parts(static_cast<unsigned>(a.rows) * a.parts), peaks(static_cast<unsigned>(a.rows) * a.peak_parts);
-        hipLaunchKernelGGL(sample_peak_kernel<T>, peaks, dim3(256), 0, s, a);
+        const dim3 parts(static_cast<unsigned>(a.rows) * a.parts);
+        hipLaunchKernelGGL(sample_peak_kernel<T>, parts, dim3(256), 0, s, a);
         hipLaunchKernelGGL(sample_bins_kernel<T>, parts, dim3(256), 0, s, a);
         hipLaunchKernelGGL(sample_cut_kernel, rows, dim3(kThreads), 0, s, a);
         hipLaunchKernelGGL(sample_gather_kernel<T>, parts, dim3(256), 0, s, a);
@@ -1118,8 +1137,6 @@ extern "C" int sandy_hip_sample(const SandyTensor* logits, const SandyTensor* te
     a.vocab = static_cast<int32_t>(vocab);
     a.parts = p.parts;
     a.per = p.per;
-    a.peak_parts = p.peak_parts;
-    a.peak_per = p.peak_per;
     a.bits = 62 - (vocab > 1 ? 64 - __builtin_clzll(static_cast<uint64_t>(vocab - 1)) : 0);
     if (a.bits > 50) a.bits = 50;
     char* w = static_cast<char*>(workspace);
