@@ -112,6 +112,9 @@ __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
 //   128 x 128, 192 x 256, 256 x 256    1024 x 11264 x 2048  36, 48, 30      2048 x 11264 x 2048  55, 52, 60
 //   4096 x 2560 x 2048   31, 26, 30    8192 x 2816 x 2816   71, 65, 77      4096 x 11264 x 2048  99, 102, 96
 //   1500 x 8192 x 4096   61, 47, 50    4096 x 4096 x 4096   70, 81, 57      4096 x 8192 x 8192   266, 237, 204
+// A short k, mostly output: 64 x 128, of which there are three a CU (128 x 128, 192 x 256 behind it):
+//   4096 x 2560 x 64     8.0, 9.8, 10.7    1000 x 5632 x 256    7.7, 8.1, 12.7    561 x 17025 x 23    15, 21, 31
+//   83 x 32000 x 704     11.2, 11.4, 17.5  634 x 11264 x 768    17.7, 13.8, 21.6
 // Few rows: the stream of the weight.  Every workgroup reads x for 16 columns, so that more rows and many columns are for tiles:
 //   1 x 11264 x 2048     7.2, 64 x 64 split 8.7      16 x 2048 x 2048  5.4, 32 x 32 split 5.9    16 x 8192 x 8192  24 against 16
 //   1 x 28672 x 8192     52, 64 x 128 split 62       4 x 16384 x 4096   19 against 17       1 x 32000 x 2048  18.3, 64 x 128 15.2
@@ -128,21 +131,21 @@ QuantForm form_of(const QuantGemm& a, bool bf16) {
     const int64_t some = std::min<int64_t>(a.groups, a.rows), rows = (a.rows + some - 1) / some;
     auto tiles = [&](int64_t m, int64_t n) { return (rows + m - 1) / m * some * ((a.n + n - 1) / n); };
     const int64_t least = tiles(64, 64), streams = int64_t{a.groups} * ((a.n + 15) / 16);
-    const int64_t alone = least <= 128 && a.blocks < 64 ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0;
-    const int64_t few = a.offsets ? (streams <= 4096 ? 2 : 0) : alone;
+    const bool brief = a.blocks <= 6;
+    const int64_t alone = least <= 128 ? (brief ? 32 : a.blocks < 64 ? 16 : 4) : least < 256 && brief ? 16 : least < 256 || a.blocks >= 64 ? 4 : 0;
+    const int64_t few = !a.offsets ? alone : streams <= 1024 ? (brief ? 16 : 8) : streams <= 4096 ? 2 : 0;
     if (rows <= few) return QuantForm::kStream;
-    if (tiles(32, 32) <= (a.blocks >= 32 ? 512 : 256)) return QuantForm::k32x32Split;
-    if (least <= 256) return QuantForm::k64x64Split;
-    if (a.offsets) {
-        if (rows > 64 && tiles(128, 128) >= 512) return QuantForm::k128x128;
-        return tiles(64, 128) <= 128 || a.blocks >= 32 ? QuantForm::k64x128Split : QuantForm::k64x128;
-    }
+    if (tiles(32, 32) <= (a.blocks >= (bf16 ? 32 : 16) ? 512 : 256)) return QuantForm::k32x32Split;
+    if (least <= 256 || a.n <= 64) return QuantForm::k64x64Split;
+    if (a.offsets && rows <= 64) return tiles(64, 128) <= 128 || a.blocks >= 32 ? QuantForm::k64x128Split : QuantForm::k64x128;
     if (tiles(64, 128) <= 256 || (rows <= 64 && a.blocks >= 32)) return QuantForm::k64x128Split;
-    if (rows <= 64) return QuantForm::k64x128;
-    if (tiles(128, 128) <= 256) return QuantForm::k128x128Split;
-    // rounds, of 512 tiles of 128 x 128 and 256 larger ones, in times of the former (36, 47 and 57 us at k = 4096)
-    auto rounds = [&](int64_t count, int64_t at_once) { return static_cast<double>((count + at_once - 1) / at_once); };
-    const double small = rounds(tiles(128, 128), 512), middle = 1.35 * rounds(tiles(192, 256), 256), large = 1.63 * rounds(tiles(256, 256), 256);
+    if (rows <= 64 || a.blocks <= 4 || (a.blocks <= 8 && tiles(128, 128) <= 256)) return QuantForm::k64x128;
+    if (tiles(128, 128) <= 256 && a.blocks >= 24) return QuantForm::k128x128Split;
+    // rounds, of 512 tiles of 128 x 128 and 256 larger ones, in times of the former (36, 47 and 57 us at k = 4096; 13.5 and 27 at
+    // k = 704; f32 outputs 60 and 113 at k = 4096).  Over 430 drawn sizes the choice is within 1 % of the best form.
+    auto rounds = [&](int64_t m, int64_t n, int64_t at_once) { return static_cast<double>((tiles(m, n) + at_once - 1) / at_once); };
+    const double small = rounds(128, 128, 512), middle = (1.25 + 2.0 / a.blocks) * rounds(192, 256, 256);
+    const double large = ((bf16 ? 1.55 : 1.85) + 3.0 / a.blocks) * rounds(256, 256, 256);
     if (bf16 && middle < std::min(small, large)) return QuantForm::k192x256;
     return large < small ? QuantForm::k256x256 : QuantForm::k128x128;
 }

@@ -60,7 +60,8 @@ __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-template <typename T, int WM, int WN, int PM, int PN, int STAGES, int SPLIT>
+// WHOLE: rows of out begin on 16-byte boundaries.
+template <typename T, bool WHOLE, int WM, int WN, int PM, int PN, int STAGES, int SPLIT>
 __global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(QuantGemm a, int m_tiles, int n_tiles) {
     using G = QuantTile<WM, WN, PM, PN, STAGES, SPLIT>;
     constexpr bool kScaled = std::is_same_v<T, BF16>;
@@ -409,7 +410,6 @@ __global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(Qua
     unsigned char* part = lds + wave * 32 * kRow;
     const int mw = 32 * WM * wm, nw = 32 * WN * wn;
     E* out = static_cast<E*>(a.out) + r0 * a.out_pitch + n0;
-    const bool whole = ((reinterpret_cast<uintptr_t>(out) | static_cast<uintptr_t>(a.out_pitch * static_cast<int64_t>(sizeof(E)))) & 15) == 0;
 #pragma unroll
     for (int t = 0; t < WM; t++) {
         if (mw + 32 * t >= xrows) break;
@@ -430,22 +430,67 @@ __global__ __launch_bounds__(64 * PM * PN * SPLIT, 1) void quant_tile_kernel(Qua
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        if constexpr (WHOLE) {
 #pragma unroll
-        for (int i = 0; i < 32 * kLanes / 64; i++) {
-            const int at = 64 * i + lane, r = mw + 32 * t + at / kLanes, n = nw + kEach * (at % kLanes);
-            const unsigned char* p = part + at / kLanes * kRow + 16 * (at % kLanes);
-            if (r >= xrows || n >= wrows) continue;
-            if (whole && n + kEach <= wrows) {
-                __builtin_nontemporal_store(*reinterpret_cast<const i32x4_t*>(p), reinterpret_cast<i32x4_t*>(out + r * a.out_pitch + n));
-            } else if (whole) {
-                for (int j = 0; j < kEach && n + j < wrows; j++) out[r * a.out_pitch + n + j] = reinterpret_cast<const E*>(p)[j];
+            for (int i = 0; i < 32 * kLanes / 64; i++) {
+                const int at = 64 * i + lane, r = mw + 32 * t + at / kLanes, n = nw + kEach * (at % kLanes);
+                const unsigned char* p = part + at / kLanes * kRow + 16 * (at % kLanes);
+                if (r >= xrows || n >= wrows) continue;
+                if (n + kEach <= wrows) {
+                    __builtin_nontemporal_store(*reinterpret_cast<const i32x4_t*>(p), reinterpret_cast<i32x4_t*>(out + r * a.out_pitch + n));
+                } else {
+                    for (int j = 0; j < kEach && n + j < wrows; j++) out[r * a.out_pitch + n + j] = reinterpret_cast<const E*>(p)[j];
+                }
             }
-        }
-        if (!whole) {
-            // rows of other alignments: neighbouring lanes write neighbouring columns
-            for (int at = lane; at < 32 * 32 * WN; at += 64) {
-                const int r = mw + 32 * t + at / (32 * WN), n = nw + at % (32 * WN);
-                if (r < xrows && n < wrows) out[r * a.out_pitch + n] = *reinterpret_cast<const E*>(part + at / (32 * WN) * kRow + sizeof(E) * (at % (32 * WN)));
+        } else {
+            // rows of other alignments: the 16-byte pieces that memory has, put together from LDS, then what is left of every
+            // row on either side, in halves of a piece and so on (2048 x 11263 x 2048: 92 us with stores of one column, 75 so)
+            const int most = min(32 * WN, wrows - nw);
+            // of a row: where it goes, how far its first boundary is, how many whole pieces follow
+            auto pieces = [&](int row, int* lead, int* full) {
+                E* const to = out + static_cast<int64_t>(mw + 32 * t + row) * a.out_pitch + nw;
+                *lead = static_cast<int>(-(reinterpret_cast<uintptr_t>(to) / sizeof(E)) & (kEach - 1));
+                *full = max(most - *lead, 0) / kEach;
+                return to;
+            };
+            int lead, full;
+#pragma unroll 1
+            for (int at = lane; at < 32 * kLanes; at += 64) {
+                const int row = at / kLanes, p = at % kLanes;
+                if (mw + 32 * t + row >= xrows) break;
+                E* const to = pieces(row, &lead, &full);
+                if (p >= full) continue;
+                const int e0 = lead + kEach * p;
+                const uint32_t* w = reinterpret_cast<const uint32_t*>(part + row * kRow + (e0 * static_cast<int>(sizeof(E)) & ~3));
+                i32x4_t v;
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[j] = static_cast<int>(sizeof(E) == 2 && (e0 & 1) ? __builtin_amdgcn_alignbit(w[j + 1], w[j], 16) : w[j]);
+                *reinterpret_cast<i32x4_t*>(to + e0) = v;
+            }
+            if (mw + 32 * t + col < xrows) {  // a lane the near side of a row, another the far
+                E* const to = pieces(col, &lead, &full);
+                const E* row = reinterpret_cast<const E*>(part + col * kRow);
+                if (lead >= most) {
+                    for (int e = half; e < most; e += 2) to[e] = row[e];
+                } else {
+                    int e = half ? lead + full * kEach : 0;
+                    const int left = half ? most - e : lead;
+#pragma unroll
+                    for (int s = 1; s < kEach; s <<= 1) {
+                        const int size = half ? kEach / 2 / s : s;  // up to a boundary growing, behind it shrinking
+                        if (!(left & size)) continue;
+                        if (size == 1) {
+                            to[e] = row[e];
+                        } else if (size == 2) {
+                            const E v[2] = {row[e], row[e + 1]};
+                            __builtin_memcpy(__builtin_assume_aligned(to + e, sizeof(v)), v, sizeof(v));
+                        } else {
+                            const E v[4] = {row[e], row[e + 1], row[e + 2], row[e + 3]};
+                            __builtin_memcpy(__builtin_assume_aligned(to + e, sizeof(v)), v, sizeof(v));
+                        }
+                        e += size;
+                    }
+                }
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

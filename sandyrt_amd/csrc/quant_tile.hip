@@ -15,7 +15,9 @@ int launch(const QuantGemm& a, Err e, hipStream_t s) {
     const int64_t some = std::min<int64_t>(a.rows, a.groups), n = (a.n + G::BN - 1) / G::BN;
     const int64_t m = a.offsets ? some + (a.rows - some) / G::BM : (a.rows + G::BM - 1) / G::BM;
     if (m * n > (int64_t{1} << 22)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
-    const auto kernel = quant_tile_kernel<T, WM, WN, PM, PN, STAGES, SPLIT>;
+    const uint64_t row_bytes = static_cast<uint64_t>(a.out_pitch) * sizeof(typename Vec8<T>::elem);
+    const auto kernel = ((reinterpret_cast<uintptr_t>(a.out) | row_bytes) & 15) == 0 ? quant_tile_kernel<T, true, WM, WN, PM, PN, STAGES, SPLIT>
+                                                                                    : quant_tile_kernel<T, false, WM, WN, PM, PN, STAGES, SPLIT>;
     SANDY_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kBytes), e, "quant tile");
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>((m * n + 7) / 8 * 8)), dim3(SPLIT * G::kThreads), kBytes, s, a, static_cast<int>(m), static_cast<int>(n));
     SANDY_HIP_TRY(hipGetLastError(), e, "quant tile launch");
