@@ -644,7 +644,7 @@ int sandy_hip_quant_moe_matmul(const SandyTensor* x, const SandyTensor* x_scales
 /* ---------------------------------------------------------------- sampling */
 
 /*
- * One token a row of logits [rows, vocab] (F32 or BF16, unit inner stride, rows any distance apart; vocab <= 2^24),
+ * One token a row of logits [rows, vocab] (F32 or BF16, unit inner stride, rows any distance apart; vocab <= 2^24, rows <= 2^17),
  * with each row's own settings, all on the device.  The reference picks on the host, greedily among equals by the
  * lowest id (src/server/Sampler.cpp:69-79,212); here too rank is by logit, then id.  A logit of -inf or NaN is never
  * drawn.  With w = exp((logit - max) / temperature):

@@ -22,6 +22,7 @@ namespace {
 // loads 32 bytes of its weight row (16 rows of whole 128-byte lines a wave) and of its x row straight into the operand
 // registers, DEPTH blocks ahead.  The waves' sums meet in LDS, in their order.  More than 16 rows go round again, the
 // weights then coming from L2.
+// One row of 28672 x 8192: 52 us, 4.5 TB/s of HBM; of 11264 x 2048 7.2 us, 3.2 TB/s, where a call that does nothing takes 2.
 template <typename T, int WAVES, int DEPTH>
 __global__ __launch_bounds__(64 * WAVES) void quant_stream_kernel(QuantGemm a) {
     __shared__ float red[WAVES][4][64];

@@ -609,6 +609,8 @@ __device__ __forceinline__ void row_tokens(const SampleArgs& a, int64_t at, F f)
     }
 }
 
+// Bound by one CU's vector instructions (40 a token to weigh it, half of them in 64 bits) and the meetings of its waves: 512
+// rows of 8000 bf16 tokens in two rounds 24 us by temperature alone, 43 with top-k 50, 45 with top-p 0.9.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     __shared__ RowShared sh;
@@ -732,6 +734,9 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
 }
 
 // ------------------------------------------------------------------ rows in parts
+// Times of each: 64 rows of 262144 bf16 logits, 33.5 MB, with top-p 0.9.
+
+// A stream from HBM: 7 us, 4.9 TB/s.  A thread keeps the eight with its maximum and looks them up again for the id.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
@@ -783,7 +788,7 @@ __device__ __forceinline__ Row row_of(const SampleArgs& a, int row, Row* shared)
 }
 
 // Counts where top_k asks for them, weights unless all of top_k's tokens are listed; the part's weight of rows that
-// nothing cuts but min_p.
+// nothing cuts but min_p.  26 us, 17 of them issuing the 40 instructions a token of its weight and bin.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
     __shared__ uint64_t weights[kBins], waves[4];
@@ -826,6 +831,7 @@ __global__ __launch_bounds__(256) void sample_bins_kernel(SampleArgs a) {
     }
 }
 
+// Sums of the parts' bins, and the cuts: 5 us, a chain of dependent loads, scans and meetings.
 __global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleArgs a) {
     __shared__ CutShared sh;
     const int row = blockIdx.x, bin = kPer * threadIdx.x;
@@ -857,6 +863,7 @@ __global__ __launch_bounds__(kThreads) void sample_cut_kernel(SampleArgs a) {
 
 // Lists the tokens in question, and sums up what a part keeps for sure from its bins.  A part lists its tokens in LDS,
 // takes as many places of the row's list at once and copies them there; what LDS has no room for goes there by itself.
+// 15 us, 2.3 TB/s: settings, bins and tokens one after the other, then a place of the list.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
     __shared__ uint64_t waves[4], places[kPartList];
@@ -908,6 +915,8 @@ struct DrawShared {
     int chosen;
 };
 
+// The listed tokens narrowed down, and the draw: the part, then the token.  A workgroup a row, 64 CUs of 256: 24 us, of which
+// settings and list 2, narrowing 3 (50 listed tokens) to 9 (650), the part 1, a block of its tokens 3 each.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     __shared__ DrawShared sh;
