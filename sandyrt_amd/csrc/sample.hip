@@ -46,7 +46,7 @@ struct Peak {
 // A row's parameters and settings.
 struct Row {
     double rate;        // log2(e) / temperature
-    float max, scale;   // a logit's bin: (max - logit) * scale
+    float max, half, scale;  // a logit's bin: (max / 2 - logit / 2) * scale, since max - logit may be beyond f32
     float top_p, least; // least: min_p
     float uniform;
     int32_t arg, bits;
@@ -195,6 +195,7 @@ __device__ __forceinline__ Row make_row(const SampleArgs& a, int row, float mx, 
     r.least = a.min_p ? a.min_p[row] : 0.0f;
     r.uniform = a.uniforms[row];
     r.max = mx;
+    r.half = 0.5f * mx;
     r.arg = arg;
     r.bits = a.bits;
     r.top_k = k > 0 && k < a.vocab ? static_cast<uint32_t>(k) : 0;
@@ -203,7 +204,7 @@ __device__ __forceinline__ Row make_row(const SampleArgs& a, int row, float mx, 
     r.rate = 1.4426950408889634074 / static_cast<double>(t);
     // bins reach to where weights vanish (2^-bits-1, and a little on), or to the lowest logit where that is nearer
     const double width = fmin(static_cast<double>(mx) - static_cast<double>(mn), (a.bits + 1.5) / r.rate);
-    r.scale = width > 0.0 ? static_cast<float>(fmin((kBins - 2) / width, 3.0e38)) : 0.0f;
+    r.scale = width > 0.0 ? static_cast<float>(fmin(2 * (kBins - 2) / width, 3.0e38)) : 0.0f;
     return r;
 }
 
@@ -252,14 +253,14 @@ __device__ __forceinline__ uint64_t weight_of(const Row& r, float l, bool all = 
 // Non-decreasing as logits fall; the last bin holds no token that weighs anything (those end a ninetieth before it, or
 // the lowest logit ends at kBins - 2).
 __device__ __forceinline__ int bin_of(const Row& r, float l) {
-    const float at = l == r.max ? 0.0f : (r.max - l) * r.scale;
+    const float at = l == r.max ? 0.0f : fmaf(l, -0.5f, r.half) * r.scale;
     const int bin = static_cast<int>(fminf(at, static_cast<float>(kBins - 2)));
     return at >= static_cast<float>(kBins - 1) ? kBins - 1 : bin;
 }
 
 // The logits between which all tokens of bins b0 .. b1 lie, a little widened: bins are rounded.
 __device__ __forceinline__ void logits_of_bins(const Row& r, int b0, int b1, float* low, float* high) {
-    const double most = r.max, wide = 1.0 / r.scale, edge = 1e-6 * fabs(most);
+    const double most = r.max, wide = 2.0 / r.scale, edge = 1e-6 * fabs(most);
     const bool all = !(fabs(most) < 3.0e38) || r.scale == 0.0f;
     *high = b0 <= 0 || all ? r.max : static_cast<float>(most - b0 * wide * (1 - 1e-6) + edge);
     *low = b1 >= kBins - 2 || all ? -__builtin_inff() : static_cast<float>(most - (b1 + 1) * wide * (1 + 1e-6) - edge);
@@ -411,7 +412,7 @@ __device__ __forceinline__ Cut find_cuts(const Row& r, const uint32_t (&c)[kPer]
     if (r.by_p()) cut.sure = min(cut.sure, p_first = sh.p_first);
     if (r.least > 0.0f) {
         // min_p's cut is at a logit: within a bin of where that falls
-        const double at = -log2(static_cast<double>(r.least)) / r.rate * static_cast<double>(r.scale);
+        const double at = -log2(static_cast<double>(r.least)) / r.rate * (0.5 * static_cast<double>(r.scale));
         if (at < kBins) {
             cut.m_first = max(static_cast<int>(at) - 1, 0);
             cut.m_last = static_cast<int>(at) + 1;

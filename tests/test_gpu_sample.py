@@ -71,6 +71,20 @@ def test_edges_of_the_settings():
         check(model_logits(rng, 8, 300, torch.float32), [u] * 8, k=k, p=[0.0, 1e-30, 0.5, last] * 2, least=[0.0, 1.0, 0.1, 0.2] * 2)
 
 
+@pytest.mark.parametrize("vocab", [40, 3000, 20000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_further_apart_than_f32_reaches(vocab, dtype):
+    """Temperatures so high that tokens weigh something whose distance from the maximum no f32 holds."""
+    rng = np.random.default_rng(vocab + 7)
+    x = torch.from_numpy(rng.uniform(-3.3e38, 3.3e38, (6, vocab))).to(dtype).cuda()
+    t = [1e37, 3e37, 1e38, 1e38, 3e38, 3e38]
+    for u in (0.2, 0.9, 1 - 2.0 ** -24):
+        check(x, [u] * 6, t=t)
+        check(x, [u] * 6, t=t, k=[3, 20, vocab - 1, vocab - 5, vocab * 4 // 5, vocab - 2])
+        check(x, [u] * 6, t=t, p=[0.5, 0.9, 0.95, 0.99, 0.999, 0.9999])
+        check(x, [u] * 6, t=t, k=[0, 0, vocab - 2, vocab - 1, 0, 30], p=[1.0, 0.99, 0.999, 0.9, 0.99, 0.9], least=[0.1, 0.3, 0.15, 0.01, 0.12, 0.2])
+
+
 @pytest.mark.parametrize("vocab", [5, 5000, 20000, 70000])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_equal_logits(vocab, dtype):
