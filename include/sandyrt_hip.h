@@ -635,7 +635,8 @@ int sandy_hip_quant_linear(const SandyTensor* x, const SandyTensor* x_scales, co
  * The grouped form (sandy_hip_moe_matmul over matrices in 8 bits, weights [E, n, k]): rows expert_offsets[e] ..
  * expert_offsets[e + 1] - 1 of x [N, k] times weight[e]^T.  expert_offsets E + 1 values (I32 or I64); an expert whose
  * two are out of order or out of 0..N is recorded (SANDY_DEVERR_OFFSETS) and writes nothing (a row that two others
- * then both claim holds either's product).  Rows of out that no expert has are left as they were.
+ * then both claim holds either's product, and where the others claim more than N rows in all, some stay as they were).
+ * Rows of out that no expert has are left as they were.
  */
 int sandy_hip_quant_moe_matmul(const SandyTensor* x, const SandyTensor* x_scales, const SandyTensor* expert_offsets,
                                const SandyTensor* weight, const SandyTensor* weight_scales, const SandyTensor* out,

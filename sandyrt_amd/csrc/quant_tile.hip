@@ -14,7 +14,7 @@ int launch(const QuantGemm& a, Err e, hipStream_t s) {
     // row tiles: of the experts, not known here, at most one each that has a row and one more for every BM further rows
     const int64_t some = std::min<int64_t>(a.rows, a.groups), n = (a.n + G::BN - 1) / G::BN;
     const int64_t m = a.offsets ? some + (a.rows - some) / G::BM : (a.rows + G::BM - 1) / G::BM;
-    if (m * n > (int64_t{1} << 22)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
+    if (m * n + 7 > UINT32_MAX / (SPLIT * G::kThreads)) return fail(e, SANDY_ERR_UNSUPPORTED, "quant product of too many tiles");
     const uint64_t row_bytes = static_cast<uint64_t>(a.out_pitch) * sizeof(typename Vec8<T>::elem);
     const auto kernel = ((reinterpret_cast<uintptr_t>(a.out) | row_bytes) & 15) == 0 ? quant_tile_kernel<T, true, WM, WN, PM, PN, STAGES, SPLIT>
                                                                                     : quant_tile_kernel<T, false, WM, WN, PM, PN, STAGES, SPLIT>;

@@ -309,6 +309,19 @@ def test_offsets_past_32_bits(form, monkeypatch):
     same(out, product(near, held), torch.bfloat16)
 
 
+def test_more_than_2_22_tiles():
+    rows, part = (1 << 28) + 70, 1 << 26
+    rng = np.random.default_rng(0)
+    w = R.whole(rng, (3, 16), 128)
+    some = R.whole(rng, ((1 << 16) + 1, 16), 1)  # an odd number of rows, again and again
+    times = -(-rows // some.payload.shape[0])
+    x = ops.QuantMatrix(some.payload.view(torch.uint8).repeat(times, 1)[:rows].view(torch.float8_e4m3fn), some.scales.repeat(times, 1)[:rows])
+    got = ops.quant_linear(x, w)
+    for a in range(0, rows, part):
+        assert torch.equal(got[a:a + part], ops.quant_linear(ops.QuantMatrix(x.payload[a:a + part], x.scales[a:a + part]), w))
+    same(got[-1000:], product(ops.QuantMatrix(x.payload[-1000:], x.scales[-1000:]), w), torch.bfloat16)
+
+
 def test_more_than_2_24_blocks():
     x = torch.randn((1 << 24) + 5, 1, device="cuda")
     q = ops.block_quant(x)
