@@ -18,6 +18,7 @@
 // Up to 8192 tokens a workgroup does a row in one launch, reading it up to four times, mostly from L2.  Longer rows are
 // cut into parts, so that few rows fill the chip, and take five launches: peak, bins, cut, gather, draw.
 #include "common.h"
+#include "sample_parts.h"
 
 #include <algorithm>
 #include <type_traits>
@@ -274,15 +275,6 @@ __device__ __forceinline__ void Cut::logits(const Row& r, float* low, float* hig
     logits_of_bins(r, b0, min(b1, limit), low, high);
 }
 
-// p * w rounded up or down, exactly; 0 <= p < 1
-__device__ __forceinline__ uint64_t part_of(float p, uint64_t w, bool up) {
-    const uint32_t u = __float_as_uint(p), e = u >> 23, m = e ? (u & 0x7fffffu) | 0x800000u : u & 0x7fffffu;
-    const int shift = 150 - static_cast<int>(e ? e : 1);  // p = m * 2^-shift, shift >= 24
-    const unsigned __int128 prod = static_cast<unsigned __int128>(m) * w;
-    if (shift >= 100) return up && prod != 0 ? 1 : 0;
-    const uint64_t q = static_cast<uint64_t>(prod >> shift);
-    return q + (up && (prod & ((static_cast<unsigned __int128>(1) << shift) - 1)) != 0 ? 1 : 0);
-}
 // top_p's part of a weight, at least; 0 where it is that of the first token alone
 __device__ __forceinline__ uint64_t nucleus(const Row& r, uint64_t weight) { return r.top_p > 0.0f ? part_of(r.top_p, weight, true) : 0; }
 
@@ -717,7 +709,12 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     static_assert(kSums <= 64);
     const uint64_t part_w = lane < (a.vocab + kBlock - 1) / kBlock * kWaves ? sh.sums[lane & (kSums - 1)] : 0, to = wave_scan(part_w);
     const uint64_t total = __shfl(to, 63, 64), target = part_of(r.uniform, total, false);
-    const int part = __builtin_ctzll(__ballot(to > target));  // (the total is above the target)
+    const uint64_t past = __ballot(to > target);
+    if (past == 0) {  // the total is above the target, unless logits change meanwhile: no place to go on from
+        if (tid == 0) store_token(a, row, -1, 0.0f);
+        return;
+    }
+    const int part = __builtin_ctzll(past);
     if (part % kWaves != wave) return;
     const uint64_t before = __shfl(to - part_w, part, 64);
     float v[8];
@@ -922,7 +919,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     __shared__ DrawShared sh;
     const int tid = threadIdx.x, row = blockIdx.x;
-    if (tid == 0) sh.row = a.settings[row], sh.cut = a.cuts[row];
+    if (tid == 0) sh.row = a.settings[row], sh.cut = a.cuts[row], sh.chosen = -1;
     __syncthreads();
     const Row& r = sh.row;
     const Cut& cut = sh.cut;
@@ -968,6 +965,10 @@ __global__ __launch_bounds__(kThreads) void sample_draw_kernel(SampleArgs a) {
     __syncthreads();
     const uint64_t total = sh.waves64[0], target = part_of(r.uniform, total, false);
     const int part = sh.chosen;
+    if (part < 0) {  // as above
+        if (tid == 0) store_token(a, row, -1, 0.0f);
+        return;
+    }
     uint64_t run = sh.before;
     __syncthreads();
     // the tokens of the part in which the sum passes the target, eight a thread at a time, the next eight requested meanwhile
