@@ -746,8 +746,9 @@ __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
         float top = -__builtin_inff();
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            top = fmaxf(top, v[j]);  // (the number, of a number and NaN)
-            mn = fminf(mn, token(v[j]) ? v[j] : __builtin_inff());
+            const bool in = token(v[j]);  // (a signalling NaN may win fmaxf, and with it hide what came before)
+            top = fmaxf(top, in ? v[j] : -__builtin_inff());
+            mn = fminf(mn, in ? v[j] : __builtin_inff());
         }
         eight = top > mx ? i : eight;
         mx = fmaxf(mx, top);
