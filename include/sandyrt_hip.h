@@ -597,7 +597,9 @@ int sandy_hip_decode_linear(const SandyTensor* x, const SandyTensor* ln_weight, 
  * payloads (U8, [.., rows, k], unit inner stride, rows apart by any pitch that keeps them from overlapping) and
  * scale bytes (U8, contiguous): [.., rows, ceil(k / 128)] with a byte for every 128 columns of a row, or
  * [.., ceil(rows / 128), ceil(k / 128)] with one for every 128 columns of 128 rows.  Values are
- * payload * 2^(c - 127) with c the block's byte; c = 255 stands for NaN.  Blocks at the ends may be short.
+ * payload * 2^(c - 127) with c the block's byte; c = 255 stands for NaN.  Values of 2^128 and more, which block_quant
+ * leaves nowhere (they take a c above 246), are infinite where they are read back and in products with f32 outputs.
+ * Blocks at the ends may be short.
  * Ranks 2 or 3.
  */
 
@@ -611,8 +613,8 @@ int sandy_hip_decode_linear(const SandyTensor* x, const SandyTensor* ln_weight, 
 int sandy_hip_block_quant(const SandyTensor* x, int64_t block_rows, const SandyTensor* payload,
                           const SandyTensor* scales, void* stream, char* err, size_t err_cap);
 
-/* What such a matrix stands for: out contiguous, F32 or BF16 (every value exact in either, but for bf16 below
- * 2^-126). */
+/* What such a matrix stands for: out contiguous, F32 or BF16 (every value below 2^128 exact in either, but for bf16
+ * below 2^-126). */
 int sandy_hip_block_dequant(const SandyTensor* payload, const SandyTensor* scales, const SandyTensor* out,
                             void* stream, char* err, size_t err_cap);
 

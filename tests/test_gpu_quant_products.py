@@ -125,6 +125,25 @@ def test_rows_of_different_ends(rows, dtype):
         same(ops.quant_moe_matmul(x, offsets_of(counts), w, dtype=dtype), grouped(x, counts, w), dtype)
 
 
+@forms
+def test_values_past_the_largest_float(form):
+    """Infinite in f32 outputs and read back; bf16 outputs, whose instruction takes the bytes, hold their products."""
+    x = ops.QuantMatrix(torch.zeros(3, 144, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[:, :130],
+                        torch.tensor([[254, 127], [247, 127], [254, 127]], dtype=torch.uint8, device="cuda"))
+    w = ops.QuantMatrix(torch.zeros(2, 144, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[:, :130],
+                        torch.tensor([[7, 127]], dtype=torch.uint8, device="cuda"))
+    for q, column in ((x, [2.0, 448.0, -1.875]), (w, [1.0, -2.0])):
+        q.payload[:, 3] = torch.tensor(column, device="cuda").to(torch.float8_e4m3fn)
+        q.payload[:, 129] = torch.ones(len(column), device="cuda").to(torch.float8_e4m3fn)
+    inf, row = float("inf"), 2.0 ** 7
+    for dtype in TYPES:
+        back = ops.block_dequant(x, dtype)[:, [3, 129]].float()
+        assert back.tolist() == [[inf, 1.0], [inf, 1.0], [-1.875 * 2.0 ** 127, 1.0]]
+    assert ops.quant_linear(x, w, dtype=torch.float32).tolist() == [[inf, -inf], [inf, -inf], [-1.875 * row + 1, 3.75 * row + 1]]
+    exact = torch.tensor([[2 * row + 1, -4 * row + 1], [449.0, -895.0], [-1.875 * row + 1, 3.75 * row + 1]])
+    assert torch.equal(ops.quant_linear(x, w).cpu(), exact.bfloat16())
+
+
 # ------------------------------------------------------------------ what the sums of bf16 outputs hold
 def cut_off(x, w):
     """(sums of magnitudes, roots of sums of squares) of what an output x [k] . w [n, k]^T may lose, where within eight
