@@ -657,8 +657,9 @@ int sandy_hip_quant_moe_matmul(const SandyTensor* x, const SandyTensor* x_scales
  * and the token drawn is the one, walking what is left in order of ids, with which the sum of w passes uniforms[row]
  * (0 <= u < 1, 24 bits) of the whole.  temperature 0 takes the first rank.  temperature, top_p, min_p: [rows] F32 or
  * NULL (1, 1, 0); top_k [rows] I32 or I64 or NULL; ids [rows] I32 or I64; probs NULL or [rows] F32, the token's share
- * of w of what is left.  Every w is held as a whole multiple of 2^-s, s = 62 - ceil(log2(vocab)) but 50 at most, sums
- * and comparisons are exact, so results do not depend on how a call is cut up; what is below 2^-s-1 weighs nothing.
+ * of w of what is left.  Every w is held as a whole multiple of 2^-s, s = 62 - ceil(log2(vocab)) but 50 at most (the
+ * nearest, or one next to it); sums of them and the comparisons of top_p and the draw are exact, min_p's is of w in f64
+ * before that rounding, so results do not depend on how a call is cut up; what is below 2^-s-1 weighs nothing.
  * A row without a token gives id -1 and probability 0; so does one with temperature negative or NaN, top_p NaN, min_p
  * above 1 or NaN, or u out of range, which is recorded (SANDY_DEVERR_SAMPLE).  `workspace` holds
  * sandy_hip_sample_workspace() bytes (16-byte aligned; NULL where that is 0): the call's alone while it runs, its contents need not be kept or

@@ -6,8 +6,8 @@
 //   t = u * sum of the weights of P and M's common tokens;  the token where their running sum, in order of ids, passes t
 //
 // Weights are whole numbers: w_i rounded to 2^-s with s = 62 - log2(vocab) (44 bits of a 262144-token vocabulary).
-// Sums of them are exact in any order, so that atomics, parts and workgroups leave no trace in the result, and every
-// comparison (top_p's and the draw's, whose factors have 24 bits) is exact too, in 128 bits.
+// Sums of them are exact in any order, so that atomics, parts and workgroups leave no trace in the result, and so are
+// comparisons of them (top_p's and the draw's, whose factors have 24 bits), in 128 bits.  min_p looks at w_i itself, in f64.
 //
 // Ranks are never formed.  Logits fall into 1023 bins of equal width from the maximum down to where weights
 // vanish; counts and weights of the bins say in which the cuts of top_k, top_p and min_p lie, and only the tokens there
@@ -209,15 +209,19 @@ __device__ __forceinline__ Row make_row(const SampleArgs& a, int row, float mx, 
     return r;
 }
 
-// (ln 2)^n / n!, n = 11 .. 0
-__device__ constexpr double kSeries[12] = {
+// (ln 2)^n / n!, n = kTerms .. 0
+constexpr int kTerms = 12;
+__device__ constexpr double kSeries[kTerms + 1] = {
+    2.56784359934882055e-11,
     4.44553827187081162e-10, 7.05491162080112336e-09, 1.01780860092396999e-07,
     1.32154867901443095e-06, 1.52527338040598411e-05, 1.54035303933816088e-04,
     1.33335581464284433e-03, 9.61812910762847688e-03, 5.55041086648215831e-02,
     2.40226506959100722e-01, 6.93147180559945286e-01, 1.0};
 // Weights of N logits at once, so that their series interleave: exp((l - max) / T) = 2^f 2^k, 1 at the maximum, f in
-// -1/2 .. 1/2 by the Taylor series of e^(f ln 2) to the 11th power (the next term is below 7e-15 of the sum), rounded to
-// the nearest multiple of 2^-bits, 52 bits of which lie behind 2^52.  Below 2^-200 it stays there, which weighs nothing.
+// -1/2 .. 1/2 by the Taylor series of e^(f ln 2) to the 12th power (the next term is below 2.4e-16 of the sum; an 11th power
+// left 8.9e-15, 7 multiples of 2^-50), rounded to a multiple of 2^-bits, 52 bits of which lie behind 2^52: the nearest, or
+// with roundings of the sum and its exponent (0.7 multiples of 2^-50 at most) one next to it.  Below 2^-200 it stays there,
+// which weighs nothing.
 // `all` false: 0 for those that min_p leaves out.  Masked logits weigh 0.
 template <int N>
 __device__ __forceinline__ void weigh(const Row& r, const float (&l)[N], bool all, uint64_t (&w)[N]) {
@@ -232,7 +236,7 @@ __device__ __forceinline__ void weigh(const Row& r, const float (&l)[N], bool al
         p[j] = kSeries[0];
     }
 #pragma unroll
-    for (int n = 1; n < 12; n++)
+    for (int n = 1; n <= kTerms; n++)
 #pragma unroll
         for (int j = 0; j < N; j++) p[j] = fma(p[j], f[j], kSeries[n]);
     auto two_to = [](int e) { return __longlong_as_double(static_cast<long long>(1023 + e) << 52); };

@@ -39,3 +39,42 @@ def test_nan_of_every_kind(vocab, dtype):
         for s in ({}, dict(t=[0.0] * 6), dict(k=[1, 3, 50, 2000, 0, 2]), dict(p=[0.5, 0.9, 0.99, 0.3, 0.8, 0.95], least=[0.0, 0.1, 0.0, 0.3, 0.01, 0.0])):
             check(x, [u] * 6, **s)
     check(x.mul_(float("nan")), [0.5] * 6)  # nothing left
+
+
+# Two logits 0 and l: exp(l / T) is above min_p by 1.5e-15 to 5.8e-15 of itself.  All are near half a power of two, where a series
+# of 2^f is worst; the comparison is in 64 bits, whose roundings (2.3e-16 of the exponent, 2.5 at most here, in base 2, and of the
+# sum) are below 1e-15 together.
+BARELY = [("-0x1.1ecd28p+1", "0x1.15aca4p+1", "0x1.6c8712p-2"), ("-0x1.6a9f24p-1", "0x1.028444p+1", "0x1.688e86p-1"),
+          ("-0x1.284cc2p-2", "0x1.1b3b8ep-2", "0x1.67b93cp-2"), ("-0x1.d7620cp-1", "0x1.5cf878p+1", "0x1.6d446ap-1"),
+          ("-0x1.0b6424p+2", "0x1.34d0dcp+1", "0x1.6a746ep-3"), ("-0x1.563dbcp+0", "0x1.f26944p+1", "0x1.6b36d0p-1"),
+          ("-0x1.f2141ap+1", "0x1.e3a5fep+1", "0x1.6da296p-2"), ("-0x1.be7df6p-2", "0x1.3ba932p+0", "0x1.677f6ap-1"),
+          ("-0x1.4e4fbcp+1", "0x1.427730p+1", "0x1.6b1f02p-2"), ("-0x1.26bc6cp+1", "0x1.541c6ap+0", "0x1.69ed66p-3"),
+          ("-0x1.526524p+1", "0x1.458eeap+1", "0x1.6a24d6p-2"), ("-0x1.b07b96p-3", "0x1.33afd0p-1", "0x1.684bcap-1"),
+          ("-0x1.26688cp+0", "0x1.ac9654p+1", "0x1.6b2a92p-1"), ("-0x1.581180p+1", "0x1.4ab5dep+1", "0x1.69cbbep-2"),
+          ("-0x1.674756p-1", "0x1.ff4bc0p+0", "0x1.685114p-1"), ("-0x1.a1a680p-3", "0x1.30cf92p-1", "0x1.6b7facp-1"),
+          ("-0x1.9ce10cp-2", "0x1.300482p+0", "0x1.6c9a0ap-1"), ("-0x1.c0f51ep-2", "0x1.44e9eap+0", "0x1.6a72b0p-1"),
+          ("-0x1.e535c6p-2", "0x1.5fd2aap+0", "0x1.6ab004p-1")]
+# A logit 0 and `n` logits l: the first token's share is below u, so that a later one is drawn, by two to four and a half multiples
+# of 2^-50 in the weight of each, which the whole weights, off by one at most, leave room for.
+SHARES = [("-0x1.5c1c88p-2", 2297, "0x1.40777ap-11"), ("-0x1.5c2240p-2", 2929, "0x1.f6b6e0p-12"), ("-0x1.62866cp-2", 3726, "0x1.8db25ap-12"),
+          ("-0x1.5fc9bap-2", 3658, "0x1.940180p-12"), ("-0x1.6a50cep-2", 2411, "0x1.3595c4p-11"), ("-0x1.614f26p-2", 2975, "0x1.f1739cp-12"),
+          ("-0x1.5c1e04p-2", 174, "0x1.0673c4p-7"), ("-0x1.615f8ap-2", 1935, "0x1.7e5594p-11")]
+
+
+@pytest.mark.parametrize("padding", [0, 8200])
+def test_weights_next_to_min_p(padding):
+    """What is kept by a few parts in 10^15."""
+    l, t, least = (np.array([float.fromhex(v) for v in column]) for column in zip(*BARELY))
+    x = torch.full((len(l), 2 + padding), -np.inf)
+    x[:, 0], x[:, 1] = 0.0, torch.from_numpy(l).float()
+    assert (x[:, 1].double().numpy() == l).all() and (t.astype(np.float32) == t).all() and (least.astype(np.float32) == least).all()
+    ids, _ = check(x.cuda(), [1 - 2.0 ** -24] * len(l), t=t, least=least)
+    assert ids.tolist() == [1] * len(l)
+
+
+@pytest.mark.parametrize("l,n,u", SHARES)
+def test_weights_next_to_a_share(l, n, u):
+    x = torch.full((1, n + 1), float.fromhex(l))
+    x[0, 0] = 0.0
+    ids, _ = check(x.cuda(), [float.fromhex(u)])
+    assert ids.item() == 1
