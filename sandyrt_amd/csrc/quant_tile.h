@@ -50,11 +50,15 @@ __device__ __forceinline__ auto some_scales(const uint8_t* row, int j, int block
 
 // 16 bytes a lane from a buffer straight into LDS, the wave's 1024 bytes in a row from `lds` on.  In flight until
 // a wait on vmcnt; the compiler does not count it (its own waits only become stricter).  (s_nop: a vector
-// instruction may just have written one of the scalars.)
+// instruction may just have written one of the scalars.)  m0 is named as overwritten, so that no value the compiler puts
+// there is taken to live across it; the warning that m0 is a reserved register is no news.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void copy_to_lds(i32x4_t buffer, int offset, int more, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(lds), "v"(offset), "s"(buffer), "s"(more)
-                 : "memory");
+                 : "memory", "m0");
 }
+#pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void wait_copies() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
