@@ -78,3 +78,36 @@ def test_weights_next_to_a_share(l, n, u):
     x[0, 0] = 0.0
     ids, _ = check(x.cuda(), [float.fromhex(u)])
     assert ids.item() == 1
+
+
+BAD = [("t", -1.0), ("t", np.nan), ("t", -np.inf), ("p", np.nan), ("least", 1.5), ("least", np.nan), ("u", 1.0), ("u", -0.1), ("u", np.nan),
+       ("u", -2.0 ** -149), ("u", np.inf)]
+
+
+@pytest.mark.parametrize("cuts", [True, False])
+@pytest.mark.parametrize("rows,vocab,bad", [(4, 8193, (1, 3)), (5, 60000, (0, 2)), (2060, 8200, (2, 1023, 1024, 1030, 2048, 2059))])
+def test_settings_out_of_range_of_rows_in_parts(rows, vocab, bad, cuts):
+    """Recorded, and such a row gives -1; its neighbours their tokens, also behind the rows that are done at a time."""
+    rng = np.random.default_rng(rows)
+    x = torch.full((rows, vocab), -np.inf)
+    at = torch.from_numpy(rng.integers(0, vocab, (rows, 12)))
+    x.scatter_(1, at, torch.from_numpy(3 * rng.standard_normal((rows, 12))).float())
+    x = x.cuda()
+    good = dict(t=0.8, p=0.9 if cuts else 1.0, least=0.01, u=0.25)
+
+    def draw(s):
+        return ops.sample(x, f32(s["u"]), temperature=f32(s["t"]), top_p=f32(s["p"]), min_p=f32(s["least"]))
+
+    fine = check(x, [good["u"]] * rows, **{n: [v] * rows for n, v in good.items() if n != "u"})
+    ops.check_device_errors()
+    for name, value in BAD:
+        s = {n: np.full(rows, v, np.float32) for n, v in good.items()}
+        s[name][list(bad)] = value
+        ids, probs = draw(s)
+        with pytest.raises(ops.SandyError, match="sample temperature"):
+            ops.check_device_errors()
+        ops.check_device_errors()
+        want, share = fine[0].clone(), fine[1].clone()
+        want[list(bad)] = -1
+        share[list(bad)] = 0.0
+        assert torch.equal(ids, want) and torch.equal(probs, share), (name, value)
