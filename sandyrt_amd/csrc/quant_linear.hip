@@ -143,7 +143,7 @@ QuantForm form_of(const QuantGemm& a, bool bf16) {
     if (rows <= 64 || a.blocks <= 4 || (a.blocks <= 8 && tiles(128, 128) <= 256)) return QuantForm::k64x128;
     if (tiles(128, 128) <= 256 && a.blocks >= 24) return QuantForm::k128x128Split;
     // rounds, of 512 tiles of 128 x 128 and 256 larger ones, in times of the former (36, 47 and 57 us at k = 4096; 13.5 and 27 at
-    // k = 704; f32 outputs 60 and 113 at k = 4096).  Over 430 drawn sizes the choice is within 1 % of the best form.
+    // k = 704; f32 outputs 60 and 113 at k = 4096).
     auto rounds = [&](int64_t m, int64_t n, int64_t at_once) { return static_cast<double>((tiles(m, n) + at_once - 1) / at_once); };
     const double small = rounds(128, 128, 512), middle = (1.25 + 2.0 / a.blocks) * rounds(192, 256, 256);
     const double large = ((bf16 ? 1.55 : 1.85) + 3.0 / a.blocks) * rounds(256, 256, 256);

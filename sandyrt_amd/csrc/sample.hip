@@ -607,7 +607,7 @@ __device__ __forceinline__ void row_tokens(const SampleArgs& a, int64_t at, F f)
 }
 
 // Bound by one CU's vector instructions (40 a token to weigh it, half of them in 64 bits) and the meetings of its waves: 512
-// rows of 8000 bf16 tokens in two rounds 24 us by temperature alone, 43 with top-k 50, 45 with top-p 0.9.
+// rows of 8000 bf16 tokens in two rounds 24 us by temperature alone, 41 with top-k 50, 43 with top-p 0.9.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
     __shared__ RowShared sh;
@@ -738,7 +738,7 @@ __global__ __launch_bounds__(kThreads) void sample_row_kernel(SampleArgs a) {
 // ------------------------------------------------------------------ rows in parts
 // Times of each: 64 rows of 262144 bf16 logits, 33.5 MB, with top-p 0.9.
 
-// A stream from HBM: 7 us, 4.9 TB/s.  A thread keeps the eight with its maximum and looks them up again for the id.
+// A stream from HBM: 9 to 14 us, 11 on average, 3.1 TB/s.  A thread keeps the eight with its maximum and looks them up again for the id.
 template <typename T>
 __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
     const int row = blockIdx.x / a.parts, part = blockIdx.x - row * a.parts;
