@@ -111,3 +111,36 @@ def test_settings_out_of_range_of_rows_in_parts(rows, vocab, bad, cuts):
         want[list(bad)] = -1
         share[list(bad)] = 0.0
         assert torch.equal(ids, want) and torch.equal(probs, share), (name, value)
+
+
+@pytest.mark.parametrize("vocab", [700, 9000])
+def test_subnormal_logits_and_temperatures(vocab):
+    """Distances that are subnormal floats, one bin for all of them."""
+    rng = np.random.default_rng(vocab + 2)
+    x = torch.from_numpy(rng.integers(-70000, 70000, (6, vocab)) * 2.0 ** -149).float().cuda()
+    assert x.abs().max() < 2.0 ** -126 and x.unique().numel() > 600
+    for t in (2.0 ** -149, 1e-42, 1e-41, 1e-40, 1e-38, 1.0):
+        check(x, rng.random(6, np.float32), t=[t] * 6)
+        check(x, rng.random(6, np.float32), t=[t] * 6, k=[1, 7, 300, vocab - 1, 0, 0], p=[1.0, 0.9, 0.5, 1.0, 0.8, 0.99], least=[0.0, 0.1, 0.0, 0.0, 0.3, 0.0])
+
+
+@pytest.mark.parametrize("vocab", [900, 9000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_infinite_logits_at_every_temperature(vocab, dtype):
+    """The likeliest at inf share all of the weight, however hot."""
+    rng = np.random.default_rng(vocab + 3)
+    x = model_logits(rng, 6, vocab, dtype)
+    for r in range(6):
+        x[r, torch.from_numpy(rng.permutation(vocab)[:r + 1])] = np.inf
+    top = torch.isinf(x)
+    for t in (1e-30, 1.0, 1e30, np.inf):
+        for s in ({}, dict(k=[1, 1, 2, 9, 300, vocab - 1]), dict(p=[0.5] * 6), dict(k=[3] * 6, p=[0.9] * 6, least=[0.2] * 6)):
+            for u in (0.0, 0.6, 1 - 2.0 ** -24):
+                finite = min(t, 1e30)  # inf / inf has no value in the plain form; every finite temperature has the same result
+                ids, probs = check(x, [u] * 6, t=[finite] * 6, **s)
+                if t != finite:
+                    names = dict(k="top_k", p="top_p", least="min_p")
+                    kw = {names[n]: torch.tensor(v, dtype=torch.int32, device="cuda") if n == "k" else f32(v) for n, v in s.items()}
+                    hot = ops.sample(x, f32([u] * 6), temperature=f32([t] * 6), **kw)
+                    assert torch.equal(hot[0], ids) and torch.equal(hot[1], probs)
+                assert bool(top[torch.arange(6, device="cuda"), ids].all())
